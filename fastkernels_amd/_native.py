@@ -107,6 +107,30 @@ _SIGNATURES = {
     "fk_merge_attn_states": (c_int, [c_void_p, c_int64, c_int64, c_void_p, c_void_p, c_void_p,
                                      c_void_p, c_void_p, c_int64, c_int64, c_int64, c_int, c_int,
                                      c_int64, c_int, c_int, c_void_p, c_void_p]),
+    "fk_update_key_bounds": (c_int, [c_void_p, c_void_p, c_int, c_void_p, c_int64, c_int64,
+                                     c_void_p, c_void_p, c_int64, c_int64, c_int, c_int, c_int,
+                                     c_int64, c_void_p]),
+    "fk_block_scores": (c_int, [c_void_p, c_int64, c_int64, c_int64, c_void_p, c_int64, c_void_p,
+                                c_int, c_void_p, c_void_p, c_int64, c_int64, c_void_p, c_void_p,
+                                c_int64, c_int64, c_int64, c_int, c_int, c_int, c_int, c_int64,
+                                c_void_p]),
+    "fk_select_blocks": (c_int, [c_void_p, c_int64, c_int64, c_int64, c_void_p, c_int64, c_int64,
+                                 c_int64, c_void_p, c_void_p, c_int64, c_int64, c_int, c_int,
+                                 c_int, c_int, c_void_p]),
+    "fk_sparse_paged_decode": (c_int, [c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_void_p,
+                                       c_int, c_void_p, c_void_p, c_void_p, c_int64, c_int64,
+                                       c_void_p, c_void_p, c_int64, c_int64, c_void_p, c_int64,
+                                       c_int64, c_int64, c_int, c_int, c_int, c_int, c_int64,
+                                       c_float, c_void_p, c_void_p, c_int64, c_void_p]),
+    "fk_sparse_paged_decode_plan": (c_int, [c_int64, c_int64, c_int, c_int, c_int, c_int,
+                                            c_void_p]),
+    "fk_shared_prefix_decode": (c_int, [c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_void_p,
+                                        c_int, c_void_p, c_void_p, c_void_p, c_int64, c_int64,
+                                        c_void_p, c_int64, c_void_p, c_void_p, c_int64, c_int64,
+                                        c_int, c_int, c_int, c_int, c_int64, c_float, c_int,
+                                        c_void_p, c_void_p, c_int64, c_void_p]),
+    "fk_shared_prefix_decode_plan": (c_int, [c_int64, c_int64, c_int64, c_int, c_int, c_int,
+                                             c_void_p]),
 }
 
 EXPORTED = tuple(_SIGNATURES)
@@ -203,3 +227,21 @@ def decode_shape(batch: int, num_heads: int, num_kv_heads: int, head_size: int, 
     call("fk_paged_decode_shape", batch, num_heads, num_kv_heads, head_size, kv_dtype, window_left,
          part_tokens, max_parts, ctypes.byref(out), ctypes.byref(out, 4), ctypes.byref(out, 8))
     return out[0], out[1], bool(out[2])
+
+
+def sparse_decode_bytes(rows: int, keep: int, num_heads: int, num_kv_heads: int, head_size: int,
+                        block_size: int) -> int:
+    """fk_sparse_paged_decode_plan: the workspace bytes of a sparse decode launch."""
+    ws = c_int64(0)
+    call("fk_sparse_paged_decode_plan", rows, keep, num_heads, num_kv_heads, head_size, block_size,
+         ctypes.byref(ws))
+    return ws.value
+
+
+def shared_prefix_bytes(batch: int, num_groups: int, max_prefix_len: int, num_heads: int,
+                        num_kv_heads: int, head_size: int) -> int:
+    """fk_shared_prefix_decode_plan: the workspace bytes of a shared-prefix launch."""
+    ws = c_int64(0)
+    call("fk_shared_prefix_decode_plan", batch, num_groups, max_prefix_len, num_heads,
+         num_kv_heads, head_size, ctypes.byref(ws))
+    return ws.value

@@ -271,3 +271,83 @@ class FlashAttnDecode(nn.Module):
              a["cache_seqlens"], a["softmax_scale"], a["part_tokens"], a["max_parts"], a["ws"],
              a["k_scale"], a["v_scale"], a["window_left"], a["sinks"])
         return a["out"]
+
+    def _page_args(self, what, q, k_cache, cache_seqlens, kwargs):
+        """The decode kwargs of the entry points below, which plan their own workspaces."""
+        pop = kwargs.pop
+        block_table = pop("block_table", None)
+        if block_table is None or cache_seqlens is None:
+            raise ValueError(f"{what}: block_table and cache_seqlens are required")
+        max_seq_len = pop("max_seq_len", None)
+        softmax_scale = pop("softmax_scale", None)
+        pop("causal", None)
+        out = pop("out", None)
+        k_scale = pop("k_scale", pop("k_descale", None))
+        v_scale = pop("v_scale", pop("v_descale", None))
+        window = pop("window_size", None)
+        if window is None:
+            window = self._window_size
+        s_aux = pop("s_aux", None)
+        if kwargs:
+            raise TypeError(f"{what}: unexpected arguments {sorted(kwargs)}")
+        hk = k_cache.shape[2]
+        if out is None:
+            out = q.new_empty((q.shape[0], self.num_heads, self.head_dim))
+        return dict(
+            out=out,
+            block_table=block_table.to(torch.int32), cache_seqlens=cache_seqlens.to(torch.int32),
+            max_seq_len=max_seq_len,
+            softmax_scale=float(ops.default_softmax_scale(self.head_dim)
+                                if softmax_scale is None else softmax_scale),
+            k_scale=self._scale_vec(k_scale, hk, q.device),
+            v_scale=self._scale_vec(v_scale, hk, q.device),
+            window_left=int(window[0]) if int(window[0]) >= 0 else -1,
+            sinks=self._sinks(s_aux, q.device))
+
+    def forward_shared_prefix(self, q, k_cache, v_cache, cache_seqlens, cu_groups, prefix_lens,
+                              max_prefix_len: int = 0, **kwargs):
+        """``forward`` for a batch in groups of rows that share a prefix, which is read once
+        for its group: rows cu_groups[g] .. cu_groups[g + 1] - 1 (int32 [groups + 1]) have the
+        same tokens at positions below prefix_lens[g] (int32 [groups]).  Their block tables
+        list the shared pages as ever; the first row's is the one read.  kwargs as forward's
+        (without num_splits).  max_prefix_len: a bound on the prefixes, if known."""
+        a = self._page_args("FlashAttnDecode.forward_shared_prefix", q, k_cache, cache_seqlens,
+                            kwargs)
+        call = torch.ops.fastkernels_amd.shared_prefix_decode if torch.compiler.is_compiling() \
+            else ops.shared_prefix_decode
+        b = q.shape[0]
+        call(self._heads(a["out"], b), self._heads(q, b), k_cache, v_cache, a["block_table"],
+             a["cache_seqlens"], cu_groups, prefix_lens, a["softmax_scale"], a["k_scale"],
+             a["v_scale"], a["window_left"], a["sinks"], int(max_prefix_len))
+        return a["out"]
+
+    def forward_sparse(self, q, k_cache, v_cache, key_bounds, cache_seqlens, num_selected: int,
+                       keep_first: int = 1, keep_last: int = 1, cu_seqlens_q=None,
+                       max_seqlen_q: int = 1, **kwargs):
+        """Decode attention over num_selected pages per query row and kv head: the first
+        keep_first, the last keep_last, and those whose key bounds (``ops.update_key_bounds``,
+        kept up to date as tokens are stored) allow the greatest logits.  One row per
+        sequence, or the rows of cu_seqlens_q (a step that checks drafted tokens).  kwargs as
+        forward's (without num_splits; no sliding window); max_seq_len, if given, bounds the
+        pages that are scored."""
+        what = "FlashAttnDecode.forward_sparse"
+        a = self._page_args(what, q, k_cache, cache_seqlens, kwargs)
+        if a["window_left"] >= 0:
+            raise NotImplementedError(f"{what}: a sliding window reads its own few pages; use "
+                                      "forward")
+        n, hk, page = q.shape[0], k_cache.shape[2], k_cache.shape[1]
+        width = a["block_table"].shape[1]
+        if a["max_seq_len"] is not None:
+            width = min(width, -(-int(a["max_seq_len"]) // page))
+        o = torch.ops.fastkernels_amd if torch.compiler.is_compiling() else ops
+        q3 = self._heads(q, n)
+        scores = torch.empty((n, hk, width), dtype=torch.float32, device=q.device)
+        o.block_scores(scores, q3, key_bounds, a["block_table"], a["cache_seqlens"], page,
+                       a["k_scale"], cu_seqlens_q, int(max_seqlen_q))
+        picked = torch.empty((n, hk, int(num_selected)), dtype=torch.int32, device=q.device)
+        o.select_blocks(picked, scores, a["cache_seqlens"], page, int(keep_first),
+                        int(keep_last), cu_seqlens_q)
+        o.sparse_paged_decode(self._heads(a["out"], n), q3, k_cache, v_cache, a["block_table"],
+                              a["cache_seqlens"], picked, a["softmax_scale"], a["k_scale"],
+                              a["v_scale"], a["sinks"], cu_seqlens_q)
+        return a["out"]

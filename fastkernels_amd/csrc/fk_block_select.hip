@@ -1,0 +1,600 @@
+// Choosing which cache pages a query attends to: per-page key bounds kept beside the cache,
+// each page's score for a query, and the pages with the best scores.
+//
+// Bounds.  For a page with keys k_0 .. k_{n-1} of one kv head, lo_d = min_i k_i[d] and
+// hi_d = max_i k_i[d].  For any query q of the head's group and any key of the page
+//   q . k <= sum_d max(q_d lo_d, q_d hi_d) = max(q, 0) . hi + min(q, 0) . lo,
+// so the score of a page bounds every logit inside it, and takes two dot products that read
+// 2 D elements instead of the page's block_size * D.  A page's score for a kv head is the
+// largest over the query heads of its group, which share the pages they attend to (and so
+// each K / V byte, as in decode).
+//
+// Bounds are elements of the cache's type: the least and greatest of values are values, so
+// nothing is rounded.  A NaN key makes the page's bounds NaN, and its score NaN; NaN is taken
+// as the highest score, so that such a page is attended to and shows.
+#include <limits.h>
+
+#include "fk_attn_tile.h"
+#include "fk_query_rows.h"
+
+namespace fk {
+namespace {
+
+// NaN-propagating minimum and maximum.
+__device__ __forceinline__ float min_nan(float a, float b) {
+  return __builtin_elementwise_minimum(a, b);
+}
+__device__ __forceinline__ float max_nan(float a, float b) {
+  return __builtin_elementwise_maximum(a, b);
+}
+
+// ---------------------------------------------------------------------------
+// update_key_bounds
+// ---------------------------------------------------------------------------
+struct BoundsParams {
+  uint8_t* bounds;
+  const uint8_t* k_cache;
+  int64_t bt_row_stride;
+  int bt_width;
+  int num_kv_heads;
+  int block_size_log2;
+  int64_t num_blocks;
+};
+
+// The elements of one 32-bit word (2 bf16 or 4 fp8) as floats, and back (exactly: the
+// values are the type's own).
+template <bool kFp8>
+struct Elems {
+  static constexpr int N = kFp8 ? 4 : 2;
+  __device__ __forceinline__ static void unpack(uint32_t w, float (&f)[N]) {
+    if constexpr (kFp8) {
+      const auto a = __builtin_amdgcn_cvt_pk_f32_fp8(w, false);
+      const auto b = __builtin_amdgcn_cvt_pk_f32_fp8(w, true);
+      f[0] = a[0];
+      f[1] = a[1];
+      f[2] = b[0];
+      f[3] = b[1];
+    } else {
+      f[0] = __uint_as_float(w << 16);
+      f[1] = __uint_as_float(w & 0xffff0000u);
+    }
+  }
+  __device__ __forceinline__ static uint32_t pack(const float (&f)[N]) {
+    if constexpr (kFp8) {
+      uint32_t w = 0;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) w |= static_cast<uint32_t>(f32_to_e4m3fn_sat(f[i])) << (8 * i);
+      return w;
+    } else {
+      return lo_pair(f32_to_bf16(f[0]), f32_to_bf16(f[1]));
+    }
+  }
+};
+
+// One wave per (page, kv head): a row of D elements takes kCl lanes of 16 bytes, so an
+// instruction reads 64 / kCl rows.  Rows past the last valid one read that one again, which
+// changes no minimum or maximum.  The pages of sequence b are those of positions
+// [len - n, len), each recomputed over all its positions < len: what is stored depends on
+// the cache alone, not on earlier calls.
+template <bool kFp8, int D>
+__global__ __launch_bounds__(256) void key_bounds_kernel(
+    BoundsParams P, const int32_t* __restrict__ bt, const int32_t* __restrict__ ctx,
+    const int32_t* __restrict__ cu) {
+  constexpr int kElt = kFp8 ? 1 : 2;
+  constexpr int kCl = D * kElt / 16;
+  constexpr int kRows = 64 / kCl;
+  using E = Elems<kFp8>;
+  const int b = blockIdx.y;
+  const int h = blockIdx.z * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int len = ctx[b];
+  const int n = cu ? cu[b + 1] - cu[b] : 1;
+  if (h >= P.num_kv_heads || n <= 0 || len <= 0) return;
+  const int j = (max(len - n, 0) >> P.block_size_log2) + static_cast<int>(blockIdx.x);
+  const int64_t pos = static_cast<int64_t>(j) << P.block_size_log2;
+  if (pos >= len || j >= P.bt_width) return;
+  const int page = bt[b * P.bt_row_stride + j];
+  if (page < 0 || page >= P.num_blocks) return;
+  const int rows = min(len - static_cast<int>(pos), 1 << P.block_size_log2);
+  const int lane = threadIdx.x & 63;
+  const int c = lane % kCl, rr = lane / kCl;
+  const int64_t row_bytes = static_cast<int64_t>(P.num_kv_heads) * D * kElt;
+  const uint8_t* src = P.k_cache + (static_cast<int64_t>(page) << P.block_size_log2) * row_bytes +
+                       static_cast<int64_t>(h) * D * kElt + 16 * c;
+  float lo[4][E::N], hi[4][E::N];
+#pragma unroll
+  for (int w = 0; w < 4; ++w)
+#pragma unroll
+    for (int e = 0; e < E::N; ++e) {
+      lo[w][e] = -kNegInf;
+      hi[w][e] = kNegInf;
+    }
+  auto fold = [&](const uint4& a, const uint4& z) {
+    const uint32_t wa[4] = {a.x, a.y, a.z, a.w}, wz[4] = {z.x, z.y, z.z, z.w};
+#pragma unroll
+    for (int w = 0; w < 4; ++w) {
+      float fa[E::N], fz[E::N];
+      E::unpack(wa[w], fa);
+      E::unpack(wz[w], fz);
+#pragma unroll
+      for (int e = 0; e < E::N; ++e) {
+        lo[w][e] = min_nan(lo[w][e], fa[e]);
+        hi[w][e] = max_nan(hi[w][e], fz[e]);
+      }
+    }
+  };
+  for (int r0 = 0; r0 < rows; r0 += 4 * kRows) {
+    uint4 x[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) x[i] = ld16(src + min(r0 + i * kRows + rr, rows - 1) * row_bytes);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) fold(x[i], x[i]);
+  }
+  uint4 a, z;
+  auto packed = [&] {
+    a = make_uint4(E::pack(lo[0]), E::pack(lo[1]), E::pack(lo[2]), E::pack(lo[3]));
+    z = make_uint4(E::pack(hi[0]), E::pack(hi[1]), E::pack(hi[2]), E::pack(hi[3]));
+  };
+  packed();
+#pragma unroll
+  for (int off = kCl; off < 64; off <<= 1) {
+    uint4 pa, pz;
+    pa.x = __shfl_xor(a.x, off, 64);
+    pa.y = __shfl_xor(a.y, off, 64);
+    pa.z = __shfl_xor(a.z, off, 64);
+    pa.w = __shfl_xor(a.w, off, 64);
+    pz.x = __shfl_xor(z.x, off, 64);
+    pz.y = __shfl_xor(z.y, off, 64);
+    pz.z = __shfl_xor(z.z, off, 64);
+    pz.w = __shfl_xor(z.w, off, 64);
+    fold(pa, pz);
+    packed();
+  }
+  if (rr == 0) {
+    uint8_t* dst = P.bounds +
+                   (static_cast<int64_t>(page) * P.num_kv_heads + h) * 2 * D * kElt + 16 * c;
+    *reinterpret_cast<uint4*>(dst) = a;
+    *reinterpret_cast<uint4*>(dst + D * kElt) = z;
+  }
+}
+
+// ---------------------------------------------------------------------------
+// block_scores
+// ---------------------------------------------------------------------------
+struct ScoreParams {
+  float* scores;
+  int64_t row_stride;   // floats between the query rows of scores
+  int64_t head_stride;  // and between its kv heads
+  int width;            // blocks per (row, head)
+  const uint16_t* q;
+  int64_t q_row_stride;
+  const uint8_t* bounds;
+  const float* k_scale;
+  int64_t bt_row_stride;
+  int bt_width;
+  int64_t rows;      // rows of q and scores
+  int token_chunks;  // groups of 16 / slots query rows per sequence
+  int num_kv_heads;
+  int gqa;
+  int slots_log2;    // column slots per query row: gqa rounded up to a power of two, at most 16
+  int block_size_log2;
+  int64_t num_blocks;
+  int tiles;         // 16-page tiles per wave
+};
+
+// One wave: 16 pages x 16 columns per MFMA tile.  The columns are 16 / slots query rows of
+// one sequence times the query heads of kv head h (a group that is no power of two repeats
+// its last head, groups above 16 take several passes over the loaded bounds); the rows of
+// the A operand are the pages' bounds, lo then hi, the B operands min(q, 0) and max(q, 0).
+template <bool kFp8, int D>
+__global__ __launch_bounds__(256) void block_scores_kernel(
+    ScoreParams P, const int32_t* __restrict__ bt, const int32_t* __restrict__ ctx,
+    const int32_t* __restrict__ cu) {
+  constexpr int kElt = kFp8 ? 1 : 2;
+  constexpr int kKc = D / 32;
+  constexpr int kLoads = kFp8 ? D / 64 : D / 32;
+  const int lane = threadIdx.x & 63;
+  const int r = lane & 15, g = lane >> 4;
+  const int h = blockIdx.z * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int b = blockIdx.y / P.token_chunks;
+  const int chunk = blockIdx.y - b * P.token_chunks;
+  if (h >= P.num_kv_heads) return;
+  const int len = ctx[b];
+  const int t0 = cu ? cu[b] : b;
+  const int n = cu ? cu[b + 1] - t0 : 1;
+  const int slots = 1 << P.slots_log2;
+  const int first = chunk * (16 >> P.slots_log2);  // this tile's first row of the sequence
+  if (first >= n || t0 < 0 || t0 + first >= P.rows) return;
+  const int i = first + (r >> P.slots_log2);       // column r's row of the sequence
+  const bool row_ok = i < n && t0 + i < P.rows;
+  const int nblk = min(pages_of(min(len - n + i + 1, len), P.block_size_log2), P.width);
+  const int most = min(min(pages_of(len, P.block_size_log2), P.bt_width), P.width);
+  const float ks = kFp8 && P.k_scale ? P.k_scale[h] : 1.f;
+  const int col_blocks = (P.gqa + 15) >> 4;
+  const uint16_t* qrow = P.q + static_cast<int64_t>(t0 + (row_ok ? i : first)) * P.q_row_stride;
+  bf16x8_t qn[kKc], qp[kKc];  // min(q, 0) and max(q, 0) of column r (of -q for a scale below 0)
+  auto load_q = [&](int cb) {
+    const int head = h * P.gqa + min(16 * cb + (r & (slots - 1)), P.gqa - 1);
+    const uint16_t* p = qrow + static_cast<int64_t>(head) * D;
+#pragma unroll
+    for (int c = 0; c < kKc; ++c) {
+      const int d0 = kFp8 ? (D / 4) * g + 8 * c : 32 * c + 8 * g;
+      const uint4 v = *reinterpret_cast<const uint4*>(p + d0);
+      const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+      uint32_t a[4], z[4];
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const uint32_t x = w[k] ^ (ks < 0.f ? 0x80008000u : 0u);
+        // by sign (a NaN goes to one side, which is enough to reach the sum)
+        const uint32_t neg = ((x >> 15) & 0x00010001u) * 0xffffu;
+        a[k] = x & neg;
+        z[k] = x & ~neg;
+      }
+      qn[c] = __builtin_bit_cast(bf16x8_t, make_uint4(a[0], a[1], a[2], a[3]));
+      qp[c] = __builtin_bit_cast(bf16x8_t, make_uint4(z[0], z[1], z[2], z[3]));
+    }
+  };
+  load_q(0);
+  const int32_t* bt_row = bt + b * P.bt_row_stride;
+  float* srow = P.scores + static_cast<int64_t>(t0 + i) * P.row_stride + h * P.head_stride;
+  const int tile_end = (P.width + 15) / 16;
+  const int tile0 = blockIdx.x * P.tiles;
+  for (int tile = tile0; tile < min(tile0 + P.tiles, tile_end); ++tile) {
+    const int j0 = 16 * tile;
+    float s[4] = {kNegInf, kNegInf, kNegInf, kNegInf};
+    if (j0 < most) {
+      const int entry = j0 + r < most ? bt_row[j0 + r] : -1;
+      const bool page_ok = entry >= 0 && entry < P.num_blocks;
+      const uint32_t ok = static_cast<uint32_t>(__ballot(page_ok)) & 0xffffu;
+      const uint8_t* row = P.bounds +
+                           (static_cast<int64_t>(page_ok ? entry : 0) * P.num_kv_heads + h) * 2 *
+                               D * kElt;
+      uint4 lo[kLoads], hi[kLoads];
+#pragma unroll
+      for (int c = 0; c < kLoads; ++c) {
+        const int at = kFp8 ? (D / 4) * g + 16 * c : (32 * c + 8 * g) * 2;
+        lo[c] = ld16(row + at);
+        hi[c] = ld16(row + D * kElt + at);
+      }
+      for (int cb = 0; cb < col_blocks; ++cb) {
+        if (cb > 0 || (col_blocks > 1 && tile > tile0)) load_q(cb);
+        uint4 kl[kKc], kh[kKc];
+        if constexpr (kFp8) {
+          DTile<true, D> a, z;
+#pragma unroll
+          for (int c = 0; c < kLoads; ++c) {
+            a.k[c] = lo[c];
+            z.k[c] = hi[c];
+          }
+          k_chunks_d(a, kl);
+          k_chunks_d(z, kh);
+        } else {
+#pragma unroll
+          for (int c = 0; c < kKc; ++c) {
+            kl[c] = lo[c];
+            kh[c] = hi[c];
+          }
+        }
+        const floatx4_t x = qk_scores_n(kl, qn), y = qk_scores_n(kh, qp);
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          float v = x[k] + y[k];
+          for (int off = 1; off < slots; off <<= 1) v = max_nan(v, __shfl_xor(v, off, 64));
+          s[k] = cb == 0 ? v : max_nan(s[k], v);
+        }
+      }
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const int page = 4 * g + k;
+        s[k] = (ok >> page & 1) && j0 + page < nblk ? s[k] * __builtin_fabsf(ks) : kNegInf;
+      }
+    }
+    if (row_ok && (r & (slots - 1)) == 0) {
+#pragma unroll
+      for (int k = 0; k < 4; ++k)
+        if (j0 + 4 * g + k < P.width) srow[j0 + 4 * g + k] = s[k];
+    }
+  }
+}
+
+// ---------------------------------------------------------------------------
+// select_blocks
+// ---------------------------------------------------------------------------
+struct SelectParams {
+  int32_t* indices;
+  int64_t out_row_stride, out_head_stride;
+  const float* scores;
+  int64_t row_stride, head_stride;
+  int width;
+  int keep, keep_first, keep_last;
+  int block_size_log2;
+  int batch;
+};
+
+constexpr int kSelThreads = 256;
+
+// Scores in ascending order of an unsigned key: NaN above all, -0 equal to +0.
+__device__ __forceinline__ uint32_t score_key(float s) {
+  if (s != s) return 0xffffffffu;
+  const uint32_t u = __float_as_uint(s + 0.f);
+  return u ^ ((u >> 31) ? 0xffffffffu : 0x80000000u);
+}
+
+// One work-group per (query row, kv head).  The key T of the lowest selected candidate is
+// found digit by digit (8 bits a pass: a histogram of the keys that agree with the digits
+// found so far, then the bin that holds the rank), and the blocks are written in order of
+// their index: the ones always kept, keys above T, and the first of the keys equal to T.
+__global__ __launch_bounds__(kSelThreads) void select_blocks_kernel(
+    SelectParams P, const int32_t* __restrict__ ctx, const int32_t* __restrict__ cu) {
+  __shared__ int hist[256];
+  __shared__ int wave_n[2][kSelThreads / 64];
+  __shared__ int found[2];
+  const int t = blockIdx.x, h = blockIdx.y;
+  int b, vis;
+  if (!query_row(cu, ctx, P.batch, t, b, vis)) return;
+  const int n = min(pages_of(vis, P.block_size_log2), P.width);
+  int32_t* out = P.indices + t * P.out_row_stride + h * P.out_head_stride;
+  const float* row = P.scores + t * P.row_stride + h * P.head_stride;
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  if (n <= P.keep) {
+    for (int k = tid; k < P.keep; k += kSelThreads) out[k] = k < n ? k : -1;
+    return;
+  }
+  const int first = P.keep_first, last = n - P.keep_last;  // candidates [first, last)
+  int need = P.keep - P.keep_first - P.keep_last;
+  uint32_t digits = 0, known = 0;
+  if (need > 0) {
+    for (int shift = 24; shift >= 0; shift -= 8) {
+      hist[tid] = 0;
+      __syncthreads();
+      for (int j = first + tid; j < last; j += kSelThreads) {
+        const uint32_t key = score_key(row[j]);
+        if ((key & known) == digits) atomicAdd(&hist[(key >> shift) & 255], 1);
+      }
+      __syncthreads();
+      // keys in bins above bin tid: the bin where that count passes `need` holds the rank
+      int above = 0;
+      for (int k = tid + 1; k < 256; ++k) above += hist[k];
+      if (above < need && above + hist[tid] >= need) {
+        found[0] = tid;
+        found[1] = need - above;
+      }
+      __syncthreads();
+      digits |= static_cast<uint32_t>(found[0]) << shift;
+      known |= 255u << shift;
+      need = found[1];
+      __syncthreads();
+    }
+  }
+  // need: how many of the keys equal to `digits` are selected.
+  int written = 0, equal = 0;
+  for (int j0 = 0; j0 < n; j0 += kSelThreads) {
+    const int j = j0 + tid;
+    const bool cand = j >= first && j < last;
+    const uint32_t key = cand ? score_key(row[j]) : 0;
+    const bool eq = cand && need > 0 && key == digits;
+    const uint64_t below = (uint64_t{1} << lane) - 1;
+    const uint64_t eqs = __ballot(eq);
+    if (lane == 0) wave_n[0][wave] = __builtin_popcountll(eqs);
+    __syncthreads();
+    int rank = equal + __builtin_popcountll(eqs & below);
+    for (int w = 0; w < kSelThreads / 64; ++w) {
+      rank += w < wave ? wave_n[0][w] : 0;
+      equal += wave_n[0][w];
+    }
+    const bool take = (j < n && !cand) || (eq && rank < need) ||
+                      (cand && P.keep > P.keep_first + P.keep_last && key > digits);
+    const uint64_t takes = __ballot(take);
+    if (lane == 0) wave_n[1][wave] = __builtin_popcountll(takes);
+    __syncthreads();
+    int at = written + __builtin_popcountll(takes & below);
+    for (int w = 0; w < kSelThreads / 64; ++w) {
+      at += w < wave ? wave_n[1][w] : 0;
+      written += wave_n[1][w];
+    }
+    if (take && at < P.keep) out[at] = j;
+    __syncthreads();
+  }
+}
+
+// ---------------------------------------------------------------------------
+// Launch
+// ---------------------------------------------------------------------------
+// Work-groups of 256 along a grid's x: their threads number less than 2^32.
+constexpr int64_t kMaxGridX = (int64_t{1} << 24) - 1;
+
+bool head_built(int d) { return d == 64 || d == 128 || d == 256; }
+
+int log2_of(int v) { return 31 - __builtin_clz(static_cast<unsigned>(v)); }
+
+// The checks of the paged arguments the entry points here share.
+int check_paged(const char* what, int kv_dtype, int64_t bt_row_stride, int64_t bt_width,
+                int64_t batch, int num_kv_heads, int head_size, int block_size,
+                int64_t num_blocks) {
+  FK_REQUIRE(batch >= 0 && batch <= 65535, "%s: batch %lld outside [0, 65535]", what,
+             static_cast<long long>(batch));
+  FK_REQUIRE(num_kv_heads > 0 && num_kv_heads <= 4 * 65535, "%s: %d kv heads", what,
+             num_kv_heads);
+  FK_REQUIRE(kv_dtype == FK_DTYPE_BF16 || kv_dtype == FK_DTYPE_FP8_E4M3FN,
+             "%s: the cache must be bf16 or fp8 e4m3fn", what);
+  FK_REQUIRE(block_size >= 16 && (block_size & (block_size - 1)) == 0,
+             "%s: block_size %d must be a power of two >= 16", what, block_size);
+  FK_REQUIRE(num_blocks > 0 && num_blocks <= INT_MAX, "%s: num_blocks %lld", what,
+             static_cast<long long>(num_blocks));
+  FK_REQUIRE(bt_width >= 0 && bt_width <= kMaxGridX && bt_row_stride >= 0,
+             "%s: block table of %lld columns", what, static_cast<long long>(bt_width));
+  if (!head_built(head_size))
+    return set_error(FK_ERR_UNSUPPORTED, "%s: head_size %d unsupported (64, 128 or 256)", what,
+                     head_size);
+  return FK_OK;
+}
+
+template <bool kFp8>
+void launch_bounds(const BoundsParams& P, int d, dim3 grid, hipStream_t s, const int32_t* bt,
+                   const int32_t* ctx, const int32_t* cu) {
+  if (d == 64)
+    hipLaunchKernelGGL((key_bounds_kernel<kFp8, 64>), grid, dim3(256), 0, s, P, bt, ctx, cu);
+  else if (d == 128)
+    hipLaunchKernelGGL((key_bounds_kernel<kFp8, 128>), grid, dim3(256), 0, s, P, bt, ctx, cu);
+  else
+    hipLaunchKernelGGL((key_bounds_kernel<kFp8, 256>), grid, dim3(256), 0, s, P, bt, ctx, cu);
+}
+
+template <bool kFp8>
+void launch_scores(const ScoreParams& P, int d, dim3 grid, hipStream_t s, const int32_t* bt,
+                   const int32_t* ctx, const int32_t* cu) {
+  if (d == 64)
+    hipLaunchKernelGGL((block_scores_kernel<kFp8, 64>), grid, dim3(256), 0, s, P, bt, ctx, cu);
+  else if (d == 128)
+    hipLaunchKernelGGL((block_scores_kernel<kFp8, 128>), grid, dim3(256), 0, s, P, bt, ctx, cu);
+  else
+    hipLaunchKernelGGL((block_scores_kernel<kFp8, 256>), grid, dim3(256), 0, s, P, bt, ctx, cu);
+}
+
+}  // namespace
+}  // namespace fk
+
+using namespace fk;
+
+extern "C" int fk_update_key_bounds(void* key_bounds, const void* k_cache, int kv_dtype,
+                                    const int32_t* block_tables, int64_t bt_row_stride,
+                                    int64_t bt_width, const int32_t* cache_seqlens,
+                                    const int32_t* cu_seqlens_q, int64_t batch,
+                                    int64_t max_seqlen_q, int num_kv_heads, int head_size,
+                                    int block_size, int64_t num_blocks, void* stream) {
+  const char* what = "fk_update_key_bounds";
+  if (int rc = check_paged(what, kv_dtype, bt_row_stride, bt_width, batch, num_kv_heads,
+                           head_size, block_size, num_blocks))
+    return rc;
+  FK_REQUIRE(max_seqlen_q >= 0 && max_seqlen_q <= INT_MAX, "%s: max_seqlen_q %lld", what,
+             static_cast<long long>(max_seqlen_q));
+  FK_REQUIRE(cu_seqlens_q || max_seqlen_q == 1,
+             "%s: without cu_seqlens_q each sequence has one new token", what);
+  if (batch == 0 || max_seqlen_q == 0 || bt_width == 0) return FK_OK;
+  FK_REQUIRE(key_bounds && k_cache && block_tables && cache_seqlens, "%s: null pointer", what);
+  FK_REQUIRE(aligned16(key_bounds) && aligned16(k_cache),
+             "%s: key_bounds and k_cache must be 16-byte aligned", what);
+  BoundsParams P;
+  P.bounds = static_cast<uint8_t*>(key_bounds);
+  P.k_cache = static_cast<const uint8_t*>(k_cache);
+  P.bt_row_stride = bt_row_stride;
+  P.bt_width = static_cast<int>(bt_width);
+  P.num_kv_heads = num_kv_heads;
+  P.block_size_log2 = log2_of(block_size);
+  P.num_blocks = num_blocks;
+  // Pages that n consecutive positions can touch.
+  int64_t pages = (max_seqlen_q + block_size - 2) / block_size + 1;
+  if (pages > bt_width) pages = bt_width;
+  const dim3 grid(static_cast<unsigned>(pages), static_cast<unsigned>(batch),
+                  static_cast<unsigned>((num_kv_heads + 3) / 4));
+  if (kv_dtype == FK_DTYPE_FP8_E4M3FN)
+    launch_bounds<true>(P, head_size, grid, as_stream(stream), block_tables, cache_seqlens,
+                        cu_seqlens_q);
+  else
+    launch_bounds<false>(P, head_size, grid, as_stream(stream), block_tables, cache_seqlens,
+                         cu_seqlens_q);
+  return check_launch(what);
+}
+
+extern "C" int fk_block_scores(float* scores, int64_t score_row_stride, int64_t score_head_stride,
+                               int64_t width, const void* q, int64_t q_row_stride,
+                               const void* key_bounds, int kv_dtype, const float* k_scale,
+                               const int32_t* block_tables, int64_t bt_row_stride,
+                               int64_t bt_width, const int32_t* cache_seqlens,
+                               const int32_t* cu_seqlens_q, int64_t batch, int64_t rows,
+                               int64_t max_seqlen_q, int num_heads, int num_kv_heads, int head_size,
+                               int block_size, int64_t num_blocks, void* stream) {
+  const char* what = "fk_block_scores";
+  if (int rc = check_paged(what, kv_dtype, bt_row_stride, bt_width, batch, num_kv_heads,
+                           head_size, block_size, num_blocks))
+    return rc;
+  FK_REQUIRE(num_heads > 0 && num_heads % num_kv_heads == 0,
+             "%s: %d query heads over %d kv heads", what, num_heads, num_kv_heads);
+  FK_REQUIRE(max_seqlen_q >= 0 && max_seqlen_q <= INT_MAX, "%s: max_seqlen_q %lld", what,
+             static_cast<long long>(max_seqlen_q));
+  FK_REQUIRE(cu_seqlens_q || max_seqlen_q == 1,
+             "%s: without cu_seqlens_q each sequence has one query row", what);
+  FK_REQUIRE(width >= 0 && width <= kMaxGridX, "%s: %lld blocks per row", what,
+             static_cast<long long>(width));
+  FK_REQUIRE(rows >= 0 && rows <= INT_MAX && (cu_seqlens_q || rows >= batch),
+             "%s: %lld query rows for %lld sequences", what, static_cast<long long>(rows),
+             static_cast<long long>(batch));
+  if (batch == 0 || rows == 0 || max_seqlen_q == 0 || width == 0) return FK_OK;
+  FK_REQUIRE(scores && q && key_bounds && block_tables && cache_seqlens, "%s: null pointer", what);
+  FK_REQUIRE(aligned16(q) && aligned16(key_bounds) && q_row_stride % 8 == 0,
+             "%s: q rows and key_bounds must be 16-byte aligned", what);
+  ScoreParams P;
+  P.scores = scores;
+  P.row_stride = score_row_stride;
+  P.head_stride = score_head_stride;
+  P.width = static_cast<int>(width);
+  P.q = static_cast<const uint16_t*>(q);
+  P.q_row_stride = q_row_stride;
+  P.bounds = static_cast<const uint8_t*>(key_bounds);
+  P.k_scale = k_scale;
+  P.bt_row_stride = bt_row_stride;
+  P.bt_width = static_cast<int>(bt_width);
+  P.rows = rows;
+  P.num_kv_heads = num_kv_heads;
+  P.gqa = num_heads / num_kv_heads;
+  P.slots_log2 = P.gqa >= 16 ? 4 : P.gqa == 1 ? 0 : log2_of(P.gqa - 1) + 1;
+  P.block_size_log2 = log2_of(block_size);
+  P.num_blocks = num_blocks;
+  const int64_t tile_rows = 16 >> P.slots_log2;
+  const int64_t chunks = (max_seqlen_q + tile_rows - 1) / tile_rows;
+  FK_REQUIRE(chunks * batch <= 65535, "%s: %lld groups of query rows are more than 65535", what,
+             static_cast<long long>(chunks * batch));
+  P.token_chunks = static_cast<int>(chunks);
+  P.tiles = 1;
+  const dim3 grid(static_cast<unsigned>((P.width + 16 * P.tiles - 1) / (16 * P.tiles)),
+                  static_cast<unsigned>(chunks * batch),
+                  static_cast<unsigned>((num_kv_heads + 3) / 4));
+  if (kv_dtype == FK_DTYPE_FP8_E4M3FN)
+    launch_scores<true>(P, head_size, grid, as_stream(stream), block_tables, cache_seqlens,
+                        cu_seqlens_q);
+  else
+    launch_scores<false>(P, head_size, grid, as_stream(stream), block_tables, cache_seqlens,
+                         cu_seqlens_q);
+  return check_launch(what);
+}
+
+extern "C" int fk_select_blocks(int32_t* block_indices, int64_t out_row_stride,
+                                int64_t out_head_stride, int64_t keep, const float* scores,
+                                int64_t score_row_stride, int64_t score_head_stride,
+                                int64_t width, const int32_t* cache_seqlens,
+                                const int32_t* cu_seqlens_q, int64_t batch, int64_t rows,
+                                int num_kv_heads, int block_size, int keep_first, int keep_last,
+                                void* stream) {
+  const char* what = "fk_select_blocks";
+  FK_REQUIRE(batch >= 0 && batch <= INT_MAX && rows >= 0 && rows <= kMaxGridX,
+             "%s: %lld rows of %lld sequences", what, static_cast<long long>(rows),
+             static_cast<long long>(batch));
+  FK_REQUIRE(num_kv_heads > 0 && num_kv_heads <= 65535, "%s: %d kv heads", what, num_kv_heads);
+  FK_REQUIRE(block_size >= 1 && (block_size & (block_size - 1)) == 0,
+             "%s: block_size %d must be a power of two", what, block_size);
+  FK_REQUIRE(width >= 0 && width <= INT_MAX - kSelThreads && keep >= 0 && keep <= INT_MAX,
+             "%s: %lld of %lld blocks", what, static_cast<long long>(keep),
+             static_cast<long long>(width));
+  FK_REQUIRE(keep_first >= 0 && keep_last >= 0 &&
+                 static_cast<int64_t>(keep_first) + keep_last <= keep,
+             "%s: keep_first %d and keep_last %d must fit in the %lld selected blocks", what,
+             keep_first, keep_last, static_cast<long long>(keep));
+  if (batch == 0 || rows == 0 || keep == 0) return FK_OK;
+  FK_REQUIRE(block_indices && (scores || width == 0) && cache_seqlens, "%s: null pointer", what);
+  SelectParams P;
+  P.indices = block_indices;
+  P.out_row_stride = out_row_stride;
+  P.out_head_stride = out_head_stride;
+  P.scores = scores;
+  P.row_stride = score_row_stride;
+  P.head_stride = score_head_stride;
+  P.width = static_cast<int>(width);
+  P.keep = static_cast<int>(keep);
+  P.keep_first = keep_first;
+  P.keep_last = keep_last;
+  P.block_size_log2 = log2_of(block_size);
+  P.batch = static_cast<int>(batch);
+  const dim3 grid(static_cast<unsigned>(rows), static_cast<unsigned>(num_kv_heads));
+  hipLaunchKernelGGL(select_blocks_kernel, grid, dim3(kSelThreads), 0, as_stream(stream), P,
+                     cache_seqlens, cu_seqlens_q);
+  return check_launch(what);
+}

@@ -697,6 +697,270 @@ def merge_attn_states(output: torch.Tensor, prefix_output: torch.Tensor, prefix_
 
 
 # ---------------------------------------------------------------------------
+# Attention that reads part of a paged cache: selected pages, shared prefixes
+# ---------------------------------------------------------------------------
+def _call_on(t: torch.Tensor, fn: str, *args) -> None:
+    """_native.call with t's device current and its current stream as the last argument."""
+    stream = _stream(t)
+    if t.get_device() == torch.cuda.current_device():
+        _native.call(fn, *args, stream)
+    else:
+        with torch.cuda.device(t.device):
+            _native.call(fn, *args, stream)
+
+
+def _check_table(what: str, block_table: torch.Tensor, cache_seqlens: torch.Tensor,
+                 cu_seqlens_q: torch.Tensor | None, rows: int | None) -> int:
+    """Checks the sequences' metadata; returns their number."""
+    if cu_seqlens_q is None:
+        batch = cache_seqlens.numel() if rows is None else rows
+    else:
+        if cu_seqlens_q.dtype != torch.int32 or cu_seqlens_q.dim() != 1 or \
+                not cu_seqlens_q.is_contiguous() or cu_seqlens_q.numel() < 1:
+            raise TypeError(f"{what}: cu_seqlens_q must be contiguous int32 [batch + 1]")
+        batch = cu_seqlens_q.numel() - 1
+    if cache_seqlens.dtype != torch.int32 or not cache_seqlens.is_contiguous() or \
+            cache_seqlens.numel() < batch:
+        raise TypeError(f"{what}: cache_seqlens must be contiguous int32 [batch]")
+    if block_table is not None:
+        if block_table.dtype != torch.int32 or block_table.dim() != 2 or \
+                (block_table.shape[1] > 1 and block_table.stride(1) != 1):
+            raise TypeError(f"{what}: block_table must be int32 [batch, max_blocks], rows "
+                            "contiguous")
+        if block_table.shape[0] < batch:
+            raise ValueError(f"{what}: block_table has fewer rows than the batch")
+    return batch
+
+
+def _check_rows(what: str, t: torch.Tensor, name: str) -> None:
+    if t.dim() != 3 or t.dtype != torch.bfloat16 or t.stride()[1:] != (t.shape[2], 1):
+        raise ValueError(f"{what}: {name} must be bf16 [rows, Hq, D] with contiguous heads")
+
+
+def _cache_tag(what: str, dtype: torch.dtype) -> int:
+    if dtype == torch.bfloat16:
+        return _native.FK_DTYPE_BF16
+    if dtype != _FP8:
+        raise TypeError(f"{what}: caches and key_bounds must be bf16 or float8_e4m3fn")
+    return _native.FK_DTYPE_FP8_E4M3FN
+
+
+def _check_scale(what: str, scale: torch.Tensor | None, name: str, heads: int) -> None:
+    if scale is not None and (scale.dtype != torch.float32 or scale.numel() != heads or
+                              not scale.is_contiguous()):
+        raise ValueError(f"{what}: {name} must be contiguous float32 [{heads}]")
+
+
+def new_key_bounds(k_cache: torch.Tensor) -> torch.Tensor:
+    """Room for the key bounds of a cache [num_blocks, block_size, Hk, D]: zeros
+    [num_blocks, Hk, 2, D] of its dtype, to be filled by :func:`update_key_bounds`."""
+    nb, _, hk, d = k_cache.shape
+    return torch.zeros(nb, hk, 2, d, dtype=k_cache.dtype, device=k_cache.device)
+
+
+def _check_bounds(what: str, key_bounds: torch.Tensor, head_size: int) -> None:
+    if key_bounds.dim() != 4 or key_bounds.shape[2] != 2 or key_bounds.shape[3] != head_size or \
+            not key_bounds.is_contiguous():
+        raise ValueError(f"{what}: key_bounds must be contiguous [num_blocks, Hk, 2, D]")
+
+
+def update_key_bounds(key_bounds: torch.Tensor, k_cache: torch.Tensor, block_table: torch.Tensor,
+                      cache_seqlens: torch.Tensor, cu_seqlens_q: torch.Tensor | None = None,
+                      max_seqlen_q: int = 1) -> None:
+    """Brings the bounds of the pages that hold each sequence's newest tokens up to date:
+    key_bounds[page, h, 0] / [page, h, 1] = the least / greatest value of each key dimension
+    over the page's tokens below cache_seqlens[b] (NaN if one is NaN).
+
+    Call it after the tokens are stored, with cache_seqlens counting them.  The newest tokens
+    are the last cu_seqlens_q[b + 1] - cu_seqlens_q[b] of sequence b (the last one without
+    cu_seqlens_q), at most max_seqlen_q.  Pages are read whole, so the result depends on the
+    cache alone: a rejected draft token is forgotten with the next call on its page."""
+    what = "update_key_bounds"
+    if k_cache.dim() != 4 or not k_cache.is_contiguous():
+        raise ValueError(f"{what}: k_cache must be contiguous [num_blocks, block_size, Hk, D]")
+    nb, bs, hk, d = k_cache.shape
+    _check_bounds(what, key_bounds, d)
+    if key_bounds.shape[:2] != (nb, hk) or key_bounds.dtype != k_cache.dtype:
+        raise ValueError(f"{what}: key_bounds must be [{nb}, {hk}, 2, {d}] of the cache's dtype")
+    tag = _cache_tag(what, k_cache.dtype)
+    batch = _check_table(what, block_table, cache_seqlens, cu_seqlens_q, None)
+    _same_device(key_bounds, k_cache, block_table, cache_seqlens, cu_seqlens_q)
+    if batch == 0:
+        return
+    _call_on(key_bounds, "fk_update_key_bounds", key_bounds.data_ptr(), k_cache.data_ptr(), tag,
+             block_table.data_ptr(), block_table.stride(0), block_table.shape[1],
+             cache_seqlens.data_ptr(), _ptr(cu_seqlens_q), batch, int(max_seqlen_q), hk, d, bs,
+             nb)
+
+
+def block_scores(scores: torch.Tensor, q: torch.Tensor, key_bounds: torch.Tensor,
+                 block_table: torch.Tensor, cache_seqlens: torch.Tensor, block_size: int,
+                 k_scale: torch.Tensor | None = None, cu_seqlens_q: torch.Tensor | None = None,
+                 max_seqlen_q: int = 1) -> None:
+    """scores[t, h, j] (float32 [rows, Hk, blocks]): an upper bound of q . k over block j of
+    row t's sequence, the greatest over the query heads of kv head h of
+    sum_d max(q_d lo_d, q_d hi_d) with the block's key_bounds (times k_scale[h] for fp8).
+    -inf for blocks the row does not see and for pages without a table entry.
+
+    Rows: one per sequence, or cu_seqlens_q [batch + 1] with at most max_seqlen_q per
+    sequence, its last tokens (row i of n sees cache_seqlens[b] - n + i + 1 keys)."""
+    what = "block_scores"
+    _check_rows(what, q, "q")
+    rows, hq, d = q.shape
+    _check_bounds(what, key_bounds, d)
+    nb, hk = key_bounds.shape[:2]
+    tag = _cache_tag(what, key_bounds.dtype)
+    if hk == 0 or hq % hk:
+        raise ValueError(f"{what}: {hq} query heads over {hk} kv heads")
+    if scores.dim() != 3 or scores.shape[:2] != (rows, hk) or scores.dtype != torch.float32 or \
+            (scores.shape[2] > 1 and scores.stride(2) != 1):
+        raise ValueError(f"{what}: scores must be float32 [rows, Hk, blocks] with contiguous "
+                         "blocks")
+    _check_scale(what, k_scale, "k_scale", hk)
+    batch = _check_table(what, block_table, cache_seqlens, cu_seqlens_q, rows)
+    _same_device(scores, q, key_bounds, block_table, cache_seqlens, cu_seqlens_q, k_scale)
+    if rows == 0 or batch == 0 or scores.shape[2] == 0:
+        return
+    _call_on(scores, "fk_block_scores", scores.data_ptr(), scores.stride(0), scores.stride(1),
+             scores.shape[2], q.data_ptr(), q.stride(0), key_bounds.data_ptr(), tag,
+             _ptr(k_scale), block_table.data_ptr(), block_table.stride(0), block_table.shape[1],
+             cache_seqlens.data_ptr(), _ptr(cu_seqlens_q), batch, rows, int(max_seqlen_q), hq, hk,
+             d, int(block_size), nb)
+
+
+def select_blocks(block_indices: torch.Tensor, scores: torch.Tensor, cache_seqlens: torch.Tensor,
+                  block_size: int, keep_first: int = 0, keep_last: int = 1,
+                  cu_seqlens_q: torch.Tensor | None = None) -> None:
+    """block_indices (int32 [rows, Hk, keep]): the blocks each row attends to per kv head, in
+    ascending order, -1 behind the last.  Of the blocks a row sees (scores' last dimension
+    bounds them), the first keep_first, the last keep_last and the ones with the highest
+    scores; of equal scores the lower index first, NaN above every number.  All of them where
+    they are at most keep."""
+    what = "select_blocks"
+    if scores.dim() != 3 or scores.dtype != torch.float32 or \
+            (scores.shape[2] > 1 and scores.stride(2) != 1):
+        raise ValueError(f"{what}: scores must be float32 [rows, Hk, blocks] with contiguous "
+                         "blocks")
+    rows, hk, width = scores.shape
+    if block_indices.dim() != 3 or block_indices.shape[:2] != (rows, hk) or \
+            block_indices.dtype != torch.int32 or \
+            (block_indices.shape[2] > 1 and block_indices.stride(2) != 1):
+        raise ValueError(f"{what}: block_indices must be int32 [rows, Hk, keep] with contiguous "
+                         "entries")
+    keep = block_indices.shape[2]
+    if keep_first < 0 or keep_last < 0 or keep_first + keep_last > keep:
+        raise ValueError(f"{what}: keep_first {keep_first} and keep_last {keep_last} must fit in "
+                         f"the {keep} selected blocks")
+    batch = _check_table(what, None, cache_seqlens, cu_seqlens_q, rows)
+    _same_device(block_indices, scores, cache_seqlens, cu_seqlens_q)
+    if rows == 0 or batch == 0 or keep == 0:
+        return
+    _call_on(scores, "fk_select_blocks", block_indices.data_ptr(), block_indices.stride(0),
+             block_indices.stride(1), keep, scores.data_ptr(), scores.stride(0),
+             scores.stride(1), width, cache_seqlens.data_ptr(), _ptr(cu_seqlens_q), batch, rows,
+             hk, int(block_size), int(keep_first), int(keep_last))
+
+
+def _check_page_attn(what, out, q, k_cache, v_cache, k_scale, v_scale, sinks) -> int:
+    _check_rows(what, q, "q")
+    _check_rows(what, out, "out")
+    if out.shape != q.shape:
+        raise ValueError(f"{what}: out must have q's shape")
+    if k_cache.dim() != 4 or v_cache.shape != k_cache.shape or k_cache.shape[3] != q.shape[2]:
+        raise ValueError(f"{what}: caches must be [num_blocks, block_size, Hk, D]")
+    if not (k_cache.is_contiguous() and v_cache.is_contiguous()):
+        raise ValueError(f"{what}: caches must be contiguous")
+    if v_cache.dtype != k_cache.dtype:
+        raise TypeError(f"{what}: caches must share a dtype")
+    tag = _cache_tag(what, k_cache.dtype)
+    _check_scale(what, k_scale, "k_scale", k_cache.shape[2])
+    _check_scale(what, v_scale, "v_scale", k_cache.shape[2])
+    _check_scale(what, sinks, "sinks", q.shape[1])
+    return tag
+
+
+def sparse_paged_decode(out: torch.Tensor, q: torch.Tensor, k_cache: torch.Tensor,
+                        v_cache: torch.Tensor, block_table: torch.Tensor,
+                        cache_seqlens: torch.Tensor, block_indices: torch.Tensor,
+                        softmax_scale: float, k_scale: torch.Tensor | None = None,
+                        v_scale: torch.Tensor | None = None, sinks: torch.Tensor | None = None,
+                        cu_seqlens_q: torch.Tensor | None = None) -> None:
+    """Decode attention into ``out`` ([rows, Hq, D] bf16) over the blocks of each row's
+    sequence that block_indices (int32 [rows, Hk, keep], as :func:`select_blocks` writes it)
+    lists for the kv head; of these, the keys the row sees.  Entries that are -1 or hold no
+    visible key are skipped; a block listed twice counts twice; a row that sees no key is
+    zero.  Rows and cu_seqlens_q as in :func:`block_scores`; scales and sinks as in
+    :func:`paged_decode`."""
+    what = "sparse_paged_decode"
+    tag = _check_page_attn(what, out, q, k_cache, v_cache, k_scale, v_scale, sinks)
+    rows, hq, d = q.shape
+    nb, bs, hk, _ = k_cache.shape
+    if block_indices.dim() != 3 or block_indices.shape[:2] != (rows, hk) or \
+            block_indices.dtype != torch.int32 or \
+            (block_indices.shape[2] > 1 and block_indices.stride(2) != 1):
+        raise ValueError(f"{what}: block_indices must be int32 [rows, Hk, keep] with contiguous "
+                         "entries")
+    batch = _check_table(what, block_table, cache_seqlens, cu_seqlens_q, rows)
+    _same_device(out, q, k_cache, v_cache, block_table, cache_seqlens, block_indices, k_scale,
+                 v_scale, sinks, cu_seqlens_q)
+    if rows == 0 or batch == 0:
+        return
+    keep = block_indices.shape[2]
+    nbytes = _native.sparse_decode_bytes(rows, keep, hq, hk, d, bs)
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=q.device) if nbytes else None
+    _call_on(q, "fk_sparse_paged_decode", out.data_ptr(), out.stride(0), q.data_ptr(),
+             q.stride(0), k_cache.data_ptr(), v_cache.data_ptr(), tag, _ptr(k_scale),
+             _ptr(v_scale), block_table.data_ptr(), block_table.stride(0), block_table.shape[1],
+             cache_seqlens.data_ptr(), _ptr(cu_seqlens_q), batch, rows, block_indices.data_ptr(),
+             block_indices.stride(0), block_indices.stride(1), keep, hq, hk, d, bs, nb,
+             float(softmax_scale), _ptr(sinks), _ptr(ws), nbytes)
+
+
+def shared_prefix_decode(out: torch.Tensor, q: torch.Tensor, k_cache: torch.Tensor,
+                         v_cache: torch.Tensor, block_table: torch.Tensor,
+                         cache_seqlens: torch.Tensor, cu_groups: torch.Tensor,
+                         prefix_lens: torch.Tensor, softmax_scale: float,
+                         k_scale: torch.Tensor | None = None,
+                         v_scale: torch.Tensor | None = None, window_left: int = -1,
+                         sinks: torch.Tensor | None = None, max_prefix_len: int = 0) -> None:
+    """:func:`paged_decode` (one query row per sequence) of a batch in groups that share a
+    prefix: rows cu_groups[g] .. cu_groups[g + 1] - 1 (int32 [groups + 1], ascending) have the
+    same tokens at positions below prefix_lens[g] (int32 [groups], any length).  Those are
+    read once for the group, through the block table of its first row, the others through
+    each row's own.  Rows outside every group share nothing; a row may be shorter than its
+    group's prefix.  max_prefix_len bounds every prefix (0: unknown); it only chooses the
+    launch shape."""
+    what = "shared_prefix_decode"
+    tag = _check_page_attn(what, out, q, k_cache, v_cache, k_scale, v_scale, sinks)
+    rows, hq, d = q.shape
+    nb, bs, hk, _ = k_cache.shape
+    for t, name in ((cu_groups, "cu_groups [groups + 1]"), (prefix_lens, "prefix_lens [groups]")):
+        if t.dtype != torch.int32 or t.dim() != 1 or not t.is_contiguous():
+            raise TypeError(f"{what}: {name} must be contiguous int32")
+    groups = cu_groups.numel() - 1
+    if groups < 0 or prefix_lens.numel() < groups:
+        raise ValueError(f"{what}: prefix_lens shorter than the groups")
+    if int(window_left) < -1:
+        raise ValueError(f"{what}: window_left must be -1 (no window) or >= 0")
+    if int(max_prefix_len) < 0:
+        raise ValueError(f"{what}: max_prefix_len must be >= 0")
+    _check_table(what, block_table, cache_seqlens, None, rows)
+    _same_device(out, q, k_cache, v_cache, block_table, cache_seqlens, cu_groups, prefix_lens,
+                 k_scale, v_scale, sinks)
+    if rows == 0:
+        return
+    bound = min(int(max_prefix_len) or block_table.shape[1] * bs, block_table.shape[1] * bs)
+    nbytes = _native.shared_prefix_bytes(rows, groups, bound, hq, hk, d)
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=q.device) if nbytes else None
+    _call_on(q, "fk_shared_prefix_decode", out.data_ptr(), out.stride(0), q.data_ptr(),
+             q.stride(0), k_cache.data_ptr(), v_cache.data_ptr(), tag, _ptr(k_scale),
+             _ptr(v_scale), block_table.data_ptr(), block_table.stride(0), block_table.shape[1],
+             cache_seqlens.data_ptr(), rows, cu_groups.data_ptr(), prefix_lens.data_ptr(), groups,
+             bound, hq, hk, d, bs, nb, float(softmax_scale), int(window_left), _ptr(sinks),
+             _ptr(ws), nbytes)
+
+
+# ---------------------------------------------------------------------------
 # torch.library registration (opaque custom ops with mutation annotations).
 # ---------------------------------------------------------------------------
 _LIB = torch.library.Library("fastkernels_amd", "DEF")
@@ -734,6 +998,22 @@ _LIB.define("silu_and_mul(Tensor! result, Tensor input) -> ()")
 _LIB.define("merge_attn_states(Tensor(a!) output, Tensor prefix_output, Tensor prefix_lse, "
             "Tensor suffix_output, Tensor suffix_lse, Tensor(b!)? output_lse, "
             "int? prefill_tokens_with_context=None, Tensor? output_scale=None) -> ()")
+_LIB.define("update_key_bounds(Tensor(a!) key_bounds, Tensor k_cache, Tensor block_table, "
+            "Tensor cache_seqlens, Tensor? cu_seqlens_q=None, int max_seqlen_q=1) -> ()")
+_LIB.define("block_scores(Tensor(a!) scores, Tensor q, Tensor key_bounds, Tensor block_table, "
+            "Tensor cache_seqlens, int block_size, Tensor? k_scale=None, "
+            "Tensor? cu_seqlens_q=None, int max_seqlen_q=1) -> ()")
+_LIB.define("select_blocks(Tensor(a!) block_indices, Tensor scores, Tensor cache_seqlens, "
+            "int block_size, int keep_first=0, int keep_last=1, Tensor? cu_seqlens_q=None) "
+            "-> ()")
+_LIB.define("sparse_paged_decode(Tensor(a!) out, Tensor q, Tensor k_cache, Tensor v_cache, "
+            "Tensor block_table, Tensor cache_seqlens, Tensor block_indices, "
+            "float softmax_scale, Tensor? k_scale=None, Tensor? v_scale=None, "
+            "Tensor? sinks=None, Tensor? cu_seqlens_q=None) -> ()")
+_LIB.define("shared_prefix_decode(Tensor(a!) out, Tensor q, Tensor k_cache, Tensor v_cache, "
+            "Tensor block_table, Tensor cache_seqlens, Tensor cu_groups, Tensor prefix_lens, "
+            "float softmax_scale, Tensor? k_scale=None, Tensor? v_scale=None, "
+            "int window_left=-1, Tensor? sinks=None, int max_prefix_len=0) -> ()")
 
 _IMPLS = {
     "rmsnorm": lambda result, input, weight, eps: rms_norm(result, input, weight, eps),
@@ -748,6 +1028,11 @@ _IMPLS = {
     "qk_norm_rope_store": qk_norm_rope_store,
     "paged_prefill": paged_prefill,
     "varlen_prefill": varlen_prefill,
+    "update_key_bounds": update_key_bounds,
+    "block_scores": block_scores,
+    "select_blocks": select_blocks,
+    "sparse_paged_decode": sparse_paged_decode,
+    "shared_prefix_decode": shared_prefix_decode,
 }
 for _name, _fn in _IMPLS.items():
     _LIB.impl(_name, _fn, "CUDA")

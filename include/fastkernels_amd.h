@@ -78,8 +78,9 @@ extern "C" {
  * header checks fk_version() / 10000 == FK_VERSION_MAJOR before binding. */
 #define FK_VERSION_MAJOR 2
 /* 2.1: fk_prefill_split_plan, fk_paged_prefill_ws, fk_varlen_prefill_ws
- * 2.2: fk_paged_decode_shape, fk_prefill_shape */
-#define FK_VERSION_MINOR 2
+ * 2.2: fk_paged_decode_shape, fk_prefill_shape
+ * 2.3: attention that reads part of the cache (the section at the end) */
+#define FK_VERSION_MINOR 3
 int fk_version(void);
 
 /* Message describing the last failing call on this thread ("" if none). */
@@ -463,6 +464,98 @@ int fk_merge_attn_states(void* out, int64_t out_token_stride, int64_t out_head_s
  * the bf16-rounded activation matches forward_native (silu_and_mul.py:19-22). */
 int fk_silu_and_mul(void* out, int64_t out_row_stride, const void* x, int64_t x_row_stride,
                     int64_t rows, int64_t d, int dtype, void* stream);
+
+/* Attention that reads part of a paged cache (library version 2.3).  No counterpart in the
+ * reference: its decode attention reads every cached token.
+ *
+ * Common arguments: block_tables is int32 [batch, >= bt_width] rows bt_row_stride apart;
+ * entries outside [0, num_blocks) and columns >= bt_width are masked.  cache_seqlens: int32
+ * [batch].  cu_seqlens_q: NULL = one query row per sequence, or int32 [batch + 1]: sequence b
+ * has the query rows [cu_seqlens_q[b], cu_seqlens_q[b+1]), its last n tokens; its i-th row
+ * sees vis = cache_seqlens[b] - n + i + 1 keys.  Rows behind the last sequence are left as
+ * they were.  max_seqlen_q bounds every sequence's rows (1 without cu_seqlens_q; it sizes the
+ * launch, rows past it are not processed).  A kv head's group is num_heads / num_kv_heads
+ * query heads, of any size.  kv_dtype: BF16 or FP8_E4M3FN; head_size 64, 128 or 256;
+ * block_size a power of two >= 16.
+ *
+ * fk_update_key_bounds: key_bounds [num_blocks, Hk, 2, head_size] of the cache's dtype; for
+ * each page that holds one of sequence b's last n tokens (n = its query rows, 1 without
+ * cu_seqlens_q), key_bounds[page, h, 0] and [page, h, 1] become the least and the greatest
+ * value of each key dimension over the page's tokens < cache_seqlens[b] (NaN if one is NaN).
+ * Whole pages are read, so the result does not depend on earlier calls.  batch <= 65535. */
+int fk_update_key_bounds(void* key_bounds, const void* k_cache, int kv_dtype,
+                         const int32_t* block_tables, int64_t bt_row_stride, int64_t bt_width,
+                         const int32_t* cache_seqlens, const int32_t* cu_seqlens_q,
+                         int64_t batch, int64_t max_seqlen_q, int num_kv_heads, int head_size,
+                         int block_size, int64_t num_blocks, void* stream);
+
+/* scores[t, h, j] (fp32; rows score_row_stride, heads score_head_stride floats apart, `width`
+ * blocks each) = the greatest over the query heads of kv head h of
+ *   sum_d max(q[t, hq, d] lo_d, q[t, hq, d] hi_d)   (lo, hi: block j's key_bounds, times
+ * k_scale[h] for fp8 pages), an upper bound of q . k over the block's keys (NaN and infinite
+ * keys give NaN or infinite scores); -inf for blocks the row does not see and for masked
+ * pages.  q: bf16 [rows, num_heads, head_size].  The groups of 16 / (group rounded up to a
+ * power of two) query rows of all sequences number at most 65535. */
+int fk_block_scores(float* scores, int64_t score_row_stride, int64_t score_head_stride,
+                    int64_t width, const void* q, int64_t q_row_stride, const void* key_bounds,
+                    int kv_dtype, const float* k_scale, const int32_t* block_tables,
+                    int64_t bt_row_stride, int64_t bt_width, const int32_t* cache_seqlens,
+                    const int32_t* cu_seqlens_q, int64_t batch, int64_t rows,
+                    int64_t max_seqlen_q, int num_heads, int num_kv_heads, int head_size,
+                    int block_size, int64_t num_blocks, void* stream);
+
+/* block_indices[t, h, 0 .. keep) (int32): the blocks row t attends to at kv head h, in
+ * ascending order, -1 behind the last.  Of the n = ceil(vis / block_size) blocks the row sees
+ * (at most `width`): all if n <= keep, else the first keep_first, the last keep_last and the
+ * ones with the highest scores among the rest; of equal scores the lower index first, NaN
+ * above every number, -0 equal to +0.  keep_first + keep_last <= keep. */
+int fk_select_blocks(int32_t* block_indices, int64_t out_row_stride, int64_t out_head_stride,
+                     int64_t keep, const float* scores, int64_t score_row_stride,
+                     int64_t score_head_stride, int64_t width, const int32_t* cache_seqlens,
+                     const int32_t* cu_seqlens_q, int64_t batch, int64_t rows, int num_kv_heads,
+                     int block_size, int keep_first, int keep_last, void* stream);
+
+/* out[t, hq] = softmax attention of q[t, hq] over its visible keys (< vis) in the blocks
+ * block_indices[t, kv head, 0 .. keep).  Entries outside the table, blocks without a visible
+ * key and masked pages are skipped, in any order; a block listed twice counts twice.  Scales
+ * and sinks as fk_paged_decode; a row that sees no key is zero.  rows <= 65535. */
+int fk_sparse_paged_decode(void* out, int64_t out_row_stride, const void* q,
+                           int64_t q_row_stride, const void* k_cache, const void* v_cache,
+                           int kv_dtype, const float* k_scale, const float* v_scale,
+                           const int32_t* block_tables, int64_t bt_row_stride, int64_t bt_width,
+                           const int32_t* cache_seqlens, const int32_t* cu_seqlens_q,
+                           int64_t batch, int64_t rows, const int32_t* block_indices,
+                           int64_t idx_row_stride, int64_t idx_head_stride, int64_t keep,
+                           int num_heads, int num_kv_heads, int head_size, int block_size,
+                           int64_t num_blocks, float scale, const float* sinks,
+                           void* workspace, int64_t workspace_bytes, void* stream);
+
+/* Workspace bytes fk_sparse_paged_decode needs at these sizes (0: none; host only). */
+int fk_sparse_paged_decode_plan(int64_t rows, int64_t keep, int num_heads, int num_kv_heads,
+                                int head_size, int block_size, int64_t* workspace_bytes);
+
+/* fk_paged_decode of the same arguments, for a batch in groups that share a prefix: rows
+ * cu_groups[g] .. cu_groups[g+1] - 1 (int32 [num_groups + 1], ascending) have the same keys
+ * and values at positions < prefix_lens[g] (int32 [num_groups]; any length), which are read
+ * once for the group, through the block table of its first row; the rows' own tables are read
+ * from there on.  Rows outside every group share nothing.  A row may be shorter than its
+ * group's prefix (0 tokens: a zero row).  max_prefix_len: a bound on every prefix, or 0 if
+ * unknown; it only chooses the launch shape. */
+int fk_shared_prefix_decode(void* out, int64_t out_row_stride, const void* q,
+                            int64_t q_row_stride, const void* k_cache, const void* v_cache,
+                            int kv_dtype, const float* k_scale, const float* v_scale,
+                            const int32_t* block_tables, int64_t bt_row_stride,
+                            int64_t bt_width, const int32_t* cache_seqlens, int64_t batch,
+                            const int32_t* cu_groups, const int32_t* prefix_lens,
+                            int64_t num_groups, int64_t max_prefix_len, int num_heads,
+                            int num_kv_heads, int head_size, int block_size, int64_t num_blocks,
+                            float scale, int window_left, const float* sinks, void* workspace,
+                            int64_t workspace_bytes, void* stream);
+
+/* Workspace bytes fk_shared_prefix_decode needs at these sizes (0: none; host only). */
+int fk_shared_prefix_decode_plan(int64_t batch, int64_t num_groups, int64_t max_prefix_len,
+                                 int num_heads, int num_kv_heads, int head_size,
+                                 int64_t* workspace_bytes);
 
 #ifdef __cplusplus
 }

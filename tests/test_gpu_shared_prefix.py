@@ -1,0 +1,180 @@
+"""Decode attention of a batch in groups that share a prefix (GPU), against the float64
+definition (``oracle.partial``).  The tolerance is that of tests/test_gpu_sparse.py."""
+from __future__ import annotations
+
+import numpy as np
+import pytest
+import torch
+
+from oracle import partial as ref
+from test_gpu_sparse import check_attn, cu_of, f64, int32, load, make_cache, poison
+
+pytestmark = pytest.mark.gpu
+
+
+def shared_tables(g, groups, dev, page):
+    """groups: list of (prefix, [own tokens per row] ), a row's length being their sum or, for
+    a negative entry, the positive length of a row shorter than the prefix; prefix None: rows
+    outside any group.  Only the first row of a group lists the prefix's whole pages."""
+    rows, pool = [], 0
+    for prefix, own in groups:
+        start = len(rows)
+        for t in own:
+            n = (prefix or 0) + t if t >= 0 else -t
+            rows.append((start, prefix or 0, n))
+    pages = max(-(-max(n, p) // page) for _, p, n in rows) + 1
+    bt = torch.full((len(rows), pages), -1, dtype=torch.int32)
+    pool = 0
+    for b, (start, prefix, n) in enumerate(rows):
+        whole = prefix // page if b != start else 0
+        for j in range(whole, -(-max(n, prefix if b == start else 0) // page)):
+            bt[b, j] = pool
+            pool += 1
+    perm = torch.randperm(pool + 3, generator=g, device=dev).to(torch.int32).cpu()
+    bt = torch.where(bt >= 0, perm[bt.clamp(min=0).long()], bt)
+    return bt.to(dev), pool + 3, [n for _, _, n in rows]
+
+
+def build(cuda, kv, hq, hk, d, page, groups, seed=0):
+    g = torch.Generator(device=cuda).manual_seed(seed + hq + d + page)
+    bt, pool, lens = shared_tables(g, groups, cuda, page)
+    k = make_cache(g, pool, page, hk, d, kv, cuda)
+    v = make_cache(g, pool, page, hk, d, kv, cuda)
+    real = [(p, o) for p, o in groups if p is not None]
+    cu = cu_of([len(o) for _, o in real], cuda)
+    pre = int32([p for p, _ in real], cuda)
+    # a prefix that ends inside a page: rows keep their own copy of that page, whose positions
+    # below the prefix hold other values; they are not read
+    at = 0
+    used = torch.zeros(pool, page, dtype=torch.bool, device=cuda)
+    for p, own in groups:
+        for i in range(len(own)):
+            n = lens[at + i]
+            for j in range(-(-n // page)):
+                lo = 0 if i == 0 else max(0, min(page, (p or 0) - j * page))
+                pg = int(bt[at + i, j])
+                if pg >= 0:
+                    used[pg, lo:max(0, min(page, n - j * page))] = True
+        if p:
+            most = min(p, max(lens[at:at + len(own)], default=0))
+            for j in range(-(-most // page)):
+                used[int(bt[at, j]), :min(page, most - j * page)] = True
+        at += len(own)
+    for c in (k, v):
+        poison(c, ~used)
+    ks = vs = None
+    if kv == "fp8":
+        ks = torch.linspace(0.1, 0.3, hk, device=cuda)
+        vs = torch.linspace(0.2, 0.4, hk, device=cuda)
+    q = torch.randn(len(lens), hq, d, generator=g, device=cuda).to(torch.bfloat16)
+    return g, q, k, v, bt, lens, cu, pre, ks, vs
+
+
+GROUPS = {
+    "one": [(200, [5, 40, 1, 0, 300])],
+    "ragged": [(333, [7, 0, -1, 20]), (64, [1]), (1000, [100, 3, -500, 250, 16, 17]),
+               (None, [90, 0, 16])],
+    "none": [(None, [30, 700, 0])],
+    "zero": [(0, [10, 0]), (0, [129])],
+    "wide": [(513, [3 + i for i in range(40)])],
+    "short": [(5, [1, 2, 3]), (15, [0, 1])],
+    "empty": [(100, []), (48, [1, 2]), (100, [])],
+    "long": [(9000, [60, 1, 2500])],
+}
+
+
+@pytest.mark.parametrize("name", list(GROUPS))
+@pytest.mark.parametrize("kv,hq,hk,d,page", [
+    ("bf16", 32, 8, 128, 16), ("fp8", 16, 2, 128, 64), ("bf16", 8, 1, 256, 16),
+    ("bf16", 10, 10, 64, 32), ("fp8", 40, 2, 64, 16), ("fp8", 12, 4, 256, 128),
+])
+def test_shared_prefix(cuda, kv, hq, hk, d, page, name):
+    from fastkernels_amd import ops
+
+    g, q, k, v, bt, lens, cu, pre, ks, vs = build(cuda, kv, hq, hk, d, page, GROUPS[name])
+    out = torch.full_like(q, 9.0)
+    ops.shared_prefix_decode(out, q, k, v, bt, int32(lens, cuda), cu, pre, d ** -0.5, ks, vs,
+                             max_prefix_len=0 if name == "ragged" else
+                             max([1, *pre.tolist()]))
+    want = ref.shared_prefix_decode(f64(q), f64(k), f64(v), bt.cpu().numpy(), lens,
+                                    cu.cpu().numpy(), pre.cpu().numpy(), d ** -0.5, f64(ks),
+                                    f64(vs))
+    check_attn(out, *want)
+
+
+@pytest.mark.parametrize("window", [0, 15, 100, 600, 5000])
+@pytest.mark.parametrize("kv,hq,hk,d,page", [("bf16", 32, 8, 128, 16), ("fp8", 24, 2, 64, 32)])
+def test_shared_prefix_window_and_sinks(cuda, kv, hq, hk, d, page, window):
+    from fastkernels_amd import ops
+
+    g, q, k, v, bt, lens, cu, pre, ks, vs = build(cuda, kv, hq, hk, d, page, GROUPS["ragged"])
+    sinks = torch.randn(hq, generator=g, device=cuda)
+    wide = torch.full((len(lens), hq + 3, d), 9.0, dtype=torch.bfloat16, device=cuda)
+    ops.shared_prefix_decode(wide[:, :hq], q, k, v, bt, int32(lens, cuda), cu, pre, d ** -0.5, ks,
+                             vs, window, sinks)
+    want = ref.shared_prefix_decode(f64(q), f64(k), f64(v), bt.cpu().numpy(), lens,
+                                    cu.cpu().numpy(), pre.cpu().numpy(), d ** -0.5, f64(ks),
+                                    f64(vs), window, f64(sinks))
+    check_attn(wide[:, :hq], *want)
+    assert bool((wide[:, hq:] == 9.0).all())
+
+
+def test_shared_prefix_is_decode(cuda):
+    """FlashAttnDecode.forward_shared_prefix beside forward, the tables listing every page."""
+    hq, hk, d, page = 32, 8, 128, 16
+    g = torch.Generator(device=cuda).manual_seed(4)
+    pre, own = 96 * page, [5, 300, 1, 44, 17, 900]
+    bt = torch.full((6, 160), -1, dtype=torch.int32, device=cuda)
+    perm = torch.randperm(1000, generator=g, device=cuda).to(torch.int32)
+    at = 96
+    for b, t in enumerate(own):
+        n = -(-t // page)
+        bt[b, :96], bt[b, 96:96 + n] = perm[:96], perm[at:at + n]
+        at += n
+    k, v = (make_cache(g, 1000, page, hk, d, "bf16", cuda) for _ in range(2))
+    q = torch.randn(6, hq * d, generator=g, device=cuda).to(torch.bfloat16)
+    ctx = int32([pre + t for t in own], cuda)
+    attn = load("flash_attn_decode", "FlashAttnDecode")(hq, hk, d)
+    got = attn.forward_shared_prefix(q, k, v, ctx, int32([0, 4, 6], cuda), int32([pre, pre], cuda),
+                                     block_table=bt, max_prefix_len=pre)
+    dense = attn(q, k, v, ctx, block_table=bt)
+    assert got.shape == dense.shape
+    want = ref.shared_prefix_decode(f64(q).reshape(6, hq, d), f64(k), f64(v), bt.cpu().numpy(),
+                                    ctx.tolist(), [0, 4, 6], [pre, pre], d ** -0.5)
+    check_attn(got, *want)
+    check_attn(dense, *want)
+
+
+def test_shared_prefix_in_graphs(cuda):
+    """Two graphs of different groups captured on one module and replayed in turn, as the
+    lengths and the prefixes change, against the eager result."""
+    hq, hk, d, page = 32, 8, 128, 16
+    _, q, k, v, bt, lens, cu, pre, _, _ = build(cuda, "bf16", hq, hk, d, page, GROUPS["one"])
+    k, v = k.nan_to_num(1.0), v.nan_to_num(1.0)
+    bt[:] = bt[:1].clamp(min=0)
+    ctx = int32(lens, cuda)
+    attn = load("flash_attn_decode", "FlashAttnDecode")(hq, hk, d)
+    two = int32([0, 2, 5], cuda)
+    two_pre = int32([64, 160], cuda)
+
+    def steps():
+        return (attn.forward_shared_prefix(q, k, v, ctx, cu, pre, block_table=bt),
+                attn.forward_shared_prefix(q, k, v, ctx, two, two_pre, block_table=bt))
+
+    steps()
+    torch.cuda.synchronize()
+    graphs, outs = [], []
+    for args in ((cu, pre), (two, two_pre)):
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            outs.append(attn.forward_shared_prefix(q, k, v, ctx, *args, block_table=bt))
+        graphs.append(graph)
+    for i, new in enumerate((lens, [205, 240, 201, 200, 0], [1, 2, 3, 170, 190])):
+        ctx.copy_(int32(new, cuda))
+        two_pre.copy_(int32([64 - 16 * i, 160 - i], cuda))
+        for graph in (graphs[i % 2], graphs[1 - i % 2]):
+            graph.replay()
+        got = [o.clone() for o in outs]
+        want = steps()
+        torch.cuda.synchronize()
+        assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
