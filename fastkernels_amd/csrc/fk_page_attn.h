@@ -1,10 +1,10 @@
-// Attention of one block of up to 16 query columns over a list of page pieces, by the waves
+// Attention of blocks of 16 query columns over a list of page pieces, by the waves
 // of one work-group: shared by the sparse and the shared-prefix decode kernels.
 //
 // A unit is a run of 16-token tiles inside one page.  The waves take the units in turn
-// (wave w of n takes units w, w + n, ...), each keeps the softmax state of its units (running
-// maximum, sum, unnormalised O, all fp32), and the states are merged through LDS with the
-// log-sum-exp rule M = max m_w, L = sum l_w 2^(m_w - M), O = sum o_w 2^(m_w - M).
+// (wave w of n takes units w, w + n, ...), each keeps the softmax state of its units (a
+// reference maximum, the sum, the unnormalised O, all fp32), and the states are merged through
+// LDS with the log-sum-exp rule M = max m_w, L = sum l_w 2^(m_w - M), O = sum o_w 2^(m_w - M).
 #pragma once
 
 #include "fk_attn_tile.h"
@@ -33,219 +33,421 @@ struct PageAttnParams {
   int batch;
 };
 
-// Waves of a work-group: their O states (columns x D floats each) take at most 64 KB of LDS.
-template <int kG, int D>
-constexpr int page_attn_waves() { return kG * D > 2048 ? 4 : 8; }
+// Softmax state of one wave over kCB blocks of 16 query columns.  Lane (r, g) holds, for
+// column r of each block, the reference maximum, its share of the sum (keys 4g .. 4g + 3 of
+// every tile) and dims (D/4) g .. (D/4) g + D/4 - 1 of O: P V is computed transposed (A = V
+// with row m = dim (D/16) m + slice, B = P), so that the column a lane rescales and divides
+// is its own.  o[cb][d][i] is dim (D/4) g + (D/16) i + d.
+//
+// Two tiles go together: their scores' layouts side by side (keys 4g .. 4g + 3 of each) are
+// the 32-key operand of the 16x16x32 MFMA once V's rows are paired alike, which does P V in
+// half the instructions of the 16-key form.
+//
+// The maximum is only moved when a score exceeds it by more than kLazyMax: until then the
+// weights grow to at most 2^8, which bf16 and the fp32 sums hold as exactly as smaller ones.
+constexpr float kLazyMax = 8.f;
+constexpr float kNoMax = -1.0e30f;  // the reference before a column's first visible key
 
-// Softmax state of one wave over up to 16 query columns.  Lane (r, g) holds column r's
-// maximum and its share of the sum, and O[column 4g + i][dims (D/16) r ..].
-template <int kG, int D, bool kFp8>
+template <int kCB, int D, bool kFp8>
 struct ColumnState {
   static constexpr int kKc = D / 32;
   static constexpr int kSl = D / 16;
-  bf16x8_t qb[kKc];
-  float m, l;
-  floatx4_t o[kSl];
+  bf16x8_t qb[kCB][kKc];
+  float m[kCB], l[kCB];
+  floatx4_t o[kCB][kSl];
 
-  // qp: the row of this lane's column (read where ok).
-  __device__ __forceinline__ void init(const uint16_t* qp, bool ok, int g) {
+  __device__ __forceinline__ void reset() {
+#pragma unroll
+    for (int cb = 0; cb < kCB; ++cb) {
+      m[cb] = kNoMax;
+      l[cb] = 0.f;
+#pragma unroll
+      for (int d = 0; d < kSl; ++d) o[cb][d] = floatx4_t{0.f, 0.f, 0.f, 0.f};
+    }
+  }
+  // qp: the row of this lane's column of block cb (read where ok); its signs are flipped by
+  // `flip` (0, or 0x80008000 where the scores' factor is negative: it is taken as positive).
+  __device__ __forceinline__ void load_q(int cb, const uint16_t* qp, bool ok, uint32_t flip,
+                                         int g) {
 #pragma unroll
     for (int c = 0; c < kKc; ++c) {
       const int d0 = kFp8 ? (D / 4) * g + 8 * c : 32 * c + 8 * g;
-      const uint4 v = ok ? *reinterpret_cast<const uint4*>(qp + d0) : make_uint4(0, 0, 0, 0);
-      qb[c] = __builtin_bit_cast(bf16x8_t, v);
+      uint4 v = ok ? *reinterpret_cast<const uint4*>(qp + d0) : make_uint4(0, 0, 0, 0);
+      v = make_uint4(v.x ^ flip, v.y ^ flip, v.z ^ flip, v.w ^ flip);
+      qb[cb][c] = __builtin_bit_cast(bf16x8_t, v);
     }
-    m = kNegInf;
-    l = 0.f;
-#pragma unroll
-    for (int d = 0; d < kSl; ++d) o[d] = floatx4_t{0.f, 0.f, 0.f, 0.f};
   }
 
-  // One tile of 16 tokens.  This lane's rows are visible where rel0 + i < span (unsigned:
-  // rel0 = position of row 4g less the first visible one); full: all 16 rows are.
-  __device__ __forceinline__ void tile(const DTile<kFp8, D>& cur, float ks, float s2,
-                                       uint32_t rel0, uint32_t span, bool full, int g) {
-    uint4 kc[kKc];
-    k_chunks_d(cur, kc);
-    const floatx4_t acc = qk_scores_n(kc, qb);
-    float s[4];
+  // Scores of two tiles (their K rows in a and b).
+  __device__ __forceinline__ void scores(const DTile<kFp8, D>& a, const DTile<kFp8, D>& b,
+                                         floatx4_t (&sa)[kCB], floatx4_t (&sb)[kCB]) const {
+    uint4 ka[kKc], kb[kKc];
+    k_chunks_d(a, ka);
+    k_chunks_d(b, kb);
 #pragma unroll
-    for (int i = 0; i < 4; ++i) s[i] = kFp8 ? acc[i] * ks * s2 : acc[i] * s2;
+    for (int cb = 0; cb < kCB; ++cb) {
+      sa[cb] = qk_scores_n(ka, qb[cb]);
+      sb[cb] = qk_scores_n(kb, qb[cb]);
+    }
+  }
+  // Scores to weights (in place; the weights are 2^(s2 score - m), s2 = scale log2(e)
+  // [k_scale] >= 0), moving the maxima where they have to.  Key i of tile a is visible to this
+  // lane's column of block cb where ra + i < lim[cb] (unsigned), likewise b; `full`: all are,
+  // to every column.
+  __device__ __forceinline__ void softmax(floatx4_t (&sa)[kCB], floatx4_t (&sb)[kCB], float s2,
+                                          uint32_t ra, uint32_t rb, const uint32_t (&lim)[kCB],
+                                          bool full) {
+    if (!full) {
+#pragma unroll
+      for (int cb = 0; cb < kCB; ++cb)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          if (!(ra + i < lim[cb])) sa[cb][i] = kNegInf;
+          if (!(rb + i < lim[cb])) sb[cb][i] = kNegInf;
+        }
+    }
+    float top[kCB];
+    bool move = false;
+#pragma unroll
+    for (int cb = 0; cb < kCB; ++cb) {
+      top[cb] = s2 * fmaxf(fmaxf(fmaxf(sa[cb][0], sa[cb][1]), fmaxf(sa[cb][2], sa[cb][3])),
+                           fmaxf(fmaxf(sb[cb][0], sb[cb][1]), fmaxf(sb[cb][2], sb[cb][3])));
+      move |= top[cb] > m[cb] + kLazyMax;
+    }
+    if (__ballot(move) != 0) {
+#pragma unroll
+      for (int cb = 0; cb < kCB; ++cb) {
+        const float m_new = fmaxf(m[cb], pair_max(top[cb]));
+        const float alpha = __builtin_amdgcn_exp2f(m[cb] - m_new);
+        m[cb] = m_new;
+        l[cb] *= alpha;
+#pragma unroll
+        for (int d = 0; d < kSl; ++d) o[cb][d] *= alpha;
+      }
+    }
+#pragma unroll
+    for (int cb = 0; cb < kCB; ++cb) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        sa[cb][i] = __builtin_amdgcn_exp2f(__builtin_fmaf(sa[cb][i], s2, -m[cb]));
+        sb[cb][i] = __builtin_amdgcn_exp2f(__builtin_fmaf(sb[cb][i], s2, -m[cb]));
+      }
+    }
+    if (!full) {  // (not left to -inf: its product with a scale of 0 is NaN)
+#pragma unroll
+      for (int cb = 0; cb < kCB; ++cb)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          if (!(ra + i < lim[cb])) sa[cb][i] = 0.f;
+          if (!(rb + i < lim[cb])) sb[cb][i] = 0.f;
+        }
+    }
+#pragma unroll
+    for (int cb = 0; cb < kCB; ++cb)
+      l[cb] += (sa[cb][0] + sa[cb][1]) + (sa[cb][2] + sa[cb][3]) +
+               ((sb[cb][0] + sb[cb][1]) + (sb[cb][2] + sb[cb][3]));
+  }
+  // O += P V.  V rows that no column sees (ra + i >= span) may hold anything: zeroed, so that
+  // a zero weight never meets a NaN.  The weights are rounded to bf16 (2^-9 relative on
+  // average, of either sign), as in the decode kernel; the sum is of the unrounded ones.
+  __device__ __forceinline__ void values(DTile<kFp8, D>& a, DTile<kFp8, D>& b,
+                                         const floatx4_t (&pa)[kCB], const floatx4_t (&pb)[kCB],
+                                         uint32_t ra, uint32_t rb, uint32_t span, bool full) {
     if (!full) {
 #pragma unroll
       for (int i = 0; i < 4; ++i)
-        if (!(rel0 + i < span)) s[i] = kNegInf;
+#pragma unroll
+        for (int q = 0; q < DTile<kFp8, D>::kVWords; ++q) {
+          a.v[i][q] = ra + i < span ? a.v[i][q] : 0u;
+          b.v[i][q] = rb + i < span ? b.v[i][q] : 0u;
+        }
     }
-    const float m_new = fmaxf(m, pair_max(fmaxf(fmaxf(s[0], s[1]), fmaxf(s[2], s[3]))));
-    const float m_use = m_new == kNegInf ? 0.f : m_new;
-    const float alpha = m_new == kNegInf ? 1.f : __builtin_amdgcn_exp2f(m - m_use);
-    float pr[4];
-    float psum = 0.f;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      pr[i] = __builtin_amdgcn_exp2f(s[i] - m_use);
-      psum += pr[i];
+    short4_t va[kSl], vb[kSl];
+    if constexpr (kFp8) {
+      const bool all[4] = {true, true, true, true};
+      v_operands_fp8(a, true, all, va);
+      v_operands_fp8(b, true, all, vb);
+    } else {
+      v_operands_w(a.v, va);
+      v_operands_w(b.v, vb);
     }
-    l = l * alpha + psum;
-    m = m_new;
-    if (__ballot(alpha != 1.f) != 0) {
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const float a = row_value<kG>(alpha, g, i);
+    for (int cb = 0; cb < kCB; ++cb) {
+      const float fa[4] = {pa[cb][0], pa[cb][1], pa[cb][2], pa[cb][3]};
+      const float fb[4] = {pb[cb][0], pb[cb][1], pb[cb][2], pb[cb][3]};
+      const uint2 x = __builtin_bit_cast(uint2, p_operand(fa));
+      const uint2 y = __builtin_bit_cast(uint2, p_operand(fb));
+      const bf16x8_t p = __builtin_bit_cast(bf16x8_t, make_uint4(x.x, x.y, y.x, y.y));
 #pragma unroll
-        for (int d = 0; d < kSl; ++d) o[d][i] *= a;
+      for (int d = 0; d < kSl; ++d) {
+        const uint2 v = __builtin_bit_cast(uint2, va[d]), w = __builtin_bit_cast(uint2, vb[d]);
+        o[cb][d] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(
+            __builtin_bit_cast(bf16x8_t, make_uint4(v.x, v.y, w.x, w.y)), p, o[cb][d], 0, 0, 0);
       }
     }
-    // The weights enter P V as bf16 (half a step, 2^-9 relative, each; their signs differ
-    // from key to key), as in the decode kernel.
-    const short4_t pa = p_operand(pr);
-    // V rows that are masked may hold anything: zeroed, so that 0 never meets a NaN.
-    short4_t vb[kSl];
-    if constexpr (kFp8) {
-      bool keep[4];
-#pragma unroll
-      for (int i = 0; i < 4; ++i) keep[i] = rel0 + i < span;
-      v_operands_fp8(cur, full, keep, vb);
-    } else {
-      uint32_t vw[4][D / 32];
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-        v_words(cur, i, full || rel0 + i < span, vw[i]);
-      v_operands_w(vw, vb);
-    }
-    pv_accumulate_n(o, pa, vb);
   }
 };
 
-// Issues the loads of the tile whose first token is slot0 (of the cache's slots), kv head
-// kvh.
+// Where a wave's lanes read a tile: byte offsets from the tile's first row of the kv head.
 template <bool kFp8, int D>
-__device__ __forceinline__ void load_page_tile(const PageAttnParams& P, int64_t slot0, int kvh,
-                                               int r, int g, DTile<kFp8, D>& t) {
-  constexpr int kElt = kFp8 ? 1 : 2;
-  const int64_t row_bytes = static_cast<int64_t>(P.num_kv_heads) * D * kElt;
-  const int64_t at = slot0 * row_bytes + static_cast<int64_t>(kvh) * D * kElt;
-  const uint8_t* krow = P.k_cache + at + r * row_bytes;
-  const uint8_t* vrow = P.v_cache + at + 4 * g * row_bytes + (D / 16) * r * kElt;
+struct TileLanes {
+  uint32_t k, v[4];
+  uint32_t bytes;  // of a tile, from its first row on
+  __device__ __forceinline__ TileLanes(int num_kv_heads, int r, int g) {
+    constexpr int kElt = kFp8 ? 1 : 2;
+    const uint32_t row = static_cast<uint32_t>(num_kv_heads) * D * kElt;
+    bytes = 15 * row + D * kElt;
+    k = r * row + (kFp8 ? (D / 4) * g : 16 * g);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v[i] = (4 * g + i) * row + (D / 16) * r * kElt;
+  }
+};
+// Issue a tile's K or V loads; row: its first row of the kv head (wave-uniform).  As buffer
+// loads: the tile's address stays in scalar registers (a descriptor of its 16 rows) and the
+// lanes' offsets never change, where plain loads took a 64-bit sum per lane and row.
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t tile_rows(const uint8_t* row, uint32_t bytes) {
+  return __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t*>(row), 0, static_cast<int>(bytes),
+                                           0x00027000);
+}
+template <bool kFp8, int D>
+__device__ __forceinline__ void load_tile_k(const uint8_t* row, const TileLanes<kFp8, D>& at,
+                                            DTile<kFp8, D>& t) {
+  const auto rows = tile_rows(row, at.bytes);
 #pragma unroll
   for (int c = 0; c < DTile<kFp8, D>::kKLoads; ++c)
-    t.k[c] = ld16(kFp8 ? krow + (D / 4) * g + 16 * c : krow + (32 * c + 8 * g) * 2);
+    t.k[c] = __builtin_bit_cast(
+        uint4, __builtin_amdgcn_raw_buffer_load_b128(rows, at.k + (kFp8 ? 16 : 64) * c, 0, 0));
+}
+template <bool kFp8, int D>
+__device__ __forceinline__ void load_tile_v(const uint8_t* row, const TileLanes<kFp8, D>& at,
+                                            DTile<kFp8, D>& t) {
+  constexpr int kWords = DTile<kFp8, D>::kVWords;
+  const auto rows = tile_rows(row, at.bytes);
 #pragma unroll
-  for (int i = 0; i < 4; ++i) ld_words(vrow + i * row_bytes, t.v[i]);
+  for (int i = 0; i < 4; ++i) {
+    if constexpr (kWords == 1) {
+      t.v[i][0] = __builtin_amdgcn_raw_buffer_load_b32(rows, at.v[i], 0, 0);
+    } else if constexpr (kWords == 2) {
+      const auto x = __builtin_amdgcn_raw_buffer_load_b64(rows, at.v[i], 0, 0);
+      t.v[i][0] = x[0];
+      t.v[i][1] = x[1];
+    } else {
+#pragma unroll
+      for (int q = 0; q < kWords; q += 4) {
+        const auto x = __builtin_amdgcn_raw_buffer_load_b128(rows, at.v[i] + 4 * q, 0, 0);
+        t.v[i][q] = x[0];
+        t.v[i][q + 1] = x[1];
+        t.v[i][q + 2] = x[2];
+        t.v[i][q + 3] = x[3];
+      }
+    }
+  }
 }
 
-// Streams units first, first + step, ... (< units) of the list into st.  unit_at(u, page,
-// tok0) gives unit u's page (-1: nothing to read) and its first token's position; a unit has
-// unit_tiles tiles of its page, of which those from position `hi` on, or wholly before `lo`,
-// are skipped.  Lane k looks up the wave's unit k, 64 at a time, and the units with something
-// to read are packed to the front, so that the tile loop only meets those.
-template <int kG, int D, bool kFp8, int U, class UnitAt>
-__device__ __forceinline__ void stream_units(const PageAttnParams& P, ColumnState<kG, D, kFp8>& st,
-                                             UnitAt unit_at, int units, int first, int step,
-                                             int unit_tiles_log2, int lo, int hi, int kvh,
-                                             float ks, int lane) {
+// Keeps the loads before it before it: the compiler otherwise sinks them to just before their
+// first use, a step later, and their latency is no longer hidden.
+__device__ __forceinline__ void loads_issued() { asm volatile("" ::: "memory"); }
+
+// What a wave's columns see of positions [from, to): lim[cb] keys from `from` on for this lane's
+// column of block cb, at most `span` for any column of the wave and at least `least`.
+template <int kCB>
+struct Limits {
+  uint32_t lim[kCB];
+  uint32_t span, least;
+};
+
+// Streams units first, first + step, ... (< units) of a list into st, of each the positions in
+// [from, to).  unit_at(u, page, tok) gives unit u's page (-1: nothing to read) and its first
+// token's position; a unit is 1 << unit_tiles_log2 tiles of its page.  Lane k looks up the
+// wave's unit k, 64 at a time, and the units with something to read are packed to the front, so
+// that the tile loop only meets those.  The K rows of the next two tiles are requested when the
+// scores have used this step's, the V rows when P V has.  limits() is asked once, when the first
+// rows are on their way.
+template <int kCB, int D, bool kFp8, class UnitAt, class LimitsOf>
+__device__ __forceinline__ void stream_units(const PageAttnParams& P,
+                                             ColumnState<kCB, D, kFp8>& st, UnitAt unit_at,
+                                             int units, int first, int step, int unit_tiles_log2,
+                                             int from, int to, LimitsOf limits, int kvh, float s2,
+                                             int lane) {
+  constexpr int kElt = kFp8 ? 1 : 2;
   const int r = lane & 15, g = lane >> 4;
-  const uint32_t span = static_cast<uint32_t>(max(hi - lo, 0));
   const int page_mask = (1 << P.block_size_log2) - 1;
+  const TileLanes<kFp8, D> at(P.num_kv_heads, r, g);
+  const int64_t row_bytes = static_cast<int64_t>(P.num_kv_heads) * D * kElt;
+  const uint8_t* const kh = P.k_cache + static_cast<int64_t>(kvh) * D * kElt;
+  const uint8_t* const vh = P.v_cache + static_cast<int64_t>(kvh) * D * kElt;
+  Limits<kCB> lm;
+  bool asked = false;
   for (int64_t u0 = first; u0 < units; u0 += static_cast<int64_t>(64) * step) {
     const int64_t u = u0 + static_cast<int64_t>(lane) * step;
     int page = -1, tok = 0;
     if (u < units) unit_at(static_cast<int>(u), page, tok);
-    const bool ok = page >= 0 && page < P.num_blocks && tok < hi &&
-                    static_cast<int64_t>(tok) + (kTile << unit_tiles_log2) > lo;
+    const bool ok = page >= 0 && page < P.num_blocks && tok < to &&
+                    static_cast<int64_t>(tok) + (kTile << unit_tiles_log2) > from;
     const uint64_t oks = __ballot(ok);
     const int n = __builtin_popcountll(oks);
+    if (n == 0) continue;
     // lane k <- the k-th lane with ok set
     const int rank = __builtin_popcountll(oks & ((uint64_t{1} << lane) - 1));
-    const int to = ok ? rank : n + (lane - rank);
-    page = __builtin_amdgcn_ds_permute(to << 2, page);
-    tok = __builtin_amdgcn_ds_permute(to << 2, tok);
+    const int dst = ok ? rank : n + (lane - rank);
+    page = __builtin_amdgcn_ds_permute(dst << 2, page);
+    tok = __builtin_amdgcn_ds_permute(dst << 2, tok);
     const int tiles = n << unit_tiles_log2;
     const int sub_mask = (1 << unit_tiles_log2) - 1;
-    for (int x0 = 0; x0 < tiles; x0 += U) {
-      DTile<kFp8, D> buf[U];
-      int t0[U];
-#pragma unroll
-      for (int k = 0; k < U; ++k) {
-        const int x = min(x0 + k, tiles - 1);
-        const int pg = __builtin_amdgcn_readlane(page, x >> unit_tiles_log2);
-        t0[k] = __builtin_amdgcn_readlane(tok, x >> unit_tiles_log2) + kTile * (x & sub_mask);
-        const int64_t slot = (static_cast<int64_t>(pg) << P.block_size_log2) +
-                             (t0[k] & page_mask);
-        load_page_tile<kFp8, D>(P, slot, kvh, r, g, buf[k]);
-      }
-#pragma unroll
-      for (int k = 0; k < U; ++k) {
-        // (unsigned: a tile that begins before lo wraps past span)
-        const uint32_t rel = static_cast<uint32_t>(t0[k]) - static_cast<uint32_t>(lo);
-        if (x0 + k < tiles)
-          st.tile(buf[k], ks, P.scale_log2, rel + 4 * g, span,
-                  rel < span && span - rel >= kTile, g);
-      }
+    // First row and position (less from; unsigned, so one before it wraps past span) of tile x.
+    auto row_of = [&](int x, uint32_t& rel) -> int64_t {
+      const int pg = __builtin_amdgcn_readlane(page, x >> unit_tiles_log2);
+      const int t0 = __builtin_amdgcn_readlane(tok, x >> unit_tiles_log2) +
+                     kTile * (x & sub_mask);
+      rel = static_cast<uint32_t>(t0) - static_cast<uint32_t>(from);
+      return ((static_cast<int64_t>(pg) << P.block_size_log2) + (t0 & page_mask)) * row_bytes;
+    };
+    DTile<kFp8, D> a, b;
+    uint32_t ra, rb;
+    int64_t at_a = row_of(0, ra), at_b = row_of(min(1, tiles - 1), rb);
+    load_tile_k(kh + at_a, at, a);
+    load_tile_k(kh + at_b, at, b);
+    load_tile_v(vh + at_a, at, a);
+    load_tile_v(vh + at_b, at, b);
+    loads_issued();
+    if (!asked) {
+      lm = limits();
+      asked = true;
+    }
+    for (int x = 0; x < tiles; x += 2) {
+      floatx4_t sa[kCB], sb[kCB];
+      st.scores(a, b, sa, sb);
+      // (past the last tiles, these are read once more: the number of loads in flight stays
+      // known to the compiler's wait counts)
+      uint32_t na, nb;
+      at_a = row_of(min(x + 2, tiles - 1), na);
+      at_b = row_of(min(x + 3, tiles - 1), nb);
+      load_tile_k(kh + at_a, at, a);
+      load_tile_k(kh + at_b, at, b);
+      loads_issued();
+      if (x + 1 >= tiles) rb = lm.span;  // no second tile: masked
+      const bool full = ra < lm.least && lm.least - ra >= kTile && rb < lm.least &&
+                        lm.least - rb >= kTile;
+      st.softmax(sa, sb, s2, ra + 4 * g, rb + 4 * g, lm.lim, full);
+      st.values(a, b, sa, sb, ra + 4 * g, rb + 4 * g, lm.span, full);
+      load_tile_v(vh + at_a, at, a);
+      load_tile_v(vh + at_b, at, b);
+      loads_issued();
+      ra = na;
+      rb = nb;
     }
   }
 }
 
-// Merges the waves' states and hands each pair of adjacent dims of each of the ncols columns
-// to emit(column, dim, x, y, M, L): x and y are O[dim], O[dim + 1] before the division.
-template <int kG, int D, bool kFp8, class Emit>
-__device__ __forceinline__ void merge_waves(ColumnState<kG, D, kFp8>& st, float* lds, int wave,
-                                            int lane, int ncols, Emit emit) {
-  constexpr int kWaves = page_attn_waves<kG, D>();
+// Merges the waves' states of all column blocks and hands each quad of adjacent dims of each
+// of the ncols columns to emit(column, dim, o, M, L): o = O[dim .. dim + 3] before the division.
+// lds: merge_lds_floats(16 kCB columns at most); every thread of the work-group calls it, and
+// may write to lds again only after a barrier.
+template <int kWaves, int D>
+constexpr int merge_lds_floats(int cols) { return kWaves * cols * (D + 4 + 2); }
+template <int kWaves, int kCB, int D, bool kFp8, class Emit>
+__device__ __forceinline__ void merge_waves(const ColumnState<kCB, D, kFp8>& st, float* lds,
+                                            int wave, int lane, int ncols, Emit emit) {
+  constexpr int kRow = D + 4;  // (rows 16 bytes apart modulo the banks)
   constexpr int kSl = D / 16;
   const int r = lane & 15, g = lane >> 4;
-  float* const xo = lds;                         // [wave][column][D]
-  float* const xm = lds + kWaves * kG * D;       // [wave][column] maximum
-  float* const xl = xm + kWaves * kG;            // [wave][column] sum
-  st.l = pair_sum(st.l);
-  if (g == 0 && r < kG) {
-    xm[wave * kG + r] = st.m;
-    xl[wave * kG + r] = st.l;
-  }
+  float2* const xm = reinterpret_cast<float2*>(lds + kWaves * ncols * kRow);  // (m, l)
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const int j = 4 * g + i;
-    if (j < kG) {
-      float* dst = xo + (wave * kG + j) * D + kSl * r;
+  for (int cb = 0; cb < kCB; ++cb) {
+    const float l = pair_sum(st.l[cb]);
+    const int j = 16 * cb + r;
+    if (j < ncols) {
+      if (g == 0) xm[wave * ncols + j] = make_float2(st.m[cb], l);
+      float* dst = lds + (wave * ncols + j) * kRow + (D / 4) * g;
 #pragma unroll
-      for (int d = 0; d < kSl; d += 4)
-        *reinterpret_cast<float4*>(dst + d) =
-            make_float4(st.o[d][i], st.o[d + 1][i], st.o[d + 2][i], st.o[d + 3][i]);
+      for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int d = 0; d < kSl; d += 4)
+          *reinterpret_cast<float4*>(dst + kSl * i + d) =
+              make_float4(st.o[cb][d][i], st.o[cb][d + 1][i], st.o[cb][d + 2][i],
+                          st.o[cb][d + 3][i]);
     }
   }
   __syncthreads();
-  for (int x = threadIdx.x; x < ncols * (D / 2); x += kWaves * 64) {
-    const int j = x / (D / 2), dim = 2 * (x % (D / 2));
-    float M = kNegInf;
-#pragma unroll
-    for (int w = 0; w < kWaves; ++w) M = fmaxf(M, xm[w * kG + j]);
-    float L = 0.f, a = 0.f, b = 0.f;
+#pragma unroll 2
+  for (int x = threadIdx.x; x < ncols * (D / 4); x += kWaves * 64) {
+    const int j = x / (D / 4), dim = 4 * (x % (D / 4));
+    float2 s[kWaves];
+    float4 o[kWaves];
 #pragma unroll
     for (int w = 0; w < kWaves; ++w) {
-      const float mw = xm[w * kG + j];
-      const float f = mw == kNegInf ? 0.f : __builtin_amdgcn_exp2f(mw - M);
-      const float2 v = *reinterpret_cast<const float2*>(xo + (w * kG + j) * D + dim);
-      L = __builtin_fmaf(xl[w * kG + j], f, L);
-      a = __builtin_fmaf(v.x, f, a);
-      b = __builtin_fmaf(v.y, f, b);
+      s[w] = xm[w * ncols + j];
+      o[w] = *reinterpret_cast<const float4*>(lds + (w * ncols + j) * kRow + dim);
     }
-    emit(j, dim, a, b, M, L);
+    float M = s[0].x;
+#pragma unroll
+    for (int w = 1; w < kWaves; ++w) M = fmaxf(M, s[w].x);
+    float L = 0.f;
+    float4 u = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+    for (int w = 0; w < kWaves; ++w) {
+      const float f = __builtin_amdgcn_exp2f(s[w].x - M);
+      L = __builtin_fmaf(s[w].y, f, L);
+      u.x = __builtin_fmaf(o[w].x, f, u.x);
+      u.y = __builtin_fmaf(o[w].y, f, u.y);
+      u.z = __builtin_fmaf(o[w].z, f, u.z);
+      u.w = __builtin_fmaf(o[w].w, f, u.w);
+    }
+    emit(j, dim, u, M, L);
   }
 }
-template <int kG, int D>
-constexpr int merge_lds_floats() { return page_attn_waves<kG, D>() * kG * (D + 2); }
+
+// A wave's state of its first column block as a partial: O [columns][D] and (m, l) per column.
+template <int kCB, int D, bool kFp8>
+__device__ __forceinline__ void write_partial(const ColumnState<kCB, D, kFp8>& st, float* o,
+                                              float* ml, int lane, int ncols) {
+  constexpr int kSl = D / 16;
+  const int r = lane & 15, g = lane >> 4;
+  const float l = pair_sum(st.l[0]);
+  if (r >= ncols) return;
+  if (g == 0) *reinterpret_cast<float2*>(ml + 2 * r) = make_float2(st.m[0], l);
+  float* dst = o + r * D + (D / 4) * g;
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+#pragma unroll
+    for (int d = 0; d < kSl; d += 4)
+      *reinterpret_cast<float4*>(dst + kSl * i + d) =
+          make_float4(st.o[0][d][i], st.o[0][d + 1][i], st.o[0][d + 2][i], st.o[0][d + 3][i]);
+}
+
+// Running log-sum-exp state of four dims of a column over partials.
+struct Folded {
+  float M, L;
+  float4 o;
+  __device__ __forceinline__ void reset() {
+    M = kNoMax;
+    L = 0.f;
+    o = make_float4(0.f, 0.f, 0.f, 0.f);
+  }
+  __device__ __forceinline__ void add(float m, float l, const float4& x) {
+    const float top = fmaxf(M, m);
+    const float fa = __builtin_amdgcn_exp2f(M - top), fb = __builtin_amdgcn_exp2f(m - top);
+    M = top;
+    L = L * fa + l * fb;
+    o.x = o.x * fa + x.x * fb;
+    o.y = o.y * fa + x.y * fb;
+    o.z = o.z * fa + x.z * fb;
+    o.w = o.w * fa + x.w * fb;
+  }
+};
 
 // Output of a finished row: O (scaled by the V scale of fp8 pages) over the sum, which the
 // head's sink joins; a row that saw no key is zero.
-__device__ __forceinline__ void write_pair(const PageAttnParams& P, int64_t row, int hq, int D,
-                                           int dim, float x, float y, float M, float L,
+__device__ __forceinline__ void write_quad(const PageAttnParams& P, int64_t row, int hq, int D,
+                                           int dim, const float4& o, float M, float L,
                                            float vsc) {
   const float sink = P.sinks ? P.sinks[hq] * kLog2e : kNegInf;
   const float l = with_sink(L, M, sink);
   const float f = l > 0.f ? vsc / l : 0.f;
-  const bf16x2_t pk = {static_cast<__bf16>(x * f), static_cast<__bf16>(y * f)};
-  *reinterpret_cast<uint32_t*>(P.out + row * P.out_row_stride + static_cast<int64_t>(hq) * D +
-                               dim) = __builtin_bit_cast(uint32_t, pk);
+  const bf16x2_t a = {static_cast<__bf16>(o.x * f), static_cast<__bf16>(o.y * f)};
+  const bf16x2_t b = {static_cast<__bf16>(o.z * f), static_cast<__bf16>(o.w * f)};
+  *reinterpret_cast<uint2*>(P.out + row * P.out_row_stride + static_cast<int64_t>(hq) * D + dim) =
+      make_uint2(__builtin_bit_cast(uint32_t, a), __builtin_bit_cast(uint32_t, b));
 }
 
 // Checks the arguments the entry points share and fills A from them.

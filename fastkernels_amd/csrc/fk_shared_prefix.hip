@@ -5,6 +5,20 @@
 // other key is read through the row's own table.  The result is that of paged decode: row b
 // attends to its keys [lo, ctx_lens[b]), lo = 0 or ctx - 1 - window_left under a sliding
 // window.  Rows outside every group share nothing.
+//
+// Work.  A group's rows times the query heads of one kv head are the columns of one matrix
+// product with the prefix's keys: blocks of kCols columns stream the prefix's 16-token tiles
+// once each (where paged decode would stream them once per row), and what a row has of its own
+// is streamed like decode's, 16 columns at most.  Both kinds are lines of tiles,
+//   prefix line: (group, kv head, block of columns) x tiles of the prefix
+//   own line:    (row, kv head, block of 16 query heads) x tiles from the prefix's end on
+// cut into equal ranges, one per work-group and one per wave, so that lengths need not be known
+// on the host and none waits for the longest.  The four waves of a work-group share a prefix
+// range's tiles (fk_page_attn.h).  Each item and range leaves one partial state; a second launch
+// merges each row's partials of both kinds.  Where the items are few, each is rounded up to
+// whole ranges, so that no range spans two (its start and end cost as much as 30 tiles).  The prefix is bound by the vector and matrix units, the
+// rest by memory: one half of the work-groups takes its prefix range first and the other half
+// last, so that a CU, which holds one of each, does both at a time.
 #include <limits.h>
 
 #include "fk_page_attn.h"
@@ -12,93 +26,593 @@
 namespace fk {
 namespace {
 
+constexpr int kWaves = 4;
+constexpr int kThreads = kWaves * 64;
+constexpr int kPreTiles = 8;      // a prefix range is a multiple of this: two tiles per wave
+constexpr int kOwnTiles = 2;      // and a wave's own range of this
+constexpr int kMaxGroups = 2048;  // (their bounds are held in LDS)
+
+// Column blocks of a prefix item.  (O takes 4 D / 16 registers per block.)
+template <int D>
+constexpr int col_blocks_of() { return D == 64 ? 4 : D == 128 ? 2 : 1; }
+constexpr int cols_of(int d) { return 16 * (d == 64 ? 4 : d == 128 ? 2 : 1); }
+
+// What the merge has to know of a row.
+struct RowRecord {
+  int64_t own_start;  // the row's first tile on the own line (its first head's)
+  int64_t pre_start;  // its group's first tile on the prefix line
+  int64_t own_range, pre_range;  // tiles of a range of each line
+  int64_t own_step, pre_step;    // places of an item on its line
+  int own_tiles;      // tiles per head (0: nothing of its own)
+  int pre_tiles;      // tiles of the prefix (0: no shared prefix)
+  int pre_item;       // its group's first prefix item
+  int col_items;      // column blocks of its group, per kv head
+  int index;          // row of its group
+  int pad_;
+};
+
 struct PrefixParams {
   PageAttnParams A;
   int num_groups;
   int window_left;
   int unit_tiles_log2;
+  int wgs;                 // work-groups that share the lines
+  int vheads;              // kv heads x blocks of 16 query heads
+  int own_cols;            // query columns of an own item: min(16, gqa)
+  float* pre_o;            // [pieces][kCols][D], then (maximum, sum) per column
+  float* pre_ml;
+  float* own_o;            // [pieces][own_cols][D]
+  float* own_ml;
+  int64_t pre_pieces;      // room for pieces of the prefix line
+  RowRecord* rows;         // [batch]
 };
 
-// Group of row b (the last with cu_groups[g] <= b), or -1.
-__device__ __forceinline__ int group_of(const int32_t* __restrict__ cu, int groups, int b) {
-  if (groups <= 0 || b < cu[0] || b >= cu[groups]) return -1;
-  int lo = 0, hi = groups;
-  while (hi - lo > 1) {
-    const int mid = (lo + hi) >> 1;
-    if (cu[mid] <= b) lo = mid; else hi = mid;
-  }
-  return lo;
-}
+// A group: its rows, and the prefix that they share in this launch: none where there is one
+// row, or under a sliding window (each row then streams its own window).
+struct Group {
+  int first, rows, prefix;
+};
+// What a row streams of its own: positions [from, ctx), through its own table from position
+// `border` on and through its group's first row's before.
+struct Own {
+  int from, ctx, border, first_row, tiles, pad_;
+  int64_t start;  // on the own line (filled where the line is walked)
+};
 
-template <int kG, int D, bool kFp8>
-__global__ __launch_bounds__((page_attn_waves<kG, D>() * 64))
-__attribute__((amdgpu_waves_per_eu(2))) void shared_prefix_kernel(
+__device__ __forceinline__ int tiles_in(int tokens) {
+  return tokens > 0 ? (tokens - 1) / kTile + 1 : 0;
+}
+__device__ __forceinline__ int64_t lane64(int64_t v, int src) {
+  const uint32_t lo = __builtin_amdgcn_readlane(static_cast<int>(v), src);
+  const uint32_t hi = __builtin_amdgcn_readlane(static_cast<int>(v >> 32), src);
+  return static_cast<int64_t>((static_cast<uint64_t>(hi) << 32) | lo);
+}
+// Inclusive sums over the lanes of a wave.
+__device__ __forceinline__ int64_t scan64(int64_t v, int lane) {
+#pragma unroll 1
+  for (int off = 1; off < 64; off <<= 1) {
+    const int64_t y = __shfl_up(v, off, 64);
+    if (lane >= off) v += y;
+  }
+  return v;
+}
+// How a line of `total` tiles in `items` items is cut into at most n ranges of `range` tiles (a
+// multiple of `quantum`); pad: items take whole ranges, which may add one range each.
+struct Cut {
+  int64_t range;
+  bool pad;
+  __device__ __forceinline__ Cut(int64_t total, int64_t items, int n, int quantum) {
+    pad = items <= n / 2;
+    // (the quotient is off by less than the one that is added)
+    range = static_cast<int64_t>(static_cast<double>(total) /
+                                 static_cast<double>(pad ? n - items : n)) + 1;
+    range = (range + quantum - 1) / quantum * quantum;
+  }
+  __device__ __forceinline__ int64_t step(int tiles) const {
+    return pad ? (tiles + range - 1) / range * range : tiles;
+  }
+};
+// The share of a line that work-group `wg` of n takes, when it has `shares` of them (n or more:
+// none).  They are dealt out to the 8 XCDs in runs (work-groups go to XCDs in turn), so that
+// neighbouring ranges, which read the same keys for the column blocks of a group, share an L2;
+// `last`: the work-groups are counted from the end.
+__device__ __forceinline__ int64_t share_of(int wg, int n, int64_t shares, bool last) {
+  if (n % 8) return last ? n - 1 - wg : wg;
+  const int per = static_cast<int>(shares + 7) / 8;
+  const int i = last ? n / 8 - 1 - (wg >> 3) : wg >> 3;
+  return i < per ? (wg & 7) * per + i : n;
+}
+__device__ __forceinline__ int uniform(int v) { return __builtin_amdgcn_readfirstlane(v); }
+
+// LDS: the merge's states (also the last work-group's tables), a chunk of rows, the groups.
+template <int D>
+constexpr int lds_rows_at() { return 4 * merge_lds_floats<kWaves, D>(cols_of(D)); }
+template <int D>
+constexpr int lds_groups_at() { return lds_rows_at<D>() + kThreads * static_cast<int>(sizeof(Own)); }
+static_assert(kMaxGroups * 12 <= lds_groups_at<64>(), "the last work-group's tables fit");
+
+template <int D, bool kFp8>
+__global__ __launch_bounds__(kThreads)
+__attribute__((amdgpu_waves_per_eu((D == 256 ? 1 : 2)))) void shared_prefix_kernel(
     PrefixParams P, const int32_t* __restrict__ bt, const int32_t* __restrict__ ctx_lens,
     const int32_t* __restrict__ cu_groups, const int32_t* __restrict__ prefix_lens) {
-  constexpr int kWaves = page_attn_waves<kG, D>();
-  constexpr int U = D == 64 ? 4 : D == 128 ? 2 : 1;
-  __shared__ __align__(16) float lds[merge_lds_floats<kG, D>()];
+  constexpr int kCB = col_blocks_of<D>();
+  constexpr int kCols = 16 * kCB;
+  extern __shared__ __align__(16) uint8_t lds_all[];
+  __shared__ int64_t wave_sum[kWaves];
+  __shared__ uint64_t wave_hits[kWaves];
+  float* const lds = reinterpret_cast<float*>(lds_all);
+  Own* const own_rows = reinterpret_cast<Own*>(lds_all + lds_rows_at<D>());
+  int* const group_first = reinterpret_cast<int*>(lds_all + lds_groups_at<D>());
+  int* const group_prefix = group_first + P.num_groups + 1;
   const PageAttnParams& A = P.A;
-  const int b = blockIdx.y;
-  const int kvh = blockIdx.x / A.col_blocks;
-  const int qbase = kvh * A.gqa + 16 * (blockIdx.x - kvh * A.col_blocks);
-  const int ncols = min(16, (kvh + 1) * A.gqa - qbase);
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int lane = threadIdx.x & 63;
   const int r = lane & 15, g = lane >> 4;
-  const int grp = group_of(cu_groups, P.num_groups, b);
-  const int prefix = grp >= 0 ? prefix_lens[grp] : 0;
-  const int64_t first_row = grp >= 0 ? max(cu_groups[grp], 0) : b;
-  const int ctx = max(ctx_lens[b], 0);
-  const int lo = P.window_left >= 0 ? max(0, ctx - 1 - P.window_left) : 0;
-  ColumnState<kG, D, kFp8> st;
-  st.init(A.q + b * A.q_row_stride + static_cast<int64_t>(qbase + r) * D, r < ncols, g);
-  const float ks = kFp8 && A.k_scale ? A.k_scale[kvh] : 1.f;
-  const float vsc = kFp8 && A.v_scale ? A.v_scale[kvh] : 1.f;
   const int tok_log2 = 4 + P.unit_tiles_log2;
-  const int32_t* own = bt + b * A.bt_row_stride;
-  const int32_t* shared = bt + first_row * A.bt_row_stride;
-  // Two passes over the units: positions below the prefix through the group's table, the
-  // others through the row's own (a unit across the border is masked in each).
-  const int border = min(prefix > 0 ? prefix : 0, ctx);
-  for (int pass = 0; pass < 2; ++pass) {
-    const int from = max(lo, pass ? border : 0), to = pass ? ctx : border;
-    if (from >= to) continue;
+  // Row and head indexes, and so every address formed from them, stay inside the batch
+  // whatever the groups say.
+  for (int i = threadIdx.x; i <= P.num_groups; i += kThreads) {
+    group_first[i] = min(max(cu_groups[i], 0), A.batch);
+    if (i < P.num_groups) {
+      const int64_t most = static_cast<int64_t>(A.bt_width) << A.block_size_log2;
+      group_prefix[i] =
+          static_cast<int>(min(static_cast<int64_t>(max(prefix_lens[i], 0)), most));
+    }
+  }
+  __syncthreads();
+  auto group_at = [&](int i) {
+    Group x{0, 0, 0};
+    if (i >= P.num_groups) return x;
+    x.first = group_first[i];
+    x.rows = group_first[i + 1] - x.first;
+    x.prefix = x.rows > 1 && P.window_left < 0 ? group_prefix[i] : 0;
+    return x;
+  };
+  // Items (kv heads x column blocks) of a group and the tiles of each.
+  auto group_items = [&](const Group& x) {
+    return x.prefix > 0 ? A.num_kv_heads * ((x.rows * A.gqa + kCols - 1) / kCols) : 0;
+  };
+  // The group that holds row b (the last one with first <= b), or -1.
+  auto group_of = [&](int b) {
+    if (P.num_groups <= 0 || b < group_first[0] || b >= group_first[P.num_groups]) return -1;
+    int lo = 0, hi = P.num_groups;
+    while (hi - lo > 1) {
+      const int mid = (lo + hi) >> 1;
+      if (group_first[mid] <= b) lo = mid; else hi = mid;
+    }
+    return lo;
+  };
+  auto own_at = [&](int b) {
+    Own w{};
+    if (b >= A.batch) return w;
+    w.ctx = max(ctx_lens[b], 0);
+    const int grp = group_of(b);
+    w.first_row = b;
+    w.from = P.window_left >= 0 ? max(0, w.ctx - 1 - P.window_left) : 0;
+    if (grp >= 0) {
+      const Group x = group_at(grp);
+      w.border = min(group_prefix[grp], w.ctx);
+      w.first_row = x.first;
+      if (x.prefix > 0) w.from = w.border;
+    }
+    // counted from the tile of `from`
+    w.tiles = w.ctx > w.from ? (w.ctx - 1) / kTile - w.from / kTile + 1 : 0;
+    return w;
+  };
+  // Inclusive sums over the work-group's threads; total: over all of them.
+  auto scan_all = [&](int64_t v, int64_t& total) {
+    const int64_t x = scan64(v, lane);
+    if (lane == 63) wave_sum[wave] = x;
+    __syncthreads();
+    int64_t before = 0;
+    total = 0;
+#pragma unroll
+    for (int w = 0; w < kWaves; ++w) {
+      before += w < wave ? wave_sum[w] : 0;
+      total += wave_sum[w];
+    }
+    __syncthreads();
+    return before + x;
+  };
+  auto prefix_cut = [&] {
+    int64_t sum = 0, n = 0;
+    for (int i = lane; i < P.num_groups; i += 64) {
+      const Group x = group_at(i);
+      sum += static_cast<int64_t>(group_items(x)) * tiles_in(x.prefix);
+      n += group_items(x);
+    }
+    return Cut(lane64(scan64(sum, lane), 63), lane64(scan64(n, lane), 63), P.wgs, kPreTiles);
+  };
+  // Streams positions [from, to) of one item through the table `table`: unit `first` and every
+  // step-th after it.
+  auto stream = [&](auto& st, const int32_t* table, int from, int to, int first, int step,
+                    auto limits, int kvh, float s2) {
     const int u0 = from >> tok_log2;
-    const int32_t* table = pass ? own : shared;
     auto unit_at = [&](int u, int& page, int& tok) {
       tok = (u0 + u) << tok_log2;
       const int j = tok >> A.block_size_log2;
       page = j < A.bt_width ? table[j] : -1;
     };
-    stream_units<kG, D, kFp8, U>(A, st, unit_at, ((to - 1) >> tok_log2) + 1 - u0, wave, kWaves,
-                                 P.unit_tiles_log2, from, to, kvh, ks, lane);
+    stream_units(A, st, unit_at, from < to ? ((to - 1) >> tok_log2) + 1 - u0 : 0, first, step,
+                 P.unit_tiles_log2, from, to, limits, kvh, s2, lane);
+  };
+  auto factor = [&](int kvh) {
+    return kFp8 && A.k_scale ? A.scale_log2 * A.k_scale[kvh] : A.scale_log2;
+  };
+
+  const int wg = blockIdx.x;
+  auto run_prefix = [&] {
+    const Cut cut = prefix_cut();
+    const int64_t S = cut.range;
+    // (all ranges, each of them some work-group's: those past the line's end are empty)
+    int64_t line = 0;  // tiles and items of the groups before the chunk
+    int64_t item0 = 0;
+    int64_t total = 0;
+    for (int i = lane; i < P.num_groups; i += 64) {
+      const Group x = group_at(i);
+      total += group_items(x) * cut.step(tiles_in(x.prefix));
+    }
+    total = lane64(scan64(total, lane), 63);
+    const int64_t w = share_of(wg, P.wgs, (total + S - 1) / S, false);
+    const int64_t t_lo = w * S, t_hi = min(total, t_lo + S);
+    for (int g0 = 0; t_lo < total && g0 < P.num_groups && line < t_hi; g0 += 64) {
+      const Group x = group_at(g0 + lane);
+      const int items = group_items(x);
+      const int64_t mine = items * cut.step(tiles_in(x.prefix));
+      const int64_t end = line + scan64(mine, lane);
+      const int64_t item_end = item0 + scan64(items, lane);
+      uint64_t hit = __ballot(mine > 0 && end > t_lo && end - mine < t_hi);
+      while (hit) {
+        const int src = __builtin_ctzll(hit);
+        hit &= hit - 1;
+        const int row0 = __builtin_amdgcn_readlane(x.first, src);
+        const int n_cols = __builtin_amdgcn_readlane(x.rows, src) * A.gqa;
+        const int prefix = __builtin_amdgcn_readlane(x.prefix, src);
+        const int n_items = __builtin_amdgcn_readlane(items, src);
+        const int64_t start = lane64(end - mine, src);
+        const int64_t first_item = lane64(item_end, src) - n_items;
+        const int64_t step = cut.step(tiles_in(prefix));
+        const int col_items = n_items / A.num_kv_heads;
+        for (int it = t_lo > start ? static_cast<int>((t_lo - start) / step) : 0;
+             it < n_items && start + it * step < t_hi; ++it) {
+          const int64_t at = start + it * step;
+          const int from = static_cast<int>(
+              min(static_cast<int64_t>(prefix), (max(t_lo, at) - at) * kTile));
+          const int to = static_cast<int>(
+              min(static_cast<int64_t>(prefix), (min(t_hi, at + step) - at) * kTile));
+          if (from >= to) continue;
+          const int kvh = it / col_items;
+          const int col0 = (it - kvh * col_items) * kCols;
+          const float s2 = factor(kvh);
+          ColumnState<kCB, D, kFp8> st;
+          st.reset();
+          int seen[kCB];  // keys of this lane's column, all of them for a column that is none
+#pragma unroll
+          for (int cb = 0; cb < kCB; ++cb) {
+            const int c = col0 + 16 * cb + r;
+            const bool ok = c < n_cols;
+            const int b = row0 + (ok ? c / A.gqa : 0);
+            const int hq = kvh * A.gqa + (ok ? c % A.gqa : 0);
+            seen[cb] = ok ? ctx_lens[b] : -1;
+            st.load_q(cb, A.q + b * A.q_row_stride + static_cast<int64_t>(hq) * D, ok,
+                      s2 < 0.f ? 0x80008000u : 0u, g);
+          }
+          auto limits = [&] {
+            Limits<kCB> x;
+            x.span = 0;
+            x.least = to - from;
+#pragma unroll
+            for (int cb = 0; cb < kCB; ++cb) {
+              const bool ok = col0 + 16 * cb + r < n_cols;
+              x.lim[cb] = ok ? max(min(to, seen[cb]) - from, 0) : to - from;
+              x.span = max(x.span, ok ? x.lim[cb] : 0u);
+              x.least = min(x.least, x.lim[cb]);
+            }
+#pragma unroll
+            for (int off = 1; off < 16; off <<= 1) {
+              x.span = max(x.span, static_cast<uint32_t>(__shfl_xor(x.span, off, 64)));
+              x.least = min(x.least, static_cast<uint32_t>(__shfl_xor(x.least, off, 64)));
+            }
+            x.span = uniform(x.span);
+            x.least = uniform(x.least);
+            return x;
+          };
+          stream(st, bt + row0 * A.bt_row_stride, from, to, wave, kWaves, limits, kvh,
+                 __builtin_fabsf(s2));
+          const int64_t piece = w + first_item + it;
+          if (piece >= P.pre_pieces) continue;  // (groups that overlap: beyond the plan)
+          float* po = P.pre_o + piece * kCols * D;
+          float* pm = P.pre_ml + piece * kCols * 2;
+          merge_waves<kWaves>(st, lds, wave, lane, min(kCols, n_cols - col0),
+                              [&](int j, int dim, const float4& o, float M, float L) {
+                                *reinterpret_cast<float4*>(po + j * D + dim) = o;
+                                if (dim == 0)
+                                  *reinterpret_cast<float2*>(pm + 2 * j) = make_float2(M, L);
+                              });
+          __syncthreads();
+        }
+      }
+      line = lane64(end, 63);
+      item0 = lane64(item_end, 63);
+    }
+  };
+
+  // The own line: a wave's range is one of 4 wgs.
+  const Own own0 = own_at(threadIdx.x);
+  int64_t own_total;
+  {
+    int64_t sum = own0.tiles;
+    for (int b = kThreads + threadIdx.x; b < A.batch; b += kThreads) sum += own_at(b).tiles;
+    scan_all(sum, own_total);
   }
-  merge_waves(st, lds, wave, lane, ncols, [&](int j, int dim, float x, float y, float M, float L) {
-    write_pair(A, b, qbase + j, D, dim, x, y, M, L, vsc);
-  });
+  const Cut own_cut(own_total * P.vheads, static_cast<int64_t>(A.batch) * P.vheads,
+                    kWaves * P.wgs, kOwnTiles);
+  if (own_cut.pad) {
+    int64_t sum = own_cut.step(own0.tiles);
+    for (int b = kThreads + threadIdx.x; b < A.batch; b += kThreads)
+      sum += own_cut.step(own_at(b).tiles);
+    scan_all(sum, own_total);
+  }
+  own_total *= P.vheads;
+
+  auto run_own = [&] {
+    const int64_t S = own_cut.range;
+    const int64_t w0 =
+        kWaves * share_of(wg, P.wgs, (own_total + kWaves * S - 1) / (kWaves * S), true);
+    const int64_t all_hi = min(own_total, (w0 + kWaves) * S);  // of the work-group
+    const int64_t w = w0 + wave;
+    const int64_t t_lo = w * S, t_hi = min(own_total, t_lo + S);
+    int64_t line = 0;
+    for (int b0 = 0; w0 * S < own_total && b0 < A.batch && line < all_hi; b0 += kThreads) {
+      Own o = b0 == 0 ? own0 : own_at(b0 + threadIdx.x);
+      const int64_t mine = own_cut.step(o.tiles) * P.vheads;
+      int64_t sum;
+      const int64_t end = line + scan_all(mine, sum);
+      line += sum;
+      o.start = end - mine;
+      const bool in = mine > 0 && end > w0 * S && o.start < all_hi;
+      if (in) own_rows[threadIdx.x] = o;
+      const uint64_t hits = __ballot(in);
+      if (lane == 0) wave_hits[wave] = hits;
+      __syncthreads();
+#pragma unroll 1
+      for (int k = 0; k < kWaves; ++k) {
+        uint64_t hit = lane64(wave_hits[k], 0);
+        while (hit) {
+          const int src = 64 * k + __builtin_ctzll(hit);
+          hit &= hit - 1;
+          const int b = b0 + src;
+          Own x = own_rows[src];
+          x.from = uniform(x.from);
+          x.ctx = uniform(x.ctx);
+          x.border = uniform(x.border);
+          x.first_row = uniform(x.first_row);
+          x.tiles = uniform(x.tiles);
+          x.start = lane64(x.start, 0);
+          const int64_t step = own_cut.step(x.tiles);
+          const int tile0 = x.from / kTile;
+          for (int v = t_lo > x.start ? static_cast<int>((t_lo - x.start) / step) : 0;
+               v < P.vheads && x.start + v * step < t_hi; ++v) {
+            const int64_t at = x.start + v * step;
+            const int64_t k_lo = max(t_lo, at) - at, k_hi = min(t_hi, at + step) - at;
+            if (k_lo >= x.tiles) continue;
+            const int from = max(x.from, kTile * (tile0 + static_cast<int>(k_lo)));
+            const int to = static_cast<int>(
+                min(static_cast<int64_t>(x.ctx), (tile0 + k_hi) * int64_t{kTile}));
+            const int kvh = v / A.col_blocks;
+            const int qbase = kvh * A.gqa + 16 * (v - kvh * A.col_blocks);
+            const int nc = min(16, (kvh + 1) * A.gqa - qbase);
+            const float s2 = factor(kvh);
+            ColumnState<1, D, kFp8> st;
+            st.reset();
+            st.load_q(0, A.q + b * A.q_row_stride + static_cast<int64_t>(qbase + r) * D, r < nc,
+                      s2 < 0.f ? 0x80008000u : 0u, g);
+            // before the border through the group's table, then through the row's own
+            const int mid = min(max(x.border, from), to);
+#pragma unroll 1
+            for (int own = mid > from ? 0 : 1; own < 2; ++own) {
+              const int lo = own ? mid : from, hi = own ? to : mid;
+              const uint32_t span = hi - lo;
+              stream(st, bt + (own ? b : x.first_row) * A.bt_row_stride, lo, hi, 0, 1,
+                     [&] { return Limits<1>{{span}, span, span}; }, kvh, __builtin_fabsf(s2));
+            }
+            const int64_t piece = w + static_cast<int64_t>(b) * P.vheads + v;
+            write_partial(st, P.own_o + piece * P.own_cols * D, P.own_ml + piece * P.own_cols * 2,
+                          lane, nc);
+          }
+        }
+      }
+      __syncthreads();
+    }
+  };
+
+  if (wg == P.wgs) {
+    // The last work-group writes the merge's records: first each group's place on the prefix
+    // line, into LDS, then the rows'.
+    int64_t* const pre_start = reinterpret_cast<int64_t*>(lds_all);
+    int* const pre_item = reinterpret_cast<int*>(pre_start + P.num_groups);
+    const Cut pre_cut = prefix_cut();
+    if (wave == 0) {
+      int64_t line = 0, item0 = 0;
+      for (int g0 = 0; g0 < P.num_groups; g0 += 64) {
+        const Group x = group_at(g0 + lane);
+        const int items = group_items(x);
+        const int64_t mine = items * pre_cut.step(tiles_in(x.prefix));
+        const int64_t end = line + scan64(mine, lane);
+        const int64_t item_end = item0 + scan64(items, lane);
+        if (g0 + lane < P.num_groups) {
+          pre_start[g0 + lane] = end - mine;
+          pre_item[g0 + lane] = static_cast<int>(item_end) - items;
+        }
+        line = lane64(end, 63);
+        item0 = lane64(item_end, 63);
+      }
+    }
+    __syncthreads();
+    int64_t line = 0;
+    for (int b0 = 0; b0 < A.batch; b0 += kThreads) {
+      const int b = b0 + threadIdx.x;
+      const Own o = own_at(b);
+      const int64_t mine = own_cut.step(o.tiles) * P.vheads;
+      int64_t sum;
+      const int64_t end = line + scan_all(mine, sum);
+      line += sum;
+      if (b >= A.batch) continue;
+      RowRecord rec{};
+      rec.own_start = end - mine;
+      rec.own_range = own_cut.range;
+      rec.own_step = own_cut.step(o.tiles);
+      rec.own_tiles = o.tiles;
+      rec.pre_range = pre_cut.range;
+      const int grp = group_of(b);
+      if (grp >= 0) {
+        const Group x = group_at(grp);
+        rec.pre_start = pre_start[grp];
+        rec.pre_tiles = tiles_in(x.prefix);
+        rec.pre_step = pre_cut.step(rec.pre_tiles);
+        rec.pre_item = pre_item[grp];
+        rec.col_items = group_items(x) / A.num_kv_heads;
+        rec.index = b - x.first;
+      }
+      P.rows[b] = rec;
+    }
+    return;
+  }
+  const bool prefix_first = wg < P.wgs / 2;
+#pragma unroll 1
+  for (int phase = 0; phase < 2; ++phase) {
+    if ((phase == 0) == prefix_first)
+      run_prefix();
+    else
+      run_own();
+  }
 }
 
-template <int kG, int D>
-void launch_fp8(bool fp8, const PrefixParams& P, dim3 grid, hipStream_t s, const int32_t* bt,
-                const int32_t* ctx, const int32_t* cu, const int32_t* pre) {
-  const dim3 block(page_attn_waves<kG, D>() * 64);
-  if (fp8)
-    hipLaunchKernelGGL((shared_prefix_kernel<kG, D, true>), grid, block, 0, s, P, bt, ctx, cu,
-                       pre);
-  else
-    hipLaunchKernelGGL((shared_prefix_kernel<kG, D, false>), grid, block, 0, s, P, bt, ctx, cu,
-                       pre);
-}
+// One work-group per (row, kv head, block of 16 query heads).  A thread folds four dims of a
+// column; where the columns leave threads over, the pieces are dealt out among them and the
+// threads' states folded through LDS.
+constexpr int kMergeThreads = 256;
+constexpr int kMergeAhead = 4;  // pieces whose loads are in flight
 template <int D>
-void launch_d(bool fp8, const PrefixParams& P, dim3 grid, hipStream_t s, const int32_t* bt,
+__global__ __launch_bounds__(kMergeThreads) void shared_prefix_merge_kernel(PrefixParams P,
+                                                                            int fp8) {
+  constexpr int kCols = cols_of(D);
+  __shared__ Folded folded[kMergeThreads];
+  const PageAttnParams& A = P.A;
+  const int b = blockIdx.y, v = blockIdx.x;
+  const int kvh = v / A.col_blocks;
+  const int in_group = 16 * (v - kvh * A.col_blocks);  // first query head, of the group
+  const int nc = min(16, A.gqa - in_group);
+  const RowRecord rec = P.rows[b];
+  const float vsc = fp8 && A.v_scale ? A.v_scale[kvh] : 1.f;
+  const int items = nc * (D / 4);
+  const int slices = max(1, kMergeThreads / items);
+  // The row's pieces on its own line: ranges w0, w0 + 1, ...
+  const int64_t own_at = rec.own_start + v * rec.own_step;
+  const int64_t own_w = rec.own_tiles ? own_at / rec.own_range : 0;
+  const int own_n = rec.own_tiles
+                        ? static_cast<int>((own_at + rec.own_tiles - 1) / rec.own_range - own_w) + 1
+                        : 0;
+  const int64_t own_col = (own_w + static_cast<int64_t>(b) * P.vheads + v) * P.own_cols;
+  for (int x0 = 0; x0 < items; x0 += kMergeThreads) {
+    const int x = x0 + static_cast<int>(threadIdx.x) % (slices > 1 ? items : kMergeThreads);
+    const int slice = slices > 1 ? threadIdx.x / items : 0;
+    const bool ok = x < items && slice < slices;
+    const int j = x / (D / 4), dim = 4 * (x % (D / 4));
+    Folded f;
+    f.reset();
+    if (ok) {
+      // ... and on the prefix line, for this column
+      int pre_n = 0;
+      int64_t pre_col = 0;
+      if (rec.pre_tiles > 0) {
+        const int c = rec.index * A.gqa + in_group + j;
+        const int it = kvh * rec.col_items + c / kCols;
+        const int64_t at = rec.pre_start + it * rec.pre_step;
+        const int64_t w = at / rec.pre_range;
+        const int64_t first = w + rec.pre_item + it;
+        pre_n = static_cast<int>(
+            min((at + rec.pre_tiles - 1) / rec.pre_range - w + 1, P.pre_pieces - first));
+        pre_col = first * kCols + c % kCols;
+      }
+      const int n = pre_n + own_n;
+      for (int k0 = slice; k0 < n; k0 += kMergeAhead * slices) {
+        float2 s[kMergeAhead];
+        float4 o[kMergeAhead];
+#pragma unroll
+        for (int u = 0; u < kMergeAhead; ++u) {
+          const int k = min(k0 + u * slices, n - 1);
+          const bool pre = k < pre_n;
+          const int64_t col = pre ? pre_col + static_cast<int64_t>(k) * kCols
+                                  : own_col + static_cast<int64_t>(k - pre_n) * P.own_cols + j;
+          s[u] = *reinterpret_cast<const float2*>((pre ? P.pre_ml : P.own_ml) + 2 * col);
+          o[u] = *reinterpret_cast<const float4*>((pre ? P.pre_o : P.own_o) + col * D + dim);
+        }
+#pragma unroll
+        for (int u = 0; u < kMergeAhead; ++u)
+          if (k0 + u * slices < n) f.add(s[u].x, s[u].y, o[u]);
+      }
+    }
+    if (slices > 1) {
+      folded[threadIdx.x] = f;
+      __syncthreads();
+      if (slice == 0)
+        for (int u = 1; u < slices; ++u) {
+          const Folded& y = folded[x + u * items];
+          f.add(y.M, y.L, y.o);
+        }
+    }
+    if (ok && slice == 0) write_quad(A, b, kvh * A.gqa + in_group + j, D, dim, f.o, f.M, f.L, vsc);
+  }
+}
+
+// Work-groups and workspace of a launch.
+struct PrefixPlan {
+  int wgs;
+  int64_t pre_pieces, own_pieces;
+  int64_t pre_o, pre_ml, own_o, own_ml, rows, bytes;  // offsets
+};
+PrefixPlan plan_of(int64_t batch, int64_t groups, int num_heads, int num_kv_heads,
+                   int head_size) {
+  PrefixPlan p{};
+  const int gqa = num_heads / num_kv_heads;
+  const int64_t cols = cols_of(head_size);
+  const int64_t vheads = static_cast<int64_t>(num_kv_heads) * ((gqa + 15) / 16);
+  const int own_cols = gqa < 16 ? gqa : 16;
+  // Two work-groups per CU where the registers leave room for them.
+  p.wgs = num_cus() * (head_size == 256 ? 1 : 2);
+  // A group that shares has two rows at the least, and rounds its columns up once.
+  const int64_t shared = groups < batch / 2 ? groups : batch / 2;
+  if (shared > 0) p.pre_pieces = p.wgs + num_kv_heads * (batch * gqa / cols + shared);
+  p.own_pieces = kWaves * p.wgs + batch * vheads;
+  auto take = [&](int64_t bytes) {
+    const int64_t at = p.bytes;
+    p.bytes += (bytes + 255) / 256 * 256;
+    return at;
+  };
+  p.pre_o = take(p.pre_pieces * cols * head_size * 4);
+  p.pre_ml = take(p.pre_pieces * cols * 8);
+  p.own_o = take(p.own_pieces * own_cols * head_size * 4);
+  p.own_ml = take(p.own_pieces * own_cols * 8);
+  p.rows = take(batch * static_cast<int64_t>(sizeof(RowRecord)));
+  return p;
+}
+
+template <int D>
+void launch_d(bool fp8, const PrefixParams& P, hipStream_t s, const int32_t* bt,
               const int32_t* ctx, const int32_t* cu, const int32_t* pre) {
-  if (P.A.gqa <= 4)
-    launch_fp8<4, D>(fp8, P, grid, s, bt, ctx, cu, pre);
-  else if (P.A.gqa <= 8)
-    launch_fp8<8, D>(fp8, P, grid, s, bt, ctx, cu, pre);
+  const dim3 grid(static_cast<unsigned>(P.wgs + 1));
+  const unsigned lds = lds_groups_at<D>() + 4 * (2 * P.num_groups + 1);
+  if (fp8)
+    hipLaunchKernelGGL((shared_prefix_kernel<D, true>), grid, dim3(kThreads), lds, s, P, bt, ctx,
+                       cu, pre);
   else
-    launch_fp8<16, D>(fp8, P, grid, s, bt, ctx, cu, pre);
+    hipLaunchKernelGGL((shared_prefix_kernel<D, false>), grid, dim3(kThreads), lds, s, P, bt, ctx,
+                       cu, pre);
+  hipLaunchKernelGGL((shared_prefix_merge_kernel<D>),
+                     dim3(static_cast<unsigned>(P.vheads), static_cast<unsigned>(P.A.batch)),
+                     dim3(kMergeThreads), 0, s, P, fp8 ? 1 : 0);
 }
 
 }  // namespace
@@ -122,8 +636,8 @@ extern "C" int fk_shared_prefix_decode(
                               num_heads, num_kv_heads, head_size, block_size, num_blocks, scale,
                               sinks))
     return rc;
-  FK_REQUIRE(num_groups >= 0 && num_groups <= INT_MAX, "%s: %lld groups", what,
-             static_cast<long long>(num_groups));
+  FK_REQUIRE(num_groups >= 0 && num_groups <= kMaxGroups, "%s: %lld groups outside [0, %d]", what,
+             static_cast<long long>(num_groups), kMaxGroups);
   FK_REQUIRE(max_prefix_len >= 0, "%s: max_prefix_len %lld", what,
              static_cast<long long>(max_prefix_len));
   FK_REQUIRE(window_left >= -1, "%s: window_left %d must be -1 or >= 0", what, window_left);
@@ -131,21 +645,34 @@ extern "C" int fk_shared_prefix_decode(
   FK_REQUIRE(out && q && k_cache && v_cache && block_tables && cache_seqlens &&
                  (num_groups == 0 || (cu_groups && prefix_lens)),
              "%s: null pointer", what);
+  const PrefixPlan plan = plan_of(batch, num_groups, num_heads, num_kv_heads, head_size);
+  if (workspace_bytes < plan.bytes || !workspace)
+    return set_error(FK_ERR_WORKSPACE, "%s: workspace of %lld bytes, %lld needed", what,
+                     static_cast<long long>(workspace_bytes), static_cast<long long>(plan.bytes));
+  FK_REQUIRE(aligned16(workspace), "%s: workspace must be 16-byte aligned", what);
+  uint8_t* ws = static_cast<uint8_t*>(workspace);
   PrefixParams P{};
   P.A = A;
   P.num_groups = static_cast<int>(num_groups);
   P.window_left = window_left;
   P.unit_tiles_log2 = A.block_size_log2 - 4 < 2 ? A.block_size_log2 - 4 : 2;
-  const dim3 grid(static_cast<unsigned>(num_kv_heads * A.col_blocks),
-                  static_cast<unsigned>(batch));
+  P.wgs = plan.wgs;
+  P.pre_pieces = plan.pre_pieces;
+  P.vheads = num_kv_heads * A.col_blocks;
+  P.own_cols = A.gqa < 16 ? A.gqa : 16;
+  P.pre_o = reinterpret_cast<float*>(ws + plan.pre_o);
+  P.pre_ml = reinterpret_cast<float*>(ws + plan.pre_ml);
+  P.own_o = reinterpret_cast<float*>(ws + plan.own_o);
+  P.own_ml = reinterpret_cast<float*>(ws + plan.own_ml);
+  P.rows = reinterpret_cast<RowRecord*>(ws + plan.rows);
   const bool fp8 = kv_dtype == FK_DTYPE_FP8_E4M3FN;
   hipStream_t s = as_stream(stream);
   if (head_size == 64)
-    launch_d<64>(fp8, P, grid, s, block_tables, cache_seqlens, cu_groups, prefix_lens);
+    launch_d<64>(fp8, P, s, block_tables, cache_seqlens, cu_groups, prefix_lens);
   else if (head_size == 128)
-    launch_d<128>(fp8, P, grid, s, block_tables, cache_seqlens, cu_groups, prefix_lens);
+    launch_d<128>(fp8, P, s, block_tables, cache_seqlens, cu_groups, prefix_lens);
   else
-    launch_d<256>(fp8, P, grid, s, block_tables, cache_seqlens, cu_groups, prefix_lens);
+    launch_d<256>(fp8, P, s, block_tables, cache_seqlens, cu_groups, prefix_lens);
   return check_launch(what);
 }
 
@@ -154,6 +681,10 @@ extern "C" int fk_shared_prefix_decode_plan(int64_t batch, int64_t num_groups,
                                             int num_kv_heads, int head_size,
                                             int64_t* workspace_bytes) {
   FK_REQUIRE(workspace_bytes, "fk_shared_prefix_decode_plan: null output pointer");
-  *workspace_bytes = 0;
+  FK_REQUIRE(batch >= 0 && batch <= 65535 && num_groups >= 0 && max_prefix_len >= 0 &&
+                 num_kv_heads > 0 && num_heads > 0 && num_heads % num_kv_heads == 0,
+             "fk_shared_prefix_decode_plan: invalid argument");
+  *workspace_bytes = batch == 0 ? 0
+                                : plan_of(batch, num_groups, num_heads, num_kv_heads, head_size).bytes;
   return FK_OK;
 }

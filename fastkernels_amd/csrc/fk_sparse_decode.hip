@@ -23,14 +23,24 @@ struct SparseParams {
   int unit_tiles_log2;
 };
 
-template <int kG, int D, bool kFp8>
-__global__ __launch_bounds__((page_attn_waves<kG, D>() * 64))
-__attribute__((amdgpu_waves_per_eu(2))) void sparse_decode_kernel(
+// Waves of a work-group.  At head size 256 the query, a step's K and V rows and O take more
+// than the 256 registers that two waves a SIMD leave: one runs there, with as much in flight.
+#ifndef XW
+#define XW 4
+#endif
+#ifndef XEU
+#define XEU 2
+#endif
+template <int D>
+constexpr int waves_of() { return D == 256 ? 4 : XW; }
+
+template <int D, bool kFp8>
+__global__ __launch_bounds__((waves_of<D>() * 64))
+__attribute__((amdgpu_waves_per_eu((D == 256 ? 1 : XEU)))) void sparse_decode_kernel(
     SparseParams P, const int32_t* __restrict__ bt, const int32_t* __restrict__ ctx,
     const int32_t* __restrict__ cu) {
-  constexpr int kWaves = page_attn_waves<kG, D>();
-  constexpr int U = D == 64 ? 4 : D == 128 ? 2 : 1;
-  __shared__ __align__(16) float lds[merge_lds_floats<kG, D>()];
+  constexpr int kWaves = waves_of<D>();
+  extern __shared__ __align__(16) float lds[];  // merge_lds_floats of the group's columns
   const PageAttnParams& A = P.A;
   const int t = blockIdx.y;
   int b, vis;
@@ -41,9 +51,11 @@ __attribute__((amdgpu_waves_per_eu(2))) void sparse_decode_kernel(
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int lane = threadIdx.x & 63;
   const int r = lane & 15, g = lane >> 4;
-  ColumnState<kG, D, kFp8> st;
-  st.init(A.q + t * A.q_row_stride + static_cast<int64_t>(qbase + r) * D, r < ncols, g);
-  const float ks = kFp8 && A.k_scale ? A.k_scale[kvh] : 1.f;
+  ColumnState<1, D, kFp8> st;
+  st.reset();
+  const float s2 = kFp8 && A.k_scale ? A.scale_log2 * A.k_scale[kvh] : A.scale_log2;
+  st.load_q(0, A.q + t * A.q_row_stride + static_cast<int64_t>(qbase + r) * D, r < ncols,
+            s2 < 0.f ? 0x80008000u : 0u, g);
   const float vsc = kFp8 && A.v_scale ? A.v_scale[kvh] : 1.f;
   const int32_t* list = P.indices + t * P.idx_row_stride + kvh * P.idx_head_stride;
   const int32_t* bt_row = bt + b * A.bt_row_stride;
@@ -58,31 +70,31 @@ __attribute__((amdgpu_waves_per_eu(2))) void sparse_decode_kernel(
     page = bt_row[j];
     tok = static_cast<int>(pos);
   };
-  stream_units<kG, D, kFp8, U>(A, st, unit_at, P.keep << per_log2, wave, kWaves,
-                               P.unit_tiles_log2, 0, max(vis, 0), kvh, ks, lane);
-  merge_waves(st, lds, wave, lane, ncols, [&](int j, int dim, float x, float y, float M, float L) {
-    write_pair(A, t, qbase + j, D, dim, x, y, M, L, vsc);
-  });
+  const uint32_t span = static_cast<uint32_t>(max(vis, 0));
+  stream_units(A, st, unit_at, P.keep << per_log2, wave, kWaves, P.unit_tiles_log2, 0,
+               max(vis, 0), [&] { return Limits<1>{{span}, span, span}; }, kvh,
+               __builtin_fabsf(s2), lane);
+  merge_waves<kWaves>(st, lds, wave, lane, ncols,
+                      [&](int j, int dim, const float4& o, float M, float L) {
+                        write_quad(A, t, qbase + j, D, dim, o, M, L, vsc);
+                      });
 }
 
-template <int kG, int D>
-void launch_fp8(bool fp8, const SparseParams& P, dim3 grid, hipStream_t s, const int32_t* bt,
-                const int32_t* ctx, const int32_t* cu) {
-  const dim3 block(page_attn_waves<kG, D>() * 64);
-  if (fp8)
-    hipLaunchKernelGGL((sparse_decode_kernel<kG, D, true>), grid, block, 0, s, P, bt, ctx, cu);
-  else
-    hipLaunchKernelGGL((sparse_decode_kernel<kG, D, false>), grid, block, 0, s, P, bt, ctx, cu);
+template <int D, bool kFp8>
+void launch_t(const SparseParams& P, dim3 grid, hipStream_t s, const int32_t* bt,
+              const int32_t* ctx, const int32_t* cu) {
+  constexpr int kWaves = waves_of<D>();
+  const int cols = P.A.gqa < 16 ? P.A.gqa : 16;
+  hipLaunchKernelGGL((sparse_decode_kernel<D, kFp8>), grid, dim3(kWaves * 64),
+                     (4 * merge_lds_floats<kWaves, D>(cols)), s, P, bt, ctx, cu);
 }
 template <int D>
 void launch_d(bool fp8, const SparseParams& P, dim3 grid, hipStream_t s, const int32_t* bt,
               const int32_t* ctx, const int32_t* cu) {
-  if (P.A.gqa <= 4)
-    launch_fp8<4, D>(fp8, P, grid, s, bt, ctx, cu);
-  else if (P.A.gqa <= 8)
-    launch_fp8<8, D>(fp8, P, grid, s, bt, ctx, cu);
+  if (fp8)
+    launch_t<D, true>(P, grid, s, bt, ctx, cu);
   else
-    launch_fp8<16, D>(fp8, P, grid, s, bt, ctx, cu);
+    launch_t<D, false>(P, grid, s, bt, ctx, cu);
 }
 
 }  // namespace

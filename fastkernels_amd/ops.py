@@ -949,7 +949,7 @@ def shared_prefix_decode(out: torch.Tensor, q: torch.Tensor, k_cache: torch.Tens
                  k_scale, v_scale, sinks)
     if rows == 0:
         return
-    bound = min(int(max_prefix_len) or block_table.shape[1] * bs, block_table.shape[1] * bs)
+    bound = int(max_prefix_len)
     nbytes = _native.shared_prefix_bytes(rows, groups, bound, hq, hk, d)
     ws = torch.empty(nbytes, dtype=torch.uint8, device=q.device) if nbytes else None
     _call_on(q, "fk_shared_prefix_decode", out.data_ptr(), out.stride(0), q.data_ptr(),
