@@ -20,6 +20,8 @@
 namespace fk {
 namespace {
 
+// Keeps the loads before it before it (the compiler may sink them to their first use).
+__device__ __forceinline__ void loads_issued() { asm volatile("" ::: "memory"); }
 // NaN-propagating minimum and maximum.
 __device__ __forceinline__ float min_nan(float a, float b) {
   return __builtin_elementwise_minimum(a, b);
@@ -61,10 +63,8 @@ struct Elems {
   }
   __device__ __forceinline__ static uint32_t pack(const float (&f)[N]) {
     if constexpr (kFp8) {
-      uint32_t w = 0;
-#pragma unroll
-      for (int i = 0; i < 4; ++i) w |= static_cast<uint32_t>(f32_to_e4m3fn_sat(f[i])) << (8 * i);
-      return w;
+      const int lo = __builtin_amdgcn_cvt_pk_fp8_f32(f[0], f[1], 0, false);
+      return static_cast<uint32_t>(__builtin_amdgcn_cvt_pk_fp8_f32(f[2], f[3], lo, true));
     } else {
       return lo_pair(f32_to_bf16(f[0]), f32_to_bf16(f[1]));
     }
@@ -178,15 +178,17 @@ struct ScoreParams {
   int slots_log2;    // column slots per query row: gqa rounded up to a power of two, at most 16
   int block_size_log2;
   int64_t num_blocks;
-  int tiles;         // 16-page tiles per wave
+  int tiles;         // 16-page tiles per wave, at most kScoreTiles
 };
 
 // One wave: 16 pages x 16 columns per MFMA tile.  The columns are 16 / slots query rows of
 // one sequence times the query heads of kv head h (a group that is no power of two repeats
 // its last head, groups above 16 take several passes over the loaded bounds); the rows of
 // the A operand are the pages' bounds, lo then hi, the B operands min(q, 0) and max(q, 0).
+constexpr int kScoreWaves = 8;  // of a work-group, a kv head each: a page's bounds are read whole
+constexpr int kScoreTiles = 4;  // of a wave at most (8: 152 us where 4 take 141)
 template <bool kFp8, int D>
-__global__ __launch_bounds__(256) void block_scores_kernel(
+__global__ __launch_bounds__(kScoreWaves * 64) void block_scores_kernel(
     ScoreParams P, const int32_t* __restrict__ bt, const int32_t* __restrict__ ctx,
     const int32_t* __restrict__ cu) {
   constexpr int kElt = kFp8 ? 1 : 2;
@@ -194,7 +196,7 @@ __global__ __launch_bounds__(256) void block_scores_kernel(
   constexpr int kLoads = kFp8 ? D / 64 : D / 32;
   const int lane = threadIdx.x & 63;
   const int r = lane & 15, g = lane >> 4;
-  const int h = blockIdx.z * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int h = blockIdx.z * (blockDim.x >> 6) + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int b = blockIdx.y / P.token_chunks;
   const int chunk = blockIdx.y - b * P.token_chunks;
   if (h >= P.num_kv_heads) return;
@@ -236,56 +238,66 @@ __global__ __launch_bounds__(256) void block_scores_kernel(
   load_q(0);
   const int32_t* bt_row = bt + b * P.bt_row_stride;
   float* srow = P.scores + static_cast<int64_t>(t0 + i) * P.row_stride + h * P.head_stride;
-  const int tile_end = (P.width + 15) / 16;
   const int tile0 = blockIdx.x * P.tiles;
-  for (int tile = tile0; tile < min(tile0 + P.tiles, tile_end); ++tile) {
-    const int j0 = 16 * tile;
-    float s[4] = {kNegInf, kNegInf, kNegInf, kNegInf};
-    if (j0 < most) {
-      const int entry = j0 + r < most ? bt_row[j0 + r] : -1;
-      const bool page_ok = entry >= 0 && entry < P.num_blocks;
-      const uint32_t ok = static_cast<uint32_t>(__ballot(page_ok)) & 0xffffu;
-      const uint8_t* row = P.bounds +
-                           (static_cast<int64_t>(page_ok ? entry : 0) * P.num_kv_heads + h) * 2 *
-                               D * kElt;
-      uint4 lo[kLoads], hi[kLoads];
+  const int tiles = min(P.tiles, (P.width + 15) / 16 - tile0);
+  const int seen = min(tiles, (most - 16 * tile0 + 15) / 16);  // tiles with pages to read
+  // Lane k holds the table's entry for the wave's page k.
+  static_assert(kScoreTiles * 16 <= 64, "a lane per page");
+  const int my_entry = 16 * tile0 + lane < most ? bt_row[16 * tile0 + lane] : -1;
+  struct Bounds {
+    uint4 lo[kLoads], hi[kLoads];
+    uint32_t ok;  // pages of the tile that can be read
+  };
+  // Issues tile x's loads (row r of a tile is page 16 x + r).
+  auto load = [&](int x, Bounds& t) {
+    const int entry = __shfl(my_entry, 16 * x + r, 64);
+    const bool ok = entry >= 0 && entry < P.num_blocks;
+    const uint8_t* row =
+        P.bounds + (static_cast<int64_t>(ok ? entry : 0) * P.num_kv_heads + h) * 2 * D * kElt;
 #pragma unroll
-      for (int c = 0; c < kLoads; ++c) {
-        const int at = kFp8 ? (D / 4) * g + 16 * c : (32 * c + 8 * g) * 2;
-        lo[c] = ld16(row + at);
-        hi[c] = ld16(row + D * kElt + at);
-      }
+    for (int c = 0; c < kLoads; ++c) {
+      const int at = kFp8 ? (D / 4) * g + 16 * c : (32 * c + 8 * g) * 2;
+      t.lo[c] = ld16(row + at);
+      t.hi[c] = ld16(row + D * kElt + at);
+    }
+    loads_issued();
+    t.ok = static_cast<uint32_t>(__ballot(ok)) & 0xffffu;
+  };
+  // Scores tile x from t, whose registers take the next tile as soon as they are free.
+  auto score = [&](int x, Bounds& t) {
+    const int j0 = 16 * (tile0 + x);
+    float s[4] = {kNegInf, kNegInf, kNegInf, kNegInf};
+    if (x < seen) {
       for (int cb = 0; cb < col_blocks; ++cb) {
-        if (cb > 0 || (col_blocks > 1 && tile > tile0)) load_q(cb);
+        if (cb > 0 || (col_blocks > 1 && x > 0)) load_q(cb);
         uint4 kl[kKc], kh[kKc];
         if constexpr (kFp8) {
           DTile<true, D> a, z;
 #pragma unroll
           for (int c = 0; c < kLoads; ++c) {
-            a.k[c] = lo[c];
-            z.k[c] = hi[c];
+            a.k[c] = t.lo[c];
+            z.k[c] = t.hi[c];
           }
           k_chunks_d(a, kl);
           k_chunks_d(z, kh);
         } else {
 #pragma unroll
           for (int c = 0; c < kKc; ++c) {
-            kl[c] = lo[c];
-            kh[c] = hi[c];
+            kl[c] = t.lo[c];
+            kh[c] = t.hi[c];
           }
         }
-        const floatx4_t x = qk_scores_n(kl, qn), y = qk_scores_n(kh, qp);
+        const floatx4_t u = qk_scores_n(kl, qn), v = qk_scores_n(kh, qp);
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          float v = x[k] + y[k];
-          for (int off = 1; off < slots; off <<= 1) v = max_nan(v, __shfl_xor(v, off, 64));
-          s[k] = cb == 0 ? v : max_nan(s[k], v);
-        }
+        for (int k = 0; k < 4; ++k) s[k] = cb == 0 ? u[k] + v[k] : max_nan(s[k], u[k] + v[k]);
       }
+      const uint32_t cur = t.ok;
+      if (x + 1 < seen) load(x + 1, t);
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
+        for (int off = 1; off < slots; off <<= 1) s[k] = max_nan(s[k], __shfl_xor(s[k], off, 64));
         const int page = 4 * g + k;
-        s[k] = (ok >> page & 1) && j0 + page < nblk ? s[k] * __builtin_fabsf(ks) : kNegInf;
+        s[k] = (cur >> page & 1) && j0 + page < nblk ? s[k] * __builtin_fabsf(ks) : kNegInf;
       }
     }
     if (row_ok && (r & (slots - 1)) == 0) {
@@ -293,7 +305,12 @@ __global__ __launch_bounds__(256) void block_scores_kernel(
       for (int k = 0; k < 4; ++k)
         if (j0 + 4 * g + k < P.width) srow[j0 + 4 * g + k] = s[k];
     }
-  }
+  };
+  // (One tile ahead: with two or three, a call that reads the most, 32 sequences of 16000 ..
+  // 131072 tokens, takes 157 and 168 us instead of 141.)
+  Bounds t;
+  if (seen > 0) load(0, t);
+  for (int x = 0; x < tiles; ++x) score(x, t);
 }
 
 // ---------------------------------------------------------------------------
@@ -310,7 +327,12 @@ struct SelectParams {
   int batch;
 };
 
-constexpr int kSelThreads = 256;
+constexpr int kSelThreads = 512;
+constexpr int kSelBins = 2048;  // 11 bits of a key
+// Keys held in LDS (one word in 17 is left free, so that threads reading runs of keys meet
+// different banks); rows with more pages are read from memory in every pass.
+constexpr int kSelLdsKeys = 32768;
+__host__ __device__ constexpr int sel_at(int j) { return j + (j >> 4); }
 
 // Scores in ascending order of an unsigned key: NaN above all, -0 equal to +0.
 __device__ __forceinline__ uint32_t score_key(float s) {
@@ -319,88 +341,135 @@ __device__ __forceinline__ uint32_t score_key(float s) {
   return u ^ ((u >> 31) ? 0xffffffffu : 0x80000000u);
 }
 
+// Inclusive sum over the work-group's threads; `total`: over all of them.  part: one word per
+// wave, not in use since the barrier before the last.
+__device__ __forceinline__ int scan_threads(int v, int* part, int tid, int& total) {
+  constexpr int kWaves = kSelThreads / 64;
+  const int lane = tid & 63, wave = tid >> 6;
+#pragma unroll
+  for (int off = 1; off < 64; off <<= 1) {
+    const int y = __shfl_up(v, off, 64);
+    if (lane >= off) v += y;
+  }
+  if (lane == 63) part[wave] = v;
+  __syncthreads();
+  int before = 0;
+  total = 0;
+#pragma unroll
+  for (int w = 0; w < kWaves; ++w) {
+    before += w < wave ? part[w] : 0;
+    total += part[w];
+  }
+  return v + before;
+}
+
 // One work-group per (query row, kv head).  The key T of the lowest selected candidate is
-// found digit by digit (8 bits a pass: a histogram of the keys that agree with the digits
-// found so far, then the bin that holds the rank), and the blocks are written in order of
-// their index: the ones always kept, keys above T, and the first of the keys equal to T.
+// found digit by digit (11, 11 and 10 bits: a histogram of the keys that agree with the digits
+// found so far, then the bin that holds the rank), until the rank takes a whole bin.  The blocks
+// are written in order of their index: each thread takes a run of them, counts what is selected
+// there (the blocks always kept, keys above T, and the first of the keys equal to T), and its
+// place is the sum of the counts before it.
+template <bool kLds>
 __global__ __launch_bounds__(kSelThreads) void select_blocks_kernel(
     SelectParams P, const int32_t* __restrict__ ctx, const int32_t* __restrict__ cu) {
-  __shared__ int hist[256];
-  __shared__ int wave_n[2][kSelThreads / 64];
-  __shared__ int found[2];
+  extern __shared__ __align__(16) uint32_t keys[];  // kLds: sel_at(width) words
+  __shared__ int hist[kSelBins];
+  __shared__ int part[2][kSelThreads / 64];
+  __shared__ int found[3];
   const int t = blockIdx.x, h = blockIdx.y;
   int b, vis;
   if (!query_row(cu, ctx, P.batch, t, b, vis)) return;
   const int n = min(pages_of(vis, P.block_size_log2), P.width);
   int32_t* out = P.indices + t * P.out_row_stride + h * P.out_head_stride;
   const float* row = P.scores + t * P.row_stride + h * P.head_stride;
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int tid = threadIdx.x;
   if (n <= P.keep) {
     for (int k = tid; k < P.keep; k += kSelThreads) out[k] = k < n ? k : -1;
     return;
   }
-  const int first = P.keep_first, last = n - P.keep_last;  // candidates [first, last)
-  int need = P.keep - P.keep_first - P.keep_last;
-  uint32_t digits = 0, known = 0;
-  if (need > 0) {
-    for (int shift = 24; shift >= 0; shift -= 8) {
-      hist[tid] = 0;
-      __syncthreads();
-      for (int j = first + tid; j < last; j += kSelThreads) {
-        const uint32_t key = score_key(row[j]);
-        if ((key & known) == digits) atomicAdd(&hist[(key >> shift) & 255], 1);
-      }
-      __syncthreads();
-      // keys in bins above bin tid: the bin where that count passes `need` holds the rank
-      int above = 0;
-      for (int k = tid + 1; k < 256; ++k) above += hist[k];
-      if (above < need && above + hist[tid] >= need) {
-        found[0] = tid;
-        found[1] = need - above;
-      }
-      __syncthreads();
-      digits |= static_cast<uint32_t>(found[0]) << shift;
-      known |= 255u << shift;
-      need = found[1];
-      __syncthreads();
-    }
+  auto key_of = [&](int j) { return kLds ? keys[sel_at(j)] : score_key(row[j]); };
+  if constexpr (kLds) {
+#pragma unroll 4
+    for (int j = tid; j < n; j += kSelThreads) keys[sel_at(j)] = score_key(row[j]);
+    __syncthreads();
   }
-  // need: how many of the keys equal to `digits` are selected.
-  int written = 0, equal = 0;
-  for (int j0 = 0; j0 < n; j0 += kSelThreads) {
-    const int j = j0 + tid;
+  const int first = P.keep_first, last = n - P.keep_last;  // candidates [first, last)
+  int need = P.keep - P.keep_first - P.keep_last;          // of which so many are selected
+  uint32_t digits = 0, known = 0;  // T, and the bits of it that count
+  // (With nothing to select among the candidates T stays above every key.)
+  bool whole = need == 0;
+  if (whole) digits = known = 0xffffffffu;
+  int equal_need = 0;  // of the keys equal to T, the first so many are selected
+  for (int pass = 0; pass < 3 && !whole; ++pass) {
+    const int shift = pass == 0 ? 21 : pass == 1 ? 10 : 0;
+    const uint32_t mask = pass == 2 ? 1023u : 2047u;
+    for (int k = tid; k < kSelBins; k += kSelThreads) hist[k] = 0;
+    __syncthreads();
+#pragma unroll 4
+    for (int j = first + tid; j < last; j += kSelThreads) {
+      const uint32_t key = key_of(j);
+      if ((key & known) == digits) atomicAdd(&hist[(key >> shift) & mask], 1);
+    }
+    __syncthreads();
+    // Thread k sums bins 2047 - 4 k .. 2044 - 4 k: the inclusive sum counts from the top.
+    int bins[4], sum = 0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      bins[i] = hist[kSelBins - 1 - 4 * tid - i];
+      sum += bins[i];
+    }
+    int total;
+    int above = scan_threads(sum, part[0], tid, total) - sum;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      if (above < need && above + bins[i] >= need) {
+        found[0] = kSelBins - 1 - 4 * tid - i;
+        found[1] = need - above;
+        found[2] = bins[i];
+      }
+      above += bins[i];
+    }
+    __syncthreads();
+    digits |= static_cast<uint32_t>(found[0]) << shift;
+    known |= mask << shift;
+    need = found[1];
+    whole = found[2] == need;  // every key of the bin is selected: the other digits do not matter
+    equal_need = need;
+  }
+  if (P.keep == P.keep_first + P.keep_last) equal_need = 0;
+  // Keys whose known digits exceed T's, and the first equal_need of those with T's.
+  const int per = (n + kSelThreads - 1) / kSelThreads;
+  const int j0 = min(n, tid * per), j1 = min(n, j0 + per);
+  int above = 0, equal = 0;
+#pragma unroll 4
+  for (int j = j0; j < j1; ++j) {
     const bool cand = j >= first && j < last;
-    const uint32_t key = cand ? score_key(row[j]) : 0;
-    const bool eq = cand && need > 0 && key == digits;
-    const uint64_t below = (uint64_t{1} << lane) - 1;
-    const uint64_t eqs = __ballot(eq);
-    if (lane == 0) wave_n[0][wave] = __builtin_popcountll(eqs);
-    __syncthreads();
-    int rank = equal + __builtin_popcountll(eqs & below);
-    for (int w = 0; w < kSelThreads / 64; ++w) {
-      rank += w < wave ? wave_n[0][w] : 0;
-      equal += wave_n[0][w];
+    const uint32_t key = cand ? key_of(j) & known : 0;
+    above += !cand || key > digits;
+    equal += cand && key == digits;
+  }
+  int total;
+  const int equal_before = scan_threads(equal, part[1], tid, total) - equal;
+  const int take_equal = min(max(equal_need - equal_before, 0), equal);
+  int at = scan_threads(above + take_equal, part[0], tid, total) - above - take_equal;
+  int left = take_equal;
+  for (int j = j0; j < j1; ++j) {
+    const bool cand = j >= first && j < last;
+    const uint32_t key = cand ? key_of(j) & known : 0;
+    const bool eq = cand && key == digits;
+    if (!cand || key > digits || (eq && left > 0)) {
+      if (at < P.keep) out[at] = j;
+      ++at;
+      left -= eq;
     }
-    const bool take = (j < n && !cand) || (eq && rank < need) ||
-                      (cand && P.keep > P.keep_first + P.keep_last && key > digits);
-    const uint64_t takes = __ballot(take);
-    if (lane == 0) wave_n[1][wave] = __builtin_popcountll(takes);
-    __syncthreads();
-    int at = written + __builtin_popcountll(takes & below);
-    for (int w = 0; w < kSelThreads / 64; ++w) {
-      at += w < wave ? wave_n[1][w] : 0;
-      written += wave_n[1][w];
-    }
-    if (take && at < P.keep) out[at] = j;
-    __syncthreads();
   }
 }
 
 // ---------------------------------------------------------------------------
 // Launch
 // ---------------------------------------------------------------------------
-// Work-groups of 256 along a grid's x: their threads number less than 2^32.
-constexpr int64_t kMaxGridX = (int64_t{1} << 24) - 1;
+// Work-groups of up to 512 threads along a grid's x: their threads number less than 2^32.
+constexpr int64_t kMaxGridX = (int64_t{1} << 23) - 1;
 
 bool head_built(int d) { return d == 64 || d == 128 || d == 256; }
 
@@ -443,11 +512,11 @@ template <bool kFp8>
 void launch_scores(const ScoreParams& P, int d, dim3 grid, hipStream_t s, const int32_t* bt,
                    const int32_t* ctx, const int32_t* cu) {
   if (d == 64)
-    hipLaunchKernelGGL((block_scores_kernel<kFp8, 64>), grid, dim3(256), 0, s, P, bt, ctx, cu);
+    hipLaunchKernelGGL((block_scores_kernel<kFp8, 64>), grid, dim3(64 * (P.num_kv_heads < kScoreWaves ? P.num_kv_heads : kScoreWaves)), 0, s, P, bt, ctx, cu);
   else if (d == 128)
-    hipLaunchKernelGGL((block_scores_kernel<kFp8, 128>), grid, dim3(256), 0, s, P, bt, ctx, cu);
+    hipLaunchKernelGGL((block_scores_kernel<kFp8, 128>), grid, dim3(64 * (P.num_kv_heads < kScoreWaves ? P.num_kv_heads : kScoreWaves)), 0, s, P, bt, ctx, cu);
   else
-    hipLaunchKernelGGL((block_scores_kernel<kFp8, 256>), grid, dim3(256), 0, s, P, bt, ctx, cu);
+    hipLaunchKernelGGL((block_scores_kernel<kFp8, 256>), grid, dim3(64 * (P.num_kv_heads < kScoreWaves ? P.num_kv_heads : kScoreWaves)), 0, s, P, bt, ctx, cu);
 }
 
 }  // namespace
@@ -544,10 +613,15 @@ extern "C" int fk_block_scores(float* scores, int64_t score_row_stride, int64_t 
   FK_REQUIRE(chunks * batch <= 65535, "%s: %lld groups of query rows are more than 65535", what,
              static_cast<long long>(chunks * batch));
   P.token_chunks = static_cast<int>(chunks);
-  P.tiles = 1;
+  // Tiles per wave: one where that leaves each SIMD under eight waves over the call, more (a
+  // wave's next tile is on its way while it scores one) where there are plenty.
+  const int64_t waves = (P.width + 15) / 16 * chunks * batch * num_kv_heads;
+  const int64_t per = waves / (int64_t{num_cus()} * 32);
+  P.tiles = static_cast<int>(per < 1 ? 1 : per > kScoreTiles ? kScoreTiles : per);
+  const int wg_heads = num_kv_heads < kScoreWaves ? num_kv_heads : kScoreWaves;
   const dim3 grid(static_cast<unsigned>((P.width + 16 * P.tiles - 1) / (16 * P.tiles)),
                   static_cast<unsigned>(chunks * batch),
-                  static_cast<unsigned>((num_kv_heads + 3) / 4));
+                  static_cast<unsigned>((num_kv_heads + wg_heads - 1) / wg_heads));
   if (kv_dtype == FK_DTYPE_FP8_E4M3FN)
     launch_scores<true>(P, head_size, grid, as_stream(stream), block_tables, cache_seqlens,
                         cu_seqlens_q);
@@ -594,7 +668,11 @@ extern "C" int fk_select_blocks(int32_t* block_indices, int64_t out_row_stride,
   P.block_size_log2 = log2_of(block_size);
   P.batch = static_cast<int>(batch);
   const dim3 grid(static_cast<unsigned>(rows), static_cast<unsigned>(num_kv_heads));
-  hipLaunchKernelGGL(select_blocks_kernel, grid, dim3(kSelThreads), 0, as_stream(stream), P,
-                     cache_seqlens, cu_seqlens_q);
+  if (P.width <= kSelLdsKeys)
+    hipLaunchKernelGGL(select_blocks_kernel<true>, grid, dim3(kSelThreads), 4 * sel_at(P.width),
+                       as_stream(stream), P, cache_seqlens, cu_seqlens_q);
+  else
+    hipLaunchKernelGGL(select_blocks_kernel<false>, grid, dim3(kSelThreads), 0, as_stream(stream),
+                       P, cache_seqlens, cu_seqlens_q);
   return check_launch(what);
 }

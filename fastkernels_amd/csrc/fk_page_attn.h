@@ -192,56 +192,26 @@ struct ColumnState {
 template <bool kFp8, int D>
 struct TileLanes {
   uint32_t k, v[4];
-  uint32_t bytes;  // of a tile, from its first row on
   __device__ __forceinline__ TileLanes(int num_kv_heads, int r, int g) {
     constexpr int kElt = kFp8 ? 1 : 2;
     const uint32_t row = static_cast<uint32_t>(num_kv_heads) * D * kElt;
-    bytes = 15 * row + D * kElt;
     k = r * row + (kFp8 ? (D / 4) * g : 16 * g);
 #pragma unroll
     for (int i = 0; i < 4; ++i) v[i] = (4 * g + i) * row + (D / 16) * r * kElt;
   }
 };
-// Issue a tile's K or V loads; row: its first row of the kv head (wave-uniform).  As buffer
-// loads: the tile's address stays in scalar registers (a descriptor of its 16 rows) and the
-// lanes' offsets never change, where plain loads took a 64-bit sum per lane and row.
-__device__ __forceinline__ __amdgpu_buffer_rsrc_t tile_rows(const uint8_t* row, uint32_t bytes) {
-  return __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t*>(row), 0, static_cast<int>(bytes),
-                                           0x00027000);
-}
+// Issue a tile's K or V loads; row: its first row of the kv head (wave-uniform).
 template <bool kFp8, int D>
 __device__ __forceinline__ void load_tile_k(const uint8_t* row, const TileLanes<kFp8, D>& at,
                                             DTile<kFp8, D>& t) {
-  const auto rows = tile_rows(row, at.bytes);
 #pragma unroll
-  for (int c = 0; c < DTile<kFp8, D>::kKLoads; ++c)
-    t.k[c] = __builtin_bit_cast(
-        uint4, __builtin_amdgcn_raw_buffer_load_b128(rows, at.k + (kFp8 ? 16 : 64) * c, 0, 0));
+  for (int c = 0; c < DTile<kFp8, D>::kKLoads; ++c) t.k[c] = ld16(row + at.k + (kFp8 ? 16 : 64) * c);
 }
 template <bool kFp8, int D>
 __device__ __forceinline__ void load_tile_v(const uint8_t* row, const TileLanes<kFp8, D>& at,
                                             DTile<kFp8, D>& t) {
-  constexpr int kWords = DTile<kFp8, D>::kVWords;
-  const auto rows = tile_rows(row, at.bytes);
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    if constexpr (kWords == 1) {
-      t.v[i][0] = __builtin_amdgcn_raw_buffer_load_b32(rows, at.v[i], 0, 0);
-    } else if constexpr (kWords == 2) {
-      const auto x = __builtin_amdgcn_raw_buffer_load_b64(rows, at.v[i], 0, 0);
-      t.v[i][0] = x[0];
-      t.v[i][1] = x[1];
-    } else {
-#pragma unroll
-      for (int q = 0; q < kWords; q += 4) {
-        const auto x = __builtin_amdgcn_raw_buffer_load_b128(rows, at.v[i] + 4 * q, 0, 0);
-        t.v[i][q] = x[0];
-        t.v[i][q + 1] = x[1];
-        t.v[i][q + 2] = x[2];
-        t.v[i][q + 3] = x[3];
-      }
-    }
-  }
+  for (int i = 0; i < 4; ++i) ld_words(row + at.v[i], t.v[i]);
 }
 
 // Keeps the loads before it before it: the compiler otherwise sinks them to just before their
@@ -435,6 +405,54 @@ struct Folded {
     o.w = o.w * fa + x.w * fb;
   }
 };
+
+// Merges the partials of nc columns, kMergeThreads threads.  A thread folds four dims of a
+// column; where the columns leave threads over, the pieces are dealt out among them and the
+// threads' states folded through LDS (`folded`, one per thread).  pieces(j) is the number of
+// column j's pieces, at(k, j, ml, o) where piece k's (m, l) and O are; emit(j, dim, o, M, L)
+// gets the merged state.
+constexpr int kMergeThreads = 256;
+constexpr int kMergeAhead = 4;  // pieces whose loads are in flight
+template <int D, class Pieces, class At, class Emit>
+__device__ __forceinline__ void merge_pieces(int nc, Folded* folded, Pieces pieces, At at,
+                                             Emit emit) {
+  const int tid = threadIdx.x;
+  const int items = nc * (D / 4);
+  const int slices = max(1, kMergeThreads / items);
+  for (int x0 = 0; x0 < items; x0 += kMergeThreads) {
+    const int x = x0 + (slices > 1 ? tid % items : tid);
+    const int slice = slices > 1 ? tid / items : 0;
+    const bool ok = x < items && slice < slices;
+    const int j = x / (D / 4), dim = 4 * (x % (D / 4));
+    Folded f;
+    f.reset();
+    const int n = ok ? pieces(j) : 0;
+    for (int k0 = slice; k0 < n; k0 += kMergeAhead * slices) {
+      float2 s[kMergeAhead];
+      float4 o[kMergeAhead];
+#pragma unroll
+      for (int u = 0; u < kMergeAhead; ++u) {
+        const float *ml, *row;
+        at(min(k0 + u * slices, n - 1), j, ml, row);
+        s[u] = *reinterpret_cast<const float2*>(ml);
+        o[u] = *reinterpret_cast<const float4*>(row + dim);
+      }
+#pragma unroll
+      for (int u = 0; u < kMergeAhead; ++u)
+        if (k0 + u * slices < n) f.add(s[u].x, s[u].y, o[u]);
+    }
+    if (slices > 1) {
+      folded[tid] = f;
+      __syncthreads();
+      if (slice == 0)
+        for (int u = 1; u < slices; ++u) {
+          const Folded& y = folded[x + u * items];
+          f.add(y.M, y.L, y.o);
+        }
+    }
+    if (ok && slice == 0) emit(j, dim, f.o, f.M, f.L);
+  }
+}
 
 // Output of a finished row: O (scaled by the V scale of fp8 pages) over the sum, which the
 // head's sink joins; a row that saw no key is zero.

@@ -489,11 +489,7 @@ __attribute__((amdgpu_waves_per_eu((D == 256 ? 1 : 2)))) void shared_prefix_kern
   }
 }
 
-// One work-group per (row, kv head, block of 16 query heads).  A thread folds four dims of a
-// column; where the columns leave threads over, the pieces are dealt out among them and the
-// threads' states folded through LDS.
-constexpr int kMergeThreads = 256;
-constexpr int kMergeAhead = 4;  // pieces whose loads are in flight
+// One work-group per (row, kv head, block of 16 query heads) merges the row's partials.
 template <int D>
 __global__ __launch_bounds__(kMergeThreads) void shared_prefix_merge_kernel(PrefixParams P,
                                                                             int fp8) {
@@ -503,68 +499,44 @@ __global__ __launch_bounds__(kMergeThreads) void shared_prefix_merge_kernel(Pref
   const int b = blockIdx.y, v = blockIdx.x;
   const int kvh = v / A.col_blocks;
   const int in_group = 16 * (v - kvh * A.col_blocks);  // first query head, of the group
-  const int nc = min(16, A.gqa - in_group);
   const RowRecord rec = P.rows[b];
   const float vsc = fp8 && A.v_scale ? A.v_scale[kvh] : 1.f;
-  const int items = nc * (D / 4);
-  const int slices = max(1, kMergeThreads / items);
-  // The row's pieces on its own line: ranges w0, w0 + 1, ...
+  // The row's pieces on its own line: ranges own_w, own_w + 1, ...
   const int64_t own_at = rec.own_start + v * rec.own_step;
   const int64_t own_w = rec.own_tiles ? own_at / rec.own_range : 0;
   const int own_n = rec.own_tiles
                         ? static_cast<int>((own_at + rec.own_tiles - 1) / rec.own_range - own_w) + 1
                         : 0;
   const int64_t own_col = (own_w + static_cast<int64_t>(b) * P.vheads + v) * P.own_cols;
-  for (int x0 = 0; x0 < items; x0 += kMergeThreads) {
-    const int x = x0 + static_cast<int>(threadIdx.x) % (slices > 1 ? items : kMergeThreads);
-    const int slice = slices > 1 ? threadIdx.x / items : 0;
-    const bool ok = x < items && slice < slices;
-    const int j = x / (D / 4), dim = 4 * (x % (D / 4));
-    Folded f;
-    f.reset();
-    if (ok) {
-      // ... and on the prefix line, for this column
-      int pre_n = 0;
-      int64_t pre_col = 0;
-      if (rec.pre_tiles > 0) {
-        const int c = rec.index * A.gqa + in_group + j;
-        const int it = kvh * rec.col_items + c / kCols;
-        const int64_t at = rec.pre_start + it * rec.pre_step;
-        const int64_t w = at / rec.pre_range;
-        const int64_t first = w + rec.pre_item + it;
-        pre_n = static_cast<int>(
-            min((at + rec.pre_tiles - 1) / rec.pre_range - w + 1, P.pre_pieces - first));
-        pre_col = first * kCols + c % kCols;
-      }
-      const int n = pre_n + own_n;
-      for (int k0 = slice; k0 < n; k0 += kMergeAhead * slices) {
-        float2 s[kMergeAhead];
-        float4 o[kMergeAhead];
-#pragma unroll
-        for (int u = 0; u < kMergeAhead; ++u) {
-          const int k = min(k0 + u * slices, n - 1);
-          const bool pre = k < pre_n;
-          const int64_t col = pre ? pre_col + static_cast<int64_t>(k) * kCols
-                                  : own_col + static_cast<int64_t>(k - pre_n) * P.own_cols + j;
-          s[u] = *reinterpret_cast<const float2*>((pre ? P.pre_ml : P.own_ml) + 2 * col);
-          o[u] = *reinterpret_cast<const float4*>((pre ? P.pre_o : P.own_o) + col * D + dim);
+  // ... and on the prefix line, found for each column.
+  int pre_n = 0;
+  int64_t pre_col = 0;
+  merge_pieces<D>(
+      min(16, A.gqa - in_group), folded,
+      [&](int j) {
+        if (rec.pre_tiles > 0) {
+          const int c = rec.index * A.gqa + in_group + j;
+          const int it = kvh * rec.col_items + c / kCols;
+          const int64_t at = rec.pre_start + it * rec.pre_step;
+          const int64_t w = at / rec.pre_range;
+          const int64_t first = w + rec.pre_item + it;
+          pre_n = static_cast<int>(max(
+              int64_t{0},
+              min((at + rec.pre_tiles - 1) / rec.pre_range - w + 1, P.pre_pieces - first)));
+          pre_col = first * kCols + c % kCols;
         }
-#pragma unroll
-        for (int u = 0; u < kMergeAhead; ++u)
-          if (k0 + u * slices < n) f.add(s[u].x, s[u].y, o[u]);
-      }
-    }
-    if (slices > 1) {
-      folded[threadIdx.x] = f;
-      __syncthreads();
-      if (slice == 0)
-        for (int u = 1; u < slices; ++u) {
-          const Folded& y = folded[x + u * items];
-          f.add(y.M, y.L, y.o);
-        }
-    }
-    if (ok && slice == 0) write_quad(A, b, kvh * A.gqa + in_group + j, D, dim, f.o, f.M, f.L, vsc);
-  }
+        return pre_n + own_n;
+      },
+      [&](int k, int j, const float*& ml, const float*& o) {
+        const bool pre = k < pre_n;
+        const int64_t col = pre ? pre_col + static_cast<int64_t>(k) * kCols
+                                : own_col + static_cast<int64_t>(k - pre_n) * P.own_cols + j;
+        ml = (pre ? P.pre_ml : P.own_ml) + 2 * col;
+        o = (pre ? P.pre_o : P.own_o) + col * D;
+      },
+      [&](int j, int dim, const float4& o, float M, float L) {
+        write_quad(A, b, kvh * A.gqa + in_group + j, D, dim, o, M, L, vsc);
+      });
 }
 
 // Work-groups and workspace of a launch.

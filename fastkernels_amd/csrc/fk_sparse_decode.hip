@@ -5,8 +5,11 @@
 //   table, or at pages that hold no visible key, are skipped; a page listed twice counts
 //   twice).  Sinks join the denominator; a row without a visible key is zero.
 //
-// One work-group per (query row, kv head, block of 16 query heads): its waves share the list
-// (fk_page_attn.h).
+// A work-group takes a share of the list of one (query row, kv head, block of 16 query heads),
+// its waves every fourth unit of the share (fk_page_attn.h).  Where the rows are too few to fill
+// the chip, the list is shared among up to kMaxParts work-groups and a second launch merges
+// their partials.  The kv head varies fastest in the grid: the rows of a sequence that check
+// drafted tokens, which mostly select the same pages, run side by side on one XCD's L2.
 #include <limits.h>
 
 #include "fk_page_attn.h"
@@ -21,28 +24,25 @@ struct SparseParams {
   int64_t idx_row_stride, idx_head_stride;
   int keep;
   int unit_tiles_log2;
+  int parts;     // work-groups per list
+  int cols;      // columns of a partial: min(16, gqa)
+  float* part_o; // [(row, virtual head), part][cols][D], then (maximum, sum) per column
+  float* part_ml;
 };
 
-// Waves of a work-group.  At head size 256 the query, a step's K and V rows and O take more
-// than the 256 registers that two waves a SIMD leave: one runs there, with as much in flight.
-#ifndef XW
-#define XW 4
-#endif
-#ifndef XEU
-#define XEU 2
-#endif
-template <int D>
-constexpr int waves_of() { return D == 256 ? 4 : XW; }
+// Registers: two waves a SIMD, or one at head size 256 (the query, a step's K and V rows and O
+// take more than 256 there).
+constexpr int kWaves = 4;
+constexpr int kMaxParts = 64;
 
 template <int D, bool kFp8>
-__global__ __launch_bounds__((waves_of<D>() * 64))
-__attribute__((amdgpu_waves_per_eu((D == 256 ? 1 : XEU)))) void sparse_decode_kernel(
+__global__ __launch_bounds__(kWaves * 64)
+__attribute__((amdgpu_waves_per_eu(D == 256 ? 1 : 2))) void sparse_decode_kernel(
     SparseParams P, const int32_t* __restrict__ bt, const int32_t* __restrict__ ctx,
     const int32_t* __restrict__ cu) {
-  constexpr int kWaves = waves_of<D>();
   extern __shared__ __align__(16) float lds[];  // merge_lds_floats of the group's columns
   const PageAttnParams& A = P.A;
-  const int t = blockIdx.y;
+  const int t = blockIdx.y, part = blockIdx.z;
   int b, vis;
   if (!query_row(cu, ctx, A.batch, t, b, vis)) return;
   const int kvh = blockIdx.x / A.col_blocks;
@@ -71,30 +71,83 @@ __attribute__((amdgpu_waves_per_eu((D == 256 ? 1 : XEU)))) void sparse_decode_ke
     tok = static_cast<int>(pos);
   };
   const uint32_t span = static_cast<uint32_t>(max(vis, 0));
-  stream_units(A, st, unit_at, P.keep << per_log2, wave, kWaves, P.unit_tiles_log2, 0,
+  stream_units(A, st, unit_at, P.keep << per_log2, kWaves * part + wave, kWaves * P.parts,
+               P.unit_tiles_log2, 0,
                max(vis, 0), [&] { return Limits<1>{{span}, span, span}; }, kvh,
                __builtin_fabsf(s2), lane);
-  merge_waves<kWaves>(st, lds, wave, lane, ncols,
-                      [&](int j, int dim, const float4& o, float M, float L) {
-                        write_quad(A, t, qbase + j, D, dim, o, M, L, vsc);
-                      });
+  if (P.parts == 1) {
+    merge_waves<kWaves>(st, lds, wave, lane, ncols,
+                        [&](int j, int dim, const float4& o, float M, float L) {
+                          write_quad(A, t, qbase + j, D, dim, o, M, L, vsc);
+                        });
+  } else {
+    const int64_t col =
+        ((static_cast<int64_t>(t) * gridDim.x + blockIdx.x) * P.parts + part) * P.cols;
+    merge_waves<kWaves>(st, lds, wave, lane, ncols,
+                        [&](int j, int dim, const float4& o, float M, float L) {
+                          *reinterpret_cast<float4*>(P.part_o + (col + j) * D + dim) = o;
+                          if (dim == 0)
+                            *reinterpret_cast<float2*>(P.part_ml + 2 * (col + j)) =
+                                make_float2(M, L);
+                        });
+  }
 }
 
-template <int D, bool kFp8>
-void launch_t(const SparseParams& P, dim3 grid, hipStream_t s, const int32_t* bt,
-              const int32_t* ctx, const int32_t* cu) {
-  constexpr int kWaves = waves_of<D>();
-  const int cols = P.A.gqa < 16 ? P.A.gqa : 16;
-  hipLaunchKernelGGL((sparse_decode_kernel<D, kFp8>), grid, dim3(kWaves * 64),
-                     (4 * merge_lds_floats<kWaves, D>(cols)), s, P, bt, ctx, cu);
-}
+// One work-group per (query row, virtual head) merges the list's parts.
 template <int D>
-void launch_d(bool fp8, const SparseParams& P, dim3 grid, hipStream_t s, const int32_t* bt,
+__global__ __launch_bounds__(kMergeThreads) void sparse_merge_kernel(
+    SparseParams P, const int32_t* __restrict__ ctx, const int32_t* __restrict__ cu, int fp8) {
+  __shared__ Folded folded[kMergeThreads];
+  const PageAttnParams& A = P.A;
+  const int t = blockIdx.y;
+  int b, vis;
+  if (!query_row(cu, ctx, A.batch, t, b, vis)) return;
+  const int kvh = blockIdx.x / A.col_blocks;
+  const int qbase = kvh * A.gqa + 16 * (blockIdx.x - kvh * A.col_blocks);
+  const float vsc = fp8 && A.v_scale ? A.v_scale[kvh] : 1.f;
+  const int64_t col0 = (static_cast<int64_t>(t) * gridDim.x + blockIdx.x) * P.parts * P.cols;
+  merge_pieces<D>(
+      min(16, (kvh + 1) * A.gqa - qbase), folded, [&](int) { return P.parts; },
+      [&](int k, int j, const float*& ml, const float*& o) {
+        const int64_t col = col0 + static_cast<int64_t>(k) * P.cols + j;
+        ml = P.part_ml + 2 * col;
+        o = P.part_o + col * D;
+      },
+      [&](int j, int dim, const float4& o, float M, float L) {
+        write_quad(A, t, qbase + j, D, dim, o, M, L, vsc);
+      });
+}
+
+// Work-groups per list: where the lists are fewer than the CUs, as many as make two per CU, each
+// with two tiles per wave at the least.  (With a list for each CU, parts only add their merge:
+// 512 lists of 2048 keys 98 us in one part, 109 in two.)
+int parts_of(int64_t rows, int64_t keep, int vheads, int block_size) {
+  const int64_t lists = rows * vheads;
+  const int64_t tiles = keep * (block_size / kTile);
+  const int64_t cus = num_cus();
+  int64_t parts = lists > 0 && lists < cus ? (2 * cus + lists - 1) / lists : 1;
+  if (parts > tiles / (2 * kWaves)) parts = tiles / (2 * kWaves);
+  return static_cast<int>(parts < 1 ? 1 : parts > kMaxParts ? kMaxParts : parts);
+}
+int64_t part_bytes(int64_t rows, int vheads, int parts, int cols, int head_size) {
+  return parts > 1 ? rows * vheads * parts * cols * (head_size + 2) * 4 : 0;
+}
+
+template <int D>
+void launch_d(bool fp8, const SparseParams& P, int64_t rows, hipStream_t s, const int32_t* bt,
               const int32_t* ctx, const int32_t* cu) {
+  const unsigned vheads = P.A.num_kv_heads * P.A.col_blocks;
+  const dim3 grid(vheads, static_cast<unsigned>(rows), static_cast<unsigned>(P.parts));
+  const unsigned lds = 4 * merge_lds_floats<kWaves, D>(P.cols);
   if (fp8)
-    launch_t<D, true>(P, grid, s, bt, ctx, cu);
+    hipLaunchKernelGGL((sparse_decode_kernel<D, true>), grid, dim3(kWaves * 64), lds, s, P, bt,
+                       ctx, cu);
   else
-    launch_t<D, false>(P, grid, s, bt, ctx, cu);
+    hipLaunchKernelGGL((sparse_decode_kernel<D, false>), grid, dim3(kWaves * 64), lds, s, P, bt,
+                       ctx, cu);
+  if (P.parts > 1)
+    hipLaunchKernelGGL((sparse_merge_kernel<D>), dim3(vheads, static_cast<unsigned>(rows)),
+                       dim3(kMergeThreads), 0, s, P, ctx, cu, fp8 ? 1 : 0);
 }
 
 }  // namespace
@@ -134,16 +187,26 @@ extern "C" int fk_sparse_paged_decode(
   P.idx_head_stride = idx_head_stride;
   P.keep = static_cast<int>(keep);
   P.unit_tiles_log2 = A.block_size_log2 - 4 < 2 ? A.block_size_log2 - 4 : 2;
-  const dim3 grid(static_cast<unsigned>(num_kv_heads * A.col_blocks),
-                  static_cast<unsigned>(rows));
+  const int vheads = num_kv_heads * A.col_blocks;
+  P.cols = A.gqa < 16 ? A.gqa : 16;
+  P.parts = parts_of(rows, keep, vheads, block_size);
+  const int64_t need = part_bytes(rows, vheads, P.parts, P.cols, head_size);
+  if (need > 0) {
+    if (!workspace || workspace_bytes < need)
+      return set_error(FK_ERR_WORKSPACE, "%s: workspace of %lld bytes, %lld needed", what,
+                       static_cast<long long>(workspace_bytes), static_cast<long long>(need));
+    FK_REQUIRE(aligned16(workspace), "%s: workspace must be 16-byte aligned", what);
+    P.part_o = static_cast<float*>(workspace);
+    P.part_ml = P.part_o + rows * vheads * P.parts * P.cols * head_size;
+  }
   const bool fp8 = kv_dtype == FK_DTYPE_FP8_E4M3FN;
   hipStream_t s = as_stream(stream);
   if (head_size == 64)
-    launch_d<64>(fp8, P, grid, s, block_tables, cache_seqlens, cu_seqlens_q);
+    launch_d<64>(fp8, P, rows, s, block_tables, cache_seqlens, cu_seqlens_q);
   else if (head_size == 128)
-    launch_d<128>(fp8, P, grid, s, block_tables, cache_seqlens, cu_seqlens_q);
+    launch_d<128>(fp8, P, rows, s, block_tables, cache_seqlens, cu_seqlens_q);
   else
-    launch_d<256>(fp8, P, grid, s, block_tables, cache_seqlens, cu_seqlens_q);
+    launch_d<256>(fp8, P, rows, s, block_tables, cache_seqlens, cu_seqlens_q);
   return check_launch(what);
 }
 
@@ -151,6 +214,13 @@ extern "C" int fk_sparse_paged_decode_plan(int64_t rows, int64_t keep, int num_h
                                            int num_kv_heads, int head_size, int block_size,
                                            int64_t* workspace_bytes) {
   FK_REQUIRE(workspace_bytes, "fk_sparse_paged_decode_plan: null output pointer");
-  *workspace_bytes = 0;
+  FK_REQUIRE(rows >= 0 && rows <= 65535 && keep >= 0 && num_kv_heads > 0 && num_heads > 0 &&
+                 num_heads % num_kv_heads == 0 && head_size > 0 && block_size >= 16 &&
+                 keep <= (INT_MAX >> 1) / (block_size / 16),
+             "fk_sparse_paged_decode_plan: invalid argument");
+  const int gqa = num_heads / num_kv_heads;
+  const int vheads = num_kv_heads * ((gqa + 15) / 16);
+  *workspace_bytes = part_bytes(rows, vheads, parts_of(rows, keep, vheads, block_size),
+                                gqa < 16 ? gqa : 16, head_size);
   return FK_OK;
 }
