@@ -13,6 +13,7 @@ stay opaque under torch.compile and are capturable in HIP graphs.
 """
 from __future__ import annotations
 
+import functools
 import math
 from typing import NamedTuple
 
@@ -73,11 +74,13 @@ def _rows(t: torch.Tensor, width: int, what: str) -> tuple[int, int]:
     return v.shape[0], v.stride(0)
 
 
-def _same_device(first: torch.Tensor, *ts: torch.Tensor | None) -> None:
+def _same_device(first: torch.Tensor, *ts: torch.Tensor | None) -> int:
+    """Refuses tensors of different devices; returns the device's index."""
     dev = first.get_device()
     for t in ts:
         if t is not None and t.get_device() != dev:
             raise ValueError(f"tensors on different devices: {first.device} vs {t.device}")
+    return dev
 
 
 # ---------------------------------------------------------------------------
@@ -699,19 +702,26 @@ def merge_attn_states(output: torch.Tensor, prefix_output: torch.Tensor, prefix_
 # ---------------------------------------------------------------------------
 # Attention that reads part of a paged cache: selected pages, shared prefixes
 # ---------------------------------------------------------------------------
-def _call_on(t: torch.Tensor, fn: str, *args) -> None:
-    """_native.call with t's device current and its current stream as the last argument."""
+def _call_on(t: torch.Tensor, dev: int, fn: str, *args) -> None:
+    """_native.call with device ``dev`` (t's) current and its current stream as the last
+    argument."""
     stream = _stream(t)
-    if t.get_device() == torch.cuda.current_device():
+    if dev == torch.cuda.current_device():
         _native.call(fn, *args, stream)
     else:
-        with torch.cuda.device(t.device):
+        with torch.cuda.device(dev):
             _native.call(fn, *args, stream)
 
 
-def _check_table(what: str, block_table: torch.Tensor, cache_seqlens: torch.Tensor,
-                 cu_seqlens_q: torch.Tensor | None, rows: int | None) -> int:
-    """Checks the sequences' metadata; returns their number."""
+@functools.lru_cache(maxsize=4096)
+def _plan_bytes(dev: int, plan, *shape: int) -> int:
+    """The workspace bytes ``plan`` asks for on a device, a function of the shape alone."""
+    with torch.cuda.device(dev):
+        return plan(*shape)
+
+
+def _check_batch(what, cache_seqlens, cu_seqlens_q, rows) -> int:
+    """Checks the sequences' lengths; returns the number of sequences."""
     if cu_seqlens_q is None:
         batch = cache_seqlens.numel() if rows is None else rows
     else:
@@ -722,22 +732,39 @@ def _check_table(what: str, block_table: torch.Tensor, cache_seqlens: torch.Tens
     if cache_seqlens.dtype != torch.int32 or not cache_seqlens.is_contiguous() or \
             cache_seqlens.numel() < batch:
         raise TypeError(f"{what}: cache_seqlens must be contiguous int32 [batch]")
-    if block_table is not None:
-        if block_table.dtype != torch.int32 or block_table.dim() != 2 or \
-                (block_table.shape[1] > 1 and block_table.stride(1) != 1):
-            raise TypeError(f"{what}: block_table must be int32 [batch, max_blocks], rows "
-                            "contiguous")
-        if block_table.shape[0] < batch:
-            raise ValueError(f"{what}: block_table has fewer rows than the batch")
     return batch
 
 
-def _check_rows(what: str, t: torch.Tensor, name: str) -> None:
-    if t.dim() != 3 or t.dtype != torch.bfloat16 or t.stride()[1:] != (t.shape[2], 1):
+def _check_table(what, block_table, batch) -> tuple[int, int]:
+    """(row stride, columns) of a block table with a row per sequence."""
+    shape, stride = block_table.shape, block_table.stride()
+    if block_table.dtype != torch.int32 or len(shape) != 2 or (shape[1] > 1 and stride[1] != 1):
+        raise TypeError(f"{what}: block_table must be int32 [batch, max_blocks], rows contiguous")
+    if shape[0] < batch:
+        raise ValueError(f"{what}: block_table has fewer rows than the batch")
+    return stride[0], shape[1]
+
+
+def _check_rows(what, t, name) -> tuple[torch.Size, int]:
+    """(shape, row stride) of bf16 rows of contiguous heads."""
+    shape = t.shape
+    stride = t.stride()
+    if len(shape) != 3 or t.dtype != torch.bfloat16 or stride[2] != 1 or stride[1] != shape[2]:
         raise ValueError(f"{what}: {name} must be bf16 [rows, Hq, D] with contiguous heads")
+    return shape, stride[0]
 
 
-def _cache_tag(what: str, dtype: torch.dtype) -> int:
+def _check_grid(what, t, name, dtype, last) -> tuple[torch.Size, int, int]:
+    """(shape, row stride, head stride) of [rows, Hk, n] values, contiguous along n."""
+    shape = t.shape
+    stride = t.stride()
+    if len(shape) != 3 or t.dtype != dtype or (shape[2] > 1 and stride[2] != 1):
+        raise ValueError(f"{what}: {name} must be {str(dtype)[6:]} [rows, Hk, {last}] with "
+                         "contiguous entries")
+    return shape, stride[0], stride[1]
+
+
+def _cache_tag(what, dtype) -> int:
     if dtype == torch.bfloat16:
         return _native.FK_DTYPE_BF16
     if dtype != _FP8:
@@ -745,10 +772,13 @@ def _cache_tag(what: str, dtype: torch.dtype) -> int:
     return _native.FK_DTYPE_FP8_E4M3FN
 
 
-def _check_scale(what: str, scale: torch.Tensor | None, name: str, heads: int) -> None:
-    if scale is not None and (scale.dtype != torch.float32 or scale.numel() != heads or
-                              not scale.is_contiguous()):
+def _check_scale(what, scale, name, heads) -> int | None:
+    """A scale's (or the sinks') pointer, None without one."""
+    if scale is None:
+        return None
+    if scale.dtype != torch.float32 or scale.numel() != heads or not scale.is_contiguous():
         raise ValueError(f"{what}: {name} must be contiguous float32 [{heads}]")
+    return scale.data_ptr()
 
 
 def new_key_bounds(k_cache: torch.Tensor) -> torch.Tensor:
@@ -758,10 +788,11 @@ def new_key_bounds(k_cache: torch.Tensor) -> torch.Tensor:
     return torch.zeros(nb, hk, 2, d, dtype=k_cache.dtype, device=k_cache.device)
 
 
-def _check_bounds(what: str, key_bounds: torch.Tensor, head_size: int) -> None:
-    if key_bounds.dim() != 4 or key_bounds.shape[2] != 2 or key_bounds.shape[3] != head_size or \
-            not key_bounds.is_contiguous():
+def _check_bounds(what, key_bounds) -> torch.Size:
+    shape = key_bounds.shape
+    if len(shape) != 4 or shape[2] != 2 or not key_bounds.is_contiguous():
         raise ValueError(f"{what}: key_bounds must be contiguous [num_blocks, Hk, 2, D]")
+    return shape
 
 
 def update_key_bounds(key_bounds: torch.Tensor, k_cache: torch.Tensor, block_table: torch.Tensor,
@@ -776,21 +807,22 @@ def update_key_bounds(key_bounds: torch.Tensor, k_cache: torch.Tensor, block_tab
     cu_seqlens_q), at most max_seqlen_q.  Pages are read whole, so the result depends on the
     cache alone: a rejected draft token is forgotten with the next call on its page."""
     what = "update_key_bounds"
-    if k_cache.dim() != 4 or not k_cache.is_contiguous():
+    shape = k_cache.shape
+    if len(shape) != 4 or not k_cache.is_contiguous():
         raise ValueError(f"{what}: k_cache must be contiguous [num_blocks, block_size, Hk, D]")
-    nb, bs, hk, d = k_cache.shape
-    _check_bounds(what, key_bounds, d)
-    if key_bounds.shape[:2] != (nb, hk) or key_bounds.dtype != k_cache.dtype:
+    nb, bs, hk, d = shape
+    dtype = k_cache.dtype
+    if _check_bounds(what, key_bounds) != (nb, hk, 2, d) or key_bounds.dtype != dtype:
         raise ValueError(f"{what}: key_bounds must be [{nb}, {hk}, 2, {d}] of the cache's dtype")
-    tag = _cache_tag(what, k_cache.dtype)
-    batch = _check_table(what, block_table, cache_seqlens, cu_seqlens_q, None)
-    _same_device(key_bounds, k_cache, block_table, cache_seqlens, cu_seqlens_q)
+    tag = _cache_tag(what, dtype)
+    batch = _check_batch(what, cache_seqlens, cu_seqlens_q, None)
+    bt_stride, bt_width = _check_table(what, block_table, batch)
+    dev = _same_device(key_bounds, k_cache, block_table, cache_seqlens, cu_seqlens_q)
     if batch == 0:
         return
-    _call_on(key_bounds, "fk_update_key_bounds", key_bounds.data_ptr(), k_cache.data_ptr(), tag,
-             block_table.data_ptr(), block_table.stride(0), block_table.shape[1],
-             cache_seqlens.data_ptr(), _ptr(cu_seqlens_q), batch, int(max_seqlen_q), hk, d, bs,
-             nb)
+    _call_on(key_bounds, dev, "fk_update_key_bounds", key_bounds.data_ptr(), k_cache.data_ptr(),
+             tag, block_table.data_ptr(), bt_stride, bt_width, cache_seqlens.data_ptr(),
+             _ptr(cu_seqlens_q), batch, int(max_seqlen_q), hk, d, bs, nb)
 
 
 def block_scores(scores: torch.Tensor, q: torch.Tensor, key_bounds: torch.Tensor,
@@ -805,27 +837,25 @@ def block_scores(scores: torch.Tensor, q: torch.Tensor, key_bounds: torch.Tensor
     Rows: one per sequence, or cu_seqlens_q [batch + 1] with at most max_seqlen_q per
     sequence, its last tokens (row i of n sees cache_seqlens[b] - n + i + 1 keys)."""
     what = "block_scores"
-    _check_rows(what, q, "q")
-    rows, hq, d = q.shape
-    _check_bounds(what, key_bounds, d)
-    nb, hk = key_bounds.shape[:2]
+    (rows, hq, d), q_stride = _check_rows(what, q, "q")
+    nb, hk, _, d_bounds = _check_bounds(what, key_bounds)
     tag = _cache_tag(what, key_bounds.dtype)
-    if hk == 0 or hq % hk:
-        raise ValueError(f"{what}: {hq} query heads over {hk} kv heads")
-    if scores.dim() != 3 or scores.shape[:2] != (rows, hk) or scores.dtype != torch.float32 or \
-            (scores.shape[2] > 1 and scores.stride(2) != 1):
-        raise ValueError(f"{what}: scores must be float32 [rows, Hk, blocks] with contiguous "
-                         "blocks")
-    _check_scale(what, k_scale, "k_scale", hk)
-    batch = _check_table(what, block_table, cache_seqlens, cu_seqlens_q, rows)
-    _same_device(scores, q, key_bounds, block_table, cache_seqlens, cu_seqlens_q, k_scale)
-    if rows == 0 or batch == 0 or scores.shape[2] == 0:
+    if hk == 0 or hq % hk or d_bounds != d:
+        raise ValueError(f"{what}: {hq} query heads of {d} over {hk} kv heads of {d_bounds}")
+    shape, row_stride, head_stride = _check_grid(what, scores, "scores", torch.float32, "blocks")
+    width = shape[2]
+    if shape[0] != rows or shape[1] != hk:
+        raise ValueError(f"{what}: scores must be [{rows}, {hk}, blocks]")
+    ks = _check_scale(what, k_scale, "k_scale", hk)
+    batch = _check_batch(what, cache_seqlens, cu_seqlens_q, rows)
+    bt_stride, bt_width = _check_table(what, block_table, batch)
+    dev = _same_device(scores, q, key_bounds, block_table, cache_seqlens, cu_seqlens_q, k_scale)
+    if rows == 0 or batch == 0 or width == 0:
         return
-    _call_on(scores, "fk_block_scores", scores.data_ptr(), scores.stride(0), scores.stride(1),
-             scores.shape[2], q.data_ptr(), q.stride(0), key_bounds.data_ptr(), tag,
-             _ptr(k_scale), block_table.data_ptr(), block_table.stride(0), block_table.shape[1],
-             cache_seqlens.data_ptr(), _ptr(cu_seqlens_q), batch, rows, int(max_seqlen_q), hq, hk,
-             d, int(block_size), nb)
+    _call_on(scores, dev, "fk_block_scores", scores.data_ptr(), row_stride, head_stride, width,
+             q.data_ptr(), q_stride, key_bounds.data_ptr(), tag, ks, block_table.data_ptr(),
+             bt_stride, bt_width, cache_seqlens.data_ptr(), _ptr(cu_seqlens_q), batch, rows,
+             int(max_seqlen_q), hq, hk, d, int(block_size), nb)
 
 
 def select_blocks(block_indices: torch.Tensor, scores: torch.Tensor, cache_seqlens: torch.Tensor,
@@ -837,46 +867,39 @@ def select_blocks(block_indices: torch.Tensor, scores: torch.Tensor, cache_seqle
     scores; of equal scores the lower index first, NaN above every number.  All of them where
     they are at most keep."""
     what = "select_blocks"
-    if scores.dim() != 3 or scores.dtype != torch.float32 or \
-            (scores.shape[2] > 1 and scores.stride(2) != 1):
-        raise ValueError(f"{what}: scores must be float32 [rows, Hk, blocks] with contiguous "
-                         "blocks")
-    rows, hk, width = scores.shape
-    if block_indices.dim() != 3 or block_indices.shape[:2] != (rows, hk) or \
-            block_indices.dtype != torch.int32 or \
-            (block_indices.shape[2] > 1 and block_indices.stride(2) != 1):
-        raise ValueError(f"{what}: block_indices must be int32 [rows, Hk, keep] with contiguous "
-                         "entries")
-    keep = block_indices.shape[2]
+    (rows, hk, width), s_row, s_head = _check_grid(what, scores, "scores", torch.float32, "blocks")
+    shape, o_row, o_head = _check_grid(what, block_indices, "block_indices", torch.int32, "keep")
+    keep = shape[2]
+    if shape[0] != rows or shape[1] != hk:
+        raise ValueError(f"{what}: block_indices must be [{rows}, {hk}, keep]")
     if keep_first < 0 or keep_last < 0 or keep_first + keep_last > keep:
         raise ValueError(f"{what}: keep_first {keep_first} and keep_last {keep_last} must fit in "
                          f"the {keep} selected blocks")
-    batch = _check_table(what, None, cache_seqlens, cu_seqlens_q, rows)
-    _same_device(block_indices, scores, cache_seqlens, cu_seqlens_q)
+    batch = _check_batch(what, cache_seqlens, cu_seqlens_q, rows)
+    dev = _same_device(block_indices, scores, cache_seqlens, cu_seqlens_q)
     if rows == 0 or batch == 0 or keep == 0:
         return
-    _call_on(scores, "fk_select_blocks", block_indices.data_ptr(), block_indices.stride(0),
-             block_indices.stride(1), keep, scores.data_ptr(), scores.stride(0),
-             scores.stride(1), width, cache_seqlens.data_ptr(), _ptr(cu_seqlens_q), batch, rows,
-             hk, int(block_size), int(keep_first), int(keep_last))
+    _call_on(scores, dev, "fk_select_blocks", block_indices.data_ptr(), o_row, o_head, keep,
+             scores.data_ptr(), s_row, s_head, width, cache_seqlens.data_ptr(),
+             _ptr(cu_seqlens_q), batch, rows, hk, int(block_size), int(keep_first),
+             int(keep_last))
 
 
-def _check_page_attn(what, out, q, k_cache, v_cache, k_scale, v_scale, sinks) -> int:
-    _check_rows(what, q, "q")
-    _check_rows(what, out, "out")
-    if out.shape != q.shape:
+def _check_page_attn(what, out, q, k_cache, v_cache):
+    """(q's shape, its and out's row strides, the caches' shape and dtype tag)."""
+    q_shape, q_stride = _check_rows(what, q, "q")
+    out_shape, out_stride = _check_rows(what, out, "out")
+    if out_shape != q_shape:
         raise ValueError(f"{what}: out must have q's shape")
-    if k_cache.dim() != 4 or v_cache.shape != k_cache.shape or k_cache.shape[3] != q.shape[2]:
+    cache = k_cache.shape
+    if len(cache) != 4 or v_cache.shape != cache or cache[3] != q_shape[2]:
         raise ValueError(f"{what}: caches must be [num_blocks, block_size, Hk, D]")
     if not (k_cache.is_contiguous() and v_cache.is_contiguous()):
         raise ValueError(f"{what}: caches must be contiguous")
-    if v_cache.dtype != k_cache.dtype:
+    dtype = k_cache.dtype
+    if v_cache.dtype != dtype:
         raise TypeError(f"{what}: caches must share a dtype")
-    tag = _cache_tag(what, k_cache.dtype)
-    _check_scale(what, k_scale, "k_scale", k_cache.shape[2])
-    _check_scale(what, v_scale, "v_scale", k_cache.shape[2])
-    _check_scale(what, sinks, "sinks", q.shape[1])
-    return tag
+    return q_shape, q_stride, out_stride, cache, _cache_tag(what, dtype)
 
 
 def sparse_paged_decode(out: torch.Tensor, q: torch.Tensor, k_cache: torch.Tensor,
@@ -892,28 +915,28 @@ def sparse_paged_decode(out: torch.Tensor, q: torch.Tensor, k_cache: torch.Tenso
     zero.  Rows and cu_seqlens_q as in :func:`block_scores`; scales and sinks as in
     :func:`paged_decode`."""
     what = "sparse_paged_decode"
-    tag = _check_page_attn(what, out, q, k_cache, v_cache, k_scale, v_scale, sinks)
-    rows, hq, d = q.shape
-    nb, bs, hk, _ = k_cache.shape
-    if block_indices.dim() != 3 or block_indices.shape[:2] != (rows, hk) or \
-            block_indices.dtype != torch.int32 or \
-            (block_indices.shape[2] > 1 and block_indices.stride(2) != 1):
-        raise ValueError(f"{what}: block_indices must be int32 [rows, Hk, keep] with contiguous "
-                         "entries")
-    batch = _check_table(what, block_table, cache_seqlens, cu_seqlens_q, rows)
-    _same_device(out, q, k_cache, v_cache, block_table, cache_seqlens, block_indices, k_scale,
-                 v_scale, sinks, cu_seqlens_q)
+    (rows, hq, d), q_stride, out_stride, (nb, bs, hk, _), tag = \
+        _check_page_attn(what, out, q, k_cache, v_cache)
+    shape, i_row, i_head = _check_grid(what, block_indices, "block_indices", torch.int32, "keep")
+    keep = shape[2]
+    if shape[0] != rows or shape[1] != hk:
+        raise ValueError(f"{what}: block_indices must be [{rows}, {hk}, keep]")
+    ks = _check_scale(what, k_scale, "k_scale", hk)
+    vs = _check_scale(what, v_scale, "v_scale", hk)
+    sink = _check_scale(what, sinks, "sinks", hq)
+    batch = _check_batch(what, cache_seqlens, cu_seqlens_q, rows)
+    bt_stride, bt_width = _check_table(what, block_table, batch)
+    dev = _same_device(out, q, k_cache, v_cache, block_table, cache_seqlens, block_indices,
+                       k_scale, v_scale, sinks, cu_seqlens_q)
     if rows == 0 or batch == 0:
         return
-    keep = block_indices.shape[2]
-    nbytes = _native.sparse_decode_bytes(rows, keep, hq, hk, d, bs)
+    nbytes = _plan_bytes(dev, _native.sparse_decode_bytes, rows, keep, hq, hk, d, bs)
     ws = torch.empty(nbytes, dtype=torch.uint8, device=q.device) if nbytes else None
-    _call_on(q, "fk_sparse_paged_decode", out.data_ptr(), out.stride(0), q.data_ptr(),
-             q.stride(0), k_cache.data_ptr(), v_cache.data_ptr(), tag, _ptr(k_scale),
-             _ptr(v_scale), block_table.data_ptr(), block_table.stride(0), block_table.shape[1],
-             cache_seqlens.data_ptr(), _ptr(cu_seqlens_q), batch, rows, block_indices.data_ptr(),
-             block_indices.stride(0), block_indices.stride(1), keep, hq, hk, d, bs, nb,
-             float(softmax_scale), _ptr(sinks), _ptr(ws), nbytes)
+    _call_on(q, dev, "fk_sparse_paged_decode", out.data_ptr(), out_stride, q.data_ptr(),
+             q_stride, k_cache.data_ptr(), v_cache.data_ptr(), tag, ks, vs,
+             block_table.data_ptr(), bt_stride, bt_width, cache_seqlens.data_ptr(),
+             _ptr(cu_seqlens_q), batch, rows, block_indices.data_ptr(), i_row, i_head, keep, hq,
+             hk, d, bs, nb, float(softmax_scale), sink, _ptr(ws), nbytes)
 
 
 def shared_prefix_decode(out: torch.Tensor, q: torch.Tensor, k_cache: torch.Tensor,
@@ -931,33 +954,36 @@ def shared_prefix_decode(out: torch.Tensor, q: torch.Tensor, k_cache: torch.Tens
     group's prefix.  max_prefix_len bounds every prefix (0: unknown); it only chooses the
     launch shape."""
     what = "shared_prefix_decode"
-    tag = _check_page_attn(what, out, q, k_cache, v_cache, k_scale, v_scale, sinks)
-    rows, hq, d = q.shape
-    nb, bs, hk, _ = k_cache.shape
+    (rows, hq, d), q_stride, out_stride, (nb, bs, hk, _), tag = \
+        _check_page_attn(what, out, q, k_cache, v_cache)
+    ks = _check_scale(what, k_scale, "k_scale", hk)
+    vs = _check_scale(what, v_scale, "v_scale", hk)
+    sink = _check_scale(what, sinks, "sinks", hq)
     for t, name in ((cu_groups, "cu_groups [groups + 1]"), (prefix_lens, "prefix_lens [groups]")):
         if t.dtype != torch.int32 or t.dim() != 1 or not t.is_contiguous():
             raise TypeError(f"{what}: {name} must be contiguous int32")
     groups = cu_groups.numel() - 1
     if groups < 0 or prefix_lens.numel() < groups:
         raise ValueError(f"{what}: prefix_lens shorter than the groups")
-    if int(window_left) < -1:
+    window_left, max_prefix_len = int(window_left), int(max_prefix_len)
+    if window_left < -1:
         raise ValueError(f"{what}: window_left must be -1 (no window) or >= 0")
-    if int(max_prefix_len) < 0:
+    if max_prefix_len < 0:
         raise ValueError(f"{what}: max_prefix_len must be >= 0")
-    _check_table(what, block_table, cache_seqlens, None, rows)
-    _same_device(out, q, k_cache, v_cache, block_table, cache_seqlens, cu_groups, prefix_lens,
-                 k_scale, v_scale, sinks)
+    batch = _check_batch(what, cache_seqlens, None, rows)
+    bt_stride, bt_width = _check_table(what, block_table, batch)
+    dev = _same_device(out, q, k_cache, v_cache, block_table, cache_seqlens, cu_groups,
+                       prefix_lens, k_scale, v_scale, sinks)
     if rows == 0:
         return
-    bound = int(max_prefix_len)
-    nbytes = _native.shared_prefix_bytes(rows, groups, bound, hq, hk, d)
-    ws = torch.empty(nbytes, dtype=torch.uint8, device=q.device) if nbytes else None
-    _call_on(q, "fk_shared_prefix_decode", out.data_ptr(), out.stride(0), q.data_ptr(),
-             q.stride(0), k_cache.data_ptr(), v_cache.data_ptr(), tag, _ptr(k_scale),
-             _ptr(v_scale), block_table.data_ptr(), block_table.stride(0), block_table.shape[1],
-             cache_seqlens.data_ptr(), rows, cu_groups.data_ptr(), prefix_lens.data_ptr(), groups,
-             bound, hq, hk, d, bs, nb, float(softmax_scale), int(window_left), _ptr(sinks),
-             _ptr(ws), nbytes)
+    nbytes = _plan_bytes(dev, _native.shared_prefix_bytes, rows, groups, max_prefix_len, hq, hk,
+                         d)
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=q.device)
+    _call_on(q, dev, "fk_shared_prefix_decode", out.data_ptr(), out_stride, q.data_ptr(),
+             q_stride, k_cache.data_ptr(), v_cache.data_ptr(), tag, ks, vs,
+             block_table.data_ptr(), bt_stride, bt_width, cache_seqlens.data_ptr(), rows,
+             cu_groups.data_ptr(), prefix_lens.data_ptr(), groups, max_prefix_len, hq, hk, d, bs,
+             nb, float(softmax_scale), window_left, sink, ws.data_ptr(), nbytes)
 
 
 # ---------------------------------------------------------------------------
