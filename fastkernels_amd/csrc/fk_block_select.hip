@@ -328,7 +328,8 @@ struct SelectParams {
 };
 
 constexpr int kSelThreads = 512;
-constexpr int kSelBins = 2048;  // 11 bits of a key
+constexpr int kSelBins = 2048;  // 11 bits of a key: four bins a thread
+static_assert(kSelBins == 4 * kSelThreads, "four bins a thread");
 // Keys held in LDS (one word in 17 is left free, so that threads reading runs of keys meet
 // different banks); rows with more pages are read from memory in every pass.
 constexpr int kSelLdsKeys = 32768;
@@ -341,26 +342,36 @@ __device__ __forceinline__ uint32_t score_key(float s) {
   return u ^ ((u >> 31) ? 0xffffffffu : 0x80000000u);
 }
 
-// Inclusive sum over the work-group's threads; `total`: over all of them.  part: one word per
-// wave, not in use since the barrier before the last.
-__device__ __forceinline__ int scan_threads(int v, int* part, int tid, int& total) {
+// Inclusive sum over the lanes of a wave: within rows of 16, then across them.
+template <int kCtrl, int kRows>
+__device__ __forceinline__ int plus_dpp(int v) {
+  return v + __builtin_amdgcn_update_dpp(0, v, kCtrl, kRows, 0xf, false);
+}
+__device__ __forceinline__ int scan_lanes(int v) {
+  v = plus_dpp<0x111, 0xf>(v);     // from the lane 1 before, 2, 4, 8
+  v = plus_dpp<0x112, 0xf>(v);
+  v = plus_dpp<0x114, 0xf>(v);
+  v = plus_dpp<0x118, 0xf>(v);
+  v = plus_dpp<0x142, 0xa>(v);     // from lane 15 of the row before, into rows 1 and 3
+  return plus_dpp<0x143, 0xc>(v);  // from lane 31, into rows 2 and 3
+}
+// Inclusive sums over the work-group's threads.  part: a word per wave and value, not in use
+// since the barrier before the last.
+template <int kN>
+__device__ __forceinline__ void scan_threads(int (&v)[kN], int (*part)[kSelThreads / 64],
+                                             int tid) {
   constexpr int kWaves = kSelThreads / 64;
   const int lane = tid & 63, wave = tid >> 6;
 #pragma unroll
-  for (int off = 1; off < 64; off <<= 1) {
-    const int y = __shfl_up(v, off, 64);
-    if (lane >= off) v += y;
+  for (int i = 0; i < kN; ++i) {
+    v[i] = scan_lanes(v[i]);
+    if (lane == 63) part[i][wave] = v[i];
   }
-  if (lane == 63) part[wave] = v;
   __syncthreads();
-  int before = 0;
-  total = 0;
 #pragma unroll
-  for (int w = 0; w < kWaves; ++w) {
-    before += w < wave ? part[w] : 0;
-    total += part[w];
-  }
-  return v + before;
+  for (int i = 0; i < kN; ++i)
+#pragma unroll
+    for (int w = 0; w < kWaves; ++w) v[i] += w < wave ? part[i][w] : 0;
 }
 
 // One work-group per (query row, kv head).  The key T of the lowest selected candidate is
@@ -388,11 +399,21 @@ __global__ __launch_bounds__(kSelThreads) void select_blocks_kernel(
     return;
   }
   auto key_of = [&](int j) { return kLds ? keys[sel_at(j)] : score_key(row[j]); };
+#pragma unroll
+  for (int i = 0; i < 4; ++i) hist[4 * tid + i] = 0;
   if constexpr (kLds) {
-#pragma unroll 4
-    for (int j = tid; j < n; j += kSelThreads) keys[sel_at(j)] = score_key(row[j]);
-    __syncthreads();
+    // (kAhead loads in flight; those past the end read the last score once more)
+    constexpr int kAhead = 8;
+    for (int j0 = tid; j0 < n; j0 += kAhead * kSelThreads) {
+      float s[kAhead];
+#pragma unroll
+      for (int u = 0; u < kAhead; ++u) s[u] = row[min(j0 + u * kSelThreads, n - 1)];
+#pragma unroll
+      for (int u = 0; u < kAhead; ++u)
+        if (j0 + u * kSelThreads < n) keys[sel_at(j0 + u * kSelThreads)] = score_key(s[u]);
+    }
   }
+  __syncthreads();
   const int first = P.keep_first, last = n - P.keep_last;  // candidates [first, last)
   int need = P.keep - P.keep_first - P.keep_last;          // of which so many are selected
   uint32_t digits = 0, known = 0;  // T, and the bits of it that count
@@ -403,23 +424,24 @@ __global__ __launch_bounds__(kSelThreads) void select_blocks_kernel(
   for (int pass = 0; pass < 3 && !whole; ++pass) {
     const int shift = pass == 0 ? 21 : pass == 1 ? 10 : 0;
     const uint32_t mask = pass == 2 ? 1023u : 2047u;
-    for (int k = tid; k < kSelBins; k += kSelThreads) hist[k] = 0;
-    __syncthreads();
 #pragma unroll 4
     for (int j = first + tid; j < last; j += kSelThreads) {
       const uint32_t key = key_of(j);
       if ((key & known) == digits) atomicAdd(&hist[(key >> shift) & mask], 1);
     }
     __syncthreads();
-    // Thread k sums bins 2047 - 4 k .. 2044 - 4 k: the inclusive sum counts from the top.
-    int bins[4], sum = 0;
+    // Thread k sums bins 2047 - 4 k .. 2044 - 4 k (and clears them for the next digit): the
+    // inclusive sum counts from the top.
+    int bins[4], sum[1] = {0};
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       bins[i] = hist[kSelBins - 1 - 4 * tid - i];
-      sum += bins[i];
+      hist[kSelBins - 1 - 4 * tid - i] = 0;
+      sum[0] += bins[i];
     }
-    int total;
-    int above = scan_threads(sum, part[0], tid, total) - sum;
+    int above = -sum[0];
+    scan_threads(sum, part, tid);
+    above += sum[0];
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       if (above < need && above + bins[i] >= need) {
@@ -440,27 +462,46 @@ __global__ __launch_bounds__(kSelThreads) void select_blocks_kernel(
   // Keys whose known digits exceed T's, and the first equal_need of those with T's.
   const int per = (n + kSelThreads - 1) / kSelThreads;
   const int j0 = min(n, tid * per), j1 = min(n, j0 + per);
+  // (from LDS a run is 64 keys at most: what is selected of it is noted in bits, and the second
+  // walk only meets those)
+  uint64_t above_bits = 0, equal_bits = 0;
   int above = 0, equal = 0;
 #pragma unroll 4
   for (int j = j0; j < j1; ++j) {
     const bool cand = j >= first && j < last;
     const uint32_t key = cand ? key_of(j) & known : 0;
-    above += !cand || key > digits;
-    equal += cand && key == digits;
+    const bool up = !cand || key > digits, eq = cand && key == digits;
+    above += up;
+    equal += eq;
+    if (kLds) {
+      above_bits |= static_cast<uint64_t>(up) << (j - j0);
+      equal_bits |= static_cast<uint64_t>(eq) << (j - j0);
+    }
   }
-  int total;
-  const int equal_before = scan_threads(equal, part[1], tid, total) - equal;
-  const int take_equal = min(max(equal_need - equal_before, 0), equal);
-  int at = scan_threads(above + take_equal, part[0], tid, total) - above - take_equal;
-  int left = take_equal;
-  for (int j = j0; j < j1; ++j) {
-    const bool cand = j >= first && j < last;
-    const uint32_t key = cand ? key_of(j) & known : 0;
-    const bool eq = cand && key == digits;
-    if (!cand || key > digits || (eq && left > 0)) {
-      if (at < P.keep) out[at] = j;
-      ++at;
+  int before[2] = {above, equal};
+  scan_threads(before, part, tid);
+  const int equal_before = before[1] - equal;
+  int left = min(max(equal_need - equal_before, 0), equal);
+  int at = before[0] - above + min(equal_before, equal_need);
+  if constexpr (kLds) {
+    for (uint64_t bits = left > 0 ? above_bits | equal_bits : above_bits; bits; bits &= bits - 1) {
+      const int k = __builtin_ctzll(bits);
+      const bool eq = equal_bits >> k & 1;
+      if (eq && left == 0) continue;
       left -= eq;
+      if (at < P.keep) out[at] = j0 + k;
+      ++at;
+    }
+  } else {
+    for (int j = j0; j < j1; ++j) {
+      const bool cand = j >= first && j < last;
+      const uint32_t key = cand ? key_of(j) & known : 0;
+      const bool eq = cand && key == digits;
+      if (!cand || key > digits || (eq && left > 0)) {
+        if (at < P.keep) out[at] = j;
+        ++at;
+        left -= eq;
+      }
     }
   }
 }
