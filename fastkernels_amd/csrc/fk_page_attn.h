@@ -48,6 +48,39 @@ struct PageAttnParams {
 constexpr float kLazyMax = 8.f;
 constexpr float kNoMax = -1.0e30f;  // the reference before a column's first visible key
 
+// K rows on their way to the scores' operand.  The operand has a key per lane (lane (r, g): 16
+// bytes at 64 c + 16 g of key r), so that loads straight into it meet another row with every
+// lane, and the cache takes them one lane at a time; and each of them takes half a cache line,
+// whose other half then waits behind the first's miss.  They are loaded in whole rows instead,
+// and a round trip through the wave's own LDS turns them.  There, chunk c holds bytes 64 c ..
+// 64 c + 63 of the 16 rows; a row's four pieces are rotated by half its number, and rows trade
+// places with their neighbours in odd chunks, so that neither side has bank conflicts.
+template <bool kFp8, int D>
+struct KChunks {
+  static constexpr int kLoads = DTile<kFp8, D>::kKLoads;
+  static constexpr int kBytes = 1024 * kLoads;  // of a tile
+  static constexpr int kPieces = 4 * kLoads;    // 16-byte pieces of a row
+  static constexpr int kRows = 64 / kPieces;    // rows per load
+  static __device__ __forceinline__ int at(int row, int chunk, int piece) {
+    return 1024 * chunk + 64 * (row ^ (chunk & 1)) + 16 * ((piece + (row >> 1)) & 3);
+  }
+  static __device__ __forceinline__ void put(const DTile<kFp8, D>& t, uint8_t* kx, int lane) {
+    const int piece = lane % kPieces;
+#pragma unroll
+    for (int i = 0; i < kLoads; ++i)
+      *reinterpret_cast<uint4*>(kx + at(kRows * i + lane / kPieces, piece >> 2, piece & 3)) =
+          t.k[i];
+  }
+  // As bf16 operands: of fp8 rows, operand 2 c + h is dims 64 c + 16 g + 8 h .. + 7.
+  static __device__ __forceinline__ void get(const uint8_t* kx, int lane, uint4 (&k)[D / 32]) {
+    DTile<kFp8, D> t;
+#pragma unroll
+    for (int c = 0; c < kLoads; ++c)
+      t.k[c] = *reinterpret_cast<const uint4*>(kx + at(lane & 15, c, lane >> 4));
+    k_chunks_d(t, k);
+  }
+};
+
 template <int kCB, int D, bool kFp8>
 struct ColumnState {
   static constexpr int kKc = D / 32;
@@ -71,19 +104,19 @@ struct ColumnState {
                                          int g) {
 #pragma unroll
     for (int c = 0; c < kKc; ++c) {
-      const int d0 = kFp8 ? (D / 4) * g + 8 * c : 32 * c + 8 * g;
+      const int d0 = kFp8 ? 64 * (c >> 1) + 16 * g + 8 * (c & 1) : 32 * c + 8 * g;
       uint4 v = ok ? *reinterpret_cast<const uint4*>(qp + d0) : make_uint4(0, 0, 0, 0);
       v = make_uint4(v.x ^ flip, v.y ^ flip, v.z ^ flip, v.w ^ flip);
       qb[cb][c] = __builtin_bit_cast(bf16x8_t, v);
     }
   }
 
-  // Scores of two tiles (their K rows in a and b).
-  __device__ __forceinline__ void scores(const DTile<kFp8, D>& a, const DTile<kFp8, D>& b,
-                                         floatx4_t (&sa)[kCB], floatx4_t (&sb)[kCB]) const {
+  // Scores of two tiles, whose K rows are in the wave's LDS kx (KChunks).
+  __device__ __forceinline__ void scores(const uint8_t* kx, int lane, floatx4_t (&sa)[kCB],
+                                         floatx4_t (&sb)[kCB]) const {
     uint4 ka[kKc], kb[kKc];
-    k_chunks_d(a, ka);
-    k_chunks_d(b, kb);
+    KChunks<kFp8, D>::get(kx, lane, ka);
+    KChunks<kFp8, D>::get(kx + KChunks<kFp8, D>::kBytes, lane, kb);
 #pragma unroll
     for (int cb = 0; cb < kCB; ++cb) {
       sa[cb] = qk_scores_n(ka, qb[cb]);
@@ -191,11 +224,14 @@ struct ColumnState {
 // Where a wave's lanes read a tile: byte offsets from the tile's first row of the kv head.
 template <bool kFp8, int D>
 struct TileLanes {
-  uint32_t k, v[4];
-  __device__ __forceinline__ TileLanes(int num_kv_heads, int r, int g) {
+  uint32_t k, k_step, v[4];
+  __device__ __forceinline__ TileLanes(int num_kv_heads, int lane) {
     constexpr int kElt = kFp8 ? 1 : 2;
+    using K = KChunks<kFp8, D>;
+    const int r = lane & 15, g = lane >> 4;
     const uint32_t row = static_cast<uint32_t>(num_kv_heads) * D * kElt;
-    k = r * row + (kFp8 ? (D / 4) * g : 16 * g);
+    k = lane / K::kPieces * row + 16 * (lane % K::kPieces);
+    k_step = K::kRows * row;
 #pragma unroll
     for (int i = 0; i < 4; ++i) v[i] = (4 * g + i) * row + (D / 16) * r * kElt;
   }
@@ -205,7 +241,8 @@ template <bool kFp8, int D>
 __device__ __forceinline__ void load_tile_k(const uint8_t* row, const TileLanes<kFp8, D>& at,
                                             DTile<kFp8, D>& t) {
 #pragma unroll
-  for (int c = 0; c < DTile<kFp8, D>::kKLoads; ++c) t.k[c] = ld16(row + at.k + (kFp8 ? 16 : 64) * c);
+  for (int i = 0; i < DTile<kFp8, D>::kKLoads; ++i)
+    t.k[i] = ld16(row + static_cast<int64_t>(i) * at.k_step + at.k);
 }
 template <bool kFp8, int D>
 __device__ __forceinline__ void load_tile_v(const uint8_t* row, const TileLanes<kFp8, D>& at,
@@ -238,11 +275,11 @@ __device__ __forceinline__ void stream_units(const PageAttnParams& P,
                                              ColumnState<kCB, D, kFp8>& st, UnitAt unit_at,
                                              int units, int first, int step, int unit_tiles_log2,
                                              int from, int to, LimitsOf limits, int kvh, float s2,
-                                             int lane) {
+                                             uint8_t* kx, int lane) {
   constexpr int kElt = kFp8 ? 1 : 2;
-  const int r = lane & 15, g = lane >> 4;
+  const int g = lane >> 4;
   const int page_mask = (1 << P.block_size_log2) - 1;
-  const TileLanes<kFp8, D> at(P.num_kv_heads, r, g);
+  const TileLanes<kFp8, D> at(P.num_kv_heads, lane);
   const int64_t row_bytes = static_cast<int64_t>(P.num_kv_heads) * D * kElt;
   const uint8_t* const kh = P.k_cache + static_cast<int64_t>(kvh) * D * kElt;
   const uint8_t* const vh = P.v_cache + static_cast<int64_t>(kvh) * D * kElt;
@@ -286,7 +323,8 @@ __device__ __forceinline__ void stream_units(const PageAttnParams& P,
     }
     for (int x = 0; x < tiles; x += 2) {
       floatx4_t sa[kCB], sb[kCB];
-      st.scores(a, b, sa, sb);
+      KChunks<kFp8, D>::put(a, kx, lane);
+      KChunks<kFp8, D>::put(b, kx + KChunks<kFp8, D>::kBytes, lane);
       // (past the last tiles, these are read once more: the number of loads in flight stays
       // known to the compiler's wait counts)
       uint32_t na, nb;
@@ -294,6 +332,8 @@ __device__ __forceinline__ void stream_units(const PageAttnParams& P,
       at_b = row_of(min(x + 3, tiles - 1), nb);
       load_tile_k(kh + at_a, at, a);
       load_tile_k(kh + at_b, at, b);
+      loads_issued();
+      st.scores(kx, lane, sa, sb);
       loads_issued();
       if (x + 1 >= tiles) rb = lm.span;  // no second tile: masked
       const bool full = ra < lm.least && lm.least - ra >= kTile && rb < lm.least &&
@@ -311,8 +351,8 @@ __device__ __forceinline__ void stream_units(const PageAttnParams& P,
 
 // Merges the waves' states of all column blocks and hands each quad of adjacent dims of each
 // of the ncols columns to emit(column, dim, o, M, L): o = O[dim .. dim + 3] before the division.
-// lds: merge_lds_floats(16 kCB columns at most); every thread of the work-group calls it, and
-// may write to lds again only after a barrier.
+// lds: merge_lds_floats(16 kCB columns at most), of the waves' K rows until all have come here;
+// every thread of the work-group calls it, and may write to lds again only after a barrier.
 template <int kWaves, int D>
 constexpr int merge_lds_floats(int cols) { return kWaves * cols * (D + 4 + 2); }
 template <int kWaves, int kCB, int D, bool kFp8, class Emit>
@@ -322,6 +362,7 @@ __device__ __forceinline__ void merge_waves(const ColumnState<kCB, D, kFp8>& st,
   constexpr int kSl = D / 16;
   const int r = lane & 15, g = lane >> 4;
   float2* const xm = reinterpret_cast<float2*>(lds + kWaves * ncols * kRow);  // (m, l)
+  __syncthreads();  // lds was the waves' K rows
 #pragma unroll
   for (int cb = 0; cb < kCB; ++cb) {
     const float l = pair_sum(st.l[cb]);

@@ -42,7 +42,7 @@ struct RowRecord {
   int64_t own_start;  // the row's first tile on the own line (its first head's)
   int64_t pre_start;  // its group's first tile on the prefix line
   int64_t own_range, pre_range;  // tiles of a range of each line
-  int64_t own_step, pre_step;    // places of an item on its line
+  int64_t pre_step;              // places of a prefix item
   int own_tiles;      // tiles per head (0: nothing of its own)
   int pre_tiles;      // tiles of the prefix (0: no shared prefix)
   int pre_item;       // its group's first prefix item
@@ -82,6 +82,11 @@ struct Own {
 __device__ __forceinline__ int tiles_in(int tokens) {
   return tokens > 0 ? (tokens - 1) / kTile + 1 : 0;
 }
+// The places of a prefix item on its line: its tiles, rounded up so that the ranges of a short
+// line do not span two items.
+__device__ __forceinline__ int64_t places_of(int prefix) {
+  return (tiles_in(prefix) + kPreTiles - 1) & -kPreTiles;
+}
 __device__ __forceinline__ int64_t lane64(int64_t v, int src) {
   const uint32_t lo = __builtin_amdgcn_readlane(static_cast<int>(v), src);
   const uint32_t hi = __builtin_amdgcn_readlane(static_cast<int>(v >> 32), src);
@@ -96,22 +101,22 @@ __device__ __forceinline__ int64_t scan64(int64_t v, int lane) {
   }
   return v;
 }
-// How a line of `total` tiles in `items` items is cut into at most n ranges of `range` tiles (a
-// multiple of `quantum`); pad: items take whole ranges, which may add one range each.
-struct Cut {
-  int64_t range;
-  bool pad;
-  __device__ __forceinline__ Cut(int64_t total, int64_t items, int n, int quantum) {
-    pad = items <= n / 2;
-    // (the quotient is off by less than the one that is added)
-    range = static_cast<int64_t>(static_cast<double>(total) /
-                                 static_cast<double>(pad ? n - items : n)) + 1;
-    range = (range + quantum - 1) / quantum * quantum;
-  }
-  __device__ __forceinline__ int64_t step(int tiles) const {
-    return pad ? (tiles + range - 1) / range * range : tiles;
-  }
-};
+// A line of `total` tiles is cut into ranges of the least multiple of `quantum` (a power of two)
+// that makes them at most n.
+__device__ __forceinline__ int64_t range_of(int64_t total, int n, int quantum) {
+  int64_t range = static_cast<int64_t>(static_cast<double>(total) / n);
+  range += range * n < total;  // (the quotient is off by less than one)
+  range = (range + quantum - 1) & -static_cast<int64_t>(quantum);
+  return max(range, static_cast<int64_t>(quantum));
+}
+// a / b (0 <= a, 0 < b) by way of a float estimate, off by one at most for quotients below 2^21.
+__device__ __forceinline__ int quotient(int64_t a, int64_t b) {
+  int64_t q = static_cast<int64_t>(static_cast<float>(a) *
+                                   __builtin_amdgcn_rcpf(static_cast<float>(b)));
+  while (q * b > a) --q;
+  while ((q + 1) * b <= a) ++q;
+  return static_cast<int>(q);
+}
 // The share of a line that work-group `wg` of n takes, when it has `shares` of them (n or more:
 // none).  They are dealt out to the 8 XCDs in runs (work-groups go to XCDs in turn), so that
 // neighbouring ranges, which read the same keys for the column blocks of a group, share an L2;
@@ -129,6 +134,10 @@ template <int D>
 constexpr int lds_rows_at() { return 4 * merge_lds_floats<kWaves, D>(cols_of(D)); }
 template <int D>
 constexpr int lds_groups_at() { return lds_rows_at<D>() + kThreads * static_cast<int>(sizeof(Own)); }
+static_assert(kWaves * 2 * KChunks<false, 64>::kBytes <= lds_rows_at<64>() &&
+                  kWaves * 2 * KChunks<false, 128>::kBytes <= lds_rows_at<128>() &&
+                  kWaves * 2 * KChunks<false, 256>::kBytes <= lds_rows_at<256>(),
+              "the waves' K rows fit");
 static_assert(kMaxGroups * 12 <= lds_groups_at<64>(), "the last work-group's tables fit");
 
 template <int D, bool kFp8>
@@ -215,14 +224,13 @@ __attribute__((amdgpu_waves_per_eu((D == 256 ? 1 : 2)))) void shared_prefix_kern
     __syncthreads();
     return before + x;
   };
-  auto prefix_cut = [&] {
-    int64_t sum = 0, n = 0;
+  auto prefix_length = [&] {
+    int64_t sum = 0;
     for (int i = lane; i < P.num_groups; i += 64) {
       const Group x = group_at(i);
-      sum += static_cast<int64_t>(group_items(x)) * tiles_in(x.prefix);
-      n += group_items(x);
+      sum += group_items(x) * places_of(x.prefix);
     }
-    return Cut(lane64(scan64(sum, lane), 63), lane64(scan64(n, lane), 63), P.wgs, kPreTiles);
+    return lane64(scan64(sum, lane), 63);
   };
   // Streams positions [from, to) of one item through the table `table`: unit `first` and every
   // step-th after it.
@@ -235,7 +243,8 @@ __attribute__((amdgpu_waves_per_eu((D == 256 ? 1 : 2)))) void shared_prefix_kern
       page = j < A.bt_width ? table[j] : -1;
     };
     stream_units(A, st, unit_at, from < to ? ((to - 1) >> tok_log2) + 1 - u0 : 0, first, step,
-                 P.unit_tiles_log2, from, to, limits, kvh, s2, lane);
+                 P.unit_tiles_log2, from, to, limits, kvh, s2,
+                 lds_all + wave * 2 * KChunks<kFp8, D>::kBytes, lane);
   };
   auto factor = [&](int kvh) {
     return kFp8 && A.k_scale ? A.scale_log2 * A.k_scale[kvh] : A.scale_log2;
@@ -243,23 +252,16 @@ __attribute__((amdgpu_waves_per_eu((D == 256 ? 1 : 2)))) void shared_prefix_kern
 
   const int wg = blockIdx.x;
   auto run_prefix = [&] {
-    const Cut cut = prefix_cut();
-    const int64_t S = cut.range;
-    // (all ranges, each of them some work-group's: those past the line's end are empty)
+    const int64_t total = prefix_length();
+    const int64_t S = range_of(total, P.wgs, kPreTiles);
     int64_t line = 0;  // tiles and items of the groups before the chunk
     int64_t item0 = 0;
-    int64_t total = 0;
-    for (int i = lane; i < P.num_groups; i += 64) {
-      const Group x = group_at(i);
-      total += group_items(x) * cut.step(tiles_in(x.prefix));
-    }
-    total = lane64(scan64(total, lane), 63);
-    const int64_t w = share_of(wg, P.wgs, (total + S - 1) / S, false);
+    const int64_t w = share_of(wg, P.wgs, quotient(total + S - 1, S), false);
     const int64_t t_lo = w * S, t_hi = min(total, t_lo + S);
     for (int g0 = 0; t_lo < total && g0 < P.num_groups && line < t_hi; g0 += 64) {
       const Group x = group_at(g0 + lane);
       const int items = group_items(x);
-      const int64_t mine = items * cut.step(tiles_in(x.prefix));
+      const int64_t mine = items * places_of(x.prefix);
       const int64_t end = line + scan64(mine, lane);
       const int64_t item_end = item0 + scan64(items, lane);
       uint64_t hit = __ballot(mine > 0 && end > t_lo && end - mine < t_hi);
@@ -272,16 +274,15 @@ __attribute__((amdgpu_waves_per_eu((D == 256 ? 1 : 2)))) void shared_prefix_kern
         const int n_items = __builtin_amdgcn_readlane(items, src);
         const int64_t start = lane64(end - mine, src);
         const int64_t first_item = lane64(item_end, src) - n_items;
-        const int64_t step = cut.step(tiles_in(prefix));
+        const int64_t step = places_of(prefix);
         const int col_items = n_items / A.num_kv_heads;
-        for (int it = t_lo > start ? static_cast<int>((t_lo - start) / step) : 0;
+        for (int it = t_lo > start ? quotient(t_lo - start, step) : 0;
              it < n_items && start + it * step < t_hi; ++it) {
           const int64_t at = start + it * step;
           const int from = static_cast<int>(
               min(static_cast<int64_t>(prefix), (max(t_lo, at) - at) * kTile));
           const int to = static_cast<int>(
               min(static_cast<int64_t>(prefix), (min(t_hi, at + step) - at) * kTile));
-          if (from >= to) continue;
           const int kvh = it / col_items;
           const int col0 = (it - kvh * col_items) * kCols;
           const float s2 = factor(kvh);
@@ -298,28 +299,39 @@ __attribute__((amdgpu_waves_per_eu((D == 256 ? 1 : 2)))) void shared_prefix_kern
             st.load_q(cb, A.q + b * A.q_row_stride + static_cast<int64_t>(hq) * D, ok,
                       s2 < 0.f ? 0x80008000u : 0u, g);
           }
-          auto limits = [&] {
-            Limits<kCB> x;
-            x.span = 0;
-            x.least = to - from;
+          // From the first multiple of the range's length on, then what is before it: so that
+          // at any time all ranges are as far past such a multiple, and the column blocks of a
+          // kv head, whose ranges begin anywhere, read the same tiles while the L2 holds them.
+          const int64_t length = S * kTile;
+          const int turn = static_cast<int>(min(
+              static_cast<int64_t>(to), quotient(from + length - 1, length) * length));
+#pragma unroll 1
+          for (int part = 0; part < 2; ++part) {
+            const int lo = part ? from : turn, hi = part ? turn : to;
+            if (lo >= hi) continue;
+            auto limits = [&] {
+              Limits<kCB> x;
+              x.span = 0;
+              x.least = hi - lo;
 #pragma unroll
-            for (int cb = 0; cb < kCB; ++cb) {
-              const bool ok = col0 + 16 * cb + r < n_cols;
-              x.lim[cb] = ok ? max(min(to, seen[cb]) - from, 0) : to - from;
-              x.span = max(x.span, ok ? x.lim[cb] : 0u);
-              x.least = min(x.least, x.lim[cb]);
-            }
+              for (int cb = 0; cb < kCB; ++cb) {
+                const bool ok = col0 + 16 * cb + r < n_cols;
+                x.lim[cb] = ok ? max(min(hi, seen[cb]) - lo, 0) : hi - lo;
+                x.span = max(x.span, ok ? x.lim[cb] : 0u);
+                x.least = min(x.least, x.lim[cb]);
+              }
 #pragma unroll
-            for (int off = 1; off < 16; off <<= 1) {
-              x.span = max(x.span, static_cast<uint32_t>(__shfl_xor(x.span, off, 64)));
-              x.least = min(x.least, static_cast<uint32_t>(__shfl_xor(x.least, off, 64)));
-            }
-            x.span = uniform(x.span);
-            x.least = uniform(x.least);
-            return x;
-          };
-          stream(st, bt + row0 * A.bt_row_stride, from, to, wave, kWaves, limits, kvh,
-                 __builtin_fabsf(s2));
+              for (int off = 1; off < 16; off <<= 1) {
+                x.span = max(x.span, static_cast<uint32_t>(__shfl_xor(x.span, off, 64)));
+                x.least = min(x.least, static_cast<uint32_t>(__shfl_xor(x.least, off, 64)));
+              }
+              x.span = uniform(x.span);
+              x.least = uniform(x.least);
+              return x;
+            };
+            stream(st, bt + row0 * A.bt_row_stride, lo, hi, wave, kWaves, limits, kvh,
+                   __builtin_fabsf(s2));
+          }
           const int64_t piece = w + first_item + it;
           if (piece >= P.pre_pieces) continue;  // (groups that overlap: beyond the plan)
           float* po = P.pre_o + piece * kCols * D;
@@ -346,27 +358,20 @@ __attribute__((amdgpu_waves_per_eu((D == 256 ? 1 : 2)))) void shared_prefix_kern
     for (int b = kThreads + threadIdx.x; b < A.batch; b += kThreads) sum += own_at(b).tiles;
     scan_all(sum, own_total);
   }
-  const Cut own_cut(own_total * P.vheads, static_cast<int64_t>(A.batch) * P.vheads,
-                    kWaves * P.wgs, kOwnTiles);
-  if (own_cut.pad) {
-    int64_t sum = own_cut.step(own0.tiles);
-    for (int b = kThreads + threadIdx.x; b < A.batch; b += kThreads)
-      sum += own_cut.step(own_at(b).tiles);
-    scan_all(sum, own_total);
-  }
   own_total *= P.vheads;
+  const int64_t own_range = range_of(own_total, kWaves * P.wgs, kOwnTiles);
 
   auto run_own = [&] {
-    const int64_t S = own_cut.range;
+    const int64_t S = own_range;
     const int64_t w0 =
-        kWaves * share_of(wg, P.wgs, (own_total + kWaves * S - 1) / (kWaves * S), true);
+        kWaves * share_of(wg, P.wgs, quotient(own_total + kWaves * S - 1, kWaves * S), true);
     const int64_t all_hi = min(own_total, (w0 + kWaves) * S);  // of the work-group
     const int64_t w = w0 + wave;
     const int64_t t_lo = w * S, t_hi = min(own_total, t_lo + S);
     int64_t line = 0;
     for (int b0 = 0; w0 * S < own_total && b0 < A.batch && line < all_hi; b0 += kThreads) {
       Own o = b0 == 0 ? own0 : own_at(b0 + threadIdx.x);
-      const int64_t mine = own_cut.step(o.tiles) * P.vheads;
+      const int64_t mine = static_cast<int64_t>(o.tiles) * P.vheads;
       int64_t sum;
       const int64_t end = line + scan_all(mine, sum);
       line += sum;
@@ -390,13 +395,11 @@ __attribute__((amdgpu_waves_per_eu((D == 256 ? 1 : 2)))) void shared_prefix_kern
           x.first_row = uniform(x.first_row);
           x.tiles = uniform(x.tiles);
           x.start = lane64(x.start, 0);
-          const int64_t step = own_cut.step(x.tiles);
           const int tile0 = x.from / kTile;
-          for (int v = t_lo > x.start ? static_cast<int>((t_lo - x.start) / step) : 0;
-               v < P.vheads && x.start + v * step < t_hi; ++v) {
-            const int64_t at = x.start + v * step;
-            const int64_t k_lo = max(t_lo, at) - at, k_hi = min(t_hi, at + step) - at;
-            if (k_lo >= x.tiles) continue;
+          for (int v = t_lo > x.start ? quotient(t_lo - x.start, x.tiles) : 0;
+               v < P.vheads && x.start + static_cast<int64_t>(v) * x.tiles < t_hi; ++v) {
+            const int64_t at = x.start + static_cast<int64_t>(v) * x.tiles;
+            const int64_t k_lo = max(t_lo, at) - at, k_hi = min(t_hi, at + x.tiles) - at;
             const int from = max(x.from, kTile * (tile0 + static_cast<int>(k_lo)));
             const int to = static_cast<int>(
                 min(static_cast<int64_t>(x.ctx), (tile0 + k_hi) * int64_t{kTile}));
@@ -432,13 +435,13 @@ __attribute__((amdgpu_waves_per_eu((D == 256 ? 1 : 2)))) void shared_prefix_kern
     // line, into LDS, then the rows'.
     int64_t* const pre_start = reinterpret_cast<int64_t*>(lds_all);
     int* const pre_item = reinterpret_cast<int*>(pre_start + P.num_groups);
-    const Cut pre_cut = prefix_cut();
+    const int64_t pre_range = range_of(prefix_length(), P.wgs, kPreTiles);
     if (wave == 0) {
       int64_t line = 0, item0 = 0;
       for (int g0 = 0; g0 < P.num_groups; g0 += 64) {
         const Group x = group_at(g0 + lane);
         const int items = group_items(x);
-        const int64_t mine = items * pre_cut.step(tiles_in(x.prefix));
+        const int64_t mine = items * places_of(x.prefix);
         const int64_t end = line + scan64(mine, lane);
         const int64_t item_end = item0 + scan64(items, lane);
         if (g0 + lane < P.num_groups) {
@@ -454,23 +457,22 @@ __attribute__((amdgpu_waves_per_eu((D == 256 ? 1 : 2)))) void shared_prefix_kern
     for (int b0 = 0; b0 < A.batch; b0 += kThreads) {
       const int b = b0 + threadIdx.x;
       const Own o = own_at(b);
-      const int64_t mine = own_cut.step(o.tiles) * P.vheads;
+      const int64_t mine = static_cast<int64_t>(o.tiles) * P.vheads;
       int64_t sum;
       const int64_t end = line + scan_all(mine, sum);
       line += sum;
       if (b >= A.batch) continue;
       RowRecord rec{};
       rec.own_start = end - mine;
-      rec.own_range = own_cut.range;
-      rec.own_step = own_cut.step(o.tiles);
+      rec.own_range = own_range;
       rec.own_tiles = o.tiles;
-      rec.pre_range = pre_cut.range;
+      rec.pre_range = pre_range;
       const int grp = group_of(b);
       if (grp >= 0) {
         const Group x = group_at(grp);
         rec.pre_start = pre_start[grp];
         rec.pre_tiles = tiles_in(x.prefix);
-        rec.pre_step = pre_cut.step(rec.pre_tiles);
+        rec.pre_step = places_of(x.prefix);
         rec.pre_item = pre_item[grp];
         rec.col_items = group_items(x) / A.num_kv_heads;
         rec.index = b - x.first;
@@ -502,10 +504,11 @@ __global__ __launch_bounds__(kMergeThreads) void shared_prefix_merge_kernel(Pref
   const RowRecord rec = P.rows[b];
   const float vsc = fp8 && A.v_scale ? A.v_scale[kvh] : 1.f;
   // The row's pieces on its own line: ranges own_w, own_w + 1, ...
-  const int64_t own_at = rec.own_start + v * rec.own_step;
-  const int64_t own_w = rec.own_tiles ? own_at / rec.own_range : 0;
+  const int64_t own_at = rec.own_start + static_cast<int64_t>(v) * rec.own_tiles;
+  const int64_t own_w = rec.own_tiles ? quotient(own_at, rec.own_range) : 0;
   const int own_n = rec.own_tiles
-                        ? static_cast<int>((own_at + rec.own_tiles - 1) / rec.own_range - own_w) + 1
+                        ? static_cast<int>(
+                              quotient(own_at + rec.own_tiles - 1, rec.own_range) - own_w) + 1
                         : 0;
   const int64_t own_col = (own_w + static_cast<int64_t>(b) * P.vheads + v) * P.own_cols;
   // ... and on the prefix line, found for each column.
@@ -518,11 +521,11 @@ __global__ __launch_bounds__(kMergeThreads) void shared_prefix_merge_kernel(Pref
           const int c = rec.index * A.gqa + in_group + j;
           const int it = kvh * rec.col_items + c / kCols;
           const int64_t at = rec.pre_start + it * rec.pre_step;
-          const int64_t w = at / rec.pre_range;
+          const int64_t w = quotient(at, rec.pre_range);
           const int64_t first = w + rec.pre_item + it;
           pre_n = static_cast<int>(max(
               int64_t{0},
-              min((at + rec.pre_tiles - 1) / rec.pre_range - w + 1, P.pre_pieces - first)));
+              min(quotient(at + rec.pre_tiles - 1, rec.pre_range) - w + 1, P.pre_pieces - first)));
           pre_col = first * kCols + c % kCols;
         }
         return pre_n + own_n;

@@ -74,7 +74,8 @@ __attribute__((amdgpu_waves_per_eu(D == 256 ? 1 : 2))) void sparse_decode_kernel
   stream_units(A, st, unit_at, P.keep << per_log2, kWaves * part + wave, kWaves * P.parts,
                P.unit_tiles_log2, 0,
                max(vis, 0), [&] { return Limits<1>{{span}, span, span}; }, kvh,
-               __builtin_fabsf(s2), lane);
+               __builtin_fabsf(s2),
+               reinterpret_cast<uint8_t*>(lds) + wave * 2 * KChunks<kFp8, D>::kBytes, lane);
   if (P.parts == 1) {
     merge_waves<kWaves>(st, lds, wave, lane, ncols,
                         [&](int j, int dim, const float4& o, float M, float L) {
@@ -138,7 +139,9 @@ void launch_d(bool fp8, const SparseParams& P, int64_t rows, hipStream_t s, cons
               const int32_t* ctx, const int32_t* cu) {
   const unsigned vheads = P.A.num_kv_heads * P.A.col_blocks;
   const dim3 grid(vheads, static_cast<unsigned>(rows), static_cast<unsigned>(P.parts));
-  const unsigned lds = 4 * merge_lds_floats<kWaves, D>(P.cols);
+  const int rows_lds = kWaves * 2 * (fp8 ? KChunks<true, D>::kBytes : KChunks<false, D>::kBytes);
+  const int merge_lds = 4 * merge_lds_floats<kWaves, D>(P.cols);
+  const unsigned lds = merge_lds > rows_lds ? merge_lds : rows_lds;
   if (fp8)
     hipLaunchKernelGGL((sparse_decode_kernel<D, true>), grid, dim3(kWaves * 64), lds, s, P, bt,
                        ctx, cu);
