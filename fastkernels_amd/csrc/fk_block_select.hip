@@ -14,14 +14,12 @@
 // as the highest score, so that such a page is attended to and shows.
 #include <limits.h>
 
-#include "fk_attn_tile.h"
+#include "fk_key_rows.h"
 #include "fk_query_rows.h"
 
 namespace fk {
 namespace {
 
-// Keeps the loads before it before it (the compiler may sink them to their first use).
-__device__ __forceinline__ void loads_issued() { asm volatile("" ::: "memory"); }
 // NaN-propagating minimum and maximum.
 __device__ __forceinline__ float min_nan(float a, float b) {
   return __builtin_elementwise_minimum(a, b);
@@ -193,7 +191,8 @@ __global__ __launch_bounds__(kScoreWaves * 64) void block_scores_kernel(
     const int32_t* __restrict__ cu) {
   constexpr int kElt = kFp8 ? 1 : 2;
   constexpr int kKc = D / 32;
-  constexpr int kLoads = kFp8 ? D / 64 : D / 32;
+  using K = KChunks<kFp8, D>;
+  extern __shared__ __align__(16) uint8_t turn[];  // K::kBytes for each wave
   const int lane = threadIdx.x & 63;
   const int r = lane & 15, g = lane >> 4;
   const int h = blockIdx.z * (blockDim.x >> 6) + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -219,7 +218,7 @@ __global__ __launch_bounds__(kScoreWaves * 64) void block_scores_kernel(
     const uint16_t* p = qrow + static_cast<int64_t>(head) * D;
 #pragma unroll
     for (int c = 0; c < kKc; ++c) {
-      const int d0 = kFp8 ? (D / 4) * g + 8 * c : 32 * c + 8 * g;
+      const int d0 = K::dims(c, g);
       const uint4 v = *reinterpret_cast<const uint4*>(p + d0);
       const uint32_t w[4] = {v.x, v.y, v.z, v.w};
       uint32_t a[4], z[4];
@@ -244,55 +243,45 @@ __global__ __launch_bounds__(kScoreWaves * 64) void block_scores_kernel(
   // Lane k holds the table's entry for the wave's page k.
   static_assert(kScoreTiles * 16 <= 64, "a lane per page");
   const int my_entry = 16 * tile0 + lane < most ? bt_row[16 * tile0 + lane] : -1;
+  const bool entry_ok = my_entry >= 0 && my_entry < P.num_blocks;
+  const uint64_t pages_ok = __ballot(entry_ok);
+  const int my_page = entry_ok ? my_entry : 0;
+  uint8_t* const kx = turn + (threadIdx.x >> 6) * K::kBytes;
+  const uint8_t* const base =
+      P.bounds + static_cast<int64_t>(h) * 2 * D * kElt + 16 * (lane % K::kPieces);
+  const int64_t page_bytes = static_cast<int64_t>(P.num_kv_heads) * 2 * D * kElt;
   struct Bounds {
-    uint4 lo[kLoads], hi[kLoads];
-    uint32_t ok;  // pages of the tile that can be read
+    DTile<kFp8, D> lo, hi;  // (k only)
   };
   // Issues tile x's loads (row r of a tile is page 16 x + r).
   auto load = [&](int x, Bounds& t) {
-    const int entry = __shfl(my_entry, 16 * x + r, 64);
-    const bool ok = entry >= 0 && entry < P.num_blocks;
-    const uint8_t* row =
-        P.bounds + (static_cast<int64_t>(ok ? entry : 0) * P.num_kv_heads + h) * 2 * D * kElt;
 #pragma unroll
-    for (int c = 0; c < kLoads; ++c) {
-      const int at = kFp8 ? (D / 4) * g + 16 * c : (32 * c + 8 * g) * 2;
-      t.lo[c] = ld16(row + at);
-      t.hi[c] = ld16(row + D * kElt + at);
+    for (int i = 0; i < K::kLoads; ++i) {
+      const uint8_t* row =
+          base + page_bytes * __shfl(my_page, 16 * x + K::kRows * i + lane / K::kPieces, 64);
+      t.lo.k[i] = ld16(row);
+      t.hi.k[i] = ld16(row + D * kElt);
     }
     loads_issued();
-    t.ok = static_cast<uint32_t>(__ballot(ok)) & 0xffffu;
   };
   // Scores tile x from t, whose registers take the next tile as soon as they are free.
   auto score = [&](int x, Bounds& t) {
     const int j0 = 16 * (tile0 + x);
     float s[4] = {kNegInf, kNegInf, kNegInf, kNegInf};
     if (x < seen) {
+      uint4 kl[kKc], kh[kKc];
+      K::put(t.lo, kx, lane);
+      K::get(kx, lane, kl);
+      K::put(t.hi, kx, lane);
+      K::get(kx, lane, kh);
+      if (x + 1 < seen) load(x + 1, t);
       for (int cb = 0; cb < col_blocks; ++cb) {
         if (cb > 0 || (col_blocks > 1 && x > 0)) load_q(cb);
-        uint4 kl[kKc], kh[kKc];
-        if constexpr (kFp8) {
-          DTile<true, D> a, z;
-#pragma unroll
-          for (int c = 0; c < kLoads; ++c) {
-            a.k[c] = t.lo[c];
-            z.k[c] = t.hi[c];
-          }
-          k_chunks_d(a, kl);
-          k_chunks_d(z, kh);
-        } else {
-#pragma unroll
-          for (int c = 0; c < kKc; ++c) {
-            kl[c] = t.lo[c];
-            kh[c] = t.hi[c];
-          }
-        }
         const floatx4_t u = qk_scores_n(kl, qn), v = qk_scores_n(kh, qp);
 #pragma unroll
         for (int k = 0; k < 4; ++k) s[k] = cb == 0 ? u[k] + v[k] : max_nan(s[k], u[k] + v[k]);
       }
-      const uint32_t cur = t.ok;
-      if (x + 1 < seen) load(x + 1, t);
+      const uint32_t cur = static_cast<uint32_t>(pages_ok >> (16 * x));
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
         for (int off = 1; off < slots; off <<= 1) s[k] = max_nan(s[k], __shfl_xor(s[k], off, 64));
@@ -552,12 +541,16 @@ void launch_bounds(const BoundsParams& P, int d, dim3 grid, hipStream_t s, const
 template <bool kFp8>
 void launch_scores(const ScoreParams& P, int d, dim3 grid, hipStream_t s, const int32_t* bt,
                    const int32_t* ctx, const int32_t* cu) {
+  const int waves = P.num_kv_heads < kScoreWaves ? P.num_kv_heads : kScoreWaves;
   if (d == 64)
-    hipLaunchKernelGGL((block_scores_kernel<kFp8, 64>), grid, dim3(64 * (P.num_kv_heads < kScoreWaves ? P.num_kv_heads : kScoreWaves)), 0, s, P, bt, ctx, cu);
+    hipLaunchKernelGGL((block_scores_kernel<kFp8, 64>), grid, dim3(64 * waves),
+                       (waves * KChunks<kFp8, 64>::kBytes), s, P, bt, ctx, cu);
   else if (d == 128)
-    hipLaunchKernelGGL((block_scores_kernel<kFp8, 128>), grid, dim3(64 * (P.num_kv_heads < kScoreWaves ? P.num_kv_heads : kScoreWaves)), 0, s, P, bt, ctx, cu);
+    hipLaunchKernelGGL((block_scores_kernel<kFp8, 128>), grid, dim3(64 * waves),
+                       (waves * KChunks<kFp8, 128>::kBytes), s, P, bt, ctx, cu);
   else
-    hipLaunchKernelGGL((block_scores_kernel<kFp8, 256>), grid, dim3(64 * (P.num_kv_heads < kScoreWaves ? P.num_kv_heads : kScoreWaves)), 0, s, P, bt, ctx, cu);
+    hipLaunchKernelGGL((block_scores_kernel<kFp8, 256>), grid, dim3(64 * waves),
+                       (waves * KChunks<kFp8, 256>::kBytes), s, P, bt, ctx, cu);
 }
 
 }  // namespace

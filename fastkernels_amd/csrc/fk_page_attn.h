@@ -7,7 +7,7 @@
 // LDS with the log-sum-exp rule M = max m_w, L = sum l_w 2^(m_w - M), O = sum o_w 2^(m_w - M).
 #pragma once
 
-#include "fk_attn_tile.h"
+#include "fk_key_rows.h"
 
 namespace fk {
 
@@ -48,39 +48,6 @@ struct PageAttnParams {
 constexpr float kLazyMax = 8.f;
 constexpr float kNoMax = -1.0e30f;  // the reference before a column's first visible key
 
-// K rows on their way to the scores' operand.  The operand has a key per lane (lane (r, g): 16
-// bytes at 64 c + 16 g of key r), so that loads straight into it meet another row with every
-// lane, and the cache takes them one lane at a time; and each of them takes half a cache line,
-// whose other half then waits behind the first's miss.  They are loaded in whole rows instead,
-// and a round trip through the wave's own LDS turns them.  There, chunk c holds bytes 64 c ..
-// 64 c + 63 of the 16 rows; a row's four pieces are rotated by half its number, and rows trade
-// places with their neighbours in odd chunks, so that neither side has bank conflicts.
-template <bool kFp8, int D>
-struct KChunks {
-  static constexpr int kLoads = DTile<kFp8, D>::kKLoads;
-  static constexpr int kBytes = 1024 * kLoads;  // of a tile
-  static constexpr int kPieces = 4 * kLoads;    // 16-byte pieces of a row
-  static constexpr int kRows = 64 / kPieces;    // rows per load
-  static __device__ __forceinline__ int at(int row, int chunk, int piece) {
-    return 1024 * chunk + 64 * (row ^ (chunk & 1)) + 16 * ((piece + (row >> 1)) & 3);
-  }
-  static __device__ __forceinline__ void put(const DTile<kFp8, D>& t, uint8_t* kx, int lane) {
-    const int piece = lane % kPieces;
-#pragma unroll
-    for (int i = 0; i < kLoads; ++i)
-      *reinterpret_cast<uint4*>(kx + at(kRows * i + lane / kPieces, piece >> 2, piece & 3)) =
-          t.k[i];
-  }
-  // As bf16 operands: of fp8 rows, operand 2 c + h is dims 64 c + 16 g + 8 h .. + 7.
-  static __device__ __forceinline__ void get(const uint8_t* kx, int lane, uint4 (&k)[D / 32]) {
-    DTile<kFp8, D> t;
-#pragma unroll
-    for (int c = 0; c < kLoads; ++c)
-      t.k[c] = *reinterpret_cast<const uint4*>(kx + at(lane & 15, c, lane >> 4));
-    k_chunks_d(t, k);
-  }
-};
-
 template <int kCB, int D, bool kFp8>
 struct ColumnState {
   static constexpr int kKc = D / 32;
@@ -104,7 +71,7 @@ struct ColumnState {
                                          int g) {
 #pragma unroll
     for (int c = 0; c < kKc; ++c) {
-      const int d0 = kFp8 ? 64 * (c >> 1) + 16 * g + 8 * (c & 1) : 32 * c + 8 * g;
+      const int d0 = KChunks<kFp8, D>::dims(c, g);
       uint4 v = ok ? *reinterpret_cast<const uint4*>(qp + d0) : make_uint4(0, 0, 0, 0);
       v = make_uint4(v.x ^ flip, v.y ^ flip, v.z ^ flip, v.w ^ flip);
       qb[cb][c] = __builtin_bit_cast(bf16x8_t, v);
@@ -250,10 +217,6 @@ __device__ __forceinline__ void load_tile_v(const uint8_t* row, const TileLanes<
 #pragma unroll
   for (int i = 0; i < 4; ++i) ld_words(row + at.v[i], t.v[i]);
 }
-
-// Keeps the loads before it before it: the compiler otherwise sinks them to just before their
-// first use, a step later, and their latency is no longer hidden.
-__device__ __forceinline__ void loads_issued() { asm volatile("" ::: "memory"); }
 
 // What a wave's columns see of positions [from, to): lim[cb] keys from `from` on for this lane's
 // column of block cb, at most `span` for any column of the wave and at least `least`.
