@@ -416,7 +416,7 @@ struct Folded {
 // column j's pieces, at(k, j, ml, o) where piece k's (m, l) and O are; emit(j, dim, o, M, L)
 // gets the merged state.
 constexpr int kMergeThreads = 256;
-constexpr int kMergeAhead = 4;  // pieces whose loads are in flight
+constexpr int kMergeAhead = 8;  // pieces whose loads are in flight
 template <int D, class Pieces, class At, class Emit>
 __device__ __forceinline__ void merge_pieces(int nc, Folded* folded, Pieces pieces, At at,
                                              Emit emit) {
