@@ -310,7 +310,8 @@ class FlashAttnDecode(nn.Module):
         for its group: rows cu_groups[g] .. cu_groups[g + 1] - 1 (int32 [groups + 1]) have the
         same tokens at positions below prefix_lens[g] (int32 [groups]).  Their block tables
         list the shared pages as ever; the first row's is the one read.  kwargs as forward's
-        (without num_splits).  max_prefix_len: a bound on the prefixes, if known."""
+        (without num_splits).  At most max_prefix_len tokens of a prefix are read once (0:
+        all); a bound keeps the workspace small."""
         a = self._page_args("FlashAttnDecode.forward_shared_prefix", q, k_cache, cache_seqlens,
                             kwargs)
         call = torch.ops.fastkernels_amd.shared_prefix_decode if torch.compiler.is_compiling() \

@@ -54,6 +54,7 @@ struct RowRecord {
 struct PrefixParams {
   PageAttnParams A;
   int num_groups;
+  int max_prefix;          // tokens of a prefix that are shared at most
   int window_left;
   int unit_tiles_log2;
   int wgs;                 // work-groups that share the lines
@@ -175,7 +176,7 @@ __attribute__((amdgpu_waves_per_eu((D == 256 ? 1 : 2)))) void shared_prefix_kern
     if (i >= P.num_groups) return x;
     x.first = group_first[i];
     x.rows = group_first[i + 1] - x.first;
-    x.prefix = x.rows > 1 && P.window_left < 0 ? group_prefix[i] : 0;
+    x.prefix = x.rows > 1 && P.window_left < 0 ? min(group_prefix[i], P.max_prefix) : 0;
     return x;
   };
   // Items (kv heads x column blocks) of a group and the tiles of each.
@@ -203,7 +204,7 @@ __attribute__((amdgpu_waves_per_eu((D == 256 ? 1 : 2)))) void shared_prefix_kern
       const Group x = group_at(grp);
       w.border = min(group_prefix[grp], w.ctx);
       w.first_row = x.first;
-      if (x.prefix > 0) w.from = w.border;
+      if (x.prefix > 0) w.from = min(x.prefix, w.ctx);
     }
     // counted from the tile of `from`
     w.tiles = w.ctx > w.from ? (w.ctx - 1) / kTile - w.from / kTile + 1 : 0;
@@ -542,14 +543,19 @@ __global__ __launch_bounds__(kMergeThreads) void shared_prefix_merge_kernel(Pref
       });
 }
 
+// The bound on the shared tokens of a prefix that an argument of 0 (none) or more stands for.
+int64_t prefix_bound(int64_t max_prefix_len) {
+  return max_prefix_len == 0 || max_prefix_len > INT_MAX ? INT_MAX : max_prefix_len;
+}
+
 // Work-groups and workspace of a launch.
 struct PrefixPlan {
   int wgs;
   int64_t pre_pieces, own_pieces;
   int64_t pre_o, pre_ml, own_o, own_ml, rows, bytes;  // offsets
 };
-PrefixPlan plan_of(int64_t batch, int64_t groups, int num_heads, int num_kv_heads,
-                   int head_size) {
+PrefixPlan plan_of(int64_t batch, int64_t groups, int64_t max_prefix, int num_heads,
+                   int num_kv_heads, int head_size) {
   PrefixPlan p{};
   const int gqa = num_heads / num_kv_heads;
   const int64_t cols = cols_of(head_size);
@@ -559,7 +565,12 @@ PrefixPlan plan_of(int64_t batch, int64_t groups, int num_heads, int num_kv_head
   p.wgs = num_cus() * (head_size == 256 ? 1 : 2);
   // A group that shares has two rows at the least, and rounds its columns up once.
   const int64_t shared = groups < batch / 2 ? groups : batch / 2;
-  if (shared > 0) p.pre_pieces = p.wgs + num_kv_heads * (batch * gqa / cols + shared);
+  if (shared > 0) {
+    const int64_t items = num_kv_heads * (batch * gqa / cols + shared);
+    const int64_t each = (max_prefix + kTile * kPreTiles - 1) / (kTile * kPreTiles);
+    // An item and a range leave a piece where they meet: as many as both at the most.
+    p.pre_pieces = items + (each < p.wgs && items * each < p.wgs ? items * each : p.wgs);
+  }
   p.own_pieces = kWaves * p.wgs + batch * vheads;
   auto take = [&](int64_t bytes) {
     const int64_t at = p.bytes;
@@ -617,10 +628,11 @@ extern "C" int fk_shared_prefix_decode(
              static_cast<long long>(max_prefix_len));
   FK_REQUIRE(window_left >= -1, "%s: window_left %d must be -1 or >= 0", what, window_left);
   if (batch == 0) return FK_OK;
+  max_prefix_len = prefix_bound(max_prefix_len);
   FK_REQUIRE(out && q && k_cache && v_cache && block_tables && cache_seqlens &&
                  (num_groups == 0 || (cu_groups && prefix_lens)),
              "%s: null pointer", what);
-  const PrefixPlan plan = plan_of(batch, num_groups, num_heads, num_kv_heads, head_size);
+  const PrefixPlan plan = plan_of(batch, num_groups, max_prefix_len, num_heads, num_kv_heads, head_size);
   if (workspace_bytes < plan.bytes || !workspace)
     return set_error(FK_ERR_WORKSPACE, "%s: workspace of %lld bytes, %lld needed", what,
                      static_cast<long long>(workspace_bytes), static_cast<long long>(plan.bytes));
@@ -629,6 +641,7 @@ extern "C" int fk_shared_prefix_decode(
   PrefixParams P{};
   P.A = A;
   P.num_groups = static_cast<int>(num_groups);
+  P.max_prefix = static_cast<int>(max_prefix_len);
   P.window_left = window_left;
   P.unit_tiles_log2 = A.block_size_log2 - 4 < 2 ? A.block_size_log2 - 4 : 2;
   P.wgs = plan.wgs;
@@ -660,6 +673,8 @@ extern "C" int fk_shared_prefix_decode_plan(int64_t batch, int64_t num_groups,
                  num_kv_heads > 0 && num_heads > 0 && num_heads % num_kv_heads == 0,
              "fk_shared_prefix_decode_plan: invalid argument");
   *workspace_bytes = batch == 0 ? 0
-                                : plan_of(batch, num_groups, num_heads, num_kv_heads, head_size).bytes;
+                                : plan_of(batch, num_groups, prefix_bound(max_prefix_len),
+                                          num_heads, num_kv_heads, head_size)
+                                      .bytes;
   return FK_OK;
 }

@@ -951,8 +951,8 @@ def shared_prefix_decode(out: torch.Tensor, q: torch.Tensor, k_cache: torch.Tens
     same tokens at positions below prefix_lens[g] (int32 [groups], any length).  Those are
     read once for the group, through the block table of its first row, the others through
     each row's own.  Rows outside every group share nothing; a row may be shorter than its
-    group's prefix.  max_prefix_len bounds every prefix (0: unknown); it only chooses the
-    launch shape."""
+    group's prefix.  At most 2048 groups; at most max_prefix_len tokens of a prefix are shared
+    (0: all of them), and a bound keeps the workspace small."""
     what = "shared_prefix_decode"
     (rows, hq, d), q_stride, out_stride, (nb, bs, hk, _), tag = \
         _check_page_attn(what, out, q, k_cache, v_cache)

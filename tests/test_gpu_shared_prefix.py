@@ -102,6 +102,20 @@ def test_shared_prefix(cuda, kv, hq, hk, d, page, name):
     check_attn(out, *want)
 
 
+@pytest.mark.parametrize("bound", [1, 16, 100, 500])
+def test_shared_prefix_bound(cuda, bound):
+    """Prefixes longer than max_prefix_len are shared up to there."""
+    from fastkernels_amd import ops
+
+    g, q, k, v, bt, lens, cu, pre, ks, vs = build(cuda, "bf16", 32, 8, 128, 16, GROUPS["ragged"])
+    out = torch.full_like(q, 9.0)
+    ops.shared_prefix_decode(out, q, k, v, bt, int32(lens, cuda), cu, pre, 128 ** -0.5,
+                             max_prefix_len=bound)
+    want = ref.shared_prefix_decode(f64(q), f64(k), f64(v), bt.cpu().numpy(), lens,
+                                    cu.cpu().numpy(), pre.cpu().numpy(), 128 ** -0.5)
+    check_attn(out, *want)
+
+
 @pytest.mark.parametrize("window", [0, 15, 100, 600, 5000])
 @pytest.mark.parametrize("kv,hq,hk,d,page", [("bf16", 32, 8, 128, 16), ("fp8", 24, 2, 64, 32)])
 def test_shared_prefix_window_and_sinks(cuda, kv, hq, hk, d, page, window):

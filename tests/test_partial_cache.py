@@ -245,3 +245,14 @@ def test_selection_keeps_what_the_bounds_promise():
     assert (s[0] >= np.where(np.arange(12)[None, :] < 11, x.max((2, 3)), -np.inf) - 1e-12).all()
     idx = ref.select_blocks(s, [n], page, 5, 1, 2)
     assert (idx[:, :, 0] == 0).all() and (idx[:, :, -2:] == [10, 11]).all()
+
+
+def test_prefix_bound_keeps_the_workspace_small():
+    N = pytest.importorskip("fastkernels_amd._native")
+    size = lambda bound, batch=8, groups=1: N.shared_prefix_bytes(batch, groups, bound, 32, 8, 128)
+    assert size(128) < size(1500) < size(0)
+    assert size(1 << 40) == size(0)
+    assert size(1500, 0) == 0
+    assert size(64, 64, 64) < size(64, 4096, 1000)
+    with pytest.raises(N.FkError):
+        size(-1)
