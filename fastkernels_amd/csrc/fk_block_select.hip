@@ -331,18 +331,24 @@ __device__ __forceinline__ uint32_t score_key(float s) {
   return u ^ ((u >> 31) ? 0xffffffffu : 0x80000000u);
 }
 
-// Inclusive sum over the lanes of a wave: within rows of 16, then across them.
-template <int kCtrl, int kRows>
-__device__ __forceinline__ int plus_dpp(int v) {
-  return v + __builtin_amdgcn_update_dpp(0, v, kCtrl, kRows, 0xf, false);
+__device__ __forceinline__ float key_score(uint32_t key) {  // (of a number)
+  return __uint_as_float(key ^ (key >> 31 ? 0x80000000u : 0xffffffffu));
 }
-__device__ __forceinline__ int scan_lanes(int v) {
-  v = plus_dpp<0x111, 0xf>(v);     // from the lane 1 before, 2, 4, 8
-  v = plus_dpp<0x112, 0xf>(v);
-  v = plus_dpp<0x114, 0xf>(v);
-  v = plus_dpp<0x118, 0xf>(v);
-  v = plus_dpp<0x142, 0xa>(v);     // from lane 15 of the row before, into rows 1 and 3
-  return plus_dpp<0x143, 0xc>(v);  // from lane 31, into rows 2 and 3
+
+// Inclusive scan over the lanes of a wave (0 is the operation's identity): within rows of 16,
+// then across them.
+template <int kCtrl, int kRows>
+__device__ __forceinline__ int moved(int v) {
+  return __builtin_amdgcn_update_dpp(0, v, kCtrl, kRows, 0xf, false);
+}
+template <class Op>
+__device__ __forceinline__ uint32_t scan_lanes(uint32_t v, Op op) {
+  v = op(v, moved<0x111, 0xf>(v));     // from the lane 1 before, 2, 4, 8
+  v = op(v, moved<0x112, 0xf>(v));
+  v = op(v, moved<0x114, 0xf>(v));
+  v = op(v, moved<0x118, 0xf>(v));
+  v = op(v, moved<0x142, 0xa>(v));     // from lane 15 of the row before, into rows 1 and 3
+  return op(v, moved<0x143, 0xc>(v));  // from lane 31, into rows 2 and 3
 }
 // Inclusive sums over the work-group's threads.  part: a word per wave and value, not in use
 // since the barrier before the last.
@@ -353,7 +359,7 @@ __device__ __forceinline__ void scan_threads(int (&v)[kN], int (*part)[kSelThrea
   const int lane = tid & 63, wave = tid >> 6;
 #pragma unroll
   for (int i = 0; i < kN; ++i) {
-    v[i] = scan_lanes(v[i]);
+    v[i] = scan_lanes(v[i], [](uint32_t a, uint32_t b) { return a + b; });
     if (lane == 63) part[i][wave] = v[i];
   }
   __syncthreads();
@@ -363,12 +369,19 @@ __device__ __forceinline__ void scan_threads(int (&v)[kN], int (*part)[kSelThrea
     for (int w = 0; w < kWaves; ++w) v[i] += w < wave ? part[i][w] : 0;
 }
 
-// One work-group per (query row, kv head).  The key T of the lowest selected candidate is
-// found digit by digit (11, 11 and 10 bits: a histogram of the keys that agree with the digits
-// found so far, then the bin that holds the rank), until the rank takes a whole bin.  The blocks
-// are written in order of their index: each thread takes a run of them, counts what is selected
-// there (the blocks always kept, keys above T, and the first of the keys equal to T), and its
-// place is the sum of the counts before it.
+// One work-group per (query row, kv head), in search of the key T of the lowest selected
+// candidate.  First the candidates' scores are counted in equal steps between the least and the
+// greatest: where the step that holds the rank has few of them, the lanes of a wave rank those.
+// Otherwise (equal scores, infinities, NaN, or more pages than LDS holds) T is found digit by
+// digit (11, 11 and 10 bits: a histogram of the keys that agree with the digits found so far,
+// then the bin that holds the rank), until the rank takes a whole bin.  The blocks are written in
+// order of their index: each thread takes a run of them, counts what is selected there (the
+// blocks always kept, keys above T, and the first of the keys equal to T), and its place is the
+// sum of the counts before it.
+//
+// Bound by latency: loads, barriers and LDS atomics in turn.  One sequence of 40000 tokens in
+// pages of 16 takes 7.3 us (8.1 by digits at once), 85 rows of 32 sequences of 16000 .. 131072
+// tokens 18.9 (20.1); 256 or 1024 threads a list take 10.6 / 24.8 and 8.4 / 23.0 by digits.
 template <bool kLds>
 __global__ __launch_bounds__(kSelThreads) void select_blocks_kernel(
     SelectParams P, const int32_t* __restrict__ ctx, const int32_t* __restrict__ cu) {
@@ -376,6 +389,9 @@ __global__ __launch_bounds__(kSelThreads) void select_blocks_kernel(
   __shared__ int hist[kSelBins];
   __shared__ int part[2][kSelThreads / 64];
   __shared__ int found[3];
+  __shared__ uint32_t range[2][kSelThreads / 64];
+  __shared__ uint32_t few[64];
+  __shared__ int few_count;
   const int t = blockIdx.x, h = blockIdx.y;
   int b, vis;
   if (!query_row(cu, ctx, P.batch, t, b, vis)) return;
@@ -390,37 +406,47 @@ __global__ __launch_bounds__(kSelThreads) void select_blocks_kernel(
   auto key_of = [&](int j) { return kLds ? keys[sel_at(j)] : score_key(row[j]); };
 #pragma unroll
   for (int i = 0; i < 4; ++i) hist[4 * tid + i] = 0;
+  const int first = P.keep_first, last = n - P.keep_last;  // candidates [first, last)
+  int need = P.keep - P.keep_first - P.keep_last;          // of which so many are selected
   if constexpr (kLds) {
     // (kAhead loads in flight; those past the end read the last score once more)
     constexpr int kAhead = 8;
+    uint32_t top = 0, bottom = 0;  // the greatest key and complement of a key
     for (int j0 = tid; j0 < n; j0 += kAhead * kSelThreads) {
       float s[kAhead];
 #pragma unroll
       for (int u = 0; u < kAhead; ++u) s[u] = row[min(j0 + u * kSelThreads, n - 1)];
 #pragma unroll
-      for (int u = 0; u < kAhead; ++u)
-        if (j0 + u * kSelThreads < n) keys[sel_at(j0 + u * kSelThreads)] = score_key(s[u]);
+      for (int u = 0; u < kAhead; ++u) {
+        const int j = j0 + u * kSelThreads;
+        if (j >= n) continue;
+        const uint32_t key = score_key(s[u]);
+        keys[sel_at(j)] = key;
+        if (j < first || j >= last) continue;
+        top = max(top, key);
+        bottom = max(bottom, ~key);
+      }
     }
+    const auto larger = [](uint32_t a, uint32_t b) { return max(a, b); };
+    top = scan_lanes(top, larger);
+    bottom = scan_lanes(bottom, larger);
+    if ((tid & 63) == 63) {
+      range[0][tid >> 6] = top;
+      range[1][tid >> 6] = bottom;
+    }
+    if (tid == 0) few_count = 0;
   }
   __syncthreads();
-  const int first = P.keep_first, last = n - P.keep_last;  // candidates [first, last)
-  int need = P.keep - P.keep_first - P.keep_last;          // of which so many are selected
   uint32_t digits = 0, known = 0;  // T, and the bits of it that count
   // (With nothing to select among the candidates T stays above every key.)
   bool whole = need == 0;
   if (whole) digits = known = 0xffffffffu;
   int equal_need = 0;  // of the keys equal to T, the first so many are selected
-  for (int pass = 0; pass < 3 && !whole; ++pass) {
-    const int shift = pass == 0 ? 21 : pass == 1 ? 10 : 0;
-    const uint32_t mask = pass == 2 ? 1023u : 2047u;
-#pragma unroll 4
-    for (int j = first + tid; j < last; j += kSelThreads) {
-      const uint32_t key = key_of(j);
-      if ((key & known) == digits) atomicAdd(&hist[(key >> shift) & mask], 1);
-    }
+  // From the counts in hist, the bin that holds rank `need` from the top: found = the bin, the
+  // rank in it, its count.  Clears the bins.
+  auto find_bin = [&] {
     __syncthreads();
-    // Thread k sums bins 2047 - 4 k .. 2044 - 4 k (and clears them for the next digit): the
-    // inclusive sum counts from the top.
+    // Thread k sums bins 2047 - 4 k .. 2044 - 4 k: the inclusive sum counts from the top.
     int bins[4], sum[1] = {0};
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
@@ -441,6 +467,63 @@ __global__ __launch_bounds__(kSelThreads) void select_blocks_kernel(
       above += bins[i];
     }
     __syncthreads();
+  };
+  if constexpr (kLds) {
+    uint32_t top = 0, bottom = 0;
+#pragma unroll
+    for (int w = 0; w < kSelThreads / 64; ++w) {
+      top = max(top, range[0][w]);
+      bottom = max(bottom, range[1][w]);
+    }
+    bottom = ~bottom;
+    // (finite scores that differ, by a number whose inverse is finite too)
+    const float low = key_score(bottom), width = key_score(top) - low;
+    if (!whole && top < 0xff800000u && bottom > 0x007fffffu && width > 1.0e-30f &&
+        width < 3.0e38f) {
+      const float scale = static_cast<float>(kSelBins) / width;
+      auto step_of = [&](uint32_t key) {  // (does not decrease with the key)
+        return min(static_cast<int>((key_score(key) - low) * scale), kSelBins - 1);
+      };
+#pragma unroll 4
+      for (int j = first + tid; j < last; j += kSelThreads) atomicAdd(&hist[step_of(key_of(j))], 1);
+      find_bin();
+      const int step = found[0], rank = found[1], count = found[2];
+      if (count <= 64) {
+#pragma unroll 4
+        for (int j = first + tid; j < last; j += kSelThreads) {
+          const uint32_t key = key_of(j);
+          if (step_of(key) != step) continue;
+          const int k = atomicAdd(&few_count, 1);
+          if (k < 64) few[k] = key;
+        }
+        __syncthreads();
+        // Every wave ranks them, a lane each.
+        const int lane = tid & 63;
+        const uint32_t mine = lane < count ? few[lane] : 0;
+        int above = 0, equal = 0;
+        for (int i = 0; i < count; ++i) {
+          const uint32_t other = __builtin_amdgcn_readlane(mine, i);
+          above += other > mine;
+          equal += other == mine;
+        }
+        const int src = __builtin_ctzll(
+            __ballot(lane < count && above < rank && rank <= above + equal));
+        digits = __builtin_amdgcn_readlane(mine, src);
+        known = 0xffffffffu;
+        equal_need = rank - __builtin_amdgcn_readlane(above, src);
+        whole = true;
+      }
+    }
+  }
+  for (int pass = 0; pass < 3 && !whole; ++pass) {
+    const int shift = pass == 0 ? 21 : pass == 1 ? 10 : 0;
+    const uint32_t mask = pass == 2 ? 1023u : 2047u;
+#pragma unroll 4
+    for (int j = first + tid; j < last; j += kSelThreads) {
+      const uint32_t key = key_of(j);
+      if ((key & known) == digits) atomicAdd(&hist[(key >> shift) & mask], 1);
+    }
+    find_bin();
     digits |= static_cast<uint32_t>(found[0]) << shift;
     known |= mask << shift;
     need = found[1];

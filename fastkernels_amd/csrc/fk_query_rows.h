@@ -8,7 +8,7 @@ namespace fk {
 // Sequence b of query row t and the keys the row sees, vis = ctx - n + i + 1 for the i-th
 // of the sequence's n rows (aligned to the end of its tokens; at most ctx).  cu == nullptr:
 // one row per sequence.  False for a row behind the last sequence.  Sequences without rows
-// are skipped by taking the last b with cu[b] <= t.
+// are skipped by taking the last b with cu[b] <= t.  Whole waves call it, with one t each.
 __device__ __forceinline__ bool query_row(const int32_t* __restrict__ cu,
                                           const int32_t* __restrict__ ctx, int batch, int t,
                                           int& b, int& vis) {
@@ -18,10 +18,16 @@ __device__ __forceinline__ bool query_row(const int32_t* __restrict__ cu,
     return t < batch;
   }
   if (batch <= 0 || t < cu[0] || t >= cu[batch]) return false;
-  int lo = 0, hi = batch;
-  while (hi - lo > 1) {
-    const int mid = (lo + hi) >> 1;
-    if (cu[mid] <= t) lo = mid; else hi = mid;
+  // The lanes look at 64 places at a time: one load's latency for up to 64 sequences, where
+  // halving takes six.
+  const int lane = threadIdx.x & 63;
+  int lo = 0, len = batch;
+  while (len > 1) {
+    const int step = (len + 63) >> 6;
+    const bool before = lane * step < len && cu[lo + lane * step] <= t;
+    const int last = max(__builtin_popcountll(__ballot(before)) - 1, 0) * step;
+    lo += last;
+    len = min(step, len - last);
   }
   b = lo;
   const int c = ctx[b];

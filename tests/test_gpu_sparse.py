@@ -232,6 +232,43 @@ def test_select_blocks(cuda, width, keep, first, last, lens, rows):
         assert (got[:, :, 0] == -7).all() and (got[:, :, -1] == -7).all()
 
 
+@pytest.mark.parametrize("kind", ["outlier", "low_outlier", "close", "negative", "denormal", "huge",
+                                  "two", "few_equal", "sorted", "tiny_steps"])
+@pytest.mark.parametrize("width,keep,first,last", [(70, 9, 1, 1), (600, 128, 1, 1), (5000, 64, 0, 2),
+                                                   (9000, 700, 3, 0)])
+def test_select_blocks_of_finite_scores(cuda, kind, width, keep, first, last):
+    """Distributions that put the lowest selected score where it is hard to find."""
+    from fastkernels_amd import ops
+
+    g = torch.Generator(device=cuda).manual_seed(width)
+    x = torch.randn(2, 1, width, generator=g, device=cuda)
+    if kind == "outlier":
+        x[:, :, width // 2] = 1e30
+    elif kind == "low_outlier":
+        x[:, :, width // 3] = -3e38
+    elif kind == "close":
+        x = 1 + (x * 50).round() * 2.0 ** -23
+    elif kind == "negative":
+        x = -x.abs() - 1
+    elif kind == "denormal":
+        x = x * 1e-40
+    elif kind == "huge":
+        x = x.clamp(-3, 3) * 1.1e38
+    elif kind == "two":
+        x = (x > 0.5).float()
+    elif kind == "few_equal":
+        x[:, :, ::width // 30] = x.flatten().sort().values[-keep]
+    elif kind == "sorted":
+        x = x.sort(dim=2, descending=True).values
+    else:
+        x = torch.arange(width, device=cuda).expand(2, 1, width) * 1e-31
+    lens = [16 * width, 16 * width - 37]
+    out = torch.full((2, 1, keep), -7, dtype=torch.int32, device=cuda)
+    ops.select_blocks(out, x.contiguous(), int32(lens, cuda), 16, first, last)
+    want = ref.select_blocks(x.cpu().numpy(), lens, 16, keep, first, last)
+    assert np.array_equal(out.cpu().numpy(), want)
+
+
 # ---------------------------------------------------------------------------
 # sparse_paged_decode
 # ---------------------------------------------------------------------------
