@@ -60,6 +60,7 @@ struct PrefixParams {
   int wgs;                 // work-groups that share the lines
   int vheads;              // kv heads x blocks of 16 query heads
   int own_cols;            // query columns of an own item: min(16, gqa)
+  int merge_cols;          // of which a work-group of the merge takes so many
   float* pre_o;            // [pieces][kCols][D], then (maximum, sum) per column
   float* pre_ml;
   float* own_o;            // [pieces][own_cols][D]
@@ -515,8 +516,9 @@ __global__ __launch_bounds__(kMergeThreads) void shared_prefix_merge_kernel(Pref
   // ... and on the prefix line, found for each column.
   int pre_n = 0;
   int64_t pre_col = 0;
+  const int j0 = blockIdx.z * P.merge_cols;
   merge_pieces<D>(
-      min(16, A.gqa - in_group), folded,
+      j0, min(P.merge_cols, min(16, A.gqa - in_group) - j0), folded,
       [&](int j) {
         if (rec.pre_tiles > 0) {
           const int c = rec.index * A.gqa + in_group + j;
@@ -597,7 +599,8 @@ void launch_d(bool fp8, const PrefixParams& P, hipStream_t s, const int32_t* bt,
     hipLaunchKernelGGL((shared_prefix_kernel<D, false>), grid, dim3(kThreads), lds, s, P, bt, ctx,
                        cu, pre);
   hipLaunchKernelGGL((shared_prefix_merge_kernel<D>),
-                     dim3(static_cast<unsigned>(P.vheads), static_cast<unsigned>(P.A.batch)),
+                     dim3(static_cast<unsigned>(P.vheads), static_cast<unsigned>(P.A.batch),
+                          (P.own_cols + P.merge_cols - 1) / P.merge_cols),
                      dim3(kMergeThreads), 0, s, P, fp8 ? 1 : 0);
 }
 
@@ -648,6 +651,7 @@ extern "C" int fk_shared_prefix_decode(
   P.pre_pieces = plan.pre_pieces;
   P.vheads = num_kv_heads * A.col_blocks;
   P.own_cols = A.gqa < 16 ? A.gqa : 16;
+  P.merge_cols = merge_cols(batch, P.vheads, P.own_cols);
   P.pre_o = reinterpret_cast<float*>(ws + plan.pre_o);
   P.pre_ml = reinterpret_cast<float*>(ws + plan.pre_ml);
   P.own_o = reinterpret_cast<float*>(ws + plan.own_o);

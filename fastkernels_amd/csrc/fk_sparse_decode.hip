@@ -26,6 +26,7 @@ struct SparseParams {
   int unit_tiles_log2;
   int parts;     // work-groups per list
   int cols;      // columns of a partial: min(16, gqa)
+  int merge_cols;  // of which a work-group of the merge takes so many
   float* part_o; // [(row, virtual head), part][cols][D], then (maximum, sum) per column
   float* part_ml;
 };
@@ -107,8 +108,9 @@ __global__ __launch_bounds__(kMergeThreads) void sparse_merge_kernel(
   const int qbase = kvh * A.gqa + 16 * (blockIdx.x - kvh * A.col_blocks);
   const float vsc = fp8 && A.v_scale ? A.v_scale[kvh] : 1.f;
   const int64_t col0 = (static_cast<int64_t>(t) * gridDim.x + blockIdx.x) * P.parts * P.cols;
+  const int j0 = blockIdx.z * P.merge_cols;
   merge_pieces<D>(
-      min(16, (kvh + 1) * A.gqa - qbase), folded, [&](int) { return P.parts; },
+      j0, min(P.merge_cols, min(16, (kvh + 1) * A.gqa - qbase) - j0), folded, [&](int) { return P.parts; },
       [&](int k, int j, const float*& ml, const float*& o) {
         const int64_t col = col0 + static_cast<int64_t>(k) * P.cols + j;
         ml = P.part_ml + 2 * col;
@@ -149,7 +151,9 @@ void launch_d(bool fp8, const SparseParams& P, int64_t rows, hipStream_t s, cons
     hipLaunchKernelGGL((sparse_decode_kernel<D, false>), grid, dim3(kWaves * 64), lds, s, P, bt,
                        ctx, cu);
   if (P.parts > 1)
-    hipLaunchKernelGGL((sparse_merge_kernel<D>), dim3(vheads, static_cast<unsigned>(rows)),
+    hipLaunchKernelGGL((sparse_merge_kernel<D>),
+                       dim3(vheads, static_cast<unsigned>(rows),
+                            (P.cols + P.merge_cols - 1) / P.merge_cols),
                        dim3(kMergeThreads), 0, s, P, ctx, cu, fp8 ? 1 : 0);
 }
 
@@ -192,6 +196,7 @@ extern "C" int fk_sparse_paged_decode(
   P.unit_tiles_log2 = A.block_size_log2 - 4 < 2 ? A.block_size_log2 - 4 : 2;
   const int vheads = num_kv_heads * A.col_blocks;
   P.cols = A.gqa < 16 ? A.gqa : 16;
+  P.merge_cols = merge_cols(rows, vheads, P.cols);
   P.parts = parts_of(rows, keep, vheads, block_size);
   const int64_t need = part_bytes(rows, vheads, P.parts, P.cols, head_size);
   if (need > 0) {
