@@ -74,6 +74,9 @@ struct Elems {
 // changes no minimum or maximum.  The pages of sequence b are those of positions
 // [len - n, len), each recomputed over all its positions < len: what is stored depends on
 // the cache alone, not on earlier calls.
+//
+// Bound by memory, by latency where the pages are few: one token of 64 sequences takes 3.2 us
+// (1.5 MB), four fp8 prompts of 1000 .. 8192 tokens in pages of 64 8.6 us (23 MB).
 template <bool kFp8, int D>
 __global__ __launch_bounds__(256) void key_bounds_kernel(
     BoundsParams P, const int32_t* __restrict__ bt, const int32_t* __restrict__ ctx,
@@ -183,6 +186,10 @@ struct ScoreParams {
 // one sequence times the query heads of kv head h (a group that is no power of two repeats
 // its last head, groups above 16 take several passes over the loaded bounds); the rows of
 // the A operand are the pages' bounds, lo then hi, the B operands min(q, 0) and max(q, 0).
+//
+// Bound by memory: 32 sequences of 16000 .. 131072 tokens in pages of 16 take 142 us (655 MB,
+// 4.6 TB/s, in pieces of 4 KB); one sequence of 40000 5.4 us.  More waves a SIMD are slower
+// there (four 158 us).
 constexpr int kScoreWaves = 8;  // of a work-group, a kv head each: a page's bounds are read whole
 constexpr int kScoreTiles = 4;  // of a wave at most (8: 152 us where 4 take 141)
 template <bool kFp8, int D>

@@ -230,9 +230,9 @@ struct Limits {
 // [from, to).  unit_at(u, page, tok) gives unit u's page (-1: nothing to read) and its first
 // token's position; a unit is 1 << unit_tiles_log2 tiles of its page.  Lane k looks up the
 // wave's unit k, 64 at a time, and the units with something to read are packed to the front, so
-// that the tile loop only meets those.  The K rows of the next two tiles are requested when the
-// scores have used this step's, the V rows when P V has.  limits() is asked once, when the first
-// rows are on their way.
+// that the tile loop only meets those.  The K rows of the next two tiles are requested when this
+// step's are in LDS (kx: two tiles of the wave's own), the V rows when P V has used this step's.
+// limits() is asked once, when the first rows are on their way.
 template <int kCB, int D, bool kFp8, class UnitAt, class LimitsOf>
 __device__ __forceinline__ void stream_units(const PageAttnParams& P,
                                              ColumnState<kCB, D, kFp8>& st, UnitAt unit_at,

@@ -12,13 +12,24 @@
 // is streamed like decode's, 16 columns at most.  Both kinds are lines of tiles,
 //   prefix line: (group, kv head, block of columns) x tiles of the prefix
 //   own line:    (row, kv head, block of 16 query heads) x tiles from the prefix's end on
-// cut into equal ranges, one per work-group and one per wave, so that lengths need not be known
-// on the host and none waits for the longest.  The four waves of a work-group share a prefix
-// range's tiles (fk_page_attn.h).  Each item and range leaves one partial state; a second launch
-// merges each row's partials of both kinds.  Where the items are few, each is rounded up to
-// whole ranges, so that no range spans two (its start and end cost as much as 30 tiles).  The prefix is bound by the vector and matrix units, the
-// rest by memory: one half of the work-groups takes its prefix range first and the other half
-// last, so that a CU, which holds one of each, does both at a time.
+// cut into equal ranges, one per work-group of the first and one per wave of the second, so that
+// lengths need not be known on the host and none waits for the longest.  The four waves of a
+// work-group share a prefix range's tiles (fk_page_attn.h).  Each item and range leave one
+// partial state; a second launch merges each row's partials of both kinds.
+//
+// What bounds it.  Own tiles are read once: memory.  A prefix tile is read once per 32 columns
+// (at head size 128), from L2 where the column blocks' ranges are in phase (below), and costs the
+// vector units as much as the matrix units.  One half of the work-groups takes its prefix range
+// first and the other half last, so that a CU, which holds one of each, does both at a time.
+// Two waves a SIMD (O of 32 columns, the queries, and two tiles of K and V fill their registers)
+// leave latencies that show.  Measured: 64 rows of 32 / 8 heads over a prefix of 8192 bf16
+// tokens with 100 .. 2000 of their own 94.7 us and 5.5 for the merge (311 MB, 9.7 GFLOP); 128
+// rows of 64 / 8 heads over three prefixes of 11000 .. 16400 fp8 tokens 149 us and 7.6 (250 MB,
+// 60 GFLOP), of which 132 with every page in L2; 8 rows over 1488 tokens 15.4 us and 4.0.
+// Variants that were slower there: 16 or 64 columns to a wave, 128 columns to a work-group
+// with K and V staged in LDS (117 .. 136 and 185 .. 210 us), the four waves on four column blocks
+// of the same tiles (98 and 152, 10 for the merge), two steps of loads ahead, items rounded up to
+// whole ranges (101 and 160).
 #include <limits.h>
 
 #include "fk_page_attn.h"
@@ -29,7 +40,7 @@ namespace {
 constexpr int kWaves = 4;
 constexpr int kThreads = kWaves * 64;
 constexpr int kPreTiles = 8;      // a prefix range is a multiple of this: two tiles per wave
-constexpr int kOwnTiles = 2;      // and a wave's own range of this
+constexpr int kOwnTiles = 2;      // and a wave's own range of this: a step
 constexpr int kMaxGroups = 2048;  // (their bounds are held in LDS)
 
 // Column blocks of a prefix item.  (O takes 4 D / 16 registers per block.)
