@@ -805,7 +805,8 @@ def update_key_bounds(key_bounds: torch.Tensor, k_cache: torch.Tensor, block_tab
     Call it after the tokens are stored, with cache_seqlens counting them.  The newest tokens
     are the last cu_seqlens_q[b + 1] - cu_seqlens_q[b] of sequence b (the last one without
     cu_seqlens_q), at most max_seqlen_q.  Pages are read whole, so the result depends on the
-    cache alone: a rejected draft token is forgotten with the next call on its page."""
+    cache alone: a rejected draft token is forgotten with the next call on its page.  A page
+    that several sequences list should be full in each of them."""
     what = "update_key_bounds"
     shape = k_cache.shape
     if len(shape) != 4 or not k_cache.is_contiguous():

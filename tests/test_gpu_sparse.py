@@ -235,7 +235,7 @@ def test_select_blocks(cuda, width, keep, first, last, lens, rows):
 @pytest.mark.parametrize("kind", ["outlier", "low_outlier", "close", "negative", "denormal", "huge",
                                   "two", "few_equal", "sorted", "tiny_steps"])
 @pytest.mark.parametrize("width,keep,first,last", [(70, 9, 1, 1), (600, 128, 1, 1), (5000, 64, 0, 2),
-                                                   (9000, 700, 3, 0)])
+                                                   (9000, 700, 3, 0), (32768, 1000, 1, 1)])
 def test_select_blocks_of_finite_scores(cuda, kind, width, keep, first, last):
     """Distributions that put the lowest selected score where it is hard to find."""
     from fastkernels_amd import ops
