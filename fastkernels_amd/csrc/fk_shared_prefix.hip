@@ -105,14 +105,32 @@ __device__ __forceinline__ int64_t lane64(int64_t v, int src) {
   const uint32_t hi = __builtin_amdgcn_readlane(static_cast<int>(v >> 32), src);
   return static_cast<int64_t>((static_cast<uint64_t>(hi) << 32) | lo);
 }
-// Inclusive sums over the lanes of a wave.
-__device__ __forceinline__ int64_t scan64(int64_t v, int lane) {
-#pragma unroll 1
-  for (int off = 1; off < 64; off <<= 1) {
-    const int64_t y = __shfl_up(v, off, 64);
-    if (lane >= off) v += y;
-  }
-  return v;
+// Inclusive sums over the lanes of a wave: within rows of 16, then across them.
+template <int kCtrl, int kRows>
+__device__ __forceinline__ int64_t plus_moved(int64_t v) {
+  const uint32_t lo = __builtin_amdgcn_update_dpp(0, static_cast<int>(v), kCtrl, kRows, 0xf, false);
+  const uint32_t hi =
+      __builtin_amdgcn_update_dpp(0, static_cast<int>(v >> 32), kCtrl, kRows, 0xf, false);
+  return v + static_cast<int64_t>((static_cast<uint64_t>(hi) << 32) | lo);
+}
+__device__ __forceinline__ int64_t scan64(int64_t v) {
+  v = plus_moved<0x111, 0xf>(v);     // from the lane 1 before, 2, 4, 8
+  v = plus_moved<0x112, 0xf>(v);
+  v = plus_moved<0x114, 0xf>(v);
+  v = plus_moved<0x118, 0xf>(v);
+  v = plus_moved<0x142, 0xa>(v);     // from lane 15 of the row before, into rows 1 and 3
+  return plus_moved<0x143, 0xc>(v);  // from lane 31, into rows 2 and 3
+}
+// v of the lane `off` places further on in the row of 16, round.
+template <int kOff>
+__device__ __forceinline__ uint32_t rotated(uint32_t v) {
+  return __builtin_amdgcn_update_dpp(0, v, 0x120 + kOff, 0xf, 0xf, false);
+}
+__device__ __forceinline__ uint32_t row_max(uint32_t v) {
+  v = max(v, rotated<8>(v));
+  v = max(v, rotated<4>(v));
+  v = max(v, rotated<2>(v));
+  return max(v, rotated<1>(v));
 }
 // A line of `total` tiles is cut into ranges of the least multiple of `quantum` (a power of two)
 // that makes them at most n.
@@ -224,7 +242,7 @@ __attribute__((amdgpu_waves_per_eu((D == 256 ? 1 : 2)))) void shared_prefix_kern
   };
   // Inclusive sums over the work-group's threads; total: over all of them.
   auto scan_all = [&](int64_t v, int64_t& total) {
-    const int64_t x = scan64(v, lane);
+    const int64_t x = scan64(v);
     if (lane == 63) wave_sum[wave] = x;
     __syncthreads();
     int64_t before = 0;
@@ -243,7 +261,7 @@ __attribute__((amdgpu_waves_per_eu((D == 256 ? 1 : 2)))) void shared_prefix_kern
       const Group x = group_at(i);
       sum += group_items(x) * places_of(x.prefix);
     }
-    return lane64(scan64(sum, lane), 63);
+    return lane64(scan64(sum), 63);
   };
   // Streams positions [from, to) of one item through the table `table`: unit `first` and every
   // step-th after it.
@@ -275,8 +293,8 @@ __attribute__((amdgpu_waves_per_eu((D == 256 ? 1 : 2)))) void shared_prefix_kern
       const Group x = group_at(g0 + lane);
       const int items = group_items(x);
       const int64_t mine = items * places_of(x.prefix);
-      const int64_t end = line + scan64(mine, lane);
-      const int64_t item_end = item0 + scan64(items, lane);
+      const int64_t end = line + scan64(mine);
+      const int64_t item_end = item0 + scan64(items);
       uint64_t hit = __ballot(mine > 0 && end > t_lo && end - mine < t_hi);
       while (hit) {
         const int src = __builtin_ctzll(hit);
@@ -333,13 +351,8 @@ __attribute__((amdgpu_waves_per_eu((D == 256 ? 1 : 2)))) void shared_prefix_kern
                 x.span = max(x.span, ok ? x.lim[cb] : 0u);
                 x.least = min(x.least, x.lim[cb]);
               }
-#pragma unroll
-              for (int off = 1; off < 16; off <<= 1) {
-                x.span = max(x.span, static_cast<uint32_t>(__shfl_xor(x.span, off, 64)));
-                x.least = min(x.least, static_cast<uint32_t>(__shfl_xor(x.least, off, 64)));
-              }
-              x.span = uniform(x.span);
-              x.least = uniform(x.least);
+              x.span = uniform(row_max(x.span));
+              x.least = ~uniform(row_max(~x.least));
               return x;
             };
             stream(st, bt + row0 * A.bt_row_stride, lo, hi, wave, kWaves, limits, kvh,
@@ -455,8 +468,8 @@ __attribute__((amdgpu_waves_per_eu((D == 256 ? 1 : 2)))) void shared_prefix_kern
         const Group x = group_at(g0 + lane);
         const int items = group_items(x);
         const int64_t mine = items * places_of(x.prefix);
-        const int64_t end = line + scan64(mine, lane);
-        const int64_t item_end = item0 + scan64(items, lane);
+        const int64_t end = line + scan64(mine);
+        const int64_t item_end = item0 + scan64(items);
         if (g0 + lane < P.num_groups) {
           pre_start[g0 + lane] = end - mine;
           pre_item[g0 + lane] = static_cast<int>(item_end) - items;
