@@ -19,13 +19,14 @@
 //
 // What bounds it.  Own tiles are read once: memory.  A prefix tile is read once per 32 columns
 // (at head size 128), from L2 where the column blocks' ranges are in phase (below), and costs the
-// vector units as much as the matrix units.  One half of the work-groups takes its prefix range
-// first and the other half last, so that a CU, which holds one of each, does both at a time.
+// vector units as much as the matrix units.  One half of the CUs takes its prefix ranges first
+// and the other half last, so that the chip does both at a time (both on each CU: 96 us where
+// this takes 87).
 // Two waves a SIMD (O of 32 columns, the queries, and two tiles of K and V fill their registers)
 // leave latencies that show.  Measured: 64 rows of 32 / 8 heads over a prefix of 8192 bf16
-// tokens with 100 .. 2000 of their own 94.7 us and 5.5 for the merge (311 MB, 9.7 GFLOP); 128
+// tokens with 100 .. 2000 of their own 87 us and 5.5 for the merge (311 MB, 9.7 GFLOP); 128
 // rows of 64 / 8 heads over three prefixes of 11000 .. 16400 fp8 tokens 149 us and 7.6 (250 MB,
-// 60 GFLOP), of which 132 with every page in L2; 8 rows over 1488 tokens 15.4 us and 4.0.
+// 60 GFLOP), of which 132 with every page in L2; 8 rows over 1488 tokens 13.9 us and 4.0.
 // Variants that were slower there: 16 or 64 columns to a wave, 128 columns to a work-group
 // with K and V staged in LDS (117 .. 136 and 185 .. 210 us), the four waves on four column blocks
 // of the same tiles (98 and 152, 10 for the merge), two steps of loads ahead, items rounded up to
@@ -507,7 +508,8 @@ __attribute__((amdgpu_waves_per_eu((D == 256 ? 1 : 2)))) void shared_prefix_kern
     }
     return;
   }
-  const bool prefix_first = wg < P.wgs / 2;
+  // (Work-groups go to the XCDs in turn and in each to its CUs, of which there is an even number.)
+  const bool prefix_first = !((wg >> 3) & 1);
 #pragma unroll 1
   for (int phase = 0; phase < 2; ++phase) {
     if ((phase == 0) == prefix_first)
