@@ -192,3 +192,37 @@ def test_shared_prefix_in_graphs(cuda):
         want = steps()
         torch.cuda.synchronize()
         assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+
+
+def test_two_streams_at_once(cuda):
+    """Shared-prefix and sparse calls that overlap on two streams, against the same calls one
+    after the other: results depend on nothing but the arguments."""
+    from fastkernels_amd import ops
+
+    hq, hk, d, page = 32, 8, 128, 16
+    calls = []
+    for seed in range(2):
+        g, q, k, v, bt, lens, cu, pre, _, _ = build(cuda, "bf16", hq, hk, d, page,
+                                                    GROUPS["ragged"], seed)
+        ctx, n = int32(lens, cuda), len(lens)
+        idx = torch.randint(-1, 60, (n, hk, 20), generator=g, device=cuda, dtype=torch.int32)
+
+        def call(out, args=(q, k, v, bt, ctx), cu=cu, pre=pre, idx=idx):
+            ops.shared_prefix_decode(out[0], *args, cu, pre, d ** -0.5)
+            ops.sparse_paged_decode(out[1], *args, idx, d ** -0.5)
+
+        calls.append((call, (2, *q.shape)))
+    want = [torch.zeros(s, dtype=torch.bfloat16, device=cuda) for _, s in calls]
+    for (call, _), out in zip(calls, want):
+        call(out)
+    got = [[torch.zeros(s, dtype=torch.bfloat16, device=cuda) for _ in range(6)] for _, s in calls]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    for i in range(6):
+        for (call, _), outs, stream in zip(calls, got, streams):
+            with torch.cuda.stream(stream):
+                call(outs[i])
+    torch.cuda.synchronize()
+    for outs, w in zip(got, want):
+        for out in outs:
+            assert torch.equal(out.view(torch.int16), w.view(torch.int16))
