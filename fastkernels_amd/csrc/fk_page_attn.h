@@ -46,7 +46,7 @@ struct PageAttnParams {
 // The maximum is only moved when a score exceeds it by more than kLazyMax: until then the
 // weights grow to at most 2^8, which bf16 and the fp32 sums hold as exactly as smaller ones.
 constexpr float kLazyMax = 8.f;
-constexpr float kNoMax = -1.0e30f;  // the reference before a column's first visible key
+constexpr float kNoMax = -3.0e38f;  // the reference before a column's first visible key
 
 template <int kCB, int D, bool kFp8>
 struct ColumnState {
@@ -97,6 +97,13 @@ struct ColumnState {
   __device__ __forceinline__ void softmax(floatx4_t (&sa)[kCB], floatx4_t (&sb)[kCB], float s2,
                                           uint32_t ra, uint32_t rb, const uint32_t (&lim)[kCB],
                                           bool full) {
+    // (Scaled first: the products are rounded alike here and in the maximum, so that no weight
+    // exceeds 2^kLazyMax however great the scores; and a scale of 0 meets no infinity.)
+#pragma unroll
+    for (int cb = 0; cb < kCB; ++cb) {
+      sa[cb] *= s2;
+      sb[cb] *= s2;
+    }
     if (!full) {
 #pragma unroll
       for (int cb = 0; cb < kCB; ++cb)
@@ -110,8 +117,8 @@ struct ColumnState {
     bool move = false;
 #pragma unroll
     for (int cb = 0; cb < kCB; ++cb) {
-      top[cb] = s2 * fmaxf(fmaxf(fmaxf(sa[cb][0], sa[cb][1]), fmaxf(sa[cb][2], sa[cb][3])),
-                           fmaxf(fmaxf(sb[cb][0], sb[cb][1]), fmaxf(sb[cb][2], sb[cb][3])));
+      top[cb] = fmaxf(fmaxf(fmaxf(sa[cb][0], sa[cb][1]), fmaxf(sa[cb][2], sa[cb][3])),
+                      fmaxf(fmaxf(sb[cb][0], sb[cb][1]), fmaxf(sb[cb][2], sb[cb][3])));
       move |= top[cb] > m[cb] + kLazyMax;
     }
     if (__ballot(move) != 0) {
@@ -129,18 +136,9 @@ struct ColumnState {
     for (int cb = 0; cb < kCB; ++cb) {
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        sa[cb][i] = __builtin_amdgcn_exp2f(__builtin_fmaf(sa[cb][i], s2, -m[cb]));
-        sb[cb][i] = __builtin_amdgcn_exp2f(__builtin_fmaf(sb[cb][i], s2, -m[cb]));
+        sa[cb][i] = __builtin_amdgcn_exp2f(sa[cb][i] - m[cb]);
+        sb[cb][i] = __builtin_amdgcn_exp2f(sb[cb][i] - m[cb]);
       }
-    }
-    if (!full) {  // (not left to -inf: its product with a scale of 0 is NaN)
-#pragma unroll
-      for (int cb = 0; cb < kCB; ++cb)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          if (!(ra + i < lim[cb])) sa[cb][i] = 0.f;
-          if (!(rb + i < lim[cb])) sb[cb][i] = 0.f;
-        }
     }
 #pragma unroll
     for (int cb = 0; cb < kCB; ++cb)

@@ -461,3 +461,53 @@ def test_sparse_in_a_graph(cuda):
         want = step()
         torch.cuda.synchronize()
         assert torch.equal(got, want) and bool(torch.isfinite(other).all())
+
+
+@pytest.mark.parametrize("rows", [1, 40])
+@pytest.mark.parametrize("sign", [-1, 1])
+def test_scores_of_great_magnitude(cuda, rows, sign):
+    """Logits of +-2^123, all equal: the mean of V, in fp32 exactly (64 small integers)."""
+    from fastkernels_amd import ops
+
+    g = torch.Generator(device=cuda).manual_seed(rows)
+    hq, hk, d, page = 4, 2, 64, 16
+    k = torch.full((4, page, hk, d), sign * 2.0 ** 60, dtype=torch.bfloat16, device=cuda)
+    v = torch.randint(-3, 4, (4, page, hk, d), generator=g, device=cuda).to(torch.bfloat16)
+    q = torch.full((rows, hq, d), 2.0 ** 60, dtype=torch.bfloat16, device=cuda)
+    bt = int32([[2, 0, 3, 1]] * rows, cuda)
+    ctx = int32([64] * rows, cuda)
+    want = v.float().sum((0, 1)).div(64).repeat_interleave(hq // hk, 0).to(torch.bfloat16)
+    sparse, prefix = torch.zeros_like(q), torch.zeros_like(q)
+    ops.sparse_paged_decode(sparse, q, k, v, bt, ctx,
+                            int32([[[0, 1, 2, 3]] * hk] * rows, cuda), d ** -0.5)
+    ops.shared_prefix_decode(prefix, q, k, v, bt, ctx, int32([0, rows], cuda), int32([40], cuda),
+                             d ** -0.5)
+    assert torch.equal(sparse, want.expand_as(q)) and torch.equal(prefix, want.expand_as(q))
+
+
+@pytest.mark.parametrize("kv", ["bf16", "fp8"])
+@pytest.mark.parametrize("d", [64, 128, 256])
+def test_one_score_above_great_ones(cuda, kv, d):
+    """Logits near +-2^100 whose rounding alone is beyond any exponent: the greatest key's V."""
+    from fastkernels_amd import ops
+
+    g = torch.Generator(device=cuda).manual_seed(d)
+    hq, hk, page, n = 4, 2, 16, 150
+    q = (torch.randn(2, hq, d, generator=g, device=cuda).abs() + 0.1) * 2.0 ** 96
+    q[1] *= -1
+    row = torch.randn(1, 1, hk, d, generator=g, device=cuda).abs() + 0.1
+    k = row.expand(10, page, hk, d).clone()
+    k[4, 3] *= 4     # the greatest logit of row 0
+    k[8, 9] *= 0.25  # and of row 1
+    dtype = FP8 if kv == "fp8" else torch.bfloat16
+    k, q = k.to(dtype), q.to(torch.bfloat16)
+    v = torch.randint(-8, 9, (10, page, hk, d), generator=g, device=cuda).to(dtype)
+    bt, ctx = int32([list(range(10))] * 2, cuda), int32([n, n], cuda)
+    one = torch.ones(hk, device=cuda) if kv == "fp8" else None
+    want = torch.stack([v[4, 3], v[8, 9]]).to(torch.bfloat16).repeat_interleave(hq // hk, 1)
+    sparse, prefix = torch.zeros_like(q), torch.zeros_like(q)
+    ops.sparse_paged_decode(sparse, q, k, v, bt, ctx,
+                            int32([[list(range(10))] * hk] * 2, cuda), 0.1, one, one)
+    ops.shared_prefix_decode(prefix, q, k, v, bt, ctx, int32([0, 2], cuda), int32([100], cuda), 0.1,
+                             one, one)
+    assert torch.equal(sparse, want) and torch.equal(prefix, want)
