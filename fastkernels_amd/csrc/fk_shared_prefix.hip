@@ -21,12 +21,12 @@
 // (at head size 128), from L2 where the column blocks' ranges are in phase (below), and costs the
 // vector units as much as the matrix units.  One half of the CUs takes its prefix ranges first
 // and the other half last, so that the chip does both at a time (both on each CU: 96 us where
-// this takes 87).
+// this took 87).
 // Two waves a SIMD (O of 32 columns, the queries, and two tiles of K and V fill their registers)
 // leave latencies that show.  Measured: 64 rows of 32 / 8 heads over a prefix of 8192 bf16
-// tokens with 100 .. 2000 of their own 87 us and 5.5 for the merge (311 MB, 9.7 GFLOP); 128
-// rows of 64 / 8 heads over three prefixes of 11000 .. 16400 fp8 tokens 149 us and 7.6 (250 MB,
-// 60 GFLOP), of which 132 with every page in L2; 8 rows over 1488 tokens 13.9 us and 4.0.
+// tokens with 100 .. 2000 of their own 83 us and 5.5 for the merge (311 MB, 9.7 GFLOP); 128
+// rows of 64 / 8 heads over three prefixes of 11000 .. 16400 fp8 tokens 142 us and 7.6 (250 MB,
+// 60 GFLOP; little less with every page in L2); 8 rows over 1488 tokens 13.9 us and 4.0.
 // Variants that were slower there: 16 or 64 columns to a wave, 128 columns to a work-group
 // with K and V staged in LDS (117 .. 136 and 185 .. 210 us), the four waves on four column blocks
 // of the same tiles (98 and 152, 10 for the merge), two steps of loads ahead, items rounded up to
