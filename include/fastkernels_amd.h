@@ -482,7 +482,8 @@ int fk_silu_and_mul(void* out, int64_t out_row_stride, const void* x, int64_t x_
  * each page that holds one of sequence b's last n tokens (n = its query rows, 1 without
  * cu_seqlens_q), key_bounds[page, h, 0] and [page, h, 1] become the least and the greatest
  * value of each key dimension over the page's tokens < cache_seqlens[b] (NaN if one is NaN).
- * Whole pages are read, so the result does not depend on earlier calls.  batch <= 65535. */
+ * Whole pages are read, so the result does not depend on earlier calls; a page that several
+ * sequences list should be full in each.  batch <= 65535. */
 int fk_update_key_bounds(void* key_bounds, const void* k_cache, int kv_dtype,
                          const int32_t* block_tables, int64_t bt_row_stride, int64_t bt_width,
                          const int32_t* cache_seqlens, const int32_t* cu_seqlens_q,

@@ -511,3 +511,40 @@ def test_one_score_above_great_ones(cuda, kv, d):
     ops.shared_prefix_decode(prefix, q, k, v, bt, ctx, int32([0, 2], cuda), int32([100], cuda), 0.1,
                              one, one)
     assert torch.equal(sparse, want) and torch.equal(prefix, want)
+
+
+@pytest.mark.parametrize("kv", ["bf16", "fp8"])
+def test_caches_past_4_gib(cuda, kv):
+    """Pages whose byte offsets pass 32 bits, against the same pages in a small cache."""
+    from fastkernels_amd import ops
+
+    g = torch.Generator(device=cuda).manual_seed(3)
+    hq, hk, d, page = 16, 8, 128, 256
+    dtype = FP8 if kv == "fp8" else torch.bfloat16
+    nb = (5 << 30) // (page * hk * d * dtype.itemsize)
+    at = [0, nb - 1, nb // 2 + 1, nb - 2]
+    small = [make_cache(g, 4, page, hk, d, kv, cuda) for _ in range(2)]
+    big = [torch.empty(nb, page, hk, d, dtype=dtype, device=cuda) for _ in range(2)]
+    for x, y in zip(big, small):
+        for i, p in enumerate(at):
+            x[p] = y[i]
+    q = torch.randn(3, hq, d, generator=g, device=cuda).to(torch.bfloat16)
+    one = torch.ones(hk, device=cuda) if kv == "fp8" else None
+    ctx = int32([1000, 1024, 700], cuda)
+    got = []
+    for (k, v), pages in ((small, [0, 1, 2, 3]), (big, at)):
+        bt = int32([pages] * 3, cuda)
+        bounds = ops.new_key_bounds(k)
+        # (of the sequence that fills them: bounds of a shared page are those of one caller)
+        ops.update_key_bounds(bounds, k, bt[1:2], ctx[1:2], int32([0, 1024], cuda), 1024)
+        scores = torch.empty(3, hk, 4, device=cuda)
+        ops.block_scores(scores, q, bounds, bt, ctx, page, one)
+        idx = torch.empty(3, hk, 3, dtype=torch.int32, device=cuda)
+        ops.select_blocks(idx, scores, ctx, page)
+        sparse, prefix = torch.empty_like(q), torch.empty_like(q)
+        ops.sparse_paged_decode(sparse, q, k, v, bt, ctx, idx, d ** -0.5, one, one)
+        ops.shared_prefix_decode(prefix, q, k, v, bt, ctx, int32([0, 3], cuda),
+                                 int32([600], cuda), d ** -0.5, one, one)
+        got.append((bounds[pages].float(), scores, idx, sparse, prefix))
+    for name, a, b in zip(("bounds", "scores", "pages", "sparse", "prefix"), *got):
+        assert torch.equal(a, b), name
