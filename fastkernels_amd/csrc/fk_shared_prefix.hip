@@ -60,7 +60,7 @@ struct RowRecord {
   int pre_item;       // its group's first prefix item
   int col_items;      // column blocks of its group, per kv head
   int index;          // row of its group
-  int pad_;
+  int short_keys;     // keys of a row shorter than its group's prefix, otherwise -1
 };
 
 struct PrefixParams {
@@ -493,6 +493,7 @@ __attribute__((amdgpu_waves_per_eu((D == 256 ? 1 : 2)))) void shared_prefix_kern
       rec.own_start = end - mine;
       rec.own_range = own_range;
       rec.own_tiles = o.tiles;
+      rec.short_keys = -1;
       rec.pre_range = pre_range;
       const int grp = group_of(b);
       if (grp >= 0) {
@@ -503,6 +504,7 @@ __attribute__((amdgpu_waves_per_eu((D == 256 ? 1 : 2)))) void shared_prefix_kern
         rec.pre_item = pre_item[grp];
         rec.col_items = group_items(x) / A.num_kv_heads;
         rec.index = b - x.first;
+        if (o.ctx < x.prefix) rec.short_keys = o.ctx;
       }
       P.rows[b] = rec;
     }
@@ -519,12 +521,83 @@ __attribute__((amdgpu_waves_per_eu((D == 256 ? 1 : 2)))) void shared_prefix_kern
   }
 }
 
-// One work-group per (row, kv head, block of 16 query heads) merges the row's partials.
+// A step of 256 keys in attend_plainly: where they are in the caches, and their weights.
+struct PlainLds {
+  int64_t row[kMergeThreads];
+  float weight[kMergeThreads], top[kMergeThreads / 64];
+};
+// Attention of query head hq of row b over positions [0, keys) read through `table`, by a merge's
+// work-group: a key a thread for the scores, a dim a thread for the sums.
 template <int D>
-__global__ __launch_bounds__(kMergeThreads) void shared_prefix_merge_kernel(PrefixParams P,
-                                                                            int fp8) {
+__device__ void attend_plainly(const PageAttnParams& A, const int32_t* __restrict__ table, int keys,
+                               bool fp8, int b, int hq, PlainLds& lds) {
+  static_assert(D <= kMergeThreads, "a dim a thread");
+  const int tid = threadIdx.x, kvh = hq / A.gqa;
+  const uint16_t* const q = A.q + b * A.q_row_stride + static_cast<int64_t>(hq) * D;
+  const float s2 = fp8 && A.k_scale ? A.scale_log2 * A.k_scale[kvh] : A.scale_log2;
+  // Index of position t's first element in the caches, -1 at a masked page.
+  auto row_at = [&](int t) -> int64_t {
+    const int j = t >> A.block_size_log2;
+    const int page = j < A.bt_width ? table[j] : -1;
+    if (page < 0 || page >= A.num_blocks) return -1;
+    const int64_t slot = (static_cast<int64_t>(page) << A.block_size_log2) +
+                         (t & ((1 << A.block_size_log2) - 1));
+    return (slot * A.num_kv_heads + kvh) * D;
+  };
+  auto value = [&](const uint8_t* cache, int64_t i) {
+    return fp8 ? __builtin_amdgcn_cvt_f32_fp8(cache[i], 0)
+               : __uint_as_float(static_cast<uint32_t>(
+                     reinterpret_cast<const uint16_t*>(cache)[i]) << 16);
+  };
+  float m = kNegInf, l = 0.f, o = 0.f;
+  for (int t0 = 0; t0 < keys; t0 += kMergeThreads) {
+    const int64_t row = t0 + tid < keys ? row_at(t0 + tid) : -1;
+    float s = kNegInf;
+    if (row >= 0) {
+      float dot = 0.f;
+      for (int d = 0; d < D; ++d)
+        dot = __builtin_fmaf(__uint_as_float(static_cast<uint32_t>(q[d]) << 16),
+                             value(A.k_cache, row + d), dot);
+      s = dot * s2;
+    }
+    float most = s;
+    for (int off = 32; off; off >>= 1) most = fmaxf(most, __shfl_xor(most, off, 64));
+    if ((tid & 63) == 0) lds.top[tid >> 6] = most;
+    __syncthreads();
+    for (int w = 0; w < kMergeThreads / 64; ++w) most = fmaxf(most, lds.top[w]);
+    const float m_new = fmaxf(m, most), used = m_new == kNegInf ? 0.f : m_new;
+    const float alpha = __builtin_amdgcn_exp2f(m - used);
+    m = m_new;
+    lds.row[tid] = row;
+    lds.weight[tid] = __builtin_amdgcn_exp2f(s - used);
+    __syncthreads();
+    l *= alpha;
+    o *= alpha;
+    for (int k = 0; k < min(kMergeThreads, keys - t0); ++k) {
+      if (lds.row[k] < 0) continue;
+      l += lds.weight[k];
+      if (tid < D) o = __builtin_fmaf(lds.weight[k], value(A.v_cache, lds.row[k] + tid), o);
+    }
+    __syncthreads();
+  }
+  l = with_sink(l, m, A.sinks ? A.sinks[hq] * kLog2e : kNegInf);
+  const float f = l > 0.f ? (fp8 && A.v_scale ? A.v_scale[kvh] : 1.f) / l : 0.f;
+  if (tid < D)
+    A.out[b * A.out_row_stride + static_cast<int64_t>(hq) * D + tid] = f32_to_bf16(o * f);
+}
+
+// One work-group per (row, kv head, block of 16 query heads) merges the row's partials.
+//
+// A row shorter than its group's prefix has zero weights for the keys that only others see, but
+// in the products with V these meet the others' values all the same: where one is infinite or
+// NaN the row's sum is NaN.  Such a row that is not finite is computed again by itself.
+template <int D>
+__global__ __launch_bounds__(kMergeThreads) void shared_prefix_merge_kernel(
+    PrefixParams P, const int32_t* __restrict__ bt, int fp8) {
   constexpr int kCols = cols_of(D);
   __shared__ Folded folded[kMergeThreads];
+  static_assert(sizeof(PlainLds) <= sizeof(folded), "the plain form's weights fit");
+  __shared__ uint32_t again;  // bits: columns to compute again
   const PageAttnParams& A = P.A;
   const int b = blockIdx.y, v = blockIdx.x;
   const int kvh = v / A.col_blocks;
@@ -543,6 +616,10 @@ __global__ __launch_bounds__(kMergeThreads) void shared_prefix_merge_kernel(Pref
   int pre_n = 0;
   int64_t pre_col = 0;
   const int j0 = blockIdx.z * P.merge_cols;
+  if (rec.short_keys >= 0) {
+    if (threadIdx.x == 0) again = 0;
+    __syncthreads();
+  }
   merge_pieces<D>(
       j0, min(P.merge_cols, min(16, A.gqa - in_group) - j0), folded,
       [&](int j) {
@@ -568,7 +645,15 @@ __global__ __launch_bounds__(kMergeThreads) void shared_prefix_merge_kernel(Pref
       },
       [&](int j, int dim, const float4& o, float M, float L) {
         write_quad(A, b, kvh * A.gqa + in_group + j, D, dim, o, M, L, vsc);
+        if (rec.short_keys >= 0 && !__builtin_isfinite((o.x + o.y) + (o.z + o.w)))
+          atomicOr(&again, 1u << j);
       });
+  if (rec.short_keys < 0) return;
+  __syncthreads();
+  for (uint32_t left = __builtin_amdgcn_readfirstlane(again); left; left &= left - 1)
+    attend_plainly<D>(A, bt + (b - rec.index) * A.bt_row_stride, rec.short_keys, fp8 != 0, b,
+                      kvh * A.gqa + in_group + __builtin_ctz(left),
+                      *reinterpret_cast<PlainLds*>(folded));
 }
 
 // The bound on the shared tokens of a prefix that an argument of 0 (none) or more stands for.
@@ -627,7 +712,7 @@ void launch_d(bool fp8, const PrefixParams& P, hipStream_t s, const int32_t* bt,
   hipLaunchKernelGGL((shared_prefix_merge_kernel<D>),
                      dim3(static_cast<unsigned>(P.vheads), static_cast<unsigned>(P.A.batch),
                           (P.own_cols + P.merge_cols - 1) / P.merge_cols),
-                     dim3(kMergeThreads), 0, s, P, fp8 ? 1 : 0);
+                     dim3(kMergeThreads), 0, s, P, bt, fp8 ? 1 : 0);
 }
 
 }  // namespace

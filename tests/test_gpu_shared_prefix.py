@@ -7,7 +7,7 @@ import pytest
 import torch
 
 from oracle import partial as ref
-from test_gpu_sparse import check_attn, cu_of, f64, int32, load, make_cache, poison
+from test_gpu_sparse import attn_tolerance, check_attn, cu_of, f64, int32, load, make_cache, poison
 
 pytestmark = pytest.mark.gpu
 
@@ -226,3 +226,62 @@ def test_two_streams_at_once(cuda):
     for outs, w in zip(got, want):
         for out in outs:
             assert torch.equal(out.view(torch.int16), w.view(torch.int16))
+
+
+# Rows of a group whose prefix is longer than some of them: (prefix, length of each row).
+SHORT_ROWS = {
+    "padding": (100, [150, 40, 0, 100, 98, 130]),
+    "first": (333, [0, 340, 333, 200, 1, 700]),
+    "many": (700, [0 if i % 7 == 3 else 13 * i + 1 for i in range(60)]),
+    "beyond": (5000, [1000, 1001, 1002, 999]),
+}
+
+
+@pytest.mark.parametrize("name", list(SHORT_ROWS))
+@pytest.mark.parametrize("kv,hq,hk,d,page,bad", [
+    ("bf16", 32, 8, 128, 16, "nan"), ("bf16", 32, 8, 128, 16, "inf"),
+    ("bf16", 40, 2, 128, 32, "-inf"), ("fp8", 16, 2, 128, 64, "nan"),
+    ("bf16", 8, 1, 256, 16, "inf"), ("bf16", 10, 10, 64, 32, "-inf"),
+    ("fp8", 12, 4, 256, 128, "nan"), ("fp8", 40, 1, 64, 16, "nan"),
+])
+def test_values_that_a_shorter_row_does_not_see(cuda, kv, hq, hk, d, page, name, bad):
+    """Keys and values of the prefix that only its longer rows see are not finite: rows that do
+    not see them are as ever, and so are the dims of the others whose values are finite."""
+    from fastkernels_amd import ops
+
+    prefix, lens = SHORT_ROWS[name]
+    g = torch.Generator(device=cuda).manual_seed(d + len(lens))
+    pages = -(-max(prefix, *lens) // page)
+    bt = torch.stack([torch.randperm(pages, generator=g, device=cuda) for _ in lens])
+    bt[:, :-(-prefix // page)] = bt[0, :-(-prefix // page)]
+    bt = (bt + 1).to(torch.int32)
+    k = make_cache(g, pages + 1, page, hk, d, kv, cuda)
+    v = make_cache(g, pages + 1, page, hk, d, kv, cuda)
+    # behind each length that ends inside the prefix: one value of V; a key behind the median
+    ends = sorted(n for n in set(lens) if 0 <= n < min(prefix, max(lens)))
+    for i, n in enumerate(ends):
+        at = (int(bt[0, n // page]), n % page, i % hk, (7 * i) % d)
+        v.view(torch.uint8 if kv == "fp8" else v.dtype)[at] = 0x7F if kv == "fp8" else float(bad)
+    mid = ends[len(ends) // 2]
+    poison(k, (int(bt[0, mid // page]), mid % page, 0, 3))
+    q = torch.randn(len(lens), hq, d, generator=g, device=cuda).to(torch.bfloat16)
+    ks = vs = None
+    if kv == "fp8":
+        ks, vs = torch.linspace(0.1, 0.3, hk, device=cuda), torch.linspace(0.2, 0.4, hk,
+                                                                          device=cuda)
+    sinks = torch.randn(hq, generator=g, device=cuda)
+    cu, pre = int32([0, len(lens)], cuda), int32([prefix], cuda)
+    out = torch.full((len(lens), hq + 1, d), 9.0, dtype=torch.bfloat16, device=cuda)[:, :hq]
+    ops.shared_prefix_decode(out, q, k, v, bt, int32(lens, cuda), cu, pre, d ** -0.5, ks, vs, -1,
+                             sinks)
+    with np.errstate(invalid="ignore"):
+        want, mean, mag = ref.shared_prefix_decode(
+            f64(q), f64(k), f64(v), bt.cpu().numpy(), lens, [0, len(lens)], [prefix], d ** -0.5,
+            f64(ks), f64(vs), -1, f64(sinks))
+    got, finite = f64(out), np.isfinite(want)
+    assert finite[lens.index(min(lens))].all()
+    assert not np.isfinite(got[~finite]).any()
+    assert np.isfinite(got[finite]).all()
+    want, mean, mag = want[finite], mean[finite], mag[finite]
+    err = (np.abs(got[finite] - want) - attn_tolerance(want, mean, mag, d)).max()
+    assert err <= 0, f"beyond the tolerance by {err}"
