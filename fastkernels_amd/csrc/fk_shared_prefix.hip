@@ -192,9 +192,9 @@ __attribute__((amdgpu_waves_per_eu((D == 256 ? 1 : 2)))) void shared_prefix_kern
   const int r = lane & 15, g = lane >> 4;
   const int tok_log2 = 4 + P.unit_tiles_log2;
   // Row and head indexes, and so every address formed from them, stay inside the batch
-  // whatever the groups say.
+  // whatever the groups say.  (Without groups there may be no cu_groups to read.)
   for (int i = threadIdx.x; i <= P.num_groups; i += kThreads) {
-    group_first[i] = min(max(cu_groups[i], 0), A.batch);
+    group_first[i] = P.num_groups > 0 ? min(max(cu_groups[i], 0), A.batch) : 0;
     if (i < P.num_groups) {
       const int64_t most = static_cast<int64_t>(A.bt_width) << A.block_size_log2;
       group_prefix[i] =

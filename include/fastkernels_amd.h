@@ -541,7 +541,8 @@ int fk_sparse_paged_decode_plan(int64_t rows, int64_t keep, int num_heads, int n
  * once for the group, through the block table of its first row; the rows' own tables are read
  * from there on.  Rows outside every group share nothing.  A row may be shorter than its
  * group's prefix (0 tokens: a zero row).  At most max_prefix_len tokens of a prefix are shared
- * (0: all of them): a bound keeps the workspace small.  At most 2048 groups. */
+ * (0: all of them): a bound keeps the workspace small.  At most 2048 groups; with none,
+ * cu_groups and prefix_lens are not read and may be NULL. */
 int fk_shared_prefix_decode(void* out, int64_t out_row_stride, const void* q,
                             int64_t q_row_stride, const void* k_cache, const void* v_cache,
                             int kv_dtype, const float* k_scale, const float* v_scale,

@@ -285,3 +285,21 @@ def test_values_that_a_shorter_row_does_not_see(cuda, kv, hq, hk, d, page, name,
     want, mean, mag = want[finite], mean[finite], mag[finite]
     err = (np.abs(got[finite] - want) - attn_tolerance(want, mean, mag, d)).max()
     assert err <= 0, f"beyond the tolerance by {err}"
+
+
+def test_no_groups_without_arrays(cuda):
+    """The C ABI with num_groups 0 takes NULL for the groups' arrays."""
+    from fastkernels_amd import _native as N
+
+    hq, hk, d, page = 32, 8, 128, 16
+    _, q, k, v, bt, lens, _, _, _, _ = build(cuda, "bf16", hq, hk, d, page, GROUPS["none"])
+    nbytes = N.shared_prefix_bytes(len(lens), 0, 0, hq, hk, d)
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=cuda)
+    out, ctx = torch.full_like(q, 9.0), int32(lens, cuda)
+    N.call("fk_shared_prefix_decode", out.data_ptr(), hq * d, q.data_ptr(), hq * d, k.data_ptr(),
+           v.data_ptr(), N.FK_DTYPE_BF16, None, None, bt.data_ptr(), bt.stride(0), bt.shape[1],
+           ctx.data_ptr(), len(lens), None, None, 0, 0, hq, hk, d, page, k.shape[0], d ** -0.5, -1,
+           None, ws.data_ptr(), nbytes, torch.cuda.current_stream().cuda_stream)
+    want = ref.shared_prefix_decode(f64(q), f64(k), f64(v), bt.cpu().numpy(), lens, [0], [],
+                                    d ** -0.5)
+    check_attn(out, *want)

@@ -256,3 +256,13 @@ def test_prefix_bound_keeps_the_workspace_small():
     assert size(64, 64, 64) < size(64, 4096, 1000)
     with pytest.raises(N.FkError):
         size(-1)
+
+
+def test_c_abi_refuses_groups_without_arrays():
+    """NULL cu_groups or prefix_lens with a group (GPU: with none they are not read)."""
+    lib, p = N.lib(), ctypes.c_void_p(0x100000)
+    for cu, pre in ((None, p), (p, None), (None, None)):
+        rc = lib.fk_shared_prefix_decode(p, 1024, p, 1024, p, p, N.FK_DTYPE_BF16, None, None, p, 4,
+                                         4, p, 2, cu, pre, 1, 0, 8, 2, 128, 16, 4, 0.1, -1, None,
+                                         p, 1 << 40, None)
+        assert rc == N.FK_ERR_INVALID_ARG and "null pointer" in last_error()
