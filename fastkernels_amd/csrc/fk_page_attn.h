@@ -46,7 +46,8 @@ struct PageAttnParams {
 // The maximum is only moved when a score exceeds it by more than kLazyMax: until then the
 // weights grow to at most 2^8, which bf16 and the fp32 sums hold as exactly as smaller ones.
 constexpr float kLazyMax = 8.f;
-constexpr float kNoMax = -3.0e38f;  // the reference before a column's first visible key
+// The reference before a column's first visible key: no finite score lies below it.
+constexpr float kNoMax = -__FLT_MAX__;
 
 template <int kCB, int D, bool kFp8>
 struct ColumnState {

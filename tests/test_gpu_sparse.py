@@ -548,3 +548,26 @@ def test_caches_past_4_gib(cuda, kv):
         got.append((bounds[pages].float(), scores, idx, sparse, prefix))
     for name, a, b in zip(("bounds", "scores", "pages", "sparse", "prefix"), *got):
         assert torch.equal(a, b), name
+
+
+@pytest.mark.parametrize("kv", ["bf16", "fp8"])
+def test_logits_next_to_the_least_float(cuda, kv):
+    """Scaled logits between -3.4e38 and -3e38, all equal: the mean of V."""
+    from fastkernels_amd import ops
+
+    g = torch.Generator(device=cuda).manual_seed(5)
+    hq, hk, d, page = 4, 2, 64, 16
+    dtype = FP8 if kv == "fp8" else torch.bfloat16
+    k = torch.full((4, page, hk, d), -1.0, device=cuda).to(dtype)
+    v = torch.randint(-3, 4, (4, page, hk, d), generator=g, device=cuda).to(dtype)
+    q = torch.full((2, hq, d), 2.0 ** 120, dtype=torch.bfloat16, device=cuda)
+    bt, ctx = int32([[2, 0, 3, 1]] * 2, cuda), int32([64, 64], cuda)
+    one = torch.ones(hk, device=cuda) if kv == "fp8" else None
+    want = v.float().sum((0, 1)).div(64).repeat_interleave(hq // hk, 0).to(torch.bfloat16)
+    # 2^126 * 2.6 * log2(e) = 3.19e38
+    sparse, prefix = torch.zeros_like(q), torch.zeros_like(q)
+    ops.sparse_paged_decode(sparse, q, k, v, bt, ctx, int32([[[0, 1, 2, 3]] * hk] * 2, cuda), 2.6,
+                            one, one)
+    ops.shared_prefix_decode(prefix, q, k, v, bt, ctx, int32([0, 2], cuda), int32([40], cuda), 2.6,
+                             one, one)
+    assert torch.equal(sparse, want.expand_as(q)) and torch.equal(prefix, want.expand_as(q))
