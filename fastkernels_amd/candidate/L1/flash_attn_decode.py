@@ -324,11 +324,12 @@ class FlashAttnDecode(nn.Module):
 
     def forward_sparse(self, q, k_cache, v_cache, key_bounds, cache_seqlens, num_selected: int,
                        keep_first: int = 1, keep_last: int = 1, cu_seqlens_q=None,
-                       max_seqlen_q: int = 1, **kwargs):
+                       max_seqlen_q: int | None = None, **kwargs):
         """Decode attention over num_selected pages per query row and kv head: the first
         keep_first, the last keep_last, and those whose key bounds (``ops.update_key_bounds``,
         kept up to date as tokens are stored) allow the greatest logits.  One row per
-        sequence, or the rows of cu_seqlens_q (a step that checks drafted tokens).  kwargs as
+        sequence, or the rows of cu_seqlens_q (a step that checks drafted tokens), at most
+        max_seqlen_q (then required) per sequence.  kwargs as
         forward's (without num_splits; no sliding window); max_seq_len, if given, bounds the
         pages that are scored."""
         what = "FlashAttnDecode.forward_sparse"
@@ -336,6 +337,8 @@ class FlashAttnDecode(nn.Module):
         if a["window_left"] >= 0:
             raise NotImplementedError(f"{what}: a sliding window reads its own few pages; use "
                                       "forward")
+        if cu_seqlens_q is not None and max_seqlen_q is None:
+            raise ValueError(f"{what}: cu_seqlens_q needs max_seqlen_q")
         n, hk, page = q.shape[0], k_cache.shape[2], k_cache.shape[1]
         width = a["block_table"].shape[1]
         if a["max_seq_len"] is not None:
@@ -344,7 +347,7 @@ class FlashAttnDecode(nn.Module):
         q3 = self._heads(q, n)
         scores = torch.empty((n, hk, width), dtype=torch.float32, device=q.device)
         o.block_scores(scores, q3, key_bounds, a["block_table"], a["cache_seqlens"], page,
-                       a["k_scale"], cu_seqlens_q, int(max_seqlen_q))
+                       a["k_scale"], cu_seqlens_q, max_seqlen_q)
         picked = torch.empty((n, hk, int(num_selected)), dtype=torch.int32, device=q.device)
         o.select_blocks(picked, scores, a["cache_seqlens"], page, int(keep_first),
                         int(keep_last), cu_seqlens_q)

@@ -735,6 +735,16 @@ def _check_batch(what, cache_seqlens, cu_seqlens_q, rows) -> int:
     return batch
 
 
+def _most_rows(what, cu_seqlens_q, max_seqlen_q) -> int:
+    """The most rows a sequence has: one without cu_seqlens_q, the caller's bound with it (the
+    lengths are on the device, and rows past a bound that is too small are not processed)."""
+    if max_seqlen_q is not None:
+        return int(max_seqlen_q)
+    if cu_seqlens_q is not None:
+        raise ValueError(f"{what}: cu_seqlens_q needs max_seqlen_q")
+    return 1
+
+
 def _check_table(what, block_table, batch) -> tuple[int, int]:
     """(row stride, columns) of a block table with a row per sequence."""
     shape, stride = block_table.shape, block_table.stride()
@@ -797,16 +807,16 @@ def _check_bounds(what, key_bounds) -> torch.Size:
 
 def update_key_bounds(key_bounds: torch.Tensor, k_cache: torch.Tensor, block_table: torch.Tensor,
                       cache_seqlens: torch.Tensor, cu_seqlens_q: torch.Tensor | None = None,
-                      max_seqlen_q: int = 1) -> None:
+                      max_seqlen_q: int | None = None) -> None:
     """Brings the bounds of the pages that hold each sequence's newest tokens up to date:
     key_bounds[page, h, 0] / [page, h, 1] = the least / greatest value of each key dimension
     over the page's tokens below cache_seqlens[b] (NaN if one is NaN).
 
     Call it after the tokens are stored, with cache_seqlens counting them.  The newest tokens
-    are the last cu_seqlens_q[b + 1] - cu_seqlens_q[b] of sequence b (the last one without
-    cu_seqlens_q), at most max_seqlen_q.  Pages are read whole, so the result depends on the
-    cache alone: a rejected draft token is forgotten with the next call on its page.  A page
-    that several sequences list should be full in each of them."""
+    are the last cu_seqlens_q[b + 1] - cu_seqlens_q[b] of sequence b, at most max_seqlen_q
+    (required with cu_seqlens_q; the last one without).  Pages are read whole, so the result
+    depends on the cache alone: a rejected draft token is forgotten with the next call on its
+    page.  A page that several sequences list should be full in each of them."""
     what = "update_key_bounds"
     shape = k_cache.shape
     if len(shape) != 4 or not k_cache.is_contiguous():
@@ -817,26 +827,27 @@ def update_key_bounds(key_bounds: torch.Tensor, k_cache: torch.Tensor, block_tab
         raise ValueError(f"{what}: key_bounds must be [{nb}, {hk}, 2, {d}] of the cache's dtype")
     tag = _cache_tag(what, dtype)
     batch = _check_batch(what, cache_seqlens, cu_seqlens_q, None)
+    most = _most_rows(what, cu_seqlens_q, max_seqlen_q)
     bt_stride, bt_width = _check_table(what, block_table, batch)
     dev = _same_device(key_bounds, k_cache, block_table, cache_seqlens, cu_seqlens_q)
     if batch == 0:
         return
     _call_on(key_bounds, dev, "fk_update_key_bounds", key_bounds.data_ptr(), k_cache.data_ptr(),
              tag, block_table.data_ptr(), bt_stride, bt_width, cache_seqlens.data_ptr(),
-             _ptr(cu_seqlens_q), batch, int(max_seqlen_q), hk, d, bs, nb)
+             _ptr(cu_seqlens_q), batch, most, hk, d, bs, nb)
 
 
 def block_scores(scores: torch.Tensor, q: torch.Tensor, key_bounds: torch.Tensor,
                  block_table: torch.Tensor, cache_seqlens: torch.Tensor, block_size: int,
                  k_scale: torch.Tensor | None = None, cu_seqlens_q: torch.Tensor | None = None,
-                 max_seqlen_q: int = 1) -> None:
+                 max_seqlen_q: int | None = None) -> None:
     """scores[t, h, j] (float32 [rows, Hk, blocks]): an upper bound of q . k over block j of
     row t's sequence, the greatest over the query heads of kv head h of
     sum_d max(q_d lo_d, q_d hi_d) with the block's key_bounds (times k_scale[h] for fp8).
     -inf for blocks the row does not see and for pages without a table entry.
 
-    Rows: one per sequence, or cu_seqlens_q [batch + 1] with at most max_seqlen_q per
-    sequence, its last tokens (row i of n sees cache_seqlens[b] - n + i + 1 keys)."""
+    Rows: one per sequence, or cu_seqlens_q [batch + 1] with at most max_seqlen_q (then
+    required) per sequence, its last tokens (row i of n sees cache_seqlens[b] - n + i + 1 keys)."""
     what = "block_scores"
     (rows, hq, d), q_stride = _check_rows(what, q, "q")
     nb, hk, _, d_bounds = _check_bounds(what, key_bounds)
@@ -849,6 +860,7 @@ def block_scores(scores: torch.Tensor, q: torch.Tensor, key_bounds: torch.Tensor
         raise ValueError(f"{what}: scores must be [{rows}, {hk}, blocks]")
     ks = _check_scale(what, k_scale, "k_scale", hk)
     batch = _check_batch(what, cache_seqlens, cu_seqlens_q, rows)
+    most = _most_rows(what, cu_seqlens_q, max_seqlen_q)
     bt_stride, bt_width = _check_table(what, block_table, batch)
     dev = _same_device(scores, q, key_bounds, block_table, cache_seqlens, cu_seqlens_q, k_scale)
     if rows == 0 or batch == 0 or width == 0:
@@ -856,7 +868,7 @@ def block_scores(scores: torch.Tensor, q: torch.Tensor, key_bounds: torch.Tensor
     _call_on(scores, dev, "fk_block_scores", scores.data_ptr(), row_stride, head_stride, width,
              q.data_ptr(), q_stride, key_bounds.data_ptr(), tag, ks, block_table.data_ptr(),
              bt_stride, bt_width, cache_seqlens.data_ptr(), _ptr(cu_seqlens_q), batch, rows,
-             int(max_seqlen_q), hq, hk, d, int(block_size), nb)
+             most, hq, hk, d, int(block_size), nb)
 
 
 def select_blocks(block_indices: torch.Tensor, scores: torch.Tensor, cache_seqlens: torch.Tensor,
@@ -1026,10 +1038,10 @@ _LIB.define("merge_attn_states(Tensor(a!) output, Tensor prefix_output, Tensor p
             "Tensor suffix_output, Tensor suffix_lse, Tensor(b!)? output_lse, "
             "int? prefill_tokens_with_context=None, Tensor? output_scale=None) -> ()")
 _LIB.define("update_key_bounds(Tensor(a!) key_bounds, Tensor k_cache, Tensor block_table, "
-            "Tensor cache_seqlens, Tensor? cu_seqlens_q=None, int max_seqlen_q=1) -> ()")
+            "Tensor cache_seqlens, Tensor? cu_seqlens_q=None, int? max_seqlen_q=None) -> ()")
 _LIB.define("block_scores(Tensor(a!) scores, Tensor q, Tensor key_bounds, Tensor block_table, "
             "Tensor cache_seqlens, int block_size, Tensor? k_scale=None, "
-            "Tensor? cu_seqlens_q=None, int max_seqlen_q=1) -> ()")
+            "Tensor? cu_seqlens_q=None, int? max_seqlen_q=None) -> ()")
 _LIB.define("select_blocks(Tensor(a!) block_indices, Tensor scores, Tensor cache_seqlens, "
             "int block_size, int keep_first=0, int keep_last=1, Tensor? cu_seqlens_q=None) "
             "-> ()")

@@ -571,3 +571,30 @@ def test_logits_next_to_the_least_float(cuda, kv):
     ops.shared_prefix_decode(prefix, q, k, v, bt, ctx, int32([0, 2], cuda), int32([40], cuda), 2.6,
                              one, one)
     assert torch.equal(sparse, want.expand_as(q)) and torch.equal(prefix, want.expand_as(q))
+
+
+def test_drafted_rows_of_several_chunks(cuda):
+    """forward_sparse of more rows per sequence than one group of score columns holds."""
+    from fastkernels_amd import ops
+
+    g = torch.Generator(device=cuda).manual_seed(8)
+    hq, hk, d, page, lens, rows = 32, 8, 128, 16, [700, 90, 333], [9, 5, 1]
+    bt, pool = tables(g, [-(-n // page) for n in lens], cuda)
+    k, v = (make_cache(g, pool, page, hk, d, "bf16", cuda) for _ in range(2))
+    bounds, ctx, cu = ops.new_key_bounds(k), int32(lens, cuda), cu_of(rows, cuda)
+    ops.update_key_bounds(bounds, k, bt, ctx, cu_of(lens, cuda), max(lens))
+    q = torch.randn(sum(rows), hq, d, generator=g, device=cuda).to(torch.bfloat16)
+    attn = load("flash_attn_decode", "FlashAttnDecode")(hq, hk, d)
+    out = attn.forward_sparse(q, k, v, bounds, ctx, 6, cu_seqlens_q=cu, max_seqlen_q=9,
+                              block_table=bt)
+    scores = torch.empty(sum(rows), hk, bt.shape[1], device=cuda)
+    ops.block_scores(scores, q, bounds, bt, ctx, page, None, cu, 9)
+    host_cu, host_bt = cu.cpu().numpy(), bt.cpu().numpy()
+    s, mag = ref.block_scores(f64(q), f64(bounds), host_bt, lens, page, bt.shape[1], None, host_cu)
+    got, seen = scores.double().cpu().numpy(), np.isfinite(s)
+    assert np.array_equal(np.isneginf(got), np.isneginf(s))
+    assert (np.abs(got[seen] - s[seen]) <= 2 * d * 2.0 ** -24 * mag[seen]).all()
+    idx = ref.select_blocks(scores.cpu().numpy(), lens, page, 6, 1, 1, host_cu)
+    want = ref.sparse_paged_decode(f64(q), f64(k), f64(v), host_bt, lens, idx, d ** -0.5, None,
+                                   None, None, host_cu)
+    check_attn(out, *want)

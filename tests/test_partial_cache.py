@@ -266,3 +266,24 @@ def test_c_abi_refuses_groups_without_arrays():
                                          4, p, 2, cu, pre, 1, 0, 8, 2, 128, 16, 4, 0.1, -1, None,
                                          p, 1 << 40, None)
         assert rc == N.FK_ERR_INVALID_ARG and "null pointer" in last_error()
+
+
+def test_rows_of_sequences_need_their_bound():
+    """cu_seqlens_q without max_seqlen_q is refused: rows past a bound of one would be left out."""
+    from fastkernels_amd.candidate.L1.flash_attn_decode import FlashAttnDecode
+
+    a, attn = args(), FlashAttnDecode(8, 2, 128)
+    for call in (
+            lambda **kw: ops.update_key_bounds(a["kb"], a["k"], a["bt"], a["ctx"], **kw),
+            lambda **kw: ops.block_scores(a["sc"], a["q"], a["kb"], a["bt"], a["ctx"], 16, **kw),
+            lambda **kw: attn.forward_sparse(a["q"], a["k"], a["k"], a["kb"], a["ctx"], 2,
+                                             block_table=a["bt"], **kw)):
+        with pytest.raises(ValueError, match="max_seqlen_q"):
+            call(cu_seqlens_q=a["cu"])
+        for kw in (dict(cu_seqlens_q=a["cu"], max_seqlen_q=1), {}):
+            with pytest.raises(RuntimeError, match="GPU only"):
+                call(**kw)
+    m = {k: v.to("meta") for k, v in a.items()}
+    o = torch.ops.fastkernels_amd
+    o.update_key_bounds(m["kb"], m["k"], m["bt"], m["ctx"], m["cu"], 2)
+    o.block_scores(m["sc"], m["q"], m["kb"], m["bt"], m["ctx"], 16, None, m["cu"], 2)
