@@ -303,3 +303,48 @@ def test_no_groups_without_arrays(cuda):
     want = ref.shared_prefix_decode(f64(q), f64(k), f64(v), bt.cpu().numpy(), lens, [0], [],
                                     d ** -0.5)
     check_attn(out, *want)
+
+
+@pytest.mark.parametrize("kv,hq,hk,d,page", [("bf16", 4, 2, 64, 16), ("fp8", 8, 1, 128, 32),
+                                             ("bf16", 2, 2, 256, 16)])
+def test_many_groups_and_rows(cuda, kv, hq, hk, d, page):
+    """More groups than a wave has lanes and more rows than a work-group has threads: groups of
+    every small size, empty and single ones among them, and rows outside any group behind."""
+    groups = []
+    for i in range(150):
+        rows = (3, 0, 8, 1, 5, 2, 9)[i % 7]
+        groups.append(((37 * i) % 250, [(11 * i + 29 * r) % 90 for r in range(rows)]))
+    groups.append((None, [(17 * r) % 70 for r in range(40)]))
+    from fastkernels_amd import ops
+
+    _, q, k, v, bt, lens, cu, pre, ks, vs = build(cuda, kv, hq, hk, d, page, groups)
+    assert len(lens) > 600 and int(cu[-1]) > 512
+    out = torch.full_like(q, 9.0)
+    ops.shared_prefix_decode(out, q, k, v, bt, int32(lens, cuda), cu, pre, d ** -0.5, ks, vs)
+    want = ref.shared_prefix_decode(f64(q), f64(k), f64(v), bt.cpu().numpy(), lens,
+                                    cu.cpu().numpy(), pre.cpu().numpy(), d ** -0.5, f64(ks),
+                                    f64(vs))
+    check_attn(out, *want)
+
+
+@pytest.mark.parametrize("backend", ["eager", "aot_eager"])
+def test_compiled_entry_points(cuda, backend):
+    """forward_sparse and forward_shared_prefix under torch.compile give what they give eagerly."""
+    hq, hk, d, page = 32, 8, 128, 16
+    g, q, k, v, bt, lens, cu, pre, _, _ = build(cuda, "bf16", hq, hk, d, page, GROUPS["one"])
+    k, v = k.nan_to_num(1.0), v.nan_to_num(1.0)
+    bt[:] = bt[:1].clamp(min=0)
+    ctx = int32(lens, cuda)
+    bounds = torch.randn(k.shape[0], hk, 2, d, generator=g, device=cuda).sort(dim=2).values.to(
+        torch.bfloat16)
+    attn = load("flash_attn_decode", "FlashAttnDecode")(hq, hk, d)
+
+    def step(q, ctx):
+        return (attn.forward_sparse(q, k, v, bounds, ctx, 9, block_table=bt, max_seq_len=512),
+                attn.forward_shared_prefix(q, k, v, ctx, cu, pre, block_table=bt))
+
+    compiled = torch.compile(step, backend=backend, fullgraph=True)
+    for shift in (0, 1):
+        want = step(q, ctx - shift)
+        got = compiled(q, ctx - shift)
+        assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])

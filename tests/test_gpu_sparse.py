@@ -598,3 +598,43 @@ def test_drafted_rows_of_several_chunks(cuda):
     want = ref.sparse_paged_decode(f64(q), f64(k), f64(v), host_bt, lens, idx, d ** -0.5, None,
                                    None, None, host_cu)
     check_attn(out, *want)
+
+
+@pytest.mark.parametrize("batch", [65, 150, 5000])
+def test_many_sequences(cuda, batch):
+    """More sequences than a wave has lanes, of 0 to 3 rows each: every operator of a step."""
+    from fastkernels_amd import ops
+
+    g = torch.Generator(device=cuda).manual_seed(batch)
+    hq, hk, d, page, keep = 4, 1, 64, 16, 2
+    lens = [(23 * b) % 90 for b in range(batch)]
+    rows = [min(lens[b], (2, 0, 1, 0, 0, 3)[b * 5 // 7 % 6]) for b in range(batch)]
+    bt, pool = tables(g, [-(-n // page) for n in lens], cuda)
+    k, v = (make_cache(g, pool, page, hk, d, "bf16", cuda) for _ in range(2))
+    cu, ctx, n = cu_of(rows, cuda), int32(lens, cuda), sum(rows) + 2
+    host_cu, host_bt = cu.cpu().numpy(), bt.cpu().numpy()
+    bounds = ops.new_key_bounds(k)
+    ops.update_key_bounds(bounds, k, bt, ctx, cu_of(lens, cuda), max(lens))
+    want = ref.update_key_bounds(np.zeros(bounds.shape), f64(k), host_bt, lens,
+                                 np.concatenate([[0], np.cumsum(lens)]))
+    assert np.array_equal(f64(bounds), want)
+    q = torch.randn(n, hq, d, generator=g, device=cuda).to(torch.bfloat16)
+    scores = torch.full((n, hk, bt.shape[1]), 7.0, device=cuda)
+    ops.block_scores(scores, q, bounds, bt, ctx, page, None, cu, 3)
+    want, mag = ref.block_scores(f64(q), f64(bounds), host_bt, lens, page, bt.shape[1], None,
+                                 host_cu)
+    got = scores.double().cpu().numpy()
+    assert (got[np.isnan(want)] == 7.0).all()
+    assert np.array_equal(np.isneginf(got), np.isneginf(want))
+    seen = np.isfinite(want)
+    assert (np.abs(got[seen] - want[seen]) <= 2 * d * 2.0 ** -24 * mag[seen]).all()
+    idx = torch.full((n, hk, keep), -7, dtype=torch.int32, device=cuda)
+    ops.select_blocks(idx, scores, ctx, page, 0, 1, cu)
+    want = ref.select_blocks(scores.cpu().numpy(), lens, page, keep, 0, 1, host_cu)
+    assert np.array_equal(idx.cpu().numpy(), want)
+    out = torch.full_like(q, 9.0)
+    ops.sparse_paged_decode(out, q, k, v, bt, ctx, idx, d ** -0.5, cu_seqlens_q=cu)
+    want = ref.sparse_paged_decode(f64(q), f64(k), f64(v), host_bt, lens, idx.cpu().numpy(),
+                                   d ** -0.5, None, None, None, host_cu)
+    seen = check_attn(out, *want)
+    assert (f64(out)[~seen] == 9.0).all()

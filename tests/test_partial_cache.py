@@ -287,3 +287,27 @@ def test_rows_of_sequences_need_their_bound():
     o = torch.ops.fastkernels_amd
     o.update_key_bounds(m["kb"], m["k"], m["bt"], m["ctx"], m["cu"], 2)
     o.block_scores(m["sc"], m["q"], m["kb"], m["bt"], m["ctx"], 16, None, m["cu"], 2)
+
+
+@pytest.mark.parametrize("how", ["sparse", "prefix"])
+def test_entry_points_compile(how):
+    """Under torch.compile each method is its custom ops, with no graph break."""
+    from fastkernels_amd.candidate.L1.flash_attn_decode import FlashAttnDecode
+
+    a, attn, calls = args(), FlashAttnDecode(8, 2, 128), []
+
+    def backend(gm, _):
+        calls.extend(str(n.target) for n in gm.graph.nodes if n.op == "call_function")
+        return lambda *_: [torch.zeros(3, 8, 128)]
+
+    def step(q):
+        if how == "sparse":
+            return attn.forward_sparse(q, a["k"], a["k"], a["kb"], a["ctx"], 2,
+                                       block_table=a["bt"], max_seq_len=64)
+        return attn.forward_shared_prefix(q, a["k"], a["k"], a["ctx"], a["gr"], a["pre"],
+                                          block_table=a["bt"])
+
+    torch.compile(step, backend=backend, fullgraph=True)(a["q"])
+    ops_called = [c.split(".")[1] for c in calls if c.startswith("fastkernels_amd.")]
+    assert ops_called == (["block_scores", "select_blocks", "sparse_paged_decode"]
+                          if how == "sparse" else ["shared_prefix_decode"])
