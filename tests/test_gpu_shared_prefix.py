@@ -348,3 +348,31 @@ def test_compiled_entry_points(cuda, backend):
         want = step(q, ctx - shift)
         got = compiled(q, ctx - shift)
         assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+
+
+@pytest.mark.parametrize("kv", ["bf16", "fp8"])
+@pytest.mark.parametrize("scale", [-0.11, 0.0])
+def test_shared_prefix_of_odd_arguments(cuda, kv, scale):
+    """Rows before the first group, prefixes of any length, lengths past the table, masked pages,
+    a scale that is not positive, key scales of either sign."""
+    from fastkernels_amd import ops
+
+    g = torch.Generator(device=cuda).manual_seed(12)
+    hq, hk, d, page, width = 16, 2, 128, 16, 12
+    lens = [40, 150, 180, 250, 10 ** 6, 0, 2 ** 31 - 1, 100, 33]
+    bt = torch.stack([torch.randperm(40, generator=g, device=cuda)[:width] for _ in lens])
+    bt = bt.to(torch.int32)
+    cu, pre = int32([2, 4, 7, 8], cuda), int32([100, 2 ** 31 - 1, 50], cuda)
+    bt[3, :6], bt[5:7] = bt[2, :6], bt[4]
+    bt[1, 0], bt[2, 1], bt[3, 9], bt[4, 3] = -1, 10 ** 6, -1, -2 ** 31
+    k, v = (make_cache(g, 40, page, hk, d, kv, cuda) for _ in range(2))
+    q = torch.randn(len(lens), hq, d, generator=g, device=cuda).to(torch.bfloat16)
+    ks = vs = None
+    if kv == "fp8":
+        ks, vs = torch.tensor([0.2, -0.3], device=cuda), torch.tensor([-0.1, 0.4], device=cuda)
+    out = torch.full_like(q, 9.0)
+    ops.shared_prefix_decode(out, q, k, v, bt, int32(lens, cuda), cu, pre, scale, ks, vs)
+    seen = [min(n, width * page) for n in lens]  # (the definition counts tokens one by one)
+    want, mean, mag = ref.shared_prefix_decode(f64(q), f64(k), f64(v), bt.cpu().numpy(), seen,
+                                               cu.tolist(), pre.tolist(), scale, f64(ks), f64(vs))
+    check_attn(out, want, np.abs(mean), np.abs(mag))

@@ -638,3 +638,39 @@ def test_many_sequences(cuda, batch):
                                    d ** -0.5, None, None, None, host_cu)
     seen = check_attn(out, *want)
     assert (f64(out)[~seen] == 9.0).all()
+
+
+@pytest.mark.parametrize("kv", ["bf16", "fp8"])
+@pytest.mark.parametrize("scale", [-0.11, 0.0])
+def test_sparse_of_odd_arguments(cuda, kv, scale):
+    """Lengths past the table, a scale that is not positive, key scales of either sign, the
+    output in place of the query."""
+    from fastkernels_amd import ops
+
+    g = torch.Generator(device=cuda).manual_seed(13)
+    hq, hk, d, page, width = 24, 2, 128, 16, 12
+    lens = [48, 10 ** 6, 2 ** 31 - 1, 0]
+    bt = torch.stack([torch.randperm(40, generator=g, device=cuda)[:width] for _ in lens])
+    bt = bt.to(torch.int32)
+    k, v = (make_cache(g, 40, page, hk, d, kv, cuda) for _ in range(2))
+    q = torch.randn(len(lens), hq, d, generator=g, device=cuda).to(torch.bfloat16)
+    ks = vs = None
+    if kv == "fp8":
+        ks, vs = torch.tensor([0.2, -0.3], device=cuda), torch.tensor([-0.1, 0.4], device=cuda)
+    bounds, ctx = ops.new_key_bounds(k), int32(lens, cuda)
+    ops.update_key_bounds(bounds, k, bt, int32([min(n, width * page) for n in lens], cuda),
+                          int32([0, 48, 240, 432, 432], cuda), 192)
+    scores = torch.empty(4, hk, width, device=cuda)
+    ops.block_scores(scores, q, bounds, bt, ctx, page, ks)
+    want, mag = ref.block_scores(f64(q), f64(bounds), bt.cpu().numpy(), lens, page, width, f64(ks))
+    got, seen = scores.double().cpu().numpy(), np.isfinite(want)
+    assert np.array_equal(np.isneginf(got), np.isneginf(want))
+    assert (np.abs(got[seen] - want[seen]) <= 2 * d * 2.0 ** -24 * mag[seen]).all()
+    idx = torch.empty(4, hk, 7, dtype=torch.int32, device=cuda)
+    ops.select_blocks(idx, scores, ctx, page, 1, 2)
+    assert np.array_equal(idx.cpu().numpy(),
+                          ref.select_blocks(scores.cpu().numpy(), lens, page, 7, 1, 2))
+    want, mean, mag = ref.sparse_paged_decode(f64(q), f64(k), f64(v), bt.cpu().numpy(), lens,
+                                              idx.cpu().numpy(), scale, f64(ks), f64(vs))
+    ops.sparse_paged_decode(q, q, k, v, bt, ctx, idx, scale, ks, vs)
+    check_attn(q, want, np.abs(mean), np.abs(mag))
