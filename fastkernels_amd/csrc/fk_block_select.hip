@@ -76,7 +76,7 @@ struct Elems {
 // the cache alone, not on earlier calls.
 //
 // Bound by memory, by latency where the pages are few: one token of 64 sequences takes 3.2 us
-// (1.5 MB), four fp8 prompts of 1000 .. 8192 tokens in pages of 64 8.6 us (23 MB).
+// (1.5 MB), four fp8 prompts of 1000 .. 8192 tokens in pages of 64 8.8 us (23 MB).
 template <bool kFp8, int D>
 __global__ __launch_bounds__(256) void key_bounds_kernel(
     BoundsParams P, const int32_t* __restrict__ bt, const int32_t* __restrict__ ctx,
@@ -187,7 +187,7 @@ struct ScoreParams {
 // its last head, groups above 16 take several passes over the loaded bounds); the rows of
 // the A operand are the pages' bounds, lo then hi, the B operands min(q, 0) and max(q, 0).
 //
-// Bound by memory: 32 sequences of 16000 .. 131072 tokens in pages of 16 take 142 us (655 MB,
+// Bound by memory: 32 sequences of 16000 .. 131072 tokens in pages of 16 take 143 us (655 MB,
 // 4.6 TB/s, in pieces of 4 KB); one sequence of 40000 5.4 us.  More waves a SIMD are slower
 // there (four 158 us).
 constexpr int kScoreWaves = 8;  // of a work-group, a kv head each: a page's bounds are read whole
@@ -387,8 +387,8 @@ __device__ __forceinline__ void scan_threads(int (&v)[kN], int (*part)[kSelThrea
 // sum of the counts before it.
 //
 // Bound by latency: loads, barriers and LDS atomics in turn.  One sequence of 40000 tokens in
-// pages of 16 takes 7.3 us (8.1 by digits at once), 85 rows of 32 sequences of 16000 .. 131072
-// tokens 18.9 (20.1); 256 or 1024 threads a list take 10.6 / 24.8 and 8.4 / 23.0 by digits.
+// pages of 16 takes 7.4 us, 85 rows of 32 sequences of 16000 .. 131072 tokens 18.6 (by digits at
+// once 8.1 and 20.1, and with 256 or 1024 threads a list 10.6 / 24.8 and 8.4 / 23.0).
 template <bool kLds>
 __global__ __launch_bounds__(kSelThreads) void select_blocks_kernel(
     SelectParams P, const int32_t* __restrict__ ctx, const int32_t* __restrict__ cu) {

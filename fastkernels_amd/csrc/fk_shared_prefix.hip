@@ -24,9 +24,12 @@
 // this took 87).
 // Two waves a SIMD (O of 32 columns, the queries, and two tiles of K and V fill their registers)
 // leave latencies that show.  Measured: 64 rows of 32 / 8 heads over a prefix of 8192 bf16
-// tokens with 100 .. 2000 of their own 83 us and 5.5 for the merge (311 MB, 9.7 GFLOP); 128
-// rows of 64 / 8 heads over three prefixes of 11000 .. 16400 fp8 tokens 142 us and 7.6 (250 MB,
-// 60 GFLOP; little less with every page in L2); 8 rows over 1488 tokens 13.9 us and 4.0.
+// tokens with 100 .. 2000 of their own 85.5 us and 5.6 for the merge (311 MB, 9.7 GFLOP); 128
+// rows of 64 / 8 heads over three prefixes of 11000 .. 16400 fp8 tokens 137 us and 7.5 (250 MB,
+// 60 GFLOP; little less with every page in L2); 8 rows over 1488 tokens 15.3 us and 4.0.  The
+// set-up of a work-group has more live than its registers hold (132 .. 160 scalars go to vector
+// registers, up to 48 vectors to scratch), which the smallest calls show; the tile loops touch
+// no scratch.
 // Variants that were slower there: 16 or 64 columns to a wave, 128 columns to a work-group
 // with K and V staged in LDS (117 .. 136 and 185 .. 210 us), the four waves on four column blocks
 // of the same tiles (98 and 152, 10 for the merge), two steps of loads ahead, items rounded up to
@@ -40,8 +43,10 @@ namespace {
 
 constexpr int kWaves = 4;
 constexpr int kThreads = kWaves * 64;
-constexpr int kPreTiles = 8;      // a prefix range is a multiple of this: two tiles per wave
-constexpr int kOwnTiles = 2;      // and a wave's own range of this: a step
+// A prefix range is a multiple of this: in pages of 16 tokens two tiles per wave; in pages of 64
+// and more two units of four tiles, which two of the waves take.
+constexpr int kPreTiles = 8;
+constexpr int kOwnTiles = 2;      // a wave's own range is a multiple of this: a step
 constexpr int kMaxGroups = 2048;  // (their bounds are held in LDS)
 
 // Column blocks of a prefix item.  (O takes 4 D / 16 registers per block.)

@@ -12,9 +12,9 @@
 // drafted tokens, which mostly select the same pages, run side by side on one XCD's L2.
 //
 // Bound by memory where the lists are many: 64 rows of 32 / 8 heads, 2048 bf16 keys a list, take
-// 96.5 us (538 MB, 5.6 TB/s); bound by the latency of its steps, partly of L2 hits, where rows
-// share pages: 85 rows that check drafted tokens over fp8 pages 52.5 us (137 MB that differ, 370
-// read).  One row takes 5.9 us and its merge 3.9.  Two or more steps of loads ahead gain nothing
+// 96.9 us (538 MB, 5.6 TB/s); bound by the latency of its steps, partly of L2 hits, where rows
+// share pages: 85 rows that check drafted tokens over fp8 pages 53.1 us (137 MB that differ, 370
+// read).  One row takes 5.8 us and its merge 4.0.  Two or more steps of loads ahead gain nothing
 // (96 and 60 us, more 148 and 63), nor does another order of the lists over the XCDs.
 #include <limits.h>
 
@@ -128,8 +128,10 @@ __global__ __launch_bounds__(kMergeThreads) void sparse_merge_kernel(
 }
 
 // Work-groups per list: where the lists are fewer than the CUs, as many as make two per CU, each
-// with two tiles per wave at the least.  (With a list for each CU, parts only add their merge:
-// 512 lists of 2048 keys 98 us in one part, 109 in two.)
+// with eight tiles at the least: two per wave in pages of 16, one or two units of a wave's own in
+// larger pages, where a unit is up to four tiles (with pages of 64 and more two of the four waves
+// then have none).  (With a list for each CU, parts only add their merge: 512 lists of 2048 keys
+// 98 us in one part, 109 in two.)
 int parts_of(int64_t rows, int64_t keep, int vheads, int block_size) {
   const int64_t lists = rows * vheads;
   const int64_t tiles = keep * (block_size / kTile);

@@ -844,7 +844,8 @@ def block_scores(scores: torch.Tensor, q: torch.Tensor, key_bounds: torch.Tensor
     """scores[t, h, j] (float32 [rows, Hk, blocks]): an upper bound of q . k over block j of
     row t's sequence, the greatest over the query heads of kv head h of
     sum_d max(q_d lo_d, q_d hi_d) with the block's key_bounds (times k_scale[h] for fp8).
-    -inf for blocks the row does not see and for pages without a table entry.
+    -inf for blocks the row does not see and for pages without a table entry; a block with
+    infinite or NaN keys may score NaN, which :func:`select_blocks` takes first.
 
     Rows: one per sequence, or cu_seqlens_q [batch + 1] with at most max_seqlen_q (then
     required) per sequence, its last tokens (row i of n sees cache_seqlens[b] - n + i + 1 keys)."""
