@@ -376,3 +376,51 @@ def test_shared_prefix_of_odd_arguments(cuda, kv, scale):
     want, mean, mag = ref.shared_prefix_decode(f64(q), f64(k), f64(v), bt.cpu().numpy(), seen,
                                                cu.tolist(), pre.tolist(), scale, f64(ks), f64(vs))
     check_attn(out, want, np.abs(mean), np.abs(mag))
+
+
+def test_most_groups(cuda):
+    """As many groups as a launch takes, of none to three rows each."""
+    from fastkernels_amd import ops
+
+    groups = [((5 * i) % 40, [(3 * i + r) % 20 for r in range((1, 2, 0, 3)[i % 4])])
+              for i in range(2048)]
+    _, q, k, v, bt, lens, cu, pre, _, _ = build(cuda, "bf16", 2, 1, 64, 16, groups)
+    out = torch.full_like(q, 9.0)
+    ops.shared_prefix_decode(out, q, k, v, bt, int32(lens, cuda), cu, pre, 0.125)
+    want = ref.shared_prefix_decode(f64(q), f64(k), f64(v), bt.cpu().numpy(), lens,
+                                    cu.cpu().numpy(), pre.cpu().numpy(), 0.125)
+    check_attn(out, *want)
+
+
+def test_most_rows(cuda):
+    """As many rows as a launch takes, each with up to a page of its own behind a page that groups
+    of 40 share, of which sparse decode lists the second: against dense float64."""
+    from fastkernels_amd import ops
+
+    n, d, page = 65535, 64, 16
+    g = torch.Generator(device=cuda).manual_seed(6)
+    k, v = (make_cache(g, 4096, page, 1, d, "bf16", cuda) for _ in range(2))
+    own = torch.randint(0, 4096, (n,), generator=g, device=cuda, dtype=torch.int32)
+    group = torch.arange(n, device=cuda) // 40
+    bt = torch.stack([(group % 1024).to(torch.int32), own], 1)
+    tail = torch.arange(n, device=cuda, dtype=torch.int32) % 17
+    ctx = tail + page
+    q = torch.randn(n, 2, d, generator=g, device=cuda).to(torch.bfloat16)
+    last = int(group[-1]) + 1
+    cu = torch.arange(last + 1, device=cuda, dtype=torch.int32).mul_(40).clamp_(max=n)
+    prefix, sparse = torch.full_like(q, 9.0), torch.full_like(q, 9.0)
+    ops.shared_prefix_decode(prefix, q, k, v, bt, ctx, cu,
+                             torch.full((last,), page, dtype=torch.int32, device=cuda), d ** -0.5)
+    idx = torch.ones(n, 1, 1, dtype=torch.int32, device=cuda)
+    rows = torch.arange(n + 1, device=cuda, dtype=torch.int32)
+    ops.sparse_paged_decode(sparse, q, k, v, bt, ctx, idx, d ** -0.5, cu_seqlens_q=rows)
+    for out, pages in ((prefix, 2), (sparse, 1)):
+        at = bt[:, 2 - pages:].long()
+        kk, vv = (x[at].view(n, pages * page, d).double() for x in (k, v))
+        seen = torch.arange(pages * page, device=cuda) < (ctx - (2 - pages) * page).unsqueeze(1)
+        x = (q.double() @ kk.transpose(1, 2).contiguous()) * d ** -0.5
+        w = torch.where(seen.unsqueeze(1), x, -float("inf")).softmax(2).nan_to_num(0.0)
+        want, mean = w @ vv, w @ vv.abs()
+        mag = (q.double().abs() @ kk.abs().transpose(1, 2).contiguous()).amax((1, 2)) * d ** -0.5
+        tol = attn_tolerance(*(t.cpu().numpy() for t in (want, mean, mag.view(-1, 1, 1))), d)
+        assert (np.abs(f64(out) - want.cpu().numpy()) <= tol).all()

@@ -311,3 +311,11 @@ def test_entry_points_compile(how):
     ops_called = [c.split(".")[1] for c in calls if c.startswith("fastkernels_amd.")]
     assert ops_called == (["block_scores", "select_blocks", "sparse_paged_decode"]
                           if how == "sparse" else ["shared_prefix_decode"])
+
+
+def test_more_groups_than_a_launch_takes_are_refused():
+    lib, p = N.lib(), ctypes.c_void_p(0x100000)
+    rc = lib.fk_shared_prefix_decode(p, 1024, p, 1024, p, p, N.FK_DTYPE_BF16, None, None, p, 4, 4, p,
+                                     3000, p, p, 2049, 0, 8, 2, 128, 16, 4, 0.1, -1, None, p,
+                                     1 << 40, None)
+    assert rc == N.FK_ERR_INVALID_ARG and "2049 groups" in last_error()
