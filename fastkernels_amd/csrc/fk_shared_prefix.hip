@@ -533,13 +533,14 @@ struct PlainLds {
 };
 // Attention of query head hq of row b over positions [0, keys) read through `table`, by a merge's
 // work-group: a key a thread for the scores, a dim a thread for the sums.
-template <int D>
+template <int D, bool kFp8>
 __device__ void attend_plainly(const PageAttnParams& A, const int32_t* __restrict__ table, int keys,
-                               bool fp8, int b, int hq, PlainLds& lds) {
+                               int b, int hq, PlainLds& lds) {
+  constexpr int kElt = kFp8 ? 1 : 2;
   static_assert(D <= kMergeThreads, "a dim a thread");
   const int tid = threadIdx.x, kvh = hq / A.gqa;
   const uint16_t* const q = A.q + b * A.q_row_stride + static_cast<int64_t>(hq) * D;
-  const float s2 = fp8 && A.k_scale ? A.scale_log2 * A.k_scale[kvh] : A.scale_log2;
+  const float s2 = kFp8 && A.k_scale ? A.scale_log2 * A.k_scale[kvh] : A.scale_log2;
   // Index of position t's first element in the caches, -1 at a masked page.
   auto row_at = [&](int t) -> int64_t {
     const int j = t >> A.block_size_log2;
@@ -549,20 +550,36 @@ __device__ void attend_plainly(const PageAttnParams& A, const int32_t* __restric
                          (t & ((1 << A.block_size_log2) - 1));
     return (slot * A.num_kv_heads + kvh) * D;
   };
-  auto value = [&](const uint8_t* cache, int64_t i) {
-    return fp8 ? __builtin_amdgcn_cvt_f32_fp8(cache[i], 0)
-               : __uint_as_float(static_cast<uint32_t>(
-                     reinterpret_cast<const uint16_t*>(cache)[i]) << 16);
+  auto value = [&](int64_t i) {
+    if constexpr (kFp8) return __builtin_amdgcn_cvt_f32_fp8(A.v_cache[i], 0);
+    return bf16_to_f32(reinterpret_cast<const uint16_t*>(A.v_cache)[i]);
   };
   float m = kNegInf, l = 0.f, o = 0.f;
   for (int t0 = 0; t0 < keys; t0 += kMergeThreads) {
     const int64_t row = t0 + tid < keys ? row_at(t0 + tid) : -1;
     float s = kNegInf;
     if (row >= 0) {
+      const uint8_t* const k = A.k_cache + row * kElt;
       float dot = 0.f;
-      for (int d = 0; d < D; ++d)
-        dot = __builtin_fmaf(__uint_as_float(static_cast<uint32_t>(q[d]) << 16),
-                             value(A.k_cache, row + d), dot);
+      for (int d = 0; d < D; d += 16 / kElt) {
+        const uint4 x = ld16(k + d * kElt);
+        const uint32_t w[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          if constexpr (kFp8) {
+            const auto a = __builtin_amdgcn_cvt_pk_f32_fp8(w[i], false);
+            const auto b = __builtin_amdgcn_cvt_pk_f32_fp8(w[i], true);
+            dot = __builtin_fmaf(bf16_to_f32(q[d + 4 * i]), a[0], dot);
+            dot = __builtin_fmaf(bf16_to_f32(q[d + 4 * i + 1]), a[1], dot);
+            dot = __builtin_fmaf(bf16_to_f32(q[d + 4 * i + 2]), b[0], dot);
+            dot = __builtin_fmaf(bf16_to_f32(q[d + 4 * i + 3]), b[1], dot);
+          } else {
+            dot = __builtin_fmaf(bf16_to_f32(q[d + 2 * i]), __uint_as_float(w[i] << 16), dot);
+            dot = __builtin_fmaf(bf16_to_f32(q[d + 2 * i + 1]),
+                                 __uint_as_float(w[i] & 0xffff0000u), dot);
+          }
+        }
+      }
       s = dot * s2;
     }
     float most = s;
@@ -578,15 +595,26 @@ __device__ void attend_plainly(const PageAttnParams& A, const int32_t* __restric
     __syncthreads();
     l *= alpha;
     o *= alpha;
-    for (int k = 0; k < min(kMergeThreads, keys - t0); ++k) {
-      if (lds.row[k] < 0) continue;
-      l += lds.weight[k];
-      if (tid < D) o = __builtin_fmaf(lds.weight[k], value(A.v_cache, lds.row[k] + tid), o);
+    // (in eights, whose loads are on their way together; without a row the weight is zero, and
+    // the value read instead does not count)
+    for (int k0 = 0; k0 < min(kMergeThreads, keys - t0); k0 += 8) {
+      float x[8];
+#pragma unroll
+      for (int k = 0; k < 8; ++k) {
+        const int64_t at = lds.row[k0 + k];
+        const float y = value(max(at, int64_t{0}) + min(tid, D - 1));
+        x[k] = at >= 0 ? y : 0.f;
+      }
+#pragma unroll
+      for (int k = 0; k < 8; ++k) {
+        l += lds.weight[k0 + k];
+        o = __builtin_fmaf(lds.weight[k0 + k], x[k], o);
+      }
     }
     __syncthreads();
   }
   l = with_sink(l, m, A.sinks ? A.sinks[hq] * kLog2e : kNegInf);
-  const float f = l > 0.f ? (fp8 && A.v_scale ? A.v_scale[kvh] : 1.f) / l : 0.f;
+  const float f = l > 0.f ? (kFp8 && A.v_scale ? A.v_scale[kvh] : 1.f) / l : 0.f;
   if (tid < D)
     A.out[b * A.out_row_stride + static_cast<int64_t>(hq) * D + tid] = f32_to_bf16(o * f);
 }
@@ -595,7 +623,9 @@ __device__ void attend_plainly(const PageAttnParams& A, const int32_t* __restric
 //
 // A row shorter than its group's prefix has zero weights for the keys that only others see, but
 // in the products with V these meet the others' values all the same: where one is infinite or
-// NaN the row's sum is NaN.  Such a row that is not finite is computed again by itself.
+// NaN the row's sum is NaN.  Such a row that is not finite is computed again by itself (its 32
+// heads over 65436 bf16 keys take 5 ms; a second pass over such ranges in the kernel above cost
+// every call 2 us in set-up).
 template <int D>
 __global__ __launch_bounds__(kMergeThreads) void shared_prefix_merge_kernel(
     PrefixParams P, const int32_t* __restrict__ bt, int fp8) {
@@ -655,10 +685,15 @@ __global__ __launch_bounds__(kMergeThreads) void shared_prefix_merge_kernel(
       });
   if (rec.short_keys < 0) return;
   __syncthreads();
-  for (uint32_t left = __builtin_amdgcn_readfirstlane(again); left; left &= left - 1)
-    attend_plainly<D>(A, bt + (b - rec.index) * A.bt_row_stride, rec.short_keys, fp8 != 0, b,
-                      kvh * A.gqa + in_group + __builtin_ctz(left),
-                      *reinterpret_cast<PlainLds*>(folded));
+  const int32_t* const table = bt + (b - rec.index) * A.bt_row_stride;
+  PlainLds& plain = *reinterpret_cast<PlainLds*>(folded);
+  for (uint32_t left = __builtin_amdgcn_readfirstlane(again); left; left &= left - 1) {
+    const int hq = kvh * A.gqa + in_group + __builtin_ctz(left);
+    if (fp8)
+      attend_plainly<D, true>(A, table, rec.short_keys, b, hq, plain);
+    else
+      attend_plainly<D, false>(A, table, rec.short_keys, b, hq, plain);
+  }
 }
 
 // The bound on the shared tokens of a prefix that an argument of 0 (none) or more stands for.
