@@ -19,7 +19,7 @@ has: 1 is a plain decode step, more is a step that checks several drafted tokens
 The 4-bit format: a block is 32 dims of one token and kv head; its scale is 2^(E - 127), one
 byte E, its values codes of {0, 0.5, 1, 1.5, 2, 3, 4, 6} with a sign.  K codes lie as
 [page, head, token, D/2] (two dims a byte, the even one low), V codes as
-[page, head, 8 tokens, 16, token, D/32], scales as [page, head, D/32, token].
+[page, head, 4 tokens, 16, token, D/32], scales as [page, head, D/32, token].
 """
 from __future__ import annotations
 
@@ -263,7 +263,7 @@ def _dequantize(packed, scales):
 
 
 def _v_rows(v):
-    """V codes [pages, Hk, page/8, 16, 8, D/32] as rows [pages, Hk, page, D/2] (a copy)."""
+    """V codes [pages, Hk, page/4, 16, 4, D/32] as rows [pages, Hk, page, D/2] (a copy)."""
     return v.permute(0, 1, 2, 4, 3, 5).flatten(4).flatten(2, 3)
 
 
@@ -284,7 +284,7 @@ def _kv4_cache(g, pool, page, hk, d):
 def _v_layout(rows):
     """The inverse of _v_rows."""
     pool, hk, page, half = rows.shape
-    return rows.view(pool, hk, page // 8, 8, 16, half // 16).permute(0, 1, 2, 4, 3, 5).contiguous()
+    return rows.view(pool, hk, page // 4, 4, 16, half // 16).permute(0, 1, 2, 4, 3, 5).contiguous()
 
 
 # ---------------------------------------------------------------------------
@@ -458,12 +458,12 @@ def _plain_kv4_chunk(s):
         packed = _pack(codes)
         scales.transpose(2, 3)[page, :, tok] = e
         if v:
-            s["v"].permute(0, 2, 4, 1, 3, 5)[page, tok // 8, tok % 8] = \
+            s["v"].permute(0, 2, 4, 1, 3, 5)[page, tok // 4, tok % 4] = \
                 packed.unflatten(-1, (16, -1))
         else:
             s["k"][page, :, tok] = packed
     page, tok = _places(s)
-    v = s["v"].permute(0, 2, 4, 1, 3, 5)[page, tok // 8, tok % 8].flatten(2)
+    v = s["v"].permute(0, 2, 4, 1, 3, 5)[page, tok // 4, tok % 4].flatten(2)
     ks, vs = (x.transpose(2, 3)[page, :, tok] for x in (s["ks"], s["vs"]))
     return (_dequantize(s["k"][page, :, tok], ks).to(torch.bfloat16),
             _dequantize(v, vs).to(torch.bfloat16))
@@ -597,8 +597,8 @@ def _kv64(s, which, pages, n):
     if which == "k":
         rows = s["k"][pages]
     else:
-        v = s["v"][pages]  # [pages, Hk, page/8, 16, 8, D/32]
-        rows = torch.stack([v[:, :, i // 8, :, i % 8].flatten(2) for i in range(s["page"])], 2)
+        v = s["v"][pages]  # [pages, Hk, page/4, 16, 4, D/32]
+        rows = torch.stack([v[:, :, i // 4, :, i % 4].flatten(2) for i in range(s["page"])], 2)
     out = torch.empty(*rows.shape[:3], 2 * rows.shape[3], dtype=torch.float64, device=DEV)
     e = e.transpose(2, 3).repeat_interleave(32, -1)
     out[..., 0::2] = _decode64(rows % 16, e[..., 0::2])
