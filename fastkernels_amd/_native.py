@@ -131,6 +131,32 @@ _SIGNATURES = {
                                         c_void_p, c_void_p, c_int64, c_void_p]),
     "fk_shared_prefix_decode_plan": (c_int, [c_int64, c_int64, c_int64, c_int, c_int, c_int,
                                              c_void_p]),
+    "fk_store_kvcache_mxfp4": (c_int, [c_void_p, c_int64, c_void_p, c_int64, c_int, c_void_p,
+                                       c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int64,
+                                       c_int, c_int, c_int, c_int64, c_void_p]),
+    "fk_gather_kvcache_mxfp4": (c_int, [c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_void_p,
+                                        c_void_p, c_void_p, c_void_p, c_int64, c_int64, c_void_p,
+                                        c_int64, c_int64, c_int, c_int, c_int, c_int64, c_void_p]),
+    "fk_mxfp4_paged_decode": (c_int, [c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_void_p,
+                                      c_void_p, c_void_p, c_void_p, c_int64, c_int64, c_void_p,
+                                      c_void_p, c_int64, c_int64, c_int64, c_int, c_int, c_int,
+                                      c_int, c_int64, c_float, c_int, c_void_p, c_void_p, c_int64,
+                                      c_void_p]),
+    "fk_mxfp4_paged_decode_plan": (c_int, [c_int64, c_int64, c_int, c_int, c_int, c_void_p]),
+    "fk_latent_norm_rope_store": (c_int, [c_void_p, c_int, c_void_p, c_void_p, c_int, c_int64,
+                                          c_void_p, c_void_p, c_int64, c_void_p, c_int64, c_void_p,
+                                          c_float, c_void_p, c_int, c_int64, c_int, c_void_p,
+                                          c_int64, c_int64, c_int, c_void_p, c_int64, c_int64,
+                                          c_void_p, c_int64, c_void_p, c_int64, c_int64, c_int,
+                                          c_int, c_void_p]),
+    "fk_gather_latent": (c_int, [c_void_p, c_int64, c_void_p, c_int, c_void_p, c_void_p, c_int64,
+                                 c_int64, c_void_p, c_int64, c_int64, c_int, c_int, c_int, c_int64,
+                                 c_void_p]),
+    "fk_latent_decode": (c_int, [c_void_p, c_int64, c_int64, c_void_p, c_int64, c_int64, c_void_p,
+                                 c_int, c_void_p, c_void_p, c_int64, c_int64, c_void_p, c_void_p,
+                                 c_int64, c_int64, c_int64, c_int, c_int, c_int, c_int, c_int64,
+                                 c_float, c_void_p, c_int64, c_void_p, c_int64, c_void_p]),
+    "fk_latent_decode_plan": (c_int, [c_int64, c_int64, c_int, c_int, c_void_p]),
 }
 
 EXPORTED = tuple(_SIGNATURES)
@@ -244,4 +270,20 @@ def shared_prefix_bytes(batch: int, num_groups: int, max_prefix_len: int, num_he
     ws = c_int64(0)
     call("fk_shared_prefix_decode_plan", batch, num_groups, max_prefix_len, num_heads,
          num_kv_heads, head_size, ctypes.byref(ws))
+    return ws.value
+
+
+def mxfp4_decode_bytes(batch: int, max_seqlen_q: int, num_heads: int, num_kv_heads: int,
+                       head_size: int) -> int:
+    """fk_mxfp4_paged_decode_plan: the workspace bytes of a decode launch over a 4-bit cache."""
+    ws = c_int64(0)
+    call("fk_mxfp4_paged_decode_plan", batch, max_seqlen_q, num_heads, num_kv_heads, head_size,
+         ctypes.byref(ws))
+    return ws.value
+
+
+def latent_decode_bytes(batch: int, max_seqlen_q: int, num_heads: int, latent_size: int) -> int:
+    """fk_latent_decode_plan: the workspace bytes of a decode launch over a latent cache."""
+    ws = c_int64(0)
+    call("fk_latent_decode_plan", batch, max_seqlen_q, num_heads, latent_size, ctypes.byref(ws))
     return ws.value

@@ -1,0 +1,654 @@
+// Decode attention over a cache of latent rows, in the absorbed form: every query head attends
+// to the same keys, a token's row of R + P values, and the values are its first R,
+//   s[t, h, j] = scale q[t, h] . row_j,   out[t, h] = sum_j softmax_j(s) row_j[0 .. R).
+//
+// The query rows of a sequence times the heads are the columns of matrix products with the
+// keys: S^T = K Q^T, then O^T += V^T P^T.  Keys come through LDS once: S reads them as rows, P V
+// the same bytes with the transpose loads.  Items (sequence, 64 columns) of 32-key steps lie on
+// one line, cut into equal ranges, one per CU (fk_lines.h).  An item inside one range is finished
+// there; of the others each part leaves a partial state, which a second launch merges.
+//
+// LDS holds a tile (32 keys) as rows of bf16; the 16-byte pieces of row t are permuted within
+// each run of 8 by (t / 2) mod 8, which with the row's length of 128 bytes more than a multiple
+// of 256 spreads what 16 lanes read at a time over all banks.
+#include "fk_lines.h"
+#include "fk_page_attn.h"
+#include "fk_query_rows.h"
+
+#include <type_traits>
+
+namespace fk {
+namespace {
+
+typedef float floatx16_t __attribute__((ext_vector_type(16)));
+
+constexpr int kWaves = 4;
+constexpr int kThreads = kWaves * 64;
+constexpr int kKeys = 32;    // of a tile
+constexpr int kBuffers = 4;  // tiles in LDS
+
+struct LatentParams {
+  uint16_t* out;
+  int64_t out_row_stride, out_head_stride;
+  const uint16_t* q;
+  int64_t q_row_stride, q_head_stride;
+  const uint8_t* cache;
+  const float* cache_scale;
+  float* lse;
+  int64_t lse_head_stride;
+  float scale_log2;
+  int num_heads;
+  int head_blocks;  // units of 32 heads of a row
+  int batch, rows, most;
+  int block_size_log2;
+  int64_t num_blocks;
+  int64_t bt_row_stride;
+  int bt_width;
+  int wgs;
+  float* o;         // [2 wgs][64][R]
+  float* ml;        // [2 wgs][64] (maximum, sum)
+  LineRecord* records;
+};
+
+// A tile in LDS.
+template <int R, int P>
+struct Tile {
+  static constexpr int kRow = 2 * (R + P);        // bytes
+  static constexpr int kPieces = kRow / 16;
+  static constexpr int kBytes = kKeys * kRow;
+  static constexpr int kMoves = kKeys * kPieces / 64;  // 64-piece moves of a tile
+  static_assert(kPieces % 8 == 0 && kKeys / 2 * kPieces % 64 == 0, "whole moves of half a tile");
+  static __device__ __forceinline__ int at(int row, int piece) {
+    return row * kRow + 16 * ((piece & ~7) | ((piece ^ (row >> 1)) & 7));
+  }
+  // Where in its half's rows of the cache (elements of kElt bytes) lane `lane` of move m of
+  // the half finds the piece that goes to LDS bytes 1024 m + 16 lane of the half.
+  template <int kElt>
+  static __device__ __forceinline__ uint32_t source(int m, int lane) {
+    const int x = 64 * m + lane;
+    const int row = x / kPieces, slot = x % kPieces;
+    return row * (R + P) * kElt + 8 * kElt * ((slot & ~7) | ((slot ^ (row >> 1)) & 7));
+  }
+};
+
+// 16 bytes from global memory straight into LDS: lane l of the wave writes at byte lds_addr + 16 l
+// what it reads at base + off.  The compiler does not see it as a load: the kernel waits for it.
+// (The scalar move covers the wait states that the load's base needs after a vector instruction
+// wrote it, and the one after the write of M0.)
+__device__ __forceinline__ void lds_load16(const uint8_t* base, uint32_t off, uint32_t lds_addr) {
+  const uint8_t* b;
+  asm volatile(
+      "s_mov_b64 %0, %2\n\t"
+      "global_load_lds_dwordx4 %1, %0"
+      : "=&s"(b)
+      : "v"(off), "s"(base), "{m0}"(lds_addr)
+      : "memory");
+}
+__device__ __forceinline__ uint32_t lds_addr_of(const void* p) {
+  return static_cast<uint32_t>(
+      reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) const uint8_t*)p));
+}
+// s_waitcnt's operand for vmcnt(0) alone (vmcnt in bits 3:0 and 15:14).
+constexpr int kNoLoads = 0x0f70;
+// Waits until at most kLeft of the wave's loads are on their way.
+template <int kLeft>
+__device__ __forceinline__ void wait_loads() {
+  asm volatile("s_waitcnt vmcnt(%0)" ::"n"(kLeft) : "memory");
+}
+__device__ __forceinline__ short4_t transposed(const uint8_t* p) {
+  typedef __attribute__((address_space(3))) short4_t* lds_short4;
+  return __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_short4)p);
+}
+__device__ __forceinline__ bf16x8_t joined(short4_t a, short4_t b) {
+  const uint2 x = __builtin_bit_cast(uint2, a), y = __builtin_bit_cast(uint2, b);
+  return __builtin_bit_cast(bf16x8_t, make_uint4(x.x, x.y, y.x, y.y));
+}
+__device__ __forceinline__ bf16x8_t masked(bf16x8_t v, const uint32_t (&m)[4]) {
+  const uint4 x = __builtin_bit_cast(uint4, v);
+  return __builtin_bit_cast(bf16x8_t,
+                            make_uint4(x.x & m[0], x.y & m[1], x.z & m[2], x.w & m[3]));
+}
+// Masks of the four words that hold eight 16-bit values, from a bit each.
+__device__ __forceinline__ void word_masks(uint32_t bits, uint32_t (&m)[4]) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    m[i] = (bits >> (2 * i) & 1 ? 0xffffu : 0u) | (bits >> (2 * i + 1) & 1 ? 0xffff0000u : 0u);
+}
+__device__ __forceinline__ uint32_t pack2(float a, float b) {
+  const bf16x2_t x = {static_cast<__bf16>(a), static_cast<__bf16>(b)};
+  return __builtin_bit_cast(uint32_t, x);
+}
+__device__ __forceinline__ float halves_max(float v) {
+  const auto c = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return fmaxf(__uint_as_float(c[0]), __uint_as_float(c[1]));
+}
+__device__ __forceinline__ float halves_sum(float v) {
+  const auto c = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return __uint_as_float(c[0]) + __uint_as_float(c[1]);
+}
+
+// The keys of a part of an item, half a tile (16) at a time.
+struct Halves {
+  const uint8_t* cache;
+  int64_t row_bytes;
+  const int32_t* table;
+  int bt_width, block_size_log2;
+  int64_t num_blocks;
+  // Page of the half that begins at key (a multiple of 16), -1: nothing to see.
+  __device__ __forceinline__ int page(int64_t key, int to) const {
+    if (key >= to) return -1;
+    const int64_t j = key >> block_size_log2;
+    const int p = j < bt_width ? table[j] : -1;
+    return p < num_blocks ? p : -1;
+  }
+  __device__ __forceinline__ const uint8_t* rows(int page, int key) const {
+    const int64_t row = (static_cast<int64_t>(max(page, 0)) << block_size_log2) +
+                        (key & ((1 << block_size_log2) - 1));
+    return cache + row * row_bytes;
+  }
+};
+
+// A sequence on the line: items of two units (32 heads of a row) in steps of a tile.
+__device__ __forceinline__ LineSeq line_seq(const LatentParams& P, const int32_t* __restrict__ cu,
+                                            const int32_t* __restrict__ ctx, int b) {
+  LineSeq x{};
+  const SeqRows s = seq_rows(cu, ctx, b, P.rows, P.most);
+  if (s.rows == 0) return x;
+  int none;
+  row_keys(s, s.rows - 1, -1, none, x.to);
+  // (past the table's end there is nothing to see)
+  x.to = static_cast<int>(min(min(static_cast<int64_t>(x.to), int64_t{0x7fffff00}),
+                              static_cast<int64_t>(P.bt_width) << P.block_size_log2));
+  x.row0 = s.row0;
+  x.rows = s.rows;
+  x.steps = x.to > 0 ? (x.to - 1) / kKeys + 1 : 1;
+  x.items = (s.rows * P.head_blocks + 1) / 2;
+  return x;
+}
+
+// Output of four dims of a finished column, and with dim == 0 its log-sum-exp.
+__device__ __forceinline__ void write_out(const LatentParams& P, int64_t row, int head, int dim,
+                                          const float4& o, float M, float L, float vsc) {
+  const float f = L > 0.f ? vsc / L : 0.f;
+  *reinterpret_cast<uint2*>(P.out + row * P.out_row_stride + head * P.out_head_stride + dim) =
+      make_uint2(pack2(o.x * f, o.y * f), pack2(o.z * f, o.w * f));
+  if (dim == 0 && P.lse)
+    P.lse[head * P.lse_head_stride + row] =
+        L > 0.f ? (M + __builtin_amdgcn_logf(L)) * 0.6931471805599453f : L == 0.f ? kNegInf : L;
+}
+
+// One work-group: items of two units of 32 heads, or 64 columns, in steps of a tile.
+//
+// The waves share S by columns and keys, wave w = (cs, ts): the 32 columns of unit cs and keys
+// 16 ts .. 16 ts + 15 (16x16x32 products), and P V by dims: wave w has dims w R / 4 .. of every
+// column (32x32x16 products), so that V is read from LDS once and K twice.  P goes through LDS,
+// and so do the columns' maxima, of which every wave then makes the same reference.  While P V of
+// a step runs, so does S of the next: two barriers a step, A before both products and B behind
+// them.
+template <int R, int P, bool kFp8>
+__global__ __launch_bounds__(kThreads)
+__attribute__((amdgpu_waves_per_eu(1, 1))) void latent_decode_kernel(
+    LatentParams A, const int32_t* __restrict__ bt, const int32_t* __restrict__ ctx_lens,
+    const int32_t* __restrict__ cu) {
+  using T = Tile<R, P>;
+  constexpr int kCols = 64;
+  constexpr int kKc = (R + P) / 32;           // products of S
+  constexpr int kOb = R / 4 / 32;             // blocks of 32 dims of a wave
+  constexpr int kMoves = T::kMoves / kWaves;  // of a wave and tile
+  static_assert(T::kMoves / 2 % kMoves == 0, "a wave's moves are of one half");
+  __shared__ LineLds<kThreads> line;
+  extern __shared__ __align__(16) uint8_t lds[];
+  uint8_t* const p_lds = lds + kBuffers * T::kBytes;       // [64 columns][32 keys] bf16
+  float* const tops = reinterpret_cast<float*>(p_lds + kCols * kKeys * 2);  // [2][64]
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int lane = threadIdx.x & 63;
+  const int r = lane & 15, g = lane >> 4;   // S
+  const int n = lane & 31, kh = lane >> 5;  // P V
+  const int ts = wave & 1, cs = wave >> 1;
+  const float vsc = kFp8 && A.cache_scale ? *A.cache_scale : 1.f;
+  const float s2 = A.scale_log2 * vsc;
+  const float abs_s2 = __builtin_fabsf(s2);
+  const uint32_t flip = s2 < 0.f ? 0x80008000u : 0u;
+  const int half = wave * kMoves / (T::kMoves / 2);
+  const int move0 = wave * kMoves % (T::kMoves / 2);  // of the half
+  uint32_t src[kMoves];
+#pragma unroll
+  for (int m = 0; m < kMoves; ++m) src[m] = T::template source<kFp8 ? 1 : 2>(move0 + m, lane);
+  const uint32_t dst0 = half * (T::kBytes / 2) + move0 * 1024;
+  const uint32_t lds0 = lds_addr_of(lds);
+  // 16 bytes (8 keys) of a column's weights, their pieces permuted against bank conflicts.
+  auto p_at = [&](int col, int key) {
+    return p_lds + col * 64 + 16 * (((key >> 3) ^ (col >> 2)) & 3) + 2 * (key & 7);
+  };
+
+  auto body = [&](int b, const LineSeq& x, int it, int s_lo, int s_hi, int64_t slot) {
+    const SeqRows sr = seq_rows(cu, ctx_lens, b, A.rows, A.most);
+    const int unit0 = it * 2;
+    const bool two = unit0 + 1 < x.rows * A.head_blocks;
+    // Row, first head and visible keys of both units.
+    int row_i[2], head0[2], hi[2];
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+      const int unit = two ? unit0 + u : unit0;
+      int none;
+      row_i[u] = unit / A.head_blocks;
+      head0[u] = 32 * (unit - row_i[u] * A.head_blocks);
+      row_keys(sr, row_i[u], -1, none, hi[u]);
+      hi[u] = uniform(hi[u]);
+    }
+    const int all_hi = min(hi[0], hi[1]), my_hi = cs ? hi[1] : hi[0];
+    const bool active = cs == 0 || two;
+    bf16x8_t qb[2][kKc];
+#pragma unroll
+    for (int cb = 0; cb < 2; ++cb) {
+      const int h = (cs ? head0[1] : head0[0]) + 16 * cb + r;
+      const bool ok = h < A.num_heads;
+      const uint16_t* const qp = A.q + (x.row0 + (cs ? row_i[1] : row_i[0])) * A.q_row_stride +
+                                 (ok ? h : 0) * A.q_head_stride + 8 * g;
+#pragma unroll
+      for (int k = 0; k < kKc; ++k) {
+        uint4 v = ok ? *reinterpret_cast<const uint4*>(qp + 32 * k) : make_uint4(0, 0, 0, 0);
+        v = make_uint4(v.x ^ flip, v.y ^ flip, v.z ^ flip, v.w ^ flip);
+        qb[cb][k] = __builtin_bit_cast(bf16x8_t, v);
+      }
+    }
+    floatx16_t o[2][kOb];  // of unit u: dims 32 d + i % 4 + 8 (i / 4) + 4 kh, column n
+#pragma unroll
+    for (int u = 0; u < 2; ++u)
+#pragma unroll
+      for (int d = 0; d < kOb; ++d)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) o[u][d][i] = 0.f;
+    // The reference maxima of S's columns (16 cb + r of unit cs), of O's (n of unit u), and this
+    // lane's share of S's columns' sums.
+    float ms[2] = {kNoMax, kNoMax}, mo[2] = {kNoMax, kNoMax}, l[2] = {0.f, 0.f};
+
+    const Halves keys{A.cache, (R + P) * (kFp8 ? 1 : 2), bt + b * A.bt_row_stride, A.bt_width,
+                      A.block_size_log2, A.num_blocks};
+    const int steps = s_hi - s_lo;
+    // The pages of the next 32 steps' halves, a lane each; and which of them, and of the 32
+    // steps before, there are.
+    int pages = -1, looked_up = -1;
+    uint64_t there = 0, there_before = 0;
+    uint2 raw[kFp8 ? kMoves : 1];
+    // Issues this wave's loads of step s: bf16 into its buffer, fp8 into `to`.
+    auto load = [&](int s, uint2 (&to)[kFp8 ? kMoves : 1]) {
+      s = min(s, steps - 1);  // (past the end, once more: as many loads are on their way)
+      const int key0 = (s_lo + s) * kKeys;
+      if (s / 32 != looked_up) {
+        looked_up = s / 32;
+        pages = keys.page(static_cast<int64_t>(key0) + 16 * lane, x.to);
+        there_before = there;
+        there = __ballot(pages >= 0);
+      }
+      const int pg = __builtin_amdgcn_readlane(pages, 2 * (s & 31) + half);
+      const uint8_t* const base = keys.rows(pg, key0 + 16 * half);
+      const uint32_t dst = lds0 + (s % kBuffers) * T::kBytes + dst0;
+#pragma unroll
+      for (int i = 0; i < kMoves; ++i) {
+        if constexpr (kFp8)
+          to[i] = ld8(base + src[i]);
+        else
+          lds_load16(base, src[i], dst + 1024 * i);
+      }
+    };
+    // fp8: what was loaded, as bf16, into step s's buffer.
+    auto put = [&](int s, const uint2 (&from)[kFp8 ? kMoves : 1]) {
+      uint8_t* const dst = lds + (s % kBuffers) * T::kBytes + dst0 + 16 * lane;
+#pragma unroll
+      for (int i = 0; i < (kFp8 ? kMoves : 0); ++i) {
+        const uint2 a = fp8x4_to_bf16x4(from[i].x), c = fp8x4_to_bf16x4(from[i].y);
+        *reinterpret_cast<uint4*>(dst + 1024 * i) = make_uint4(a.x, a.y, c.x, c.y);
+      }
+    };
+    auto halves_of = [&](int s) -> uint32_t {
+      return (s / 32 == looked_up ? there : there_before) >> (2 * (s & 31)) & 3;
+    };
+    // Whether every column sees all keys of step s.
+    auto whole = [&](int s) { return (s_lo + s + 1) * kKeys <= all_hi && halves_of(s) == 3; };
+
+    floatx4_t p[2];
+    // S of step s, and its columns' maxima.
+    auto scores = [&](int s, auto is_masked) {
+      const uint8_t* const tile = lds + (s % kBuffers) * T::kBytes;
+#pragma unroll
+      for (int cb = 0; cb < 2; ++cb) p[cb] = floatx4_t{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int k = 0; k < kKc; ++k) {
+        const uint4 a = *reinterpret_cast<const uint4*>(tile + T::at(16 * ts + r, 4 * k + g));
+#pragma unroll
+        for (int cb = 0; cb < 2; ++cb)
+          p[cb] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, a),
+                                                          qb[cb][k], p[cb], 0, 0, 0);
+      }
+      p[0] *= abs_s2;
+      p[1] *= abs_s2;
+      if constexpr (decltype(is_masked)::value) {
+        const int t0 = (s_lo + s) * kKeys + 16 * ts + 4 * g;
+        const bool there_ = halves_of(s) >> ts & 1;
+#pragma unroll
+        for (int cb = 0; cb < 2; ++cb)
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            if (!(there_ && t0 + i < my_hi)) p[cb][i] = kNegInf;
+      }
+#pragma unroll
+      for (int cb = 0; cb < 2; ++cb) {
+        const float top =
+            pair_max(fmaxf(fmaxf(p[cb][0], p[cb][1]), fmaxf(p[cb][2], p[cb][3])));
+        if (g == 0) tops[64 * ts + 32 * cs + 16 * cb + r] = top;
+      }
+    };
+    // The references, moved where they have to be; weights from p, into LDS.
+    auto weights = [&] {
+      float t[2];
+      bool move = false;
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        t[u] = fmaxf(tops[32 * u + n], tops[64 + 32 * u + n]);
+        move |= (u == 0 || two) && t[u] > mo[u] + kLazyMax;
+      }
+      if (__ballot(move) != 0) {
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+          const float m_new = fmaxf(mo[u], t[u]);
+          const float alpha = __builtin_amdgcn_exp2f(mo[u] - m_new);
+          mo[u] = m_new;
+#pragma unroll
+          for (int d = 0; d < kOb; ++d)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) o[u][d][i] *= alpha;
+        }
+#pragma unroll
+        for (int cb = 0; cb < 2; ++cb) {
+          const int c = 32 * cs + 16 * cb + r;
+          const float m_new = fmaxf(ms[cb], fmaxf(tops[c], tops[64 + c]));
+          l[cb] *= __builtin_amdgcn_exp2f(ms[cb] - m_new);
+          ms[cb] = m_new;
+        }
+      }
+      if (!active) return;
+      // The weights are rounded to bf16 for P V (2^-9 relative at most, of either sign); their
+      // sum is of the unrounded ones.
+#pragma unroll
+      for (int cb = 0; cb < 2; ++cb) {
+        float e[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) e[i] = __builtin_amdgcn_exp2f(p[cb][i] - ms[cb]);
+        l[cb] += (e[0] + e[1]) + (e[2] + e[3]);
+        *reinterpret_cast<uint2*>(p_at(32 * cs + 16 * cb + r, 16 * ts + 4 * g)) =
+            make_uint2(pack2(e[0], e[1]), pack2(e[2], e[3]));
+      }
+    };
+    // O += P V of step s.  Operands of 16 keys (k): lane (n, kh) has keys 16 k + 8 kh .. + 7.  In
+    // a transpose load, lane 4 a + q of each 16 addresses key a and dims 4 q .. 4 q + 3.
+    auto values = [&](int s, auto is_masked) {
+      constexpr bool kMasked = decltype(is_masked)::value;
+      const uint8_t* const tile = lds + (s % kBuffers) * T::kBytes;
+      const int a4 = r >> 2, piece = wave * (R / 32) + 2 * (g & 1) + ((lane & 3) >> 1);
+#pragma unroll
+      for (int k = 0; k < 2; ++k) {
+        bf16x8_t w[2];
+#pragma unroll
+        for (int u = 0; u < 2; ++u)
+          w[u] = __builtin_bit_cast(
+              bf16x8_t, *reinterpret_cast<const uint4*>(p_at(32 * u + n, 16 * k + 8 * kh)));
+        // Keys that the row does not see may hold anything, infinities and NaN among it: zeros.
+        uint32_t mask[2][4];
+        if constexpr (kMasked) {
+          const uint32_t halves = halves_of(s);
+#pragma unroll
+          for (int u = 0; u < 2; ++u) {
+            uint32_t bits = 0;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+              const int t = (s_lo + s) * kKeys + 16 * k + 8 * kh + i;
+              bits |= (halves >> k & 1) && t < hi[u] ? 1u << i : 0u;
+            }
+            word_masks(bits, mask[u]);
+          }
+        }
+        const int row = 16 * k + 8 * kh + a4;
+#pragma unroll
+        for (int d = 0; d < kOb; ++d) {
+          const uint8_t* const at = tile + 8 * (lane & 1);
+          const bf16x8_t v = joined(transposed(at + T::at(row, 4 * d + piece)),
+                                    transposed(at + T::at(row + 4, 4 * d + piece)));
+          o[0][d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kMasked ? masked(v, mask[0]) : v, w[0],
+                                                            o[0][d], 0, 0, 0);
+          if (two)
+            o[1][d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kMasked ? masked(v, mask[1]) : v,
+                                                              w[1], o[1][d], 0, 0, 0);
+        }
+      }
+    };
+
+    // (the queries have come: the waits in the loop count the loads above alone)
+    __builtin_amdgcn_s_waitcnt(kNoLoads);
+    if constexpr (kFp8) {
+      uint2 raw0[kMoves], raw1[kMoves];
+      load(0, raw0);
+      load(1, raw1);
+      load(2, raw);
+      put(0, raw0);
+      put(1, raw1);
+    } else {
+#pragma unroll 1
+      for (int s = 0; s < kBuffers; ++s) load(s, raw);
+      wait_loads<(kBuffers - 1) * kMoves>();
+    }
+    __syncthreads();
+    if (active) scores(0, std::true_type{});
+    __syncthreads();
+    weights();
+    auto step = [&](int s, auto is_masked) {
+      if constexpr (!kFp8) wait_loads<(kBuffers - 2) * kMoves>();
+      __syncthreads();  // A: step s's weights and step s + 1's tile are in LDS
+      values(s, is_masked);
+      if (s + 1 >= steps) return;
+      if (active) scores(s + 1, is_masked);
+      __syncthreads();  // B: the maxima are in LDS, step s's tile and weights have been read
+      if constexpr (kFp8) {
+        put(s + 2, raw);
+        load(s + 3, raw);
+      } else {
+        load(s + kBuffers, raw);
+      }
+      weights();
+    };
+    // (a loop of its own for the steps from the first one on that is not whole)
+    int s = 0;
+#pragma unroll 1
+    for (; s + 1 < steps && whole(s) && whole(s + 1); ++s) step(s, std::false_type{});
+#pragma unroll 1
+    for (; s < steps; ++s) step(s, std::true_type{});
+    wait_loads<0>();
+
+    // The columns' sums, of both waves and all lanes that have keys of theirs.
+#pragma unroll
+    for (int cb = 0; cb < 2; ++cb) {
+      l[cb] = pair_sum(l[cb]);
+      if (g == 0) tops[64 * ts + 32 * cs + 16 * cb + r] = l[cb];
+    }
+    __syncthreads();
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+      const int c = 32 * u + n, head = head0[u] + n;
+      if ((u == 1 && !two) || head >= A.num_heads) continue;
+      const float L = tops[c] + tops[64 + c];
+      float* const po = A.o + (slot * kCols + c) * R;
+      if (slot >= 0 && wave == 0 && kh == 0)
+        *reinterpret_cast<float2*>(A.ml + (slot * kCols + c) * 2) = make_float2(mo[u], L);
+#pragma unroll
+      for (int d = 0; d < kOb; ++d)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const float4 z = make_float4(o[u][d][4 * i], o[u][d][4 * i + 1], o[u][d][4 * i + 2],
+                                       o[u][d][4 * i + 3]);
+          const int dim = wave * (R / 4) + 32 * d + 8 * i + 4 * kh;
+          if (slot < 0)
+            write_out(A, x.row0 + row_i[u], head, dim, z, mo[u], L, vsc);
+          else
+            *reinterpret_cast<float4*>(po + dim) = z;
+        }
+    }
+    __syncthreads();
+  };
+  walk_line<kThreads>(line, A.batch, A.wgs, blockIdx.x, 1, A.records,
+                      [&](int b) { return line_seq(A, cu, ctx_lens, b); }, body);
+}
+
+// One work-group per (query row, some of its heads): merges the pieces of an item that ranges cut.
+template <int R>
+__global__ __launch_bounds__(kMergeThreads) void latent_merge_kernel(
+    LatentParams A, const int32_t* __restrict__ ctx_lens, const int32_t* __restrict__ cu,
+    int heads, int fp8) {
+  __shared__ Folded folded[kMergeThreads];
+  const int t = blockIdx.y;
+  int b, vis;
+  if (!query_row(cu, ctx_lens, A.batch, t, b, vis)) return;
+  const SeqRows s = seq_rows(cu, ctx_lens, b, A.rows, A.most);
+  const int i = t - s.row0;
+  if (i >= s.rows) return;
+  const LineRecord rec = A.records[b];
+  const float vsc = fp8 && A.cache_scale ? *A.cache_scale : 1.f;
+  const int h0 = blockIdx.x * heads, h1 = min(h0 + heads, A.num_heads);
+  // Unit by unit of the row's heads.
+  for (int h = h0; h < h1;) {
+    const int unit = i * A.head_blocks + h / 32;
+    const int in = 32 * (unit & 1) + h % 32;
+    const int nc = min(h1, (h / 32 + 1) * 32) - h;
+    const LinePieces pieces(rec, unit >> 1);
+    if (pieces.n > 1) {
+      merge_pieces<R>(
+          0, nc, folded, [&](int) { return pieces.n; },
+          [&](int k, int x, const float*& ml, const float*& o) {
+            const int64_t at = pieces.slot(k) * 64 + in + x;
+            ml = A.ml + 2 * at;
+            o = A.o + at * R;
+          },
+          [&](int x, int dim, const float4& o, float M, float L) {
+            write_out(A, t, h + x, dim, o, M, L, vsc);
+          });
+      __syncthreads();
+    }
+    h += nc;
+  }
+}
+
+struct LatentPlan {
+  int wgs;
+  int64_t o, ml, records, bytes;
+};
+LatentPlan plan_of(int64_t batch, int latent_size) {
+  LatentPlan p{};
+  p.wgs = num_cus();
+  auto take = [&](int64_t bytes) {
+    const int64_t at = p.bytes;
+    p.bytes += (bytes + 255) / 256 * 256;
+    return at;
+  };
+  p.o = take(int64_t{2} * p.wgs * 64 * latent_size * 4);
+  p.ml = take(int64_t{2} * p.wgs * 64 * 8);
+  p.records = take(batch * static_cast<int64_t>(sizeof(LineRecord)));
+  return p;
+}
+
+template <int R, int P, bool kFp8>
+void launch(const LatentParams& A, hipStream_t s, const int32_t* bt, const int32_t* ctx,
+            const int32_t* cu) {
+  const unsigned lds = kBuffers * Tile<R, P>::kBytes + 64 * kKeys * 2 + 2 * 64 * 4;
+  hipLaunchKernelGGL((latent_decode_kernel<R, P, kFp8>), dim3(A.wgs + 1), dim3(kThreads), lds, s,
+                     A, bt, ctx, cu);
+  const int heads = merge_cols(A.rows, 1, A.num_heads);
+  hipLaunchKernelGGL((latent_merge_kernel<R>), dim3((A.num_heads + heads - 1) / heads, A.rows),
+                     dim3(kMergeThreads), 0, s, A, ctx, cu, heads, kFp8 ? 1 : 0);
+}
+
+}  // namespace
+}  // namespace fk
+
+using namespace fk;
+
+extern "C" int fk_latent_decode(void* out, int64_t out_row_stride, int64_t out_head_stride,
+                                const void* q, int64_t q_row_stride, int64_t q_head_stride,
+                                const void* cache, int cache_dtype, const float* cache_scale,
+                                const int32_t* block_tables, int64_t bt_row_stride,
+                                int64_t bt_width, const int32_t* cache_seqlens,
+                                const int32_t* cu_seqlens_q, int64_t batch, int64_t rows,
+                                int64_t max_seqlen_q, int num_heads, int latent_size,
+                                int rope_size, int block_size, int64_t num_blocks, float scale,
+                                float* lse, int64_t lse_head_stride, void* workspace,
+                                int64_t workspace_bytes, void* stream) {
+  const char* what = "fk_latent_decode";
+  FK_REQUIRE(batch >= 0 && batch <= 65535 && rows >= 0 && rows <= 65535,
+             "%s: batch %lld or rows %lld outside [0, 65535]", what, static_cast<long long>(batch),
+             static_cast<long long>(rows));
+  FK_REQUIRE(num_heads > 0 && num_heads <= 65535, "%s: %d heads", what, num_heads);
+  FK_REQUIRE(max_seqlen_q >= 1 && max_seqlen_q <= 65535 && max_seqlen_q * num_heads <= 0x7fffffff,
+             "%s: max_seqlen_q %lld", what, static_cast<long long>(max_seqlen_q));
+  FK_REQUIRE(cache_dtype == FK_DTYPE_BF16 || cache_dtype == FK_DTYPE_FP8_E4M3FN,
+             "%s: the cache must be bf16 or fp8 e4m3fn", what);
+  FK_REQUIRE(block_size >= 16 && block_size <= (1 << 30) && (block_size & (block_size - 1)) == 0,
+             "%s: block_size %d must be a power of two >= 16", what, block_size);
+  FK_REQUIRE(num_blocks > 0 && num_blocks <= 0x7fffffff, "%s: num_blocks %lld", what,
+             static_cast<long long>(num_blocks));
+  FK_REQUIRE(bt_width >= 0 && bt_width <= 0x7fffffff && bt_row_stride >= 0,
+             "%s: block table of %lld columns", what, static_cast<long long>(bt_width));
+  if (latent_size != 512 || rope_size != 64)
+    return set_error(FK_ERR_UNSUPPORTED, "%s: rows of %d + %d unsupported (512 + 64)", what,
+                     latent_size, rope_size);
+  FK_REQUIRE(aligned16(q) && aligned16(out) && aligned16(cache) && q_row_stride % 8 == 0 &&
+                 q_head_stride % 8 == 0 && out_row_stride % 8 == 0 && out_head_stride % 8 == 0,
+             "%s: q, out and the cache must have 16-byte aligned rows", what);
+  if (batch == 0 || rows == 0) return FK_OK;
+  FK_REQUIRE(out && q && cache && block_tables && cache_seqlens, "%s: null pointer", what);
+  if (!cu_seqlens_q) max_seqlen_q = 1;
+  const LatentPlan plan = plan_of(batch, latent_size);
+  if (workspace_bytes < plan.bytes || !workspace)
+    return set_error(FK_ERR_WORKSPACE, "%s: workspace of %lld bytes, %lld needed", what,
+                     static_cast<long long>(workspace_bytes), static_cast<long long>(plan.bytes));
+  FK_REQUIRE(aligned16(workspace), "%s: workspace must be 16-byte aligned", what);
+  uint8_t* const ws = static_cast<uint8_t*>(workspace);
+  LatentParams A{};
+  A.out = static_cast<uint16_t*>(out);
+  A.out_row_stride = out_row_stride;
+  A.out_head_stride = out_head_stride;
+  A.q = static_cast<const uint16_t*>(q);
+  A.q_row_stride = q_row_stride;
+  A.q_head_stride = q_head_stride;
+  A.cache = static_cast<const uint8_t*>(cache);
+  A.cache_scale = cache_scale;
+  A.lse = lse;
+  A.lse_head_stride = lse_head_stride;
+  A.scale_log2 = scale * kLog2e;
+  A.num_heads = num_heads;
+  A.batch = static_cast<int>(batch);
+  A.rows = static_cast<int>(rows);
+  A.most = static_cast<int>(max_seqlen_q);
+  A.block_size_log2 = 31 - __builtin_clz(static_cast<unsigned>(block_size));
+  A.num_blocks = num_blocks;
+  A.bt_row_stride = bt_row_stride;
+  A.bt_width = static_cast<int>(bt_width);
+  A.wgs = plan.wgs;
+  A.head_blocks = (num_heads + 31) / 32;
+  A.o = reinterpret_cast<float*>(ws + plan.o);
+  A.ml = reinterpret_cast<float*>(ws + plan.ml);
+  A.records = reinterpret_cast<LineRecord*>(ws + plan.records);
+  hipStream_t s = as_stream(stream);
+  if (cache_dtype == FK_DTYPE_FP8_E4M3FN)
+    launch<512, 64, true>(A, s, block_tables, cache_seqlens, cu_seqlens_q);
+  else
+    launch<512, 64, false>(A, s, block_tables, cache_seqlens, cu_seqlens_q);
+  return check_launch(what);
+}
+
+extern "C" int fk_latent_decode_plan(int64_t batch, int64_t max_seqlen_q, int num_heads,
+                                     int latent_size, int64_t* workspace_bytes) {
+  FK_REQUIRE(workspace_bytes, "fk_latent_decode_plan: null output pointer");
+  FK_REQUIRE(batch >= 0 && batch <= 65535 && max_seqlen_q >= 1 && max_seqlen_q <= 65535 &&
+                 num_heads > 0 && num_heads <= 65535 && latent_size > 0 && latent_size <= 65536,
+             "fk_latent_decode_plan: invalid argument");
+  *workspace_bytes = batch == 0 ? 0 : plan_of(batch, latent_size).bytes;
+  return FK_OK;
+}

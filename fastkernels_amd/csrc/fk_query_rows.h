@@ -5,19 +5,10 @@
 
 namespace fk {
 
-// Sequence b of query row t and the keys the row sees, vis = ctx - n + i + 1 for the i-th
-// of the sequence's n rows (aligned to the end of its tokens; at most ctx).  cu == nullptr:
-// one row per sequence.  False for a row behind the last sequence.  Sequences without rows
-// are skipped by taking the last b with cu[b] <= t.  Whole waves call it, with one t each.
-__device__ __forceinline__ bool query_row(const int32_t* __restrict__ cu,
-                                          const int32_t* __restrict__ ctx, int batch, int t,
-                                          int& b, int& vis) {
-  if (cu == nullptr) {
-    b = t;
-    vis = t < batch ? ctx[t] : 0;
-    return t < batch;
-  }
-  if (batch <= 0 || t < cu[0] || t >= cu[batch]) return false;
+// Sequence of row t (cu[b] <= t < cu[b + 1]), or -1 for a row of none.  Sequences without rows are
+// skipped by taking the last b with cu[b] <= t.  Whole waves call it, with one t each.
+__device__ __forceinline__ int sequence_of(const int32_t* __restrict__ cu, int batch, int t) {
+  if (batch <= 0 || t < cu[0] || t >= cu[batch]) return -1;
   // The lanes look at 64 places at a time: one load's latency for up to 64 sequences, where
   // halving takes six.
   const int lane = threadIdx.x & 63;
@@ -29,7 +20,23 @@ __device__ __forceinline__ bool query_row(const int32_t* __restrict__ cu,
     lo += last;
     len = min(step, len - last);
   }
-  b = lo;
+  return lo;
+}
+
+// Sequence b of query row t and the keys the row sees, vis = ctx - n + i + 1 for the i-th
+// of the sequence's n rows (aligned to the end of its tokens; at most ctx).  cu == nullptr:
+// one row per sequence.  False for a row behind the last sequence.  Whole waves call it, with one
+// t each.
+__device__ __forceinline__ bool query_row(const int32_t* __restrict__ cu,
+                                          const int32_t* __restrict__ ctx, int batch, int t,
+                                          int& b, int& vis) {
+  if (cu == nullptr) {
+    b = t;
+    vis = t < batch ? ctx[t] : 0;
+    return t < batch;
+  }
+  b = sequence_of(cu, batch, t);
+  if (b < 0) return false;
   const int c = ctx[b];
   // (cu[b + 1] > t here, so at least one of the sequence's rows is not before this one.)
   vis = c - (cu[b + 1] - 1 - t);

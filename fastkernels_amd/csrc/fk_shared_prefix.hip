@@ -36,6 +36,7 @@
 // whole ranges (101 and 160).
 #include <limits.h>
 
+#include "fk_lines.h"
 #include "fk_page_attn.h"
 
 namespace fk {
@@ -106,27 +107,6 @@ __device__ __forceinline__ int tiles_in(int tokens) {
 __device__ __forceinline__ int64_t places_of(int prefix) {
   return (tiles_in(prefix) + kPreTiles - 1) & -kPreTiles;
 }
-__device__ __forceinline__ int64_t lane64(int64_t v, int src) {
-  const uint32_t lo = __builtin_amdgcn_readlane(static_cast<int>(v), src);
-  const uint32_t hi = __builtin_amdgcn_readlane(static_cast<int>(v >> 32), src);
-  return static_cast<int64_t>((static_cast<uint64_t>(hi) << 32) | lo);
-}
-// Inclusive sums over the lanes of a wave: within rows of 16, then across them.
-template <int kCtrl, int kRows>
-__device__ __forceinline__ int64_t plus_moved(int64_t v) {
-  const uint32_t lo = __builtin_amdgcn_update_dpp(0, static_cast<int>(v), kCtrl, kRows, 0xf, false);
-  const uint32_t hi =
-      __builtin_amdgcn_update_dpp(0, static_cast<int>(v >> 32), kCtrl, kRows, 0xf, false);
-  return v + static_cast<int64_t>((static_cast<uint64_t>(hi) << 32) | lo);
-}
-__device__ __forceinline__ int64_t scan64(int64_t v) {
-  v = plus_moved<0x111, 0xf>(v);     // from the lane 1 before, 2, 4, 8
-  v = plus_moved<0x112, 0xf>(v);
-  v = plus_moved<0x114, 0xf>(v);
-  v = plus_moved<0x118, 0xf>(v);
-  v = plus_moved<0x142, 0xa>(v);     // from lane 15 of the row before, into rows 1 and 3
-  return plus_moved<0x143, 0xc>(v);  // from lane 31, into rows 2 and 3
-}
 // v of the lane `off` places further on in the row of 16, round.
 template <int kOff>
 __device__ __forceinline__ uint32_t rotated(uint32_t v) {
@@ -138,34 +118,6 @@ __device__ __forceinline__ uint32_t row_max(uint32_t v) {
   v = max(v, rotated<2>(v));
   return max(v, rotated<1>(v));
 }
-// A line of `total` tiles is cut into ranges of the least multiple of `quantum` (a power of two)
-// that makes them at most n.
-__device__ __forceinline__ int64_t range_of(int64_t total, int n, int quantum) {
-  int64_t range = static_cast<int64_t>(static_cast<double>(total) / n);
-  range += range * n < total;  // (the quotient is off by less than one)
-  range = (range + quantum - 1) & -static_cast<int64_t>(quantum);
-  return max(range, static_cast<int64_t>(quantum));
-}
-// a / b (0 <= a, 0 < b) by way of a float estimate, off by one at most for quotients below 2^21.
-__device__ __forceinline__ int quotient(int64_t a, int64_t b) {
-  int64_t q = static_cast<int64_t>(static_cast<float>(a) *
-                                   __builtin_amdgcn_rcpf(static_cast<float>(b)));
-  while (q * b > a) --q;
-  while ((q + 1) * b <= a) ++q;
-  return static_cast<int>(q);
-}
-// The share of a line that work-group `wg` of n takes, when it has `shares` of them (n or more:
-// none).  They are dealt out to the 8 XCDs in runs (work-groups go to XCDs in turn), so that
-// neighbouring ranges, which read the same keys for the column blocks of a group, share an L2;
-// `last`: the work-groups are counted from the end.
-__device__ __forceinline__ int64_t share_of(int wg, int n, int64_t shares, bool last) {
-  if (n % 8) return last ? n - 1 - wg : wg;
-  const int per = static_cast<int>(shares + 7) / 8;
-  const int i = last ? n / 8 - 1 - (wg >> 3) : wg >> 3;
-  return i < per ? (wg & 7) * per + i : n;
-}
-__device__ __forceinline__ int uniform(int v) { return __builtin_amdgcn_readfirstlane(v); }
-
 // LDS: the merge's states (also the last work-group's tables), a chunk of rows, the groups.
 template <int D>
 constexpr int lds_rows_at() { return 4 * merge_lds_floats<kWaves, D>(cols_of(D)); }

@@ -53,6 +53,8 @@ int num_cus() {
 // 2.2.0: fk_paged_decode_shape and fk_prefill_shape added.
 // 2.3.0: fk_update_key_bounds, fk_block_scores, fk_select_blocks, fk_sparse_paged_decode,
 // fk_shared_prefix_decode and the plans of the last two added.
+// 2.4.0: the 4-bit cache (fk_*_mxfp4, fk_mxfp4_paged_decode and its plan) and the latent cache
+// (fk_latent_norm_rope_store, fk_gather_latent, fk_latent_decode and its plan) added.
 extern "C" int fk_version(void) { return FK_VERSION_MAJOR * 10000 + FK_VERSION_MINOR * 100; }
 
 extern "C" const char* fk_last_error(void) { return fk::g_last_error; }

@@ -1001,6 +1001,316 @@ def shared_prefix_decode(out: torch.Tensor, q: torch.Tensor, k_cache: torch.Tens
 
 
 # ---------------------------------------------------------------------------
+# A paged cache held in 4 bits (OCP microscaling fp4)
+# ---------------------------------------------------------------------------
+class Mxfp4Cache(NamedTuple):
+    """Codes and scales of a 4-bit cache (uint8; layouts in include/fastkernels_amd.h)."""
+    k_cache: torch.Tensor   # [num_blocks, Hk, block_size, D / 2]
+    v_cache: torch.Tensor   # [num_blocks, Hk, block_size / 4, 16, 4, D / 32]
+    k_scales: torch.Tensor  # [num_blocks, Hk, D / 32, block_size]
+    v_scales: torch.Tensor  # [num_blocks, Hk, D / 32, block_size]
+
+
+def new_mxfp4_cache(num_blocks: int, block_size: int, num_kv_heads: int, head_dim: int,
+                    device) -> Mxfp4Cache:
+    """A 4-bit cache of zeros: (D + D / 16) bytes a token and kv head, K and V together."""
+    if head_dim not in (64, 128, 256) or block_size < 16 or block_size & (block_size - 1):
+        raise ValueError(f"new_mxfp4_cache: head_dim {head_dim} must be 64, 128 or 256, block_size "
+                         f"{block_size} a power of two >= 16")
+    codes, blocks = head_dim // 2, head_dim // 32
+
+    def zeros(*shape):
+        return torch.zeros(num_blocks, num_kv_heads, *shape, dtype=torch.uint8, device=device)
+    return Mxfp4Cache(zeros(block_size, codes), zeros(block_size // 4, 16, 4, blocks),
+                      zeros(blocks, block_size), zeros(blocks, block_size))
+
+
+def _check_mxfp4(what, k_cache, v_cache, k_scales, v_scales) -> tuple[int, int, int, int]:
+    """(num_blocks, Hk, block_size, D) of a 4-bit cache."""
+    shape = k_cache.shape
+    if len(shape) != 4:
+        raise ValueError(f"{what}: k_cache must be [num_blocks, Hk, block_size, D / 2]")
+    nb, hk, bs, half = shape
+    scales = (nb, hk, half // 16, bs)
+    if v_cache.shape != (nb, hk, bs // 4, 16, 4, half // 16):
+        raise ValueError(f"{what}: v_cache must be [num_blocks, Hk, block_size / 4, 16, 4, D / 32]")
+    if k_scales.shape != scales or v_scales.shape != scales:
+        raise ValueError(f"{what}: k_scales and v_scales must be [num_blocks, Hk, D / 32, "
+                         "block_size]")
+    for t in (k_cache, v_cache, k_scales, v_scales):
+        if t.dtype != torch.uint8 or not t.is_contiguous():
+            raise ValueError(f"{what}: codes and scales must be contiguous uint8")
+    return nb, hk, bs, 2 * half
+
+
+def _check_slots(what, slot_mapping, tokens) -> int:
+    """Checks a slot mapping; returns whether it is int64."""
+    i64 = slot_mapping.dtype == torch.int64
+    if not (i64 or slot_mapping.dtype == torch.int32) or not slot_mapping.is_contiguous():
+        raise TypeError(f"{what}: slot_mapping must be contiguous int32 or int64")
+    if slot_mapping.numel() < tokens:
+        raise ValueError(f"{what}: slot_mapping shorter than the token count")
+    return int(i64)
+
+
+def _check_cu_k(what, cu_seqlens_k) -> int:
+    """Checks the contexts' first rows; returns the number of sequences."""
+    if cu_seqlens_k.dtype != torch.int32 or cu_seqlens_k.dim() != 1 or \
+            not cu_seqlens_k.is_contiguous() or cu_seqlens_k.numel() < 1:
+        raise TypeError(f"{what}: cu_seqlens_k must be contiguous int32 [batch + 1]")
+    return cu_seqlens_k.numel() - 1
+
+
+def store_kvcache_mxfp4(key: torch.Tensor, value: torch.Tensor, k_cache: torch.Tensor,
+                        v_cache: torch.Tensor, k_scales: torch.Tensor, v_scales: torch.Tensor,
+                        slot_mapping: torch.Tensor) -> None:
+    """:func:`store_kvcache` into a 4-bit cache (:class:`Mxfp4Cache`): key/value [N, Hk, D] of
+    float32, float16 or bfloat16, slot_mapping (-1 skips; otherwise distinct).  Each 32 dims of a
+    row share a power of two, the exponent of their greatest magnitude rounded to two significant
+    bits, less 2; values are rounded to the nearest of {0, 0.5, 1, 1.5, 2, 3, 4, 6} times it, ties
+    to the even code.  32 dims with an infinity or a NaN become NaN."""
+    what = "store_kvcache_mxfp4"
+    if key.dim() != 3 or value.shape != key.shape:
+        raise ValueError(f"{what}: key/value must be [N, num_kv_heads, head_dim]")
+    n, hk, d = key.shape
+    nb, hk_cache, bs, d_cache = _check_mxfp4(what, k_cache, v_cache, k_scales, v_scales)
+    if (hk_cache, d_cache) != (hk, d):
+        raise ValueError(f"{what}: rows of {hk} heads of {d} into a cache of {hk_cache} of "
+                         f"{d_cache}")
+    if value.dtype != key.dtype:
+        raise TypeError(f"{what}: key and value must share a dtype")
+    tag = _tag(key, what)
+    for t, nm in ((key, "key"), (value, "value")):
+        if t.stride(2) != 1 or (hk > 1 and t.stride(1) != d):
+            raise ValueError(f"{what}: {nm} rows must be [Hk, D] contiguous")
+    i64 = _check_slots(what, slot_mapping, n)
+    dev = _same_device(key, value, k_cache, v_cache, k_scales, v_scales, slot_mapping)
+    if n == 0:
+        return
+    _call_on(key, dev, "fk_store_kvcache_mxfp4", key.data_ptr(), key.stride(0), value.data_ptr(),
+             value.stride(0), tag, k_cache.data_ptr(), v_cache.data_ptr(), k_scales.data_ptr(),
+             v_scales.data_ptr(), slot_mapping.data_ptr(), i64, n, hk, d, bs, nb)
+
+
+def gather_kvcache_mxfp4(key: torch.Tensor, value: torch.Tensor, k_cache: torch.Tensor,
+                         v_cache: torch.Tensor, k_scales: torch.Tensor, v_scales: torch.Tensor,
+                         block_table: torch.Tensor, cu_seqlens_k: torch.Tensor) -> None:
+    """key / value (bf16 [rows, Hk, D]): row cu_seqlens_k[b] + i becomes what a 4-bit cache holds
+    of position i of sequence b, exactly (zeros where block_table has no page); rows behind the
+    last sequence stay as they were.  The dense keys that :func:`varlen_prefill` takes for a chunk
+    of a prompt over such a cache."""
+    what = "gather_kvcache_mxfp4"
+    nb, hk, bs, d = _check_mxfp4(what, k_cache, v_cache, k_scales, v_scales)
+    for t, nm in ((key, "key"), (value, "value")):
+        if t.dim() != 3 or t.dtype != torch.bfloat16 or t.shape[1:] != (hk, d) or \
+                t.stride(2) != 1 or (hk > 1 and t.stride(1) != d):
+            raise ValueError(f"{what}: {nm} must be bf16 [rows, {hk}, {d}] with contiguous rows")
+    if value.shape != key.shape:
+        raise ValueError(f"{what}: key and value must have the same rows")
+    batch = _check_cu_k(what, cu_seqlens_k)
+    bt_stride, bt_width = _check_table(what, block_table, batch)
+    dev = _same_device(key, value, k_cache, v_cache, k_scales, v_scales, block_table,
+                       cu_seqlens_k)
+    rows = key.shape[0]
+    if rows == 0 or batch == 0:
+        return
+    _call_on(key, dev, "fk_gather_kvcache_mxfp4", key.data_ptr(), key.stride(0),
+             value.data_ptr(), value.stride(0), k_cache.data_ptr(), v_cache.data_ptr(),
+             k_scales.data_ptr(), v_scales.data_ptr(), block_table.data_ptr(), bt_stride,
+             bt_width, cu_seqlens_k.data_ptr(), batch, rows, hk, d, bs, nb)
+
+
+def mxfp4_paged_decode(out: torch.Tensor, q: torch.Tensor, k_cache: torch.Tensor,
+                       v_cache: torch.Tensor, k_scales: torch.Tensor, v_scales: torch.Tensor,
+                       block_table: torch.Tensor, cache_seqlens: torch.Tensor,
+                       softmax_scale: float, window_left: int = -1,
+                       sinks: torch.Tensor | None = None,
+                       cu_seqlens_q: torch.Tensor | None = None,
+                       max_seqlen_q: int | None = None) -> None:
+    """:func:`paged_decode` over a 4-bit cache into ``out`` ([rows, Hq, D] bf16): one query row
+    per sequence, or cu_seqlens_q [batch + 1] with at most max_seqlen_q (then required) per
+    sequence, its last tokens (row i of n sees the first cache_seqlens[b] - n + i + 1 keys, under a
+    window the last window_left + 1 of them).  sinks as in :func:`paged_decode`; a row that
+    sees no key is zero; rows behind the last sequence stay as they were."""
+    what = "mxfp4_paged_decode"
+    (rows, hq, d), q_stride = _check_rows(what, q, "q")
+    out_shape, out_stride = _check_rows(what, out, "out")
+    if out_shape != q.shape:
+        raise ValueError(f"{what}: out must have q's shape")
+    nb, hk, bs, d_cache = _check_mxfp4(what, k_cache, v_cache, k_scales, v_scales)
+    if d_cache != d or hk == 0 or hq % hk:
+        raise ValueError(f"{what}: {hq} query heads of {d} over {hk} kv heads of {d_cache}")
+    window_left = int(window_left)
+    if window_left < -1:
+        raise ValueError(f"{what}: window_left must be -1 (no window) or >= 0")
+    sink = _check_scale(what, sinks, "sinks", hq)
+    batch = _check_batch(what, cache_seqlens, cu_seqlens_q, rows)
+    most = _most_rows(what, cu_seqlens_q, max_seqlen_q)
+    bt_stride, bt_width = _check_table(what, block_table, batch)
+    dev = _same_device(out, q, k_cache, v_cache, k_scales, v_scales, block_table, cache_seqlens,
+                       sinks, cu_seqlens_q)
+    if rows == 0 or batch == 0:
+        return
+    nbytes = _plan_bytes(dev, _native.mxfp4_decode_bytes, batch, most, hq, hk, d)
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=q.device)
+    _call_on(q, dev, "fk_mxfp4_paged_decode", out.data_ptr(), out_stride, q.data_ptr(), q_stride,
+             k_cache.data_ptr(), v_cache.data_ptr(), k_scales.data_ptr(), v_scales.data_ptr(),
+             block_table.data_ptr(), bt_stride, bt_width, cache_seqlens.data_ptr(),
+             _ptr(cu_seqlens_q), batch, rows, most, hq, hk, d, bs, nb, float(softmax_scale),
+             window_left, sink, ws.data_ptr(), nbytes)
+
+
+# ---------------------------------------------------------------------------
+# Latent attention: keys and values from one row a token, which all heads share
+# ---------------------------------------------------------------------------
+_ROPE = 64  # dims of a latent row's rotary part
+
+
+def _check_latent(what, cache, scale) -> tuple[torch.Size, int, int | None]:
+    """(shape, dtype tag, scale's pointer) of a latent cache."""
+    shape = cache.shape
+    if len(shape) != 3 or not cache.is_contiguous():
+        raise ValueError(f"{what}: cache must be contiguous [num_blocks, block_size, latent + "
+                         "rope]")
+    if cache.dtype == torch.bfloat16:
+        tag = _native.FK_DTYPE_BF16
+    elif cache.dtype == _FP8:
+        tag = _native.FK_DTYPE_FP8_E4M3FN
+    else:
+        raise TypeError(f"{what}: cache must be bf16 or float8_e4m3fn")
+    return shape, tag, _check_scale(what, scale, "scale", 1)
+
+
+def _check_strided(what, t, name, shape) -> tuple[int, ...]:
+    """The strides of a bf16 tensor of this shape, contiguous along its last dimension."""
+    if t.dtype != torch.bfloat16 or t.shape != shape or t.stride(-1) != 1:
+        raise ValueError(f"{what}: {name} must be bf16 {list(shape)}, contiguous along the last "
+                         "dimension")
+    return t.stride()
+
+
+def latent_norm_rope_store(cache: torch.Tensor, slot_mapping: torch.Tensor,
+                           positions: torch.Tensor, latent: torch.Tensor,
+                           key_rope: torch.Tensor, cos_sin_cache: torch.Tensor, is_neox: bool,
+                           weight: torch.Tensor | None = None, eps: float = 1e-6,
+                           scale: torch.Tensor | None = None,
+                           query_rope: torch.Tensor | None = None,
+                           query_out: torch.Tensor | None = None,
+                           latent_out: torch.Tensor | None = None,
+                           key_rope_out: torch.Tensor | None = None) -> None:
+    """One launch for the steps between the projections and attention over a latent cache
+    ([num_blocks, block_size, latent + rope], bf16 or float8_e4m3fn): c = rmsnorm(latent) with
+    ``weight`` (without: latent as it is), k = key_rope rotated by ``positions``, the row [c | k]
+    (divided by ``scale``, float32 [1]) to slot_mapping[t] (-1 skips; otherwise distinct), and
+    query_out = query_rope rotated.
+
+    latent [N, R], key_rope [N, P], query_rope / query_out [N, H, P] are bf16, contiguous along the
+    last dimension: views of the projections' outputs and of the absorbed queries.  latent_out and
+    key_rope_out, if given, take c and k.  Every output may be its own input.  All of it is
+    computed in float32 and rounded once."""
+    what = "latent_norm_rope_store"
+    (nb, bs, width), tag, sp = _check_latent(what, cache, scale)
+    if latent.dim() != 2 or key_rope.dim() != 2:
+        raise ValueError(f"{what}: latent must be [N, R], key_rope [N, P]")
+    (n, r), p = latent.shape, key_rope.shape[1]
+    if width != r + p:
+        raise ValueError(f"{what}: rows of {r} + {p} into a cache of {width}")
+    ls = _check_strided(what, latent, "latent", (n, r))
+    ks = _check_strided(what, key_rope, "key_rope", (n, p))
+    if positions.dtype != torch.int64 or not positions.is_contiguous() or positions.numel() < n:
+        raise TypeError(f"{what}: positions must be contiguous int64 [N]")
+    if cos_sin_cache.dim() != 2 or cos_sin_cache.shape[1] != p or \
+            not cos_sin_cache.is_contiguous() or \
+            cos_sin_cache.dtype not in (torch.float32, torch.bfloat16):
+        raise ValueError(f"{what}: cos_sin_cache must be contiguous float32 or bf16 "
+                         f"[max_pos, {p}]")
+    if weight is not None and (weight.dtype != torch.bfloat16 or weight.shape != (r,) or
+                               not weight.is_contiguous()):
+        raise ValueError(f"{what}: weight must be contiguous bf16 [{r}]")
+    if (query_rope is None) != (query_out is None):
+        raise ValueError(f"{what}: pass both query_rope and query_out, or neither")
+    heads, qs, qos = 0, (0, 0), (0, 0)
+    if query_rope is not None:
+        heads = query_rope.shape[1] if query_rope.dim() == 3 else 0
+        qs = _check_strided(what, query_rope, "query_rope", (n, heads, p))
+        qos = _check_strided(what, query_out, "query_out", (n, heads, p))
+    los = (0,) if latent_out is None else _check_strided(what, latent_out, "latent_out", (n, r))
+    kos = (0,) if key_rope_out is None else \
+        _check_strided(what, key_rope_out, "key_rope_out", (n, p))
+    i64 = _check_slots(what, slot_mapping, n)
+    dev = _same_device(cache, slot_mapping, positions, latent, key_rope, cos_sin_cache, weight,
+                       scale, query_rope, query_out, latent_out, key_rope_out)
+    if n == 0:
+        return
+    _call_on(cache, dev, "fk_latent_norm_rope_store", cache.data_ptr(), tag, sp,
+             slot_mapping.data_ptr(), i64, nb * bs, positions.data_ptr(), latent.data_ptr(),
+             ls[0], key_rope.data_ptr(), ks[0], _ptr(weight), float(eps),
+             cos_sin_cache.data_ptr(), _tag(cos_sin_cache, what), cos_sin_cache.shape[0],
+             int(bool(is_neox)), _ptr(query_rope), qs[0], qs[1], heads, _ptr(query_out), qos[0],
+             qos[1], _ptr(latent_out), los[0], _ptr(key_rope_out), kos[0], n, r, p)
+
+
+def gather_latent(out: torch.Tensor, cache: torch.Tensor, block_table: torch.Tensor,
+                  cu_seqlens_k: torch.Tensor, scale: torch.Tensor | None = None) -> None:
+    """out (bf16 [rows, latent + rope]): row cu_seqlens_k[b] + i becomes the latent cache's row of
+    position i of sequence b (times ``scale``; zeros where block_table has no page); rows behind
+    the last sequence stay as they were.  What the expanded form projects up to the keys and values
+    of :func:`varlen_prefill` at head sizes 192 / 128."""
+    what = "gather_latent"
+    (nb, bs, width), tag, sp = _check_latent(what, cache, scale)
+    if out.dim() != 2 or out.shape[1] != width:
+        raise ValueError(f"{what}: out must be bf16 [rows, {width}]")
+    rows = out.shape[0]
+    stride = _check_strided(what, out, "out", (rows, width))
+    batch = _check_cu_k(what, cu_seqlens_k)
+    bt_stride, bt_width = _check_table(what, block_table, batch)
+    dev = _same_device(out, cache, block_table, cu_seqlens_k, scale)
+    if rows == 0 or batch == 0:
+        return
+    _call_on(out, dev, "fk_gather_latent", out.data_ptr(), stride[0], cache.data_ptr(), tag, sp,
+             block_table.data_ptr(), bt_stride, bt_width, cu_seqlens_k.data_ptr(), batch, rows,
+             width - _ROPE, _ROPE, bs, nb)
+
+
+def latent_decode(out: torch.Tensor, q: torch.Tensor, cache: torch.Tensor,
+                  block_table: torch.Tensor, cache_seqlens: torch.Tensor, softmax_scale: float,
+                  scale: torch.Tensor | None = None, cu_seqlens_q: torch.Tensor | None = None,
+                  max_seqlen_q: int | None = None, lse: torch.Tensor | None = None) -> None:
+    """Latent attention in the absorbed form: q [rows, H, latent + rope] (the queries projected to
+    the latent space, then their rotated parts) attends to the rows of the cache, whose first
+    ``latent`` dims are the values: out [rows, H, latent], both bf16 with any row and head strides.
+    ``scale`` (float32 [1]) is an fp8 cache's.  lse (float32 [H, rows]): the log-sum-exp of each
+    row's logits, -inf for a row without keys, for :func:`merge_attn_states`.
+
+    Rows: one per sequence, or cu_seqlens_q [batch + 1] with at most max_seqlen_q (then required)
+    per sequence, its last tokens (row i of n sees the first cache_seqlens[b] - n + i + 1 keys).  A
+    row that sees no key is zero; rows behind the last sequence stay as they were."""
+    what = "latent_decode"
+    (nb, bs, width), tag, sp = _check_latent(what, cache, scale)
+    if q.dim() != 3 or q.shape[2] != width:
+        raise ValueError(f"{what}: q must be bf16 [rows, H, {width}]")
+    rows, heads, _ = q.shape
+    qs = _check_strided(what, q, "q", (rows, heads, width))
+    os_ = _check_strided(what, out, "out", (rows, heads, width - _ROPE))
+    if lse is not None and (lse.dtype != torch.float32 or lse.shape != (heads, rows) or
+                            (rows > 1 and lse.stride(1) != 1)):
+        raise ValueError(f"{what}: lse must be float32 [{heads}, {rows}], contiguous along rows")
+    batch = _check_batch(what, cache_seqlens, cu_seqlens_q, rows)
+    most = _most_rows(what, cu_seqlens_q, max_seqlen_q)
+    bt_stride, bt_width = _check_table(what, block_table, batch)
+    dev = _same_device(out, q, cache, block_table, cache_seqlens, scale, cu_seqlens_q, lse)
+    if rows == 0 or batch == 0 or heads == 0:
+        return
+    nbytes = _plan_bytes(dev, _native.latent_decode_bytes, batch, most, heads, width - _ROPE)
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=q.device)
+    _call_on(q, dev, "fk_latent_decode", out.data_ptr(), os_[0], os_[1], q.data_ptr(), qs[0],
+             qs[1], cache.data_ptr(), tag, sp, block_table.data_ptr(), bt_stride, bt_width,
+             cache_seqlens.data_ptr(), _ptr(cu_seqlens_q), batch, rows, most, heads,
+             width - _ROPE, _ROPE, bs, nb, float(softmax_scale), _ptr(lse),
+             0 if lse is None else lse.stride(0), ws.data_ptr(), nbytes)
+
+
+# ---------------------------------------------------------------------------
 # torch.library registration (opaque custom ops with mutation annotations).
 # ---------------------------------------------------------------------------
 _LIB = torch.library.Library("fastkernels_amd", "DEF")
@@ -1054,6 +1364,26 @@ _LIB.define("shared_prefix_decode(Tensor(a!) out, Tensor q, Tensor k_cache, Tens
             "Tensor block_table, Tensor cache_seqlens, Tensor cu_groups, Tensor prefix_lens, "
             "float softmax_scale, Tensor? k_scale=None, Tensor? v_scale=None, "
             "int window_left=-1, Tensor? sinks=None, int max_prefix_len=0) -> ()")
+_LIB.define("store_kvcache_mxfp4(Tensor key, Tensor value, Tensor(a!) k_cache, "
+            "Tensor(b!) v_cache, Tensor(c!) k_scales, Tensor(d!) v_scales, Tensor slot_mapping) "
+            "-> ()")
+_LIB.define("gather_kvcache_mxfp4(Tensor(a!) key, Tensor(b!) value, Tensor k_cache, "
+            "Tensor v_cache, Tensor k_scales, Tensor v_scales, Tensor block_table, "
+            "Tensor cu_seqlens_k) -> ()")
+_LIB.define("mxfp4_paged_decode(Tensor(a!) out, Tensor q, Tensor k_cache, Tensor v_cache, "
+            "Tensor k_scales, Tensor v_scales, Tensor block_table, Tensor cache_seqlens, "
+            "float softmax_scale, int window_left=-1, Tensor? sinks=None, "
+            "Tensor? cu_seqlens_q=None, int? max_seqlen_q=None) -> ()")
+_LIB.define("latent_norm_rope_store(Tensor(a!) cache, Tensor slot_mapping, Tensor positions, "
+            "Tensor latent, Tensor key_rope, Tensor cos_sin_cache, bool is_neox, "
+            "Tensor? weight=None, float eps=1e-6, Tensor? scale=None, Tensor? query_rope=None, "
+            "Tensor(b!)? query_out=None, Tensor(c!)? latent_out=None, "
+            "Tensor(d!)? key_rope_out=None) -> ()")
+_LIB.define("gather_latent(Tensor(a!) out, Tensor cache, Tensor block_table, "
+            "Tensor cu_seqlens_k, Tensor? scale=None) -> ()")
+_LIB.define("latent_decode(Tensor(a!) out, Tensor q, Tensor cache, Tensor block_table, "
+            "Tensor cache_seqlens, float softmax_scale, Tensor? scale=None, "
+            "Tensor? cu_seqlens_q=None, int? max_seqlen_q=None, Tensor(b!)? lse=None) -> ()")
 
 _IMPLS = {
     "rmsnorm": lambda result, input, weight, eps: rms_norm(result, input, weight, eps),
@@ -1073,6 +1403,12 @@ _IMPLS = {
     "select_blocks": select_blocks,
     "sparse_paged_decode": sparse_paged_decode,
     "shared_prefix_decode": shared_prefix_decode,
+    "store_kvcache_mxfp4": store_kvcache_mxfp4,
+    "gather_kvcache_mxfp4": gather_kvcache_mxfp4,
+    "mxfp4_paged_decode": mxfp4_paged_decode,
+    "latent_norm_rope_store": latent_norm_rope_store,
+    "gather_latent": gather_latent,
+    "latent_decode": latent_decode,
 }
 for _name, _fn in _IMPLS.items():
     _LIB.impl(_name, _fn, "CUDA")

@@ -79,8 +79,9 @@ extern "C" {
 #define FK_VERSION_MAJOR 2
 /* 2.1: fk_prefill_split_plan, fk_paged_prefill_ws, fk_varlen_prefill_ws
  * 2.2: fk_paged_decode_shape, fk_prefill_shape
- * 2.3: attention that reads part of the cache (the section at the end) */
-#define FK_VERSION_MINOR 3
+ * 2.3: attention that reads part of the cache
+ * 2.4: the 4-bit cache and the latent cache (the sections at the end) */
+#define FK_VERSION_MINOR 4
 int fk_version(void);
 
 /* Message describing the last failing call on this thread ("" if none). */
@@ -558,6 +559,120 @@ int fk_shared_prefix_decode(void* out, int64_t out_row_stride, const void* q,
 int fk_shared_prefix_decode_plan(int64_t batch, int64_t num_groups, int64_t max_prefix_len,
                                  int num_heads, int num_kv_heads, int head_size,
                                  int64_t* workspace_bytes);
+
+/* A paged cache held in 4 bits (library version 2.4).  No counterpart in the reference.
+ *
+ * The format is OCP microscaling fp4: the values of a block (32 dims of one token and kv head)
+ * are a power of two 2^(E - 127) times e2m1 codes, {0, 0.5, 1, 1.5, 2, 3, 4, 6} with a sign; E is
+ * one byte, 255 makes the block NaN.  With D = head_size, of bytes:
+ *   k_cache   [num_blocks, Hk, block_size, D / 2]           two dims a byte, the even one low
+ *   v_cache   [num_blocks, Hk, block_size / 4, 16, 4, D / 32]
+ *             dims (D/16) i .. (D/16) (i + 1) - 1 of four tokens side by side
+ *   k_scales, v_scales  [num_blocks, Hk, D / 32, block_size]
+ * all 16-byte aligned.  head_size 64, 128 or 256; block_size a power of two >= 16.  Block tables
+ * and cu_seqlens_q as in the section above.
+ *
+ * fk_store_kvcache_mxfp4: key and value rows [tokens, Hk, D] of F32, F16 or BF16 (rows
+ * key_row_stride / value_row_stride elements apart) go to slot slot_mapping[t] = page *
+ * block_size + place (int32 or int64; skipped outside [0, num_blocks * block_size); distinct).
+ * A block's E is the exponent of its greatest magnitude, rounded to two significant bits, less
+ * 2 (at least 0); values are rounded to the nearest code, ties to the even one, so that none is
+ * off by more than half a step.  A block with an infinity or a NaN is NaN. */
+int fk_store_kvcache_mxfp4(const void* key, int64_t key_row_stride, const void* value,
+                           int64_t value_row_stride, int dtype, void* k_cache, void* v_cache,
+                           void* k_scales, void* v_scales, const void* slot_mapping,
+                           int slot_is_i64, int64_t tokens, int num_kv_heads, int head_size,
+                           int block_size, int64_t num_blocks, void* stream);
+
+/* Rows cu_seqlens_k[b] + i of key and value (bf16 [rows, Hk, D], row strides in elements,
+ * 16-byte aligned) = what the cache holds of position i of sequence b, exactly; zeros at masked
+ * pages.  cu_seqlens_k: int32 [batch + 1]; rows behind the last sequence are left as they
+ * were.  Dense keys for fk_varlen_prefill over a context that is held in 4 bits. */
+int fk_gather_kvcache_mxfp4(void* key, int64_t key_row_stride, void* value,
+                            int64_t value_row_stride, const void* k_cache, const void* v_cache,
+                            const void* k_scales, const void* v_scales,
+                            const int32_t* block_tables, int64_t bt_row_stride, int64_t bt_width,
+                            const int32_t* cu_seqlens_k, int64_t batch, int64_t rows,
+                            int num_kv_heads, int head_size, int block_size, int64_t num_blocks,
+                            void* stream);
+
+/* out[t, hq] = softmax attention of q[t, hq] (bf16 [rows, num_heads, D], heads contiguous) over
+ * the keys it sees: the last window_left + 1 (-1: all) of its sequence's first vis.  sinks as
+ * fk_paged_decode; a row that sees no key is zero.  Keys that a row does not see may hold
+ * anything.  rows and max_seqlen_q <= 65535. */
+int fk_mxfp4_paged_decode(void* out, int64_t out_row_stride, const void* q, int64_t q_row_stride,
+                          const void* k_cache, const void* v_cache, const void* k_scales,
+                          const void* v_scales, const int32_t* block_tables,
+                          int64_t bt_row_stride, int64_t bt_width, const int32_t* cache_seqlens,
+                          const int32_t* cu_seqlens_q, int64_t batch, int64_t rows,
+                          int64_t max_seqlen_q, int num_heads, int num_kv_heads, int head_size,
+                          int block_size, int64_t num_blocks, float scale, int window_left,
+                          const float* sinks, void* workspace, int64_t workspace_bytes,
+                          void* stream);
+
+/* Workspace bytes fk_mxfp4_paged_decode needs at these sizes (host only). */
+int fk_mxfp4_paged_decode_plan(int64_t batch, int64_t max_seqlen_q, int num_heads,
+                               int num_kv_heads, int head_size, int64_t* workspace_bytes);
+
+/* Attention with keys and values from one latent row a token (library version 2.4): the cache
+ * side of MLA (fastkernels/tasks/baseline/L2/mla_attention_impl.py).  The cache is
+ * [num_blocks, block_size, latent_size + rope_size] of BF16 or FP8_E4M3FN, 16-byte aligned;
+ * latent_size 512, rope_size 64; block_size a power of two >= 16.  cache_scale: device fp32
+ * scalar or NULL (1); a value is its code times the scale.  Block tables and cu_seqlens_q as in
+ * the section above.
+ *
+ * fk_latent_norm_rope_store: for each token t
+ *   c = latent[t] / sqrt(mean(latent[t]^2) + eps) * weight   (as it is with weight NULL),
+ *   k = key_rope[t] rotated by positions[t],   query_out[t, h] = query_rope[t, h] rotated alike
+ * (int64 positions; not rotated outside [0, max_position)); cos_sin [max_position, rope_size]: cos
+ * then sin, F32 or BF16; is_neox: pairs (i, i + rope_size / 2), else (2 i, 2 i + 1)), and the row
+ * [c | k] / cache_scale goes to slot slot_mapping[t] (int32 or int64; skipped outside
+ * [0, num_slots); distinct), fp8 rounded to nearest even and saturated at 448.  latent_out and
+ * key_out (or NULL) take c and k in bf16.  Everything is computed in fp32 and rounded once.
+ * Tensors are bf16 with rows and heads 16-byte aligned; each output may be its input.
+ * num_heads 0: no queries. */
+int fk_latent_norm_rope_store(void* cache, int cache_dtype, const float* cache_scale,
+                              const void* slot_mapping, int slot_is_i64, int64_t num_slots,
+                              const int64_t* positions, const void* latent,
+                              int64_t latent_row_stride, const void* key_rope,
+                              int64_t key_row_stride, const void* weight, float eps,
+                              const void* cos_sin, int cos_sin_dtype, int64_t max_position,
+                              int is_neox, const void* query_rope, int64_t q_row_stride,
+                              int64_t q_head_stride, int num_heads, void* query_out,
+                              int64_t qo_row_stride, int64_t qo_head_stride, void* latent_out,
+                              int64_t latent_out_row_stride, void* key_out,
+                              int64_t key_out_row_stride, int64_t tokens, int latent_size,
+                              int rope_size, void* stream);
+
+/* Row cu_seqlens_k[b] + i of out (bf16 [rows, latent_size + rope_size], 16-byte aligned) = the
+ * cache's row of position i of sequence b (times cache_scale); zeros at masked pages; rows behind
+ * the last sequence are left as they were.  What the expanded form projects up to keys and
+ * values (fk_varlen_prefill at head sizes 192 / 128). */
+int fk_gather_latent(void* out, int64_t out_row_stride, const void* cache, int cache_dtype,
+                     const float* cache_scale, const int32_t* block_tables,
+                     int64_t bt_row_stride, int64_t bt_width, const int32_t* cu_seqlens_k,
+                     int64_t batch, int64_t rows, int latent_size, int rope_size, int block_size,
+                     int64_t num_blocks, void* stream);
+
+/* The absorbed form: out[t, h] (bf16 [rows, num_heads, latent_size]) = sum_j w_j c_j, w the
+ * softmax of scale q[t, h] . [c_j | k_j] over the first vis keys of the row's sequence; q bf16
+ * [rows, num_heads, latent_size + rope_size].  Row and head strides in elements, 16-byte
+ * aligned.  lse (or NULL): fp32 [num_heads, rows], heads lse_head_stride apart: the natural log of
+ * the softmax's denominator.  A row that sees no key is zero, its lse -infinity.  Keys that a row
+ * does not see may hold anything.  batch, rows and max_seqlen_q <= 65535. */
+int fk_latent_decode(void* out, int64_t out_row_stride, int64_t out_head_stride, const void* q,
+                     int64_t q_row_stride, int64_t q_head_stride, const void* cache,
+                     int cache_dtype, const float* cache_scale, const int32_t* block_tables,
+                     int64_t bt_row_stride, int64_t bt_width, const int32_t* cache_seqlens,
+                     const int32_t* cu_seqlens_q, int64_t batch, int64_t rows,
+                     int64_t max_seqlen_q, int num_heads, int latent_size, int rope_size,
+                     int block_size, int64_t num_blocks, float scale, float* lse,
+                     int64_t lse_head_stride, void* workspace, int64_t workspace_bytes,
+                     void* stream);
+
+/* Workspace bytes fk_latent_decode needs at these sizes (host only). */
+int fk_latent_decode_plan(int64_t batch, int64_t max_seqlen_q, int num_heads, int latent_size,
+                          int64_t* workspace_bytes);
 
 #ifdef __cplusplus
 }
