@@ -39,14 +39,15 @@ struct LatentParams {
   float scale_log2;
   int num_heads;
   int head_blocks;  // units of 32 heads of a row
+  int units;        // of an item
   int batch, rows, most;
   int block_size_log2;
   int64_t num_blocks;
   int64_t bt_row_stride;
   int bt_width;
   int wgs;
-  float* o;         // [2 wgs][64][R]
-  float* ml;        // [2 wgs][64] (maximum, sum)
+  float* o;         // [2 wgs][32 units][R]
+  float* ml;        // [2 wgs][32 units] (maximum, sum)
   LineRecord* records;
 };
 
@@ -148,9 +149,33 @@ struct Halves {
   }
 };
 
-// A sequence on the line: items of two units (32 heads of a row) in steps of a tile.
+// O *= alpha, in place among the accumulators: the compiler would copy them out and back around
+// every step for it.  (The waits: vector instructions read a product's result 18 later at the
+// earliest, and products what those wrote 2 later.)
+template <int N>
+__device__ __forceinline__ void scale_acc(floatx16_t (&o)[N], float alpha) {
+#pragma unroll
+  for (int d = 0; d < N; ++d) {
+    asm volatile("s_nop 15\n\ts_nop 3" : "+a"(o[d]), "+v"(alpha));
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      float x = o[d][i], t;
+      asm volatile(
+          "v_accvgpr_read_b32 %1, %0\n\t"
+          "v_mul_f32 %1, %1, %2\n\t"
+          "v_accvgpr_write_b32 %0, %1"
+          : "+a"(x), "=&v"(t)
+          : "v"(alpha));
+      o[d][i] = x;
+    }
+    asm volatile("s_nop 3" : "+a"(o[d]));
+  }
+}
+
+// A sequence on the line: items of `units` units (32 heads of a row) in steps of a tile.
 __device__ __forceinline__ LineSeq line_seq(const LatentParams& P, const int32_t* __restrict__ cu,
-                                            const int32_t* __restrict__ ctx, int b) {
+                                            const int32_t* __restrict__ ctx, int b,
+                                            int units) {
   LineSeq x{};
   const SeqRows s = seq_rows(cu, ctx, b, P.rows, P.most);
   if (s.rows == 0) return x;
@@ -162,7 +187,7 @@ __device__ __forceinline__ LineSeq line_seq(const LatentParams& P, const int32_t
   x.row0 = s.row0;
   x.rows = s.rows;
   x.steps = x.to > 0 ? (x.to - 1) / kKeys + 1 : 1;
-  x.items = (s.rows * P.head_blocks + 1) / 2;
+  x.items = (s.rows * P.head_blocks + units - 1) / units;
   return x;
 }
 
@@ -177,29 +202,32 @@ __device__ __forceinline__ void write_out(const LatentParams& P, int64_t row, in
         L > 0.f ? (M + __builtin_amdgcn_logf(L)) * 0.6931471805599453f : L == 0.f ? kNegInf : L;
 }
 
-// One work-group: items of two units of 32 heads, or 64 columns, in steps of a tile.
+// One work-group: items of kUnits units of 32 heads (of one query row each), in steps of a tile.
 //
-// The waves share S by columns and keys, wave w = (cs, ts): the 32 columns of unit cs and keys
+// The waves share S by columns and keys, wave w = (cs, ts): half cs of the columns and keys
 // 16 ts .. 16 ts + 15 (16x16x32 products), and P V by dims: wave w has dims w R / 4 .. of every
 // column (32x32x16 products), so that V is read from LDS once and K twice.  P goes through LDS,
 // and so do the columns' maxima, of which every wave then makes the same reference.  While P V of
 // a step runs, so does S of the next: two barriers a step, A before both products and B behind
 // them.
-template <int R, int P, bool kFp8>
+template <int R, int P, int kUnits, bool kFp8>
 __global__ __launch_bounds__(kThreads)
 __attribute__((amdgpu_waves_per_eu(1, 1))) void latent_decode_kernel(
     LatentParams A, const int32_t* __restrict__ bt, const int32_t* __restrict__ ctx_lens,
     const int32_t* __restrict__ cu) {
   using T = Tile<R, P>;
-  constexpr int kCols = 64;
+  constexpr int kCols = 32 * kUnits;
+  constexpr int kCB = kUnits;                 // blocks of 16 columns of a wave's S
   constexpr int kKc = (R + P) / 32;           // products of S
   constexpr int kOb = R / 4 / 32;             // blocks of 32 dims of a wave
   constexpr int kMoves = T::kMoves / kWaves;  // of a wave and tile
   static_assert(T::kMoves / 2 % kMoves == 0, "a wave's moves are of one half");
+  constexpr int kGroup = 6;  // K operands read from LDS at a time
+  static_assert(kKc % kGroup == 0 && kOb % 2 == 0, "whole groups");
   __shared__ LineLds<kThreads> line;
   extern __shared__ __align__(16) uint8_t lds[];
-  uint8_t* const p_lds = lds + kBuffers * T::kBytes;       // [64 columns][32 keys] bf16
-  float* const tops = reinterpret_cast<float*>(p_lds + kCols * kKeys * 2);  // [2][64]
+  uint8_t* const p_lds = lds + kBuffers * T::kBytes;       // [columns][32 keys] bf16
+  float* const tops = reinterpret_cast<float*>(p_lds + kCols * kKeys * 2);  // [2][columns]
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int lane = threadIdx.x & 63;
   const int r = lane & 15, g = lane >> 4;   // S
@@ -223,28 +251,30 @@ __attribute__((amdgpu_waves_per_eu(1, 1))) void latent_decode_kernel(
 
   auto body = [&](int b, const LineSeq& x, int it, int s_lo, int s_hi, int64_t slot) {
     const SeqRows sr = seq_rows(cu, ctx_lens, b, A.rows, A.most);
-    const int unit0 = it * 2;
-    const bool two = unit0 + 1 < x.rows * A.head_blocks;
-    // Row, first head and visible keys of both units.
-    int row_i[2], head0[2], hi[2];
+    // Row, first head and visible keys of the units; one that there is not has no heads.
+    int row_i[kUnits], head0[kUnits], hi[kUnits];
 #pragma unroll
-    for (int u = 0; u < 2; ++u) {
-      const int unit = two ? unit0 + u : unit0;
+    for (int u = 0; u < kUnits; ++u) {
+      const int unit = min(it * kUnits + u, x.rows * A.head_blocks - 1);
       int none;
       row_i[u] = unit / A.head_blocks;
-      head0[u] = 32 * (unit - row_i[u] * A.head_blocks);
+      head0[u] = it * kUnits + u > unit ? A.num_heads
+                                        : 32 * (unit - row_i[u] * A.head_blocks);
       row_keys(sr, row_i[u], -1, none, hi[u]);
       hi[u] = uniform(hi[u]);
     }
-    const int all_hi = min(hi[0], hi[1]), my_hi = cs ? hi[1] : hi[0];
-    const bool active = cs == 0 || two;
-    bf16x8_t qb[2][kKc];
+    const int all_hi = min(hi[0], hi[kUnits - 1]);
+    const int su = kUnits == 2 ? cs : 0;  // unit of S's columns
+    const int my_hi = su ? hi[kUnits - 1] : hi[0];
+    const int s_col = 16 * kCB * cs + r;  // first of S's columns
+    bf16x8_t qb[kCB][kKc];
 #pragma unroll
-    for (int cb = 0; cb < 2; ++cb) {
-      const int h = (cs ? head0[1] : head0[0]) + 16 * cb + r;
+    for (int cb = 0; cb < kCB; ++cb) {
+      const int h = (su ? head0[kUnits - 1] : head0[0]) + (s_col + 16 * cb) % 32;
       const bool ok = h < A.num_heads;
-      const uint16_t* const qp = A.q + (x.row0 + (cs ? row_i[1] : row_i[0])) * A.q_row_stride +
-                                 (ok ? h : 0) * A.q_head_stride + 8 * g;
+      const uint16_t* const qp =
+          A.q + (x.row0 + (su ? row_i[kUnits - 1] : row_i[0])) * A.q_row_stride +
+          (ok ? h : 0) * A.q_head_stride + 8 * g;
 #pragma unroll
       for (int k = 0; k < kKc; ++k) {
         uint4 v = ok ? *reinterpret_cast<const uint4*>(qp + 32 * k) : make_uint4(0, 0, 0, 0);
@@ -252,16 +282,20 @@ __attribute__((amdgpu_waves_per_eu(1, 1))) void latent_decode_kernel(
         qb[cb][k] = __builtin_bit_cast(bf16x8_t, v);
       }
     }
-    floatx16_t o[2][kOb];  // of unit u: dims 32 d + i % 4 + 8 (i / 4) + 4 kh, column n
+    floatx16_t o[kUnits][kOb];  // dims 32 d + i % 4 + 8 (i / 4) + 4 kh of column n of unit u
 #pragma unroll
-    for (int u = 0; u < 2; ++u)
+    for (int u = 0; u < kUnits; ++u)
 #pragma unroll
       for (int d = 0; d < kOb; ++d)
 #pragma unroll
         for (int i = 0; i < 16; ++i) o[u][d][i] = 0.f;
-    // The reference maxima of S's columns (16 cb + r of unit cs), of O's (n of unit u), and this
-    // lane's share of S's columns' sums.
-    float ms[2] = {kNoMax, kNoMax}, mo[2] = {kNoMax, kNoMax}, l[2] = {0.f, 0.f};
+    // The reference maxima of S's columns, of O's, and this lane's share of S's columns' sums.
+    float ms[kCB], mo[kUnits], l[kCB];
+#pragma unroll
+    for (int u = 0; u < kUnits; ++u) {
+      ms[u] = mo[u] = kNoMax;
+      l[u] = 0.f;
+    }
 
     const Halves keys{A.cache, (R + P) * (kFp8 ? 1 : 2), bt + b * A.bt_row_stride, A.bt_width,
                       A.block_size_log2, A.num_blocks};
@@ -307,118 +341,157 @@ __attribute__((amdgpu_waves_per_eu(1, 1))) void latent_decode_kernel(
     // Whether every column sees all keys of step s.
     auto whole = [&](int s) { return (s_lo + s + 1) * kKeys <= all_hi && halves_of(s) == 3; };
 
-    floatx4_t p[2];
-    // S of step s, and its columns' maxima.
+    floatx4_t p[kCB];
+    // S of step s, and its columns' maxima.  Operands come in groups, one ahead of the products.
+    // Piece 4 k + g of a row: of its place, k / 2 moves it by 128 bytes, k % 2 by a permutation.
+    const uint32_t k_at[2] = {static_cast<uint32_t>(T::at(16 * ts + r, g)),
+                              static_cast<uint32_t>(T::at(16 * ts + r, 4 + g))};
     auto scores = [&](int s, auto is_masked) {
       const uint8_t* const tile = lds + (s % kBuffers) * T::kBytes;
+      const uint8_t* const at[2] = {tile + k_at[0], tile + k_at[1]};
+      uint4 kx[2][kGroup];
 #pragma unroll
-      for (int cb = 0; cb < 2; ++cb) p[cb] = floatx4_t{0.f, 0.f, 0.f, 0.f};
+      for (int j = 0; j < kGroup; ++j)
+        kx[0][j] = *reinterpret_cast<const uint4*>(at[j & 1] + 128 * (j >> 1));
 #pragma unroll
-      for (int k = 0; k < kKc; ++k) {
-        const uint4 a = *reinterpret_cast<const uint4*>(tile + T::at(16 * ts + r, 4 * k + g));
+      for (int cb = 0; cb < kCB; ++cb) p[cb] = floatx4_t{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-        for (int cb = 0; cb < 2; ++cb)
-          p[cb] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, a),
-                                                          qb[cb][k], p[cb], 0, 0, 0);
+      for (int k0 = 0; k0 < kKc; k0 += kGroup) {
+        const int now = k0 / kGroup & 1;
+        if (k0 + kGroup < kKc) {
+#pragma unroll
+          for (int j = 0; j < kGroup; ++j)
+            kx[now ^ 1][j] = *reinterpret_cast<const uint4*>(at[j & 1] +
+                                                             128 * ((k0 + kGroup + j) >> 1));
+        }
+        loads_issued();
+#pragma unroll
+        for (int j = 0; j < kGroup; ++j)
+#pragma unroll
+          for (int cb = 0; cb < kCB; ++cb)
+            p[cb] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(
+                __builtin_bit_cast(bf16x8_t, kx[now][j]), qb[cb][k0 + j], p[cb], 0, 0, 0);
       }
-      p[0] *= abs_s2;
-      p[1] *= abs_s2;
+#pragma unroll
+      for (int cb = 0; cb < kCB; ++cb) p[cb] *= abs_s2;
       if constexpr (decltype(is_masked)::value) {
         const int t0 = (s_lo + s) * kKeys + 16 * ts + 4 * g;
         const bool there_ = halves_of(s) >> ts & 1;
 #pragma unroll
-        for (int cb = 0; cb < 2; ++cb)
+        for (int cb = 0; cb < kCB; ++cb)
 #pragma unroll
           for (int i = 0; i < 4; ++i)
             if (!(there_ && t0 + i < my_hi)) p[cb][i] = kNegInf;
       }
 #pragma unroll
-      for (int cb = 0; cb < 2; ++cb) {
+      for (int cb = 0; cb < kCB; ++cb) {
         const float top =
             pair_max(fmaxf(fmaxf(p[cb][0], p[cb][1]), fmaxf(p[cb][2], p[cb][3])));
-        if (g == 0) tops[64 * ts + 32 * cs + 16 * cb + r] = top;
+        if (g == 0) tops[kCols * ts + s_col + 16 * cb] = top;
       }
     };
     // The references, moved where they have to be; weights from p, into LDS.
     auto weights = [&] {
-      float t[2];
+      float t[kUnits];
       bool move = false;
 #pragma unroll
-      for (int u = 0; u < 2; ++u) {
-        t[u] = fmaxf(tops[32 * u + n], tops[64 + 32 * u + n]);
-        move |= (u == 0 || two) && t[u] > mo[u] + kLazyMax;
+      for (int u = 0; u < kUnits; ++u) {
+        t[u] = fmaxf(tops[32 * u + n], tops[kCols + 32 * u + n]);
+        move |= t[u] > mo[u] + kLazyMax;
       }
       if (__ballot(move) != 0) {
 #pragma unroll
-        for (int u = 0; u < 2; ++u) {
+        for (int u = 0; u < kUnits; ++u) {
           const float m_new = fmaxf(mo[u], t[u]);
-          const float alpha = __builtin_amdgcn_exp2f(mo[u] - m_new);
+          scale_acc(o[u], __builtin_amdgcn_exp2f(mo[u] - m_new));
           mo[u] = m_new;
-#pragma unroll
-          for (int d = 0; d < kOb; ++d)
-#pragma unroll
-            for (int i = 0; i < 16; ++i) o[u][d][i] *= alpha;
         }
 #pragma unroll
-        for (int cb = 0; cb < 2; ++cb) {
-          const int c = 32 * cs + 16 * cb + r;
-          const float m_new = fmaxf(ms[cb], fmaxf(tops[c], tops[64 + c]));
+        for (int cb = 0; cb < kCB; ++cb) {
+          const int c = s_col + 16 * cb;
+          const float m_new = fmaxf(ms[cb], fmaxf(tops[c], tops[kCols + c]));
           l[cb] *= __builtin_amdgcn_exp2f(ms[cb] - m_new);
           ms[cb] = m_new;
         }
       }
-      if (!active) return;
       // The weights are rounded to bf16 for P V (2^-9 relative at most, of either sign); their
       // sum is of the unrounded ones.
 #pragma unroll
-      for (int cb = 0; cb < 2; ++cb) {
+      for (int cb = 0; cb < kCB; ++cb) {
         float e[4];
 #pragma unroll
         for (int i = 0; i < 4; ++i) e[i] = __builtin_amdgcn_exp2f(p[cb][i] - ms[cb]);
         l[cb] += (e[0] + e[1]) + (e[2] + e[3]);
-        *reinterpret_cast<uint2*>(p_at(32 * cs + 16 * cb + r, 16 * ts + 4 * g)) =
+        *reinterpret_cast<uint2*>(p_at(s_col + 16 * cb, 16 * ts + 4 * g)) =
             make_uint2(pack2(e[0], e[1]), pack2(e[2], e[3]));
       }
     };
     // O += P V of step s.  Operands of 16 keys (k): lane (n, kh) has keys 16 k + 8 kh .. + 7.  In
-    // a transpose load, lane 4 a + q of each 16 addresses key a and dims 4 q .. 4 q + 3.
+    // a transpose load, lane 4 a + q of each 16 addresses key a and dims 4 q .. 4 q + 3; block d's
+    // place in a row moves by 128 bytes with d / 2 and by a permutation with d % 2.
+    uint32_t v_at[2][2];
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+#pragma unroll
+      for (int d = 0; d < 2; ++d)
+        v_at[h][d] = 8 * (lane & 1) +
+                     T::at(8 * kh + 4 * h + (r >> 2),
+                           wave * (R / 32) + 4 * d + 2 * (g & 1) + ((lane & 3) >> 1));
+    const uint8_t* const p_from = p_at(n, 8 * kh);  // keys 16 on: pieces 2 on, of four, permuted
+    const int p_next = 32 - 64 * (((kh ^ (n >> 2)) & 3) >> 1);
     auto values = [&](int s, auto is_masked) {
       constexpr bool kMasked = decltype(is_masked)::value;
       const uint8_t* const tile = lds + (s % kBuffers) * T::kBytes;
-      const int a4 = r >> 2, piece = wave * (R / 32) + 2 * (g & 1) + ((lane & 3) >> 1);
+      const uint8_t* const at[2][2] = {{tile + v_at[0][0], tile + v_at[0][1]},
+                                       {tile + v_at[1][0], tile + v_at[1][1]}};
+      auto v_operand = [&](int x) {  // keys 16 (x / kOb) on, block x % kOb
+        const int k = x / kOb, d = x % kOb;
+        const int off = 16 * k * T::kRow + 128 * (d >> 1);
+        return joined(transposed(at[0][d & 1] + off), transposed(at[1][d & 1] + off));
+      };
+      bf16x8_t w[2][kUnits];
 #pragma unroll
-      for (int k = 0; k < 2; ++k) {
-        bf16x8_t w[2];
+      for (int k = 0; k < 2; ++k)
 #pragma unroll
-        for (int u = 0; u < 2; ++u)
-          w[u] = __builtin_bit_cast(
-              bf16x8_t, *reinterpret_cast<const uint4*>(p_at(32 * u + n, 16 * k + 8 * kh)));
-        // Keys that the row does not see may hold anything, infinities and NaN among it: zeros.
-        uint32_t mask[2][4];
-        if constexpr (kMasked) {
-          const uint32_t halves = halves_of(s);
+        for (int u = 0; u < kUnits; ++u)
+          w[k][u] = __builtin_bit_cast(
+              bf16x8_t, *reinterpret_cast<const uint4*>(p_from + 64 * 32 * u + k * p_next));
+      // Keys that the row does not see may hold anything, infinities and NaN among it: zeros.
+      uint32_t mask[2][kUnits][4];
+      if constexpr (kMasked) {
+        const uint32_t halves = halves_of(s);
 #pragma unroll
-          for (int u = 0; u < 2; ++u) {
+        for (int k = 0; k < 2; ++k)
+#pragma unroll
+          for (int u = 0; u < kUnits; ++u) {
             uint32_t bits = 0;
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
               const int t = (s_lo + s) * kKeys + 16 * k + 8 * kh + i;
               bits |= (halves >> k & 1) && t < hi[u] ? 1u << i : 0u;
             }
-            word_masks(bits, mask[u]);
+            word_masks(bits, mask[k][u]);
           }
-        }
-        const int row = 16 * k + 8 * kh + a4;
+      }
+      constexpr int kVGroup = 2;
+      bf16x8_t v[2][kVGroup];
 #pragma unroll
-        for (int d = 0; d < kOb; ++d) {
-          const uint8_t* const at = tile + 8 * (lane & 1);
-          const bf16x8_t v = joined(transposed(at + T::at(row, 4 * d + piece)),
-                                    transposed(at + T::at(row + 4, 4 * d + piece)));
-          o[0][d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kMasked ? masked(v, mask[0]) : v, w[0],
-                                                            o[0][d], 0, 0, 0);
-          if (two)
-            o[1][d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kMasked ? masked(v, mask[1]) : v,
-                                                              w[1], o[1][d], 0, 0, 0);
+      for (int j = 0; j < kVGroup; ++j) v[0][j] = v_operand(j);
+#pragma unroll
+      for (int x0 = 0; x0 < 2 * kOb; x0 += kVGroup) {
+        const int now = x0 / kVGroup & 1;
+        if (x0 + kVGroup < 2 * kOb) {
+#pragma unroll
+          for (int j = 0; j < kVGroup; ++j) v[now ^ 1][j] = v_operand(x0 + kVGroup + j);
+        }
+        loads_issued();
+#pragma unroll
+        for (int j = 0; j < kVGroup; ++j) {
+          const int k = (x0 + j) / kOb, d = (x0 + j) % kOb;
+#pragma unroll
+          for (int u = 0; u < kUnits; ++u)
+            o[u][d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(
+                kMasked ? masked(v[now][j], mask[k][u]) : v[now][j], w[k][u], o[u][d], 0, 0, 0);
         }
       }
     };
@@ -438,7 +511,7 @@ __attribute__((amdgpu_waves_per_eu(1, 1))) void latent_decode_kernel(
       wait_loads<(kBuffers - 1) * kMoves>();
     }
     __syncthreads();
-    if (active) scores(0, std::true_type{});
+    scores(0, std::true_type{});
     __syncthreads();
     weights();
     auto step = [&](int s, auto is_masked) {
@@ -446,7 +519,7 @@ __attribute__((amdgpu_waves_per_eu(1, 1))) void latent_decode_kernel(
       __syncthreads();  // A: step s's weights and step s + 1's tile are in LDS
       values(s, is_masked);
       if (s + 1 >= steps) return;
-      if (active) scores(s + 1, is_masked);
+      scores(s + 1, is_masked);
       __syncthreads();  // B: the maxima are in LDS, step s's tile and weights have been read
       if constexpr (kFp8) {
         put(s + 2, raw);
@@ -466,16 +539,16 @@ __attribute__((amdgpu_waves_per_eu(1, 1))) void latent_decode_kernel(
 
     // The columns' sums, of both waves and all lanes that have keys of theirs.
 #pragma unroll
-    for (int cb = 0; cb < 2; ++cb) {
+    for (int cb = 0; cb < kCB; ++cb) {
       l[cb] = pair_sum(l[cb]);
-      if (g == 0) tops[64 * ts + 32 * cs + 16 * cb + r] = l[cb];
+      if (g == 0) tops[kCols * ts + s_col + 16 * cb] = l[cb];
     }
     __syncthreads();
 #pragma unroll
-    for (int u = 0; u < 2; ++u) {
+    for (int u = 0; u < kUnits; ++u) {
       const int c = 32 * u + n, head = head0[u] + n;
-      if ((u == 1 && !two) || head >= A.num_heads) continue;
-      const float L = tops[c] + tops[64 + c];
+      if (head >= A.num_heads) continue;
+      const float L = tops[c] + tops[kCols + c];
       float* const po = A.o + (slot * kCols + c) * R;
       if (slot >= 0 && wave == 0 && kh == 0)
         *reinterpret_cast<float2*>(A.ml + (slot * kCols + c) * 2) = make_float2(mo[u], L);
@@ -495,7 +568,7 @@ __attribute__((amdgpu_waves_per_eu(1, 1))) void latent_decode_kernel(
     __syncthreads();
   };
   walk_line<kThreads>(line, A.batch, A.wgs, blockIdx.x, 1, A.records,
-                      [&](int b) { return line_seq(A, cu, ctx_lens, b); }, body);
+                      [&](int b) { return line_seq(A, cu, ctx_lens, b, kUnits); }, body);
 }
 
 // One work-group per (query row, some of its heads): merges the pieces of an item that ranges cut.
@@ -516,14 +589,14 @@ __global__ __launch_bounds__(kMergeThreads) void latent_merge_kernel(
   // Unit by unit of the row's heads.
   for (int h = h0; h < h1;) {
     const int unit = i * A.head_blocks + h / 32;
-    const int in = 32 * (unit & 1) + h % 32;
+    const int in = 32 * (unit % A.units) + h % 32;
     const int nc = min(h1, (h / 32 + 1) * 32) - h;
-    const LinePieces pieces(rec, unit >> 1);
+    const LinePieces pieces(rec, unit / A.units);
     if (pieces.n > 1) {
       merge_pieces<R>(
           0, nc, folded, [&](int) { return pieces.n; },
           [&](int k, int x, const float*& ml, const float*& o) {
-            const int64_t at = pieces.slot(k) * 64 + in + x;
+            const int64_t at = pieces.slot(k) * (32 * A.units) + in + x;
             ml = A.ml + 2 * at;
             o = A.o + at * R;
           },
@@ -537,19 +610,20 @@ __global__ __launch_bounds__(kMergeThreads) void latent_merge_kernel(
 }
 
 struct LatentPlan {
-  int wgs;
+  int wgs, units;
   int64_t o, ml, records, bytes;
 };
-LatentPlan plan_of(int64_t batch, int latent_size) {
+LatentPlan plan_of(int64_t batch, int64_t max_seqlen_q, int num_heads, int latent_size) {
   LatentPlan p{};
+  p.units = max_seqlen_q * ((num_heads + 31) / 32) > 1 ? 2 : 1;
   p.wgs = num_cus();
   auto take = [&](int64_t bytes) {
     const int64_t at = p.bytes;
     p.bytes += (bytes + 255) / 256 * 256;
     return at;
   };
-  p.o = take(int64_t{2} * p.wgs * 64 * latent_size * 4);
-  p.ml = take(int64_t{2} * p.wgs * 64 * 8);
+  p.o = take(int64_t{2} * p.wgs * 32 * p.units * latent_size * 4);
+  p.ml = take(int64_t{2} * p.wgs * 32 * p.units * 8);
   p.records = take(batch * static_cast<int64_t>(sizeof(LineRecord)));
   return p;
 }
@@ -557,9 +631,13 @@ LatentPlan plan_of(int64_t batch, int latent_size) {
 template <int R, int P, bool kFp8>
 void launch(const LatentParams& A, hipStream_t s, const int32_t* bt, const int32_t* ctx,
             const int32_t* cu) {
-  const unsigned lds = kBuffers * Tile<R, P>::kBytes + 64 * kKeys * 2 + 2 * 64 * 4;
-  hipLaunchKernelGGL((latent_decode_kernel<R, P, kFp8>), dim3(A.wgs + 1), dim3(kThreads), lds, s,
-                     A, bt, ctx, cu);
+  const unsigned lds = kBuffers * Tile<R, P>::kBytes + 32 * A.units * (kKeys * 2 + 2 * 4);
+  if (A.units == 1)
+    hipLaunchKernelGGL((latent_decode_kernel<R, P, 1, kFp8>), dim3(A.wgs + 1), dim3(kThreads),
+                       lds, s, A, bt, ctx, cu);
+  else
+    hipLaunchKernelGGL((latent_decode_kernel<R, P, 2, kFp8>), dim3(A.wgs + 1), dim3(kThreads),
+                       lds, s, A, bt, ctx, cu);
   const int heads = merge_cols(A.rows, 1, A.num_heads);
   hipLaunchKernelGGL((latent_merge_kernel<R>), dim3((A.num_heads + heads - 1) / heads, A.rows),
                      dim3(kMergeThreads), 0, s, A, ctx, cu, heads, kFp8 ? 1 : 0);
@@ -604,7 +682,7 @@ extern "C" int fk_latent_decode(void* out, int64_t out_row_stride, int64_t out_h
   if (batch == 0 || rows == 0) return FK_OK;
   FK_REQUIRE(out && q && cache && block_tables && cache_seqlens, "%s: null pointer", what);
   if (!cu_seqlens_q) max_seqlen_q = 1;
-  const LatentPlan plan = plan_of(batch, latent_size);
+  const LatentPlan plan = plan_of(batch, max_seqlen_q, num_heads, latent_size);
   if (workspace_bytes < plan.bytes || !workspace)
     return set_error(FK_ERR_WORKSPACE, "%s: workspace of %lld bytes, %lld needed", what,
                      static_cast<long long>(workspace_bytes), static_cast<long long>(plan.bytes));
@@ -632,6 +710,7 @@ extern "C" int fk_latent_decode(void* out, int64_t out_row_stride, int64_t out_h
   A.bt_width = static_cast<int>(bt_width);
   A.wgs = plan.wgs;
   A.head_blocks = (num_heads + 31) / 32;
+  A.units = plan.units;
   A.o = reinterpret_cast<float*>(ws + plan.o);
   A.ml = reinterpret_cast<float*>(ws + plan.ml);
   A.records = reinterpret_cast<LineRecord*>(ws + plan.records);
@@ -649,6 +728,6 @@ extern "C" int fk_latent_decode_plan(int64_t batch, int64_t max_seqlen_q, int nu
   FK_REQUIRE(batch >= 0 && batch <= 65535 && max_seqlen_q >= 1 && max_seqlen_q <= 65535 &&
                  num_heads > 0 && num_heads <= 65535 && latent_size > 0 && latent_size <= 65536,
              "fk_latent_decode_plan: invalid argument");
-  *workspace_bytes = batch == 0 ? 0 : plan_of(batch, latent_size).bytes;
+  *workspace_bytes = batch == 0 ? 0 : plan_of(batch, max_seqlen_q, num_heads, latent_size).bytes;
   return FK_OK;
 }
