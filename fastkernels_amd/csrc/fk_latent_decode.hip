@@ -172,20 +172,16 @@ __device__ __forceinline__ void scale_acc(floatx16_t (&o)[N], float alpha) {
   }
 }
 
-// A sequence on the line: items of `units` units (32 heads of a row) in steps of a tile.
-__device__ __forceinline__ LineSeq line_seq(const LatentParams& P, const int32_t* __restrict__ cu,
-                                            const int32_t* __restrict__ ctx, int b,
-                                            int units) {
-  LineSeq x{};
-  const SeqRows s = seq_rows(cu, ctx, b, P.rows, P.most);
-  if (s.rows == 0) return x;
+// A sequence's items: `units` units (32 heads of a row) each, in steps of a tile.
+__device__ __forceinline__ LineItems line_items(const LatentParams& P, const SeqRows& s,
+                                                int units) {
+  LineItems x;
   int none;
+  x.from = 0;
   row_keys(s, s.rows - 1, -1, none, x.to);
   // (past the table's end there is nothing to see)
   x.to = static_cast<int>(min(min(static_cast<int64_t>(x.to), int64_t{0x7fffff00}),
                               static_cast<int64_t>(P.bt_width) << P.block_size_log2));
-  x.row0 = s.row0;
-  x.rows = s.rows;
   x.steps = x.to > 0 ? (x.to - 1) / kKeys + 1 : 1;
   x.items = (s.rows * P.head_blocks + units - 1) / units;
   return x;
@@ -207,9 +203,12 @@ __device__ __forceinline__ void write_out(const LatentParams& P, int64_t row, in
 // The waves share S by columns and keys, wave w = (cs, ts): half cs of the columns and keys
 // 16 ts .. 16 ts + 15 (16x16x32 products), and P V by dims: wave w has dims w R / 4 .. of every
 // column (32x32x16 products), so that V is read from LDS once and K twice.  P goes through LDS,
-// and so do the columns' maxima, of which every wave then makes the same reference.  While P V of
-// a step runs, so does S of the next: two barriers a step, A before both products and B behind
-// them.
+// and so do the columns' maxima.
+//
+// A step has one barrier.  Behind it come S of the next step and P V of this one, with the next
+// step's softmax among the products of the latter: its weights are made with the reference maxima
+// as they are, and only where the maxima, which are all known behind the next barrier, ask for
+// others is P made again.
 template <int R, int P, int kUnits, bool kFp8>
 __global__ __launch_bounds__(kThreads)
 __attribute__((amdgpu_waves_per_eu(1, 1))) void latent_decode_kernel(
@@ -222,12 +221,14 @@ __attribute__((amdgpu_waves_per_eu(1, 1))) void latent_decode_kernel(
   constexpr int kOb = R / 4 / 32;             // blocks of 32 dims of a wave
   constexpr int kMoves = T::kMoves / kWaves;  // of a wave and tile
   static_assert(T::kMoves / 2 % kMoves == 0, "a wave's moves are of one half");
-  constexpr int kGroup = 6;  // K operands read from LDS at a time
+  constexpr int kGroup = kFp8 && kUnits == 2 ? 2 : 3;  // K operands read from LDS at a time
   static_assert(kKc % kGroup == 0 && kOb % 2 == 0, "whole groups");
   __shared__ LineLds<kThreads> line;
   extern __shared__ __align__(16) uint8_t lds[];
-  uint8_t* const p_lds = lds + kBuffers * T::kBytes;       // [columns][32 keys] bf16
-  float* const tops = reinterpret_cast<float*>(p_lds + kCols * kKeys * 2);  // [2][columns]
+  uint8_t* const p_lds = lds + kBuffers * T::kBytes;  // of two steps, [columns][32 keys] bf16
+  constexpr int kP = kCols * kKeys * 2;
+  // [two steps][2 halves of the keys][columns]
+  float* const tops = reinterpret_cast<float*>(p_lds + 2 * kP);
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int lane = threadIdx.x & 63;
   const int r = lane & 15, g = lane >> 4;   // S
@@ -249,13 +250,13 @@ __attribute__((amdgpu_waves_per_eu(1, 1))) void latent_decode_kernel(
     return p_lds + col * 64 + 16 * (((key >> 3) ^ (col >> 2)) & 3) + 2 * (key & 7);
   };
 
-  auto body = [&](int b, const LineSeq& x, int it, int s_lo, int s_hi, int64_t slot) {
-    const SeqRows sr = seq_rows(cu, ctx_lens, b, A.rows, A.most);
+  auto body = [&](int b, const SeqRows& sr, const LineItems& x, int it, int s_lo, int s_hi,
+                  int64_t slot) {
     // Row, first head and visible keys of the units; one that there is not has no heads.
     int row_i[kUnits], head0[kUnits], hi[kUnits];
 #pragma unroll
     for (int u = 0; u < kUnits; ++u) {
-      const int unit = min(it * kUnits + u, x.rows * A.head_blocks - 1);
+      const int unit = min(it * kUnits + u, sr.rows * A.head_blocks - 1);
       int none;
       row_i[u] = unit / A.head_blocks;
       head0[u] = it * kUnits + u > unit ? A.num_heads
@@ -267,21 +268,6 @@ __attribute__((amdgpu_waves_per_eu(1, 1))) void latent_decode_kernel(
     const int su = kUnits == 2 ? cs : 0;  // unit of S's columns
     const int my_hi = su ? hi[kUnits - 1] : hi[0];
     const int s_col = 16 * kCB * cs + r;  // first of S's columns
-    bf16x8_t qb[kCB][kKc];
-#pragma unroll
-    for (int cb = 0; cb < kCB; ++cb) {
-      const int h = (su ? head0[kUnits - 1] : head0[0]) + (s_col + 16 * cb) % 32;
-      const bool ok = h < A.num_heads;
-      const uint16_t* const qp =
-          A.q + (x.row0 + (su ? row_i[kUnits - 1] : row_i[0])) * A.q_row_stride +
-          (ok ? h : 0) * A.q_head_stride + 8 * g;
-#pragma unroll
-      for (int k = 0; k < kKc; ++k) {
-        uint4 v = ok ? *reinterpret_cast<const uint4*>(qp + 32 * k) : make_uint4(0, 0, 0, 0);
-        v = make_uint4(v.x ^ flip, v.y ^ flip, v.z ^ flip, v.w ^ flip);
-        qb[cb][k] = __builtin_bit_cast(bf16x8_t, v);
-      }
-    }
     floatx16_t o[kUnits][kOb];  // dims 32 d + i % 4 + 8 (i / 4) + 4 kh of column n of unit u
 #pragma unroll
     for (int u = 0; u < kUnits; ++u)
@@ -289,12 +275,13 @@ __attribute__((amdgpu_waves_per_eu(1, 1))) void latent_decode_kernel(
       for (int d = 0; d < kOb; ++d)
 #pragma unroll
         for (int i = 0; i < 16; ++i) o[u][d][i] = 0.f;
-    // The reference maxima of S's columns, of O's, and this lane's share of S's columns' sums.
-    float ms[kCB], mo[kUnits], l[kCB];
+    // The reference maxima of S's columns, of O's, this lane's share of S's columns' sums, and of
+    // that the last step's.
+    float ms[kCB], mo[kUnits], l[kCB], last[kCB];
 #pragma unroll
     for (int u = 0; u < kUnits; ++u) {
       ms[u] = mo[u] = kNoMax;
-      l[u] = 0.f;
+      l[u] = last[u] = 0.f;
     }
 
     const Halves keys{A.cache, (R + P) * (kFp8 ? 1 : 2), bt + b * A.bt_row_stride, A.bt_width,
@@ -305,8 +292,12 @@ __attribute__((amdgpu_waves_per_eu(1, 1))) void latent_decode_kernel(
     int pages = -1, looked_up = -1;
     uint64_t there = 0, there_before = 0;
     uint2 raw[kFp8 ? kMoves : 1];
-    // Issues this wave's loads of step s: bf16 into its buffer, fp8 into `to`.
-    auto load = [&](int s, uint2 (&to)[kFp8 ? kMoves : 1]) {
+    // This wave's loads of step s: where from, and bf16: where to.
+    struct Moves {
+      const uint8_t* from;
+      uint32_t to;
+    };
+    auto moves_of = [&](int s) {
       s = min(s, steps - 1);  // (past the end, once more: as many loads are on their way)
       const int key0 = (s_lo + s) * kKeys;
       if (s / 32 != looked_up) {
@@ -316,22 +307,26 @@ __attribute__((amdgpu_waves_per_eu(1, 1))) void latent_decode_kernel(
         there = __ballot(pages >= 0);
       }
       const int pg = __builtin_amdgcn_readlane(pages, 2 * (s & 31) + half);
-      const uint8_t* const base = keys.rows(pg, key0 + 16 * half);
-      const uint32_t dst = lds0 + (s % kBuffers) * T::kBytes + dst0;
+      return Moves{keys.rows(pg, key0 + 16 * half), lds0 + (s % kBuffers) * T::kBytes + dst0};
+    };
+    // Issues the i-th of them: bf16 into LDS, fp8 into raw.
+    auto issue = [&](const Moves& m, int i) {
+      if constexpr (kFp8)
+        raw[i] = ld8(m.from + src[i]);
+      else
+        lds_load16(m.from, src[i], m.to + 1024 * i);
+    };
+    auto load = [&](int s) {
+      const Moves m = moves_of(s);
 #pragma unroll
-      for (int i = 0; i < kMoves; ++i) {
-        if constexpr (kFp8)
-          to[i] = ld8(base + src[i]);
-        else
-          lds_load16(base, src[i], dst + 1024 * i);
-      }
+      for (int i = 0; i < kMoves; ++i) issue(m, i);
     };
     // fp8: what was loaded, as bf16, into step s's buffer.
-    auto put = [&](int s, const uint2 (&from)[kFp8 ? kMoves : 1]) {
+    auto put = [&](int s) {
       uint8_t* const dst = lds + (s % kBuffers) * T::kBytes + dst0 + 16 * lane;
 #pragma unroll
       for (int i = 0; i < (kFp8 ? kMoves : 0); ++i) {
-        const uint2 a = fp8x4_to_bf16x4(from[i].x), c = fp8x4_to_bf16x4(from[i].y);
+        const uint2 a = fp8x4_to_bf16x4(raw[i].x), c = fp8x4_to_bf16x4(raw[i].y);
         *reinterpret_cast<uint4*>(dst + 1024 * i) = make_uint4(a.x, a.y, c.x, c.y);
       }
     };
@@ -341,12 +336,31 @@ __attribute__((amdgpu_waves_per_eu(1, 1))) void latent_decode_kernel(
     // Whether every column sees all keys of step s.
     auto whole = [&](int s) { return (s_lo + s + 1) * kKeys <= all_hi && halves_of(s) == 3; };
 
-    floatx4_t p[kCB];
-    // S of step s, and its columns' maxima.  Operands come in groups, one ahead of the products.
-    // Piece 4 k + g of a row: of its place, k / 2 moves it by 128 bytes, k % 2 by a permutation.
+    // The first steps' loads, and the queries behind them.
+    load(0);
+    if constexpr (kFp8) put(0);
+    load(1);
+    bf16x8_t qb[kCB][kKc];
+#pragma unroll
+    for (int cb = 0; cb < kCB; ++cb) {
+      const int h = (su ? head0[kUnits - 1] : head0[0]) + (s_col + 16 * cb) % 32;
+      const bool ok = h < A.num_heads;
+      const uint16_t* const qp =
+          A.q + (sr.row0 + (su ? row_i[kUnits - 1] : row_i[0])) * A.q_row_stride +
+          (ok ? h : 0) * A.q_head_stride + 8 * g;
+#pragma unroll
+      for (int k = 0; k < kKc; ++k) {
+        uint4 v = ok ? *reinterpret_cast<const uint4*>(qp + 32 * k) : make_uint4(0, 0, 0, 0);
+        v = make_uint4(v.x ^ flip, v.y ^ flip, v.z ^ flip, v.w ^ flip);
+        qb[cb][k] = __builtin_bit_cast(bf16x8_t, v);
+      }
+    }
+    // S of step s, in logits.  Operands come in groups, one ahead of the products.  Piece 4 k + g
+    // of a row: of its place, k / 2 moves it by 128 bytes, k % 2 by a permutation.
     const uint32_t k_at[2] = {static_cast<uint32_t>(T::at(16 * ts + r, g)),
                               static_cast<uint32_t>(T::at(16 * ts + r, 4 + g))};
-    auto scores = [&](int s, auto is_masked) {
+    // (among(x): what to do among the products of the x-th group)
+    auto scores = [&](int s, floatx4_t (&p)[kCB], auto among) {
       const uint8_t* const tile = lds + (s % kBuffers) * T::kBytes;
       const uint8_t* const at[2] = {tile + k_at[0], tile + k_at[1]};
       uint4 kx[2][kGroup];
@@ -361,10 +375,11 @@ __attribute__((amdgpu_waves_per_eu(1, 1))) void latent_decode_kernel(
         if (k0 + kGroup < kKc) {
 #pragma unroll
           for (int j = 0; j < kGroup; ++j)
-            kx[now ^ 1][j] = *reinterpret_cast<const uint4*>(at[j & 1] +
+            kx[now ^ 1][j] = *reinterpret_cast<const uint4*>(at[(k0 + kGroup + j) & 1] +
                                                              128 * ((k0 + kGroup + j) >> 1));
         }
-        loads_issued();
+        among(k0 / kGroup);
+        __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
         for (int j = 0; j < kGroup; ++j)
 #pragma unroll
@@ -372,59 +387,64 @@ __attribute__((amdgpu_waves_per_eu(1, 1))) void latent_decode_kernel(
             p[cb] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(
                 __builtin_bit_cast(bf16x8_t, kx[now][j]), qb[cb][k0 + j], p[cb], 0, 0, 0);
       }
+    };
+    // The softmax of step s, in four parts: logits, their maxima, weights.
+    // (The weights are rounded to bf16 for P V, 2^-9 relative at most, of either sign; their sum
+    // is of the unrounded ones.)
+    auto logits = [&](int s, floatx4_t (&p)[kCB]) {
+      // (keys that this lane's column sees, from its first one on; without a branch, which would
+      // part the products around it)
+      const int seen = halves_of(s) >> ts & 1 ? my_hi - ((s_lo + s) * kKeys + 16 * ts + 4 * g) : 0;
 #pragma unroll
-      for (int cb = 0; cb < kCB; ++cb) p[cb] *= abs_s2;
-      if constexpr (decltype(is_masked)::value) {
-        const int t0 = (s_lo + s) * kKeys + 16 * ts + 4 * g;
-        const bool there_ = halves_of(s) >> ts & 1;
+      for (int cb = 0; cb < kCB; ++cb)
 #pragma unroll
-        for (int cb = 0; cb < kCB; ++cb)
-#pragma unroll
-          for (int i = 0; i < 4; ++i)
-            if (!(there_ && t0 + i < my_hi)) p[cb][i] = kNegInf;
-      }
+        for (int i = 0; i < 4; ++i) p[cb][i] = i < seen ? p[cb][i] * abs_s2 : kNegInf;
+    };
+    auto maxima = [&](int s, const floatx4_t (&p)[kCB]) {
 #pragma unroll
       for (int cb = 0; cb < kCB; ++cb) {
         const float top =
             pair_max(fmaxf(fmaxf(p[cb][0], p[cb][1]), fmaxf(p[cb][2], p[cb][3])));
-        if (g == 0) tops[kCols * ts + s_col + 16 * cb] = top;
+        tops[(s & 1) * 2 * kCols + kCols * ts + s_col + 16 * cb] = top;
       }
     };
-    // The references, moved where they have to be; weights from p, into LDS.
-    auto weights = [&] {
-      float t[kUnits];
-      bool move = false;
+    auto weights = [&](int s, const floatx4_t (&p)[kCB], int cb) {
+      float e[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) e[i] = __builtin_amdgcn_exp2f(p[cb][i] - ms[cb]);
+      last[cb] = (e[0] + e[1]) + (e[2] + e[3]);
+      *reinterpret_cast<uint2*>(p_at(s_col + 16 * cb, 16 * ts + 4 * g) + (s & 1) * kP) =
+          make_uint2(pack2(e[0], e[1]), pack2(e[2], e[3]));
+    };
+    // Whether a maximum is too far above its reference (uniform: every wave has the same ones);
+    // then the references move and the step's weights are made again.
+    auto too_far = [&](const float (&t)[kUnits]) {
+      bool far = false;
+#pragma unroll
+      for (int u = 0; u < kUnits; ++u) far |= t[u] > mo[u] + kLazyMax;
+      return __ballot(far) != 0;
+    };
+    auto move = [&](int s, const floatx4_t (&p)[kCB], const float (&t)[kUnits]) {
 #pragma unroll
       for (int u = 0; u < kUnits; ++u) {
-        t[u] = fmaxf(tops[32 * u + n], tops[kCols + 32 * u + n]);
-        move |= t[u] > mo[u] + kLazyMax;
+        const float m_new = fmaxf(mo[u], t[u]);
+        scale_acc(o[u], __builtin_amdgcn_exp2f(mo[u] - m_new));
+        mo[u] = m_new;
       }
-      if (__ballot(move) != 0) {
-#pragma unroll
-        for (int u = 0; u < kUnits; ++u) {
-          const float m_new = fmaxf(mo[u], t[u]);
-          scale_acc(o[u], __builtin_amdgcn_exp2f(mo[u] - m_new));
-          mo[u] = m_new;
-        }
-#pragma unroll
-        for (int cb = 0; cb < kCB; ++cb) {
-          const int c = s_col + 16 * cb;
-          const float m_new = fmaxf(ms[cb], fmaxf(tops[c], tops[kCols + c]));
-          l[cb] *= __builtin_amdgcn_exp2f(ms[cb] - m_new);
-          ms[cb] = m_new;
-        }
-      }
-      // The weights are rounded to bf16 for P V (2^-9 relative at most, of either sign); their
-      // sum is of the unrounded ones.
+      const float* const top = tops + (s & 1) * 2 * kCols;
 #pragma unroll
       for (int cb = 0; cb < kCB; ++cb) {
-        float e[4];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) e[i] = __builtin_amdgcn_exp2f(p[cb][i] - ms[cb]);
-        l[cb] += (e[0] + e[1]) + (e[2] + e[3]);
-        *reinterpret_cast<uint2*>(p_at(s_col + 16 * cb, 16 * ts + 4 * g)) =
-            make_uint2(pack2(e[0], e[1]), pack2(e[2], e[3]));
+        const int c = s_col + 16 * cb;
+        const float m_new = fmaxf(ms[cb], fmaxf(top[c], top[kCols + c]));
+        l[cb] *= __builtin_amdgcn_exp2f(ms[cb] - m_new);
+        ms[cb] = m_new;
+        weights(s, p, cb);
       }
+      __syncthreads();
+    };
+    auto count = [&] {
+#pragma unroll
+      for (int cb = 0; cb < kCB; ++cb) l[cb] += last[cb];
     };
     // O += P V of step s.  Operands of 16 keys (k): lane (n, kh) has keys 16 k + 8 kh .. + 7.  In
     // a transpose load, lane 4 a + q of each 16 addresses key a and dims 4 q .. 4 q + 3; block d's
@@ -439,23 +459,32 @@ __attribute__((amdgpu_waves_per_eu(1, 1))) void latent_decode_kernel(
                            wave * (R / 32) + 4 * d + 2 * (g & 1) + ((lane & 3) >> 1));
     const uint8_t* const p_from = p_at(n, 8 * kh);  // keys 16 on: pieces 2 on, of four, permuted
     const int p_next = 32 - 64 * (((kh ^ (n >> 2)) & 3) >> 1);
-    auto values = [&](int s, auto is_masked) {
-      constexpr bool kMasked = decltype(is_masked)::value;
-      const uint8_t* const tile = lds + (s % kBuffers) * T::kBytes;
-      const uint8_t* const at[2][2] = {{tile + v_at[0][0], tile + v_at[0][1]},
-                                       {tile + v_at[1][0], tile + v_at[1][1]}};
-      auto v_operand = [&](int x) {  // keys 16 (x / kOb) on, block x % kOb
-        const int k = x / kOb, d = x % kOb;
-        const int off = 16 * k * T::kRow + 128 * (d >> 1);
-        return joined(transposed(at[0][d & 1] + off), transposed(at[1][d & 1] + off));
-      };
-      bf16x8_t w[2][kUnits];
+    auto v_operand = [&](const uint8_t* tile, int x) {  // keys 16 (x / kOb) on, block x % kOb
+      const int k = x / kOb, d = x % kOb;
+      const int off = 16 * k * T::kRow + 128 * (d >> 1);
+      return joined(transposed(tile + v_at[0][d & 1] + off), transposed(tile + v_at[1][d & 1] + off));
+    };
+    // The first operands of P V of step s: its weights, and V's of the first group.
+    constexpr int kVGroup = kOb / 2;
+    struct First {
+      bf16x8_t w[2][kUnits], v[kVGroup];
+    };
+    auto first_operands = [&](int s, First& f) {
 #pragma unroll
       for (int k = 0; k < 2; ++k)
 #pragma unroll
         for (int u = 0; u < kUnits; ++u)
-          w[k][u] = __builtin_bit_cast(
-              bf16x8_t, *reinterpret_cast<const uint4*>(p_from + 64 * 32 * u + k * p_next));
+          f.w[k][u] = __builtin_bit_cast(
+              bf16x8_t, *reinterpret_cast<const uint4*>(p_from + (s & 1) * kP + 64 * 32 * u +
+                                                        k * p_next));
+#pragma unroll
+      for (int j = 0; j < kVGroup; ++j)
+        f.v[j] = v_operand(lds + (s % kBuffers) * T::kBytes, j);
+    };
+    // (among(x): what to do among the products of the x-th quarter)
+    auto values = [&](int s, const First& f, auto is_masked, auto among) {
+      constexpr bool kMasked = decltype(is_masked)::value;
+      const uint8_t* const tile = lds + (s % kBuffers) * T::kBytes;
       // Keys that the row does not see may hold anything, infinities and NaN among it: zeros.
       uint32_t mask[2][kUnits][4];
       if constexpr (kMasked) {
@@ -473,111 +502,162 @@ __attribute__((amdgpu_waves_per_eu(1, 1))) void latent_decode_kernel(
             word_masks(bits, mask[k][u]);
           }
       }
-      constexpr int kVGroup = 2;
       bf16x8_t v[2][kVGroup];
 #pragma unroll
-      for (int j = 0; j < kVGroup; ++j) v[0][j] = v_operand(j);
+      for (int j = 0; j < kVGroup; ++j) v[0][j] = f.v[j];
 #pragma unroll
       for (int x0 = 0; x0 < 2 * kOb; x0 += kVGroup) {
         const int now = x0 / kVGroup & 1;
         if (x0 + kVGroup < 2 * kOb) {
 #pragma unroll
-          for (int j = 0; j < kVGroup; ++j) v[now ^ 1][j] = v_operand(x0 + kVGroup + j);
+          for (int j = 0; j < kVGroup; ++j) v[now ^ 1][j] = v_operand(tile, x0 + kVGroup + j);
         }
-        loads_issued();
+        __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
         for (int j = 0; j < kVGroup; ++j) {
           const int k = (x0 + j) / kOb, d = (x0 + j) % kOb;
 #pragma unroll
           for (int u = 0; u < kUnits; ++u)
             o[u][d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(
-                kMasked ? masked(v[now][j], mask[k][u]) : v[now][j], w[k][u], o[u][d], 0, 0, 0);
+                kMasked ? masked(v[now][j], mask[k][u]) : v[now][j], f.w[k][u], o[u][d], 0, 0, 0);
         }
+        among(x0 / kVGroup);
       }
     };
 
-    // (the queries have come: the waits in the loop count the loads above alone)
-    __builtin_amdgcn_s_waitcnt(kNoLoads);
-    if constexpr (kFp8) {
-      uint2 raw0[kMoves], raw1[kMoves];
-      load(0, raw0);
-      load(1, raw1);
-      load(2, raw);
-      put(0, raw0);
-      put(1, raw1);
-    } else {
-#pragma unroll 1
-      for (int s = 0; s < kBuffers; ++s) load(s, raw);
-      wait_loads<(kBuffers - 1) * kMoves>();
-    }
-    __syncthreads();
-    scores(0, std::true_type{});
-    __syncthreads();
-    weights();
-    auto step = [&](int s, auto is_masked) {
-      if constexpr (!kFp8) wait_loads<(kBuffers - 2) * kMoves>();
-      __syncthreads();  // A: step s's weights and step s + 1's tile are in LDS
-      values(s, is_masked);
-      if (s + 1 >= steps) return;
-      scores(s + 1, is_masked);
-      __syncthreads();  // B: the maxima are in LDS, step s's tile and weights have been read
-      if constexpr (kFp8) {
-        put(s + 2, raw);
-        load(s + 3, raw);
-      } else {
-        load(s + kBuffers, raw);
+    floatx4_t p[kCB], next[kCB];
+    // A step's barrier: step s's weights and maxima and step s + 1's tile are in LDS, and step
+    // s - 1 is done with.  Its loads, of step s + 3, are issued among its products, so that the
+    // waves do not wait for their addresses to be taken.
+    auto enter = [&](int s, float (&t)[kUnits]) {
+      if constexpr (!kFp8) wait_loads<kMoves>();
+      __syncthreads();
+      if constexpr (kFp8) put(s + 2);
+#pragma unroll
+      for (int u = 0; u < kUnits; ++u) {
+        const float* const top = tops + (s & 1) * 2 * kCols + 32 * u + n;
+        t[u] = fmaxf(top[0], top[kCols]);
       }
-      weights();
     };
-    // (a loop of its own for the steps from the first one on that is not whole)
+    const auto nothing = [](int) {};
+    float t[kUnits];
+    First f;
+    if constexpr (!kFp8) wait_loads<0>();
+    __syncthreads();
+    if constexpr (kFp8) put(1);
+    load(2);
+    scores(0, p, nothing);
+    logits(0, p);
+    maxima(0, p);
+    __syncthreads();
+    // The first references.
+#pragma unroll
+    for (int u = 0; u < kUnits; ++u) {
+      const int c = s_col + 16 * u;
+      mo[u] = fmaxf(kNoMax, fmaxf(tops[32 * u + n], tops[kCols + 32 * u + n]));
+      ms[u] = fmaxf(kNoMax, fmaxf(tops[c], tops[kCols + c]));
+      weights(0, p, u);
+    }
+    enter(0, t);
     int s = 0;
 #pragma unroll 1
-    for (; s + 1 < steps && whole(s) && whole(s + 1); ++s) step(s, std::false_type{});
+    while (true) {  // (step s has been entered)
+      if (too_far(t)) move(s, p, t);
+      if (s + 1 < steps && whole(s)) {
+        // The steps that need nothing special, in a loop of their own: where such a step met
+        // another, the compiler would copy O around.
 #pragma unroll 1
-    for (; s < steps; ++s) step(s, std::true_type{});
+        do {
+          count();
+          const Moves m = moves_of(s + 3);
+          scores(s + 1, next, [&](int x) {
+            issue(m, x);
+            if (x == kKc / kGroup - 1) first_operands(s, f);
+          });
+          constexpr int kDone = kKc / kGroup;
+          static_assert(kDone <= kMoves && kDone + 8 >= kMoves, "every load is issued once");
+          values(s, f, std::false_type{}, [&](int x) {
+            if (x == 0) logits(s + 1, next);
+            if (x == 1) maxima(s + 1, next);
+            if (x >= 2 && x - 2 < kCB) weights(s + 1, next, x - 2);
+#pragma unroll
+            for (int i = 0; i < 2; ++i)
+              if (kDone + 2 * x + i < kMoves) issue(m, kDone + 2 * x + i);
+          });
+#pragma unroll
+          for (int cb = 0; cb < kCB; ++cb) p[cb] = next[cb];
+          ++s;
+          enter(s, t);
+        } while (s + 1 < steps && whole(s) && !too_far(t));
+      } else {
+        count();
+        load(s + 3);
+        first_operands(s, f);
+        values(s, f, std::true_type{}, nothing);
+        if (++s == steps) break;
+        scores(s, p, nothing);
+        logits(s, p);
+        maxima(s, p);
+#pragma unroll
+        for (int cb = 0; cb < kCB; ++cb) weights(s, p, cb);
+        enter(s, t);
+      }
+    }
     wait_loads<0>();
+    __syncthreads();
 
-    // The columns' sums, of both waves and all lanes that have keys of theirs.
+    // The states, through LDS: the columns' sums, of both waves and all lanes that have keys of
+    // theirs, and O, which leaves in whole rows.
+    constexpr int kRow = R + 4;  // floats
+    float* const xo = reinterpret_cast<float*>(lds);
+    static_assert(4 * kCols * kRow <= kBuffers * T::kBytes, "O fits");
 #pragma unroll
     for (int cb = 0; cb < kCB; ++cb) {
       l[cb] = pair_sum(l[cb]);
-      if (g == 0) tops[kCols * ts + s_col + 16 * cb] = l[cb];
+      tops[kCols * ts + s_col + 16 * cb] = l[cb];
     }
-    __syncthreads();
 #pragma unroll
     for (int u = 0; u < kUnits; ++u) {
-      const int c = 32 * u + n, head = head0[u] + n;
-      if (head >= A.num_heads) continue;
-      const float L = tops[c] + tops[kCols + c];
-      float* const po = A.o + (slot * kCols + c) * R;
-      if (slot >= 0 && wave == 0 && kh == 0)
-        *reinterpret_cast<float2*>(A.ml + (slot * kCols + c) * 2) = make_float2(mo[u], L);
+      if (wave == 0) tops[2 * kCols + 32 * u + n] = mo[u];
+      float* const to = xo + (32 * u + n) * kRow + wave * (R / 4) + 4 * kh;
 #pragma unroll
       for (int d = 0; d < kOb; ++d)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const float4 z = make_float4(o[u][d][4 * i], o[u][d][4 * i + 1], o[u][d][4 * i + 2],
-                                       o[u][d][4 * i + 3]);
-          const int dim = wave * (R / 4) + 32 * d + 8 * i + 4 * kh;
-          if (slot < 0)
-            write_out(A, x.row0 + row_i[u], head, dim, z, mo[u], L, vsc);
-          else
-            *reinterpret_cast<float4*>(po + dim) = z;
-        }
+        for (int i = 0; i < 4; ++i)
+          *reinterpret_cast<float4*>(to + 32 * d + 8 * i) = make_float4(
+              o[u][d][4 * i], o[u][d][4 * i + 1], o[u][d][4 * i + 2], o[u][d][4 * i + 3]);
+    }
+    __syncthreads();
+#pragma unroll 4
+    for (int i = threadIdx.x; i < kCols * (R / 4); i += kThreads) {
+      const int c = i / (R / 4), dim = 4 * (i % (R / 4));
+      const int u = c / 32, head = (u ? head0[kUnits - 1] : head0[0]) + c % 32;
+      if (head >= A.num_heads) continue;
+      const float4 z = *reinterpret_cast<const float4*>(xo + c * kRow + dim);
+      const float L = tops[c] + tops[kCols + c], M = tops[2 * kCols + c];
+      if (slot < 0) {
+        write_out(A, sr.row0 + (u ? row_i[kUnits - 1] : row_i[0]), head, dim, z, M, L, vsc);
+      } else {
+        *reinterpret_cast<float4*>(A.o + (slot * kCols + c) * R + dim) = z;
+        if (dim == 0)
+          *reinterpret_cast<float2*>(A.ml + (slot * kCols + c) * 2) = make_float2(M, L);
+      }
     }
     __syncthreads();
   };
   walk_line<kThreads>(line, A.batch, A.wgs, blockIdx.x, 1, A.records,
-                      [&](int b) { return line_seq(A, cu, ctx_lens, b, kUnits); }, body);
+                      [&](int b) { return seq_rows(cu, ctx_lens, b, A.rows, A.most); },
+                      [&](const SeqRows& s) { return line_items(A, s, kUnits); }, body);
 }
 
-// One work-group per (query row, some of its heads): merges the pieces of an item that ranges cut.
-template <int R>
+// One work-group per (query row, some of its heads, kDims of their dims): merges the pieces of an
+// item that ranges cut.
+template <int R, int kDims>
 __global__ __launch_bounds__(kMergeThreads) void latent_merge_kernel(
     LatentParams A, const int32_t* __restrict__ ctx_lens, const int32_t* __restrict__ cu,
     int heads, int fp8) {
   __shared__ Folded folded[kMergeThreads];
-  const int t = blockIdx.y;
+  const int t = blockIdx.y, dim0 = blockIdx.z * kDims;
   int b, vis;
   if (!query_row(cu, ctx_lens, A.batch, t, b, vis)) return;
   const SeqRows s = seq_rows(cu, ctx_lens, b, A.rows, A.most);
@@ -593,15 +673,15 @@ __global__ __launch_bounds__(kMergeThreads) void latent_merge_kernel(
     const int nc = min(h1, (h / 32 + 1) * 32) - h;
     const LinePieces pieces(rec, unit / A.units);
     if (pieces.n > 1) {
-      merge_pieces<R>(
+      merge_pieces<kDims>(
           0, nc, folded, [&](int) { return pieces.n; },
           [&](int k, int x, const float*& ml, const float*& o) {
             const int64_t at = pieces.slot(k) * (32 * A.units) + in + x;
             ml = A.ml + 2 * at;
-            o = A.o + at * R;
+            o = A.o + at * R + dim0;
           },
           [&](int x, int dim, const float4& o, float M, float L) {
-            write_out(A, t, h + x, dim, o, M, L, vsc);
+            write_out(A, t, h + x, dim0 + dim, o, M, L, vsc);
           });
       __syncthreads();
     }
@@ -631,16 +711,23 @@ LatentPlan plan_of(int64_t batch, int64_t max_seqlen_q, int num_heads, int laten
 template <int R, int P, bool kFp8>
 void launch(const LatentParams& A, hipStream_t s, const int32_t* bt, const int32_t* ctx,
             const int32_t* cu) {
-  const unsigned lds = kBuffers * Tile<R, P>::kBytes + 32 * A.units * (kKeys * 2 + 2 * 4);
+  const unsigned lds = kBuffers * Tile<R, P>::kBytes + 2 * 32 * A.units * (kKeys * 2 + 2 * 4);
   if (A.units == 1)
     hipLaunchKernelGGL((latent_decode_kernel<R, P, 1, kFp8>), dim3(A.wgs + 1), dim3(kThreads),
                        lds, s, A, bt, ctx, cu);
   else
     hipLaunchKernelGGL((latent_decode_kernel<R, P, 2, kFp8>), dim3(A.wgs + 1), dim3(kThreads),
                        lds, s, A, bt, ctx, cu);
+  // Where rows and heads do not make two work-groups a CU, the dims are dealt out too, and with
+  // them threads to share a column's pieces.
   const int heads = merge_cols(A.rows, 1, A.num_heads);
-  hipLaunchKernelGGL((latent_merge_kernel<R>), dim3((A.num_heads + heads - 1) / heads, A.rows),
-                     dim3(kMergeThreads), 0, s, A, ctx, cu, heads, kFp8 ? 1 : 0);
+  const dim3 grid((A.num_heads + heads - 1) / heads, A.rows);
+  if (static_cast<int64_t>(grid.x) * grid.y < num_cus())
+    hipLaunchKernelGGL((latent_merge_kernel<R, 64>), dim3(grid.x, grid.y, R / 64),
+                       dim3(kMergeThreads), 0, s, A, ctx, cu, heads, kFp8 ? 1 : 0);
+  else
+    hipLaunchKernelGGL((latent_merge_kernel<R, R>), grid, dim3(kMergeThreads), 0, s, A, ctx, cu,
+                       heads, kFp8 ? 1 : 0);
 }
 
 }  // namespace

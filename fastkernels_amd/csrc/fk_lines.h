@@ -55,34 +55,18 @@ __device__ __forceinline__ int64_t share_of(int wg, int n, int64_t shares, bool 
   return i < per ? (wg & 7) * per + i : n;
 }
 
-// One sequence's items on a line: `items` of `steps` steps each, laid end to end.
-struct LineSeq {
-  int row0, rows;   // its query rows
-  int from, to;     // keys that any of them sees
-  int steps, items;
-  int64_t start;    // first step on the line (filled where the line is walked)
-};
-// Where the merge finds a sequence's items on the line.
-struct LineRecord {
-  int64_t start, range;
-  int steps, pad_;
-};
-// Partial states of the items that ranges cut: a range has one slot for an item that begins
-// before it and one for an item that begins in it and goes on behind it.
-__device__ __forceinline__ int64_t line_slot(int64_t wg, bool begins) {
-  return 2 * wg + (begins ? 1 : 0);
-}
-
 // Query rows of sequence b (cu == nullptr: one each), inside [0, rows) whatever cu says, and at
 // most `most`; and the keys they see: row i of n the last window_left + 1 (all: -1) before
 // ctx - n + i + 1, whether the rows processed are all n or not.
 struct SeqRows {
   int row0, rows, all, ctx;
+  int64_t start;  // its first step on the line (filled where that is walked)
 };
 __device__ __forceinline__ SeqRows seq_rows(const int32_t* __restrict__ cu,
                                             const int32_t* __restrict__ ctx, int b, int rows,
                                             int most) {
   SeqRows s;
+  s.start = 0;
   s.ctx = max(ctx[b], 0);
   if (cu == nullptr) {
     s.row0 = b;
@@ -104,23 +88,40 @@ __device__ __forceinline__ void row_keys(const SeqRows& s, int i, int window_lef
   lo = window_left >= 0 ? max(0, hi - 1 - window_left) : 0;
 }
 
+// Its items on a line: `items` of `steps` steps each, laid end to end, over the keys [from, to)
+// that any of its rows sees.
+struct LineItems {
+  int from, to;
+  int steps, items;
+};
+// Where the merge finds a sequence's items on the line.
+struct LineRecord {
+  int64_t start, range;
+  int steps, pad_;
+};
+// Partial states of the items that ranges cut: a range has one slot for an item that begins
+// before it and one for an item that begins in it and goes on behind it.
+__device__ __forceinline__ int64_t line_slot(int64_t wg, bool begins) {
+  return 2 * wg + (begins ? 1 : 0);
+}
+
 // What walk_line holds in LDS.
 template <int kThreads>
 struct LineLds {
-  int64_t start[kThreads];
+  SeqRows seq[kThreads];
   int64_t sum[kThreads / 64];
   uint64_t hits[kThreads / 64];
 };
 
-// Walks the share of work-group `wg` of `wgs` on the line of `batch` sequences, which
-// seq_at(b) describes: body(b, sequence, item, first step, end step, slot) for each item's part
-// in it, uniform over the work-group; slot: -1 where the part is the whole item, otherwise where
-// its partial state goes.  Work-group wgs writes every sequence's record instead.  Every thread
-// of the work-group calls it; the line's sequences with items have at least one step.
-template <int kThreads, class SeqAt, class Body>
+// Walks the share of work-group `wg` of `wgs` on the line of `batch` sequences, seq_at(b) their
+// rows and items_of(rows) their items: body(b, rows, items, item, first step, end step, slot) for
+// each item's part in it, uniform over the work-group; slot: -1 where the part is the whole item,
+// otherwise where its partial state goes.  Work-group wgs writes every sequence's record instead.
+// Every thread of the work-group calls it; items have at least one step.
+template <int kThreads, class SeqAt, class ItemsOf, class Body>
 __device__ __forceinline__ void walk_line(LineLds<kThreads>& lds, int batch, int wgs, int wg,
                                           int quantum, LineRecord* __restrict__ records,
-                                          SeqAt seq_at, Body body) {
+                                          SeqAt seq_at, ItemsOf items_of, Body body) {
   constexpr int kWaves = kThreads / 64;
   const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63;
   auto scan_all = [&](int64_t v, int64_t& total) {
@@ -137,13 +138,17 @@ __device__ __forceinline__ void walk_line(LineLds<kThreads>& lds, int batch, int
     __syncthreads();
     return before + x;
   };
-  auto length = [](const LineSeq& x) { return static_cast<int64_t>(x.steps) * x.items; };
   auto at = [&](int b) {
-    LineSeq x{};
+    SeqRows x{};
     if (b < batch) x = seq_at(b);
     return x;
   };
-  const LineSeq first = at(tid);
+  auto length = [&](const SeqRows& x) {
+    if (x.rows == 0) return int64_t{0};
+    const LineItems it = items_of(x);
+    return static_cast<int64_t>(it.steps) * it.items;
+  };
+  const SeqRows first = at(tid);
   int64_t sum = length(first), total;
   for (int b = kThreads + tid; b < batch; b += kThreads) sum += length(at(b));
   scan_all(sum, total);
@@ -155,17 +160,17 @@ __device__ __forceinline__ void walk_line(LineLds<kThreads>& lds, int batch, int
   const int64_t t_hi = writes ? total : min(total, t_lo + S);
   int64_t line = 0;
   for (int b0 = 0; t_lo < total && b0 < batch && line < t_hi; b0 += kThreads) {
-    LineSeq x = b0 == 0 ? first : at(b0 + tid);
+    SeqRows x = b0 == 0 ? first : at(b0 + tid);
     const int64_t mine = length(x);
     const int64_t end = line + scan_all(mine, sum);
     line += sum;
     x.start = end - mine;
     if (writes) {
-      if (b0 + tid < batch) records[b0 + tid] = LineRecord{x.start, S, x.steps, 0};
+      if (mine > 0) records[b0 + tid] = LineRecord{x.start, S, items_of(x).steps, 0};
       continue;
     }
     const bool in = mine > 0 && end > t_lo && x.start < t_hi;
-    if (in) lds.start[tid] = x.start;
+    if (in) lds.seq[tid] = x;
     const uint64_t hits = __ballot(in);
     if (lane == 0) lds.hits[wave] = hits;
     __syncthreads();
@@ -175,15 +180,20 @@ __device__ __forceinline__ void walk_line(LineLds<kThreads>& lds, int batch, int
       while (hit) {
         const int src = 64 * k + __builtin_ctzll(hit);
         hit &= hit - 1;
-        LineSeq y = seq_at(b0 + src);
-        y.start = lane64(lds.start[src], 0);
-        for (int it = t_lo > y.start ? quotient(t_lo - y.start, y.steps) : 0;
-             it < y.items && y.start + static_cast<int64_t>(it) * y.steps < t_hi; ++it) {
-          const int64_t s0 = y.start + static_cast<int64_t>(it) * y.steps;
+        SeqRows y = lds.seq[src];
+        y.row0 = uniform(y.row0);
+        y.rows = uniform(y.rows);
+        y.all = uniform(y.all);
+        y.ctx = uniform(y.ctx);
+        y.start = lane64(y.start, 0);
+        const LineItems z = items_of(y);
+        for (int it = t_lo > y.start ? quotient(t_lo - y.start, z.steps) : 0;
+             it < z.items && y.start + static_cast<int64_t>(it) * z.steps < t_hi; ++it) {
+          const int64_t s0 = y.start + static_cast<int64_t>(it) * z.steps;
           const int lo = static_cast<int>(max(t_lo, s0) - s0);
-          const int hi = static_cast<int>(min(t_hi, s0 + y.steps) - s0);
-          const bool whole = lo == 0 && hi == y.steps;
-          body(b0 + src, y, it, lo, hi, whole ? int64_t{-1} : line_slot(w, lo == 0));
+          const int hi = static_cast<int>(min(t_hi, s0 + z.steps) - s0);
+          const bool whole = lo == 0 && hi == z.steps;
+          body(b0 + src, y, z, it, lo, hi, whole ? int64_t{-1} : line_slot(w, lo == 0));
         }
       }
     }

@@ -177,29 +177,25 @@ __attribute__((amdgpu_waves_per_eu(2))) void mxfp4_decode_kernel(
   const float s2 = A.scale_log2;
   const int page_mask = (1 << A.block_size_log2) - 1;
 
-  auto seq_at = [&](int b) {
-    LineSeq x{};
-    const SeqRows s = seq_rows(cu, ctx_lens, b, P.rows, P.most);
-    if (s.rows == 0) return x;
+  auto items_of = [&](const SeqRows& s) {
+    LineItems x;
     int none;
     row_keys(s, 0, P.window_left, x.from, none);
     row_keys(s, s.rows - 1, P.window_left, none, x.to);
-    x.row0 = s.row0;
-    x.rows = s.rows;
     // (past the table's end there is nothing to see)
-    x.to = static_cast<int>(min(static_cast<int64_t>(x.to),
+    x.to = static_cast<int>(min(min(static_cast<int64_t>(x.to), int64_t{0x7fffff00}),
                                 static_cast<int64_t>(A.bt_width) << A.block_size_log2));
     x.from &= -kStep;
     x.steps = x.to > x.from ? (x.to - x.from - 1) / kStep + 1 : 1;
     x.items = A.num_kv_heads * ((s.rows * A.gqa + kCols - 1) / kCols);
     return x;
   };
-  auto body = [&](int b, const LineSeq& x, int it, int s_lo, int s_hi, int64_t slot) {
+  auto body = [&](int b, const SeqRows& sr, const LineItems& x, int it, int s_lo, int s_hi,
+                  int64_t slot) {
     const int col_items = x.items / A.num_kv_heads;
     const int kvh = it / col_items;
     const int col0 = (it - kvh * col_items) * kCols;
-    const int n_cols = min(kCols, x.rows * A.gqa - col0);
-    const SeqRows sr = seq_rows(cu, ctx_lens, b, P.rows, P.most);
+    const int n_cols = min(kCols, sr.rows * A.gqa - col0);
     ColumnState<kCB, D, false> st;
     st.reset();
     int lo[kCB], hi[kCB];  // keys that this lane's column sees
@@ -211,7 +207,7 @@ __attribute__((amdgpu_waves_per_eu(2))) void mxfp4_decode_kernel(
       const int i = ok ? (col0 + c) / A.gqa : 0, hq = kvh * A.gqa + (ok ? (col0 + c) % A.gqa : 0);
       row_keys(sr, i, P.window_left, lo[cb], hi[cb]);
       const uint16_t* const qp =
-          A.q + (x.row0 + i) * A.q_row_stride + static_cast<int64_t>(hq) * D + g * (D / 4);
+          A.q + (sr.row0 + i) * A.q_row_stride + static_cast<int64_t>(hq) * D + g * (D / 4);
 #pragma unroll
       for (int k = 0; k < D / 32; ++k) {
         const uint32_t flip = s2 < 0.f ? 0x80008000u : 0u;
@@ -329,7 +325,7 @@ __attribute__((amdgpu_waves_per_eu(2))) void mxfp4_decode_kernel(
     merge_waves<kWaves>(st, lds, wave, lane, n_cols,
                         [&](int j, int dim, const float4& o, float M, float L) {
                           if (slot < 0) {
-                            write_quad(A, x.row0 + (col0 + j) / A.gqa,
+                            write_quad(A, sr.row0 + (col0 + j) / A.gqa,
                                        kvh * A.gqa + (col0 + j) % A.gqa, D, dim, o, M, L, 1.f);
                             return;
                           }
@@ -339,7 +335,9 @@ __attribute__((amdgpu_waves_per_eu(2))) void mxfp4_decode_kernel(
                         });
     __syncthreads();
   };
-  walk_line<kThreads>(line, A.batch, P.wgs, blockIdx.x, kWaves, P.records, seq_at, body);
+  walk_line<kThreads>(line, A.batch, P.wgs, blockIdx.x, kWaves, P.records,
+                      [&](int b) { return seq_rows(cu, ctx_lens, b, P.rows, P.most); }, items_of,
+                      body);
 }
 
 // One work-group per (query row, kv head, some of its columns): merges the pieces of an item that
