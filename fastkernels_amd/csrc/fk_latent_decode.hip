@@ -24,8 +24,11 @@ typedef float floatx16_t __attribute__((ext_vector_type(16)));
 
 constexpr int kWaves = 4;
 constexpr int kThreads = kWaves * 64;
+constexpr int kSeqs = 128;   // sequences looked at together
 constexpr int kKeys = 32;    // of a tile
-constexpr int kBuffers = 4;  // tiles in LDS
+// (Weights to 2^32: with values up to 2^90 their sums stay finite.  No logits of trained models come
+// near it.)
+constexpr float kFar = 32.f;
 
 struct LatentParams {
   uint16_t* out;
@@ -57,18 +60,17 @@ struct Tile {
   static constexpr int kRow = 2 * (R + P);        // bytes
   static constexpr int kPieces = kRow / 16;
   static constexpr int kBytes = kKeys * kRow;
-  static constexpr int kMoves = kKeys * kPieces / 64;  // 64-piece moves of a tile
-  static_assert(kPieces % 8 == 0 && kKeys / 2 * kPieces % 64 == 0, "whole moves of half a tile");
+  static constexpr int kMoves = kPieces / 8;  // of 64 pieces, of eight rows
+  static_assert(kPieces % 8 == 0, "whole runs of pieces, whole moves of eight rows");
   static __device__ __forceinline__ int at(int row, int piece) {
     return row * kRow + 16 * ((piece & ~7) | ((piece ^ (row >> 1)) & 7));
   }
-  // Where in its half's rows of the cache (elements of kElt bytes) lane `lane` of move m of
-  // the half finds the piece that goes to LDS bytes 1024 m + 16 lane of the half.
-  template <int kElt>
-  static __device__ __forceinline__ uint32_t source(int m, int lane) {
+  // Where in its eight rows of the cache a lane finds the piece that goes to LDS bytes
+  // 1024 m + 16 lane of them (rows from a multiple of 8 on, `odd`: not of 16).
+  static __device__ __forceinline__ uint32_t source(int m, int lane, bool odd) {
     const int x = 64 * m + lane;
     const int row = x / kPieces, slot = x % kPieces;
-    return row * (R + P) * kElt + 8 * kElt * ((slot & ~7) | ((slot ^ (row >> 1)) & 7));
+    return row * kRow + 16 * ((slot & ~7) | ((slot ^ ((row >> 1) + (odd ? 4 : 0))) & 7));
   }
 };
 
@@ -81,6 +83,16 @@ __device__ __forceinline__ void lds_load16(const uint8_t* base, uint32_t off, ui
   asm volatile(
       "s_mov_b64 %0, %2\n\t"
       "global_load_lds_dwordx4 %1, %0"
+      : "=&s"(b)
+      : "v"(off), "s"(base), "{m0}"(lds_addr)
+      : "memory");
+}
+// ... and 4 bytes, at 4 l.
+__device__ __forceinline__ void lds_load4(const uint8_t* base, uint32_t off, uint32_t lds_addr) {
+  const uint8_t* b;
+  asm volatile(
+      "s_mov_b64 %0, %2\n\t"
+      "global_load_lds_dword %1, %0"
       : "=&s"(b)
       : "v"(off), "s"(base), "{m0}"(lds_addr)
       : "memory");
@@ -104,30 +116,10 @@ __device__ __forceinline__ bf16x8_t joined(short4_t a, short4_t b) {
   const uint2 x = __builtin_bit_cast(uint2, a), y = __builtin_bit_cast(uint2, b);
   return __builtin_bit_cast(bf16x8_t, make_uint4(x.x, x.y, y.x, y.y));
 }
-__device__ __forceinline__ bf16x8_t masked(bf16x8_t v, const uint32_t (&m)[4]) {
-  const uint4 x = __builtin_bit_cast(uint4, v);
-  return __builtin_bit_cast(bf16x8_t,
-                            make_uint4(x.x & m[0], x.y & m[1], x.z & m[2], x.w & m[3]));
-}
-// Masks of the four words that hold eight 16-bit values, from a bit each.
-__device__ __forceinline__ void word_masks(uint32_t bits, uint32_t (&m)[4]) {
-#pragma unroll
-  for (int i = 0; i < 4; ++i)
-    m[i] = (bits >> (2 * i) & 1 ? 0xffffu : 0u) | (bits >> (2 * i + 1) & 1 ? 0xffff0000u : 0u);
-}
 __device__ __forceinline__ uint32_t pack2(float a, float b) {
   const bf16x2_t x = {static_cast<__bf16>(a), static_cast<__bf16>(b)};
   return __builtin_bit_cast(uint32_t, x);
 }
-__device__ __forceinline__ float halves_max(float v) {
-  const auto c = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
-  return fmaxf(__uint_as_float(c[0]), __uint_as_float(c[1]));
-}
-__device__ __forceinline__ float halves_sum(float v) {
-  const auto c = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
-  return __uint_as_float(c[0]) + __uint_as_float(c[1]);
-}
-
 // The keys of a part of an item, half a tile (16) at a time.
 struct Halves {
   const uint8_t* cache;
@@ -149,30 +141,7 @@ struct Halves {
   }
 };
 
-// O *= alpha, in place among the accumulators: the compiler would copy them out and back around
-// every step for it.  (The waits: vector instructions read a product's result 18 later at the
-// earliest, and products what those wrote 2 later.)
-template <int N>
-__device__ __forceinline__ void scale_acc(floatx16_t (&o)[N], float alpha) {
-#pragma unroll
-  for (int d = 0; d < N; ++d) {
-    asm volatile("s_nop 15\n\ts_nop 3" : "+a"(o[d]), "+v"(alpha));
-#pragma unroll
-    for (int i = 0; i < 16; ++i) {
-      float x = o[d][i], t;
-      asm volatile(
-          "v_accvgpr_read_b32 %1, %0\n\t"
-          "v_mul_f32 %1, %1, %2\n\t"
-          "v_accvgpr_write_b32 %0, %1"
-          : "+a"(x), "=&v"(t)
-          : "v"(alpha));
-      o[d][i] = x;
-    }
-    asm volatile("s_nop 3" : "+a"(o[d]));
-  }
-}
-
-// A sequence's items: `units` units (32 heads of a row) each, in steps of a tile.
+// A sequence's items: `units` units of 32 heads of a row each, in steps of a tile.
 __device__ __forceinline__ LineItems line_items(const LatentParams& P, const SeqRows& s,
                                                 int units) {
   LineItems x;
@@ -183,7 +152,7 @@ __device__ __forceinline__ LineItems line_items(const LatentParams& P, const Seq
   x.to = static_cast<int>(min(min(static_cast<int64_t>(x.to), int64_t{0x7fffff00}),
                               static_cast<int64_t>(P.bt_width) << P.block_size_log2));
   x.steps = x.to > 0 ? (x.to - 1) / kKeys + 1 : 1;
-  x.items = (s.rows * P.head_blocks + units - 1) / units;
+  x.items = s.rows * ((P.head_blocks + units - 1) / units);
   return x;
 }
 
@@ -198,7 +167,7 @@ __device__ __forceinline__ void write_out(const LatentParams& P, int64_t row, in
         L > 0.f ? (M + __builtin_amdgcn_logf(L)) * 0.6931471805599453f : L == 0.f ? kNegInf : L;
 }
 
-// One work-group: items of kUnits units of 32 heads (of one query row each), in steps of a tile.
+// One work-group: items of kUnits units of 32 heads of a query row, in steps of a tile.
 //
 // The waves share S by columns and keys, wave w = (cs, ts): half cs of the columns and keys
 // 16 ts .. 16 ts + 15 (16x16x32 products), and P V by dims: wave w has dims w R / 4 .. of every
@@ -206,9 +175,13 @@ __device__ __forceinline__ void write_out(const LatentParams& P, int64_t row, in
 // and so do the columns' maxima.
 //
 // A step has one barrier.  Behind it come S of the next step and P V of this one, with the next
-// step's softmax among the products of the latter: its weights are made with the reference maxima
-// as they are, and only where the maxima, which are all known behind the next barrier, ask for
-// others is P made again.
+// step's softmax among the products of the latter.
+//
+// A column's weights are 2^(logit - m), m the maximum of the first step: bf16 and the fp32 sums
+// hold great weights as exactly as small ones, and O is not rescaled.  Where a later maximum, which
+// all waves know behind the next barrier, is 2^kFar times that, the part is taken in two: the state
+// so far goes to memory, and what follows begins again with its own maximum and is merged with it.
+constexpr int tiles_of(bool fp8) { return fp8 ? 3 : 4; }
 template <int R, int P, int kUnits, bool kFp8>
 __global__ __launch_bounds__(kThreads)
 __attribute__((amdgpu_waves_per_eu(1, 1))) void latent_decode_kernel(
@@ -216,16 +189,21 @@ __attribute__((amdgpu_waves_per_eu(1, 1))) void latent_decode_kernel(
     const int32_t* __restrict__ cu) {
   using T = Tile<R, P>;
   constexpr int kCols = 32 * kUnits;
-  constexpr int kCB = kUnits;                 // blocks of 16 columns of a wave's S
-  constexpr int kKc = (R + P) / 32;           // products of S
-  constexpr int kOb = R / 4 / 32;             // blocks of 32 dims of a wave
-  constexpr int kMoves = T::kMoves / kWaves;  // of a wave and tile
-  static_assert(T::kMoves / 2 % kMoves == 0, "a wave's moves are of one half");
-  constexpr int kGroup = kFp8 && kUnits == 2 ? 2 : 3;  // K operands read from LDS at a time
+  constexpr int kCB = kUnits;            // blocks of 16 columns of a wave's S
+  constexpr int kKc = (R + P) / 32;      // products of S
+  constexpr int kOb = R / 4 / 32;        // blocks of 32 dims of a wave
+  constexpr int kGroup = 3;              // K operands read from LDS at a time
+  constexpr int kMoves = T::kMoves;      // of a wave and tile: eight rows
   static_assert(kKc % kGroup == 0 && kOb % 2 == 0, "whole groups");
-  __shared__ LineLds<kThreads> line;
+  // Tiles in LDS: bf16 four, of which two are on their way; fp8 three, and the codes of two to
+  // come (a wave's own eight rows each).
+  constexpr int kBuffers = tiles_of(kFp8);
+  constexpr int kCodes = 8 * (R + P);    // bytes of a wave's codes of a tile
+  constexpr int kWide = kCodes / 1024, kCodeMoves = kWide + kCodes % 1024 / 256;
+  static_assert(kCodes % 512 == 0, "whole moves");
+  __shared__ LineLds<kThreads, kSeqs> line;
   extern __shared__ __align__(16) uint8_t lds[];
-  uint8_t* const p_lds = lds + kBuffers * T::kBytes;  // of two steps, [columns][32 keys] bf16
+  uint8_t* const p_lds = lds + 4 * T::kBytes;  // of two steps, [columns][32 keys] bf16
   constexpr int kP = kCols * kKeys * 2;
   // [two steps][2 halves of the keys][columns]
   float* const tops = reinterpret_cast<float*>(p_lds + 2 * kP);
@@ -238,35 +216,28 @@ __attribute__((amdgpu_waves_per_eu(1, 1))) void latent_decode_kernel(
   const float s2 = A.scale_log2 * vsc;
   const float abs_s2 = __builtin_fabsf(s2);
   const uint32_t flip = s2 < 0.f ? 0x80008000u : 0u;
-  const int half = wave * kMoves / (T::kMoves / 2);
-  const int move0 = wave * kMoves % (T::kMoves / 2);  // of the half
-  uint32_t src[kMoves];
+  // A wave loads eight rows of a tile.
+  uint32_t src[kFp8 ? 1 : kMoves];
 #pragma unroll
-  for (int m = 0; m < kMoves; ++m) src[m] = T::template source<kFp8 ? 1 : 2>(move0 + m, lane);
-  const uint32_t dst0 = half * (T::kBytes / 2) + move0 * 1024;
+  for (int m = 0; m < (kFp8 ? 1 : kMoves); ++m)
+    src[m] = kFp8 ? lane : T::source(m, lane, wave & 1);
   const uint32_t lds0 = lds_addr_of(lds);
   // 16 bytes (8 keys) of a column's weights, their pieces permuted against bank conflicts.
   auto p_at = [&](int col, int key) {
     return p_lds + col * 64 + 16 * (((key >> 3) ^ (col >> 2)) & 3) + 2 * (key & 7);
   };
 
-  auto body = [&](int b, const SeqRows& sr, const LineItems& x, int it, int s_lo, int s_hi,
-                  int64_t slot) {
-    // Row, first head and visible keys of the units; one that there is not has no heads.
-    int row_i[kUnits], head0[kUnits], hi[kUnits];
-#pragma unroll
-    for (int u = 0; u < kUnits; ++u) {
-      const int unit = min(it * kUnits + u, sr.rows * A.head_blocks - 1);
-      int none;
-      row_i[u] = unit / A.head_blocks;
-      head0[u] = it * kUnits + u > unit ? A.num_heads
-                                        : 32 * (unit - row_i[u] * A.head_blocks);
-      row_keys(sr, row_i[u], -1, none, hi[u]);
-      hi[u] = uniform(hi[u]);
-    }
-    const int all_hi = min(hi[0], hi[kUnits - 1]);
-    const int su = kUnits == 2 ? cs : 0;  // unit of S's columns
-    const int my_hi = su ? hi[kUnits - 1] : hi[0];
+  // One go at the steps [s_lo, s_hi) of a part: returns where it stopped, s_hi or where the maxima
+  // ask for other references.  Its state goes to slot `to`, or for -1 to the output, if it got to the
+  // end, otherwise to `spare` (`to` itself if that is a slot); `more`: merged with the one there.
+  auto attempt = [&](int b, const SeqRows& sr, const LineItems& x, int it, int s_lo, int s_hi,
+                     int64_t to, int64_t spare, bool more) -> int {
+    // kUnits blocks of 32 heads of one query row, which sees keys [0, hi).
+    const int items = (A.head_blocks + kUnits - 1) / kUnits;  // of a row
+    const int row = it / items, head0 = 32 * kUnits * (it - row * items);
+    int none, hi;
+    row_keys(sr, row, -1, none, hi);
+    hi = uniform(hi);
     const int s_col = 16 * kCB * cs + r;  // first of S's columns
     floatx16_t o[kUnits][kOb];  // dims 32 d + i % 4 + 8 (i / 4) + 4 kh of column n of unit u
 #pragma unroll
@@ -287,67 +258,98 @@ __attribute__((amdgpu_waves_per_eu(1, 1))) void latent_decode_kernel(
     const Halves keys{A.cache, (R + P) * (kFp8 ? 1 : 2), bt + b * A.bt_row_stride, A.bt_width,
                       A.block_size_log2, A.num_blocks};
     const int steps = s_hi - s_lo;
-    // The pages of the next 32 steps' halves, a lane each; and which of them, and of the 32
-    // steps before, there are.
+    // The pages of 32 steps' halves, a lane each; and which of them, and of the 32 steps before,
+    // there are.
     int pages = -1, looked_up = -1;
     uint64_t there = 0, there_before = 0;
-    uint2 raw[kFp8 ? kMoves : 1];
-    // This wave's loads of step s: where from, and bf16: where to.
+    auto known = [&](int s) { return min(s, steps - 1) / 32 == looked_up; };
+    auto look_up = [&](int s) {  // before the loads of step s
+      if (known(s)) return;
+      looked_up = min(s, steps - 1) / 32;
+      pages = keys.page((static_cast<int64_t>(s_lo) + 32 * looked_up) * kKeys + 16 * lane, x.to);
+      there_before = there;
+      there = __ballot(pages >= 0);
+    };
+    // Keys that the row sees of eight rows of step s, from its key `at` on.
+    auto seen = [&](int s, int at) -> int {
+      const uint64_t t = s / 32 == looked_up ? there : there_before;
+      return t >> (2 * (s & 31) + (at >> 4)) & 1 ? hi - ((s_lo + s) * kKeys + at) : 0;
+    };
+    // This wave's loads of step s (past the end, once more of the last: as many are on their way):
+    // where from, and where to.
     struct Moves {
       const uint8_t* from;
       uint32_t to;
     };
     auto moves_of = [&](int s) {
-      s = min(s, steps - 1);  // (past the end, once more: as many loads are on their way)
-      const int key0 = (s_lo + s) * kKeys;
-      if (s / 32 != looked_up) {
-        looked_up = s / 32;
-        pages = keys.page(static_cast<int64_t>(key0) + 16 * lane, x.to);
-        there_before = there;
-        there = __ballot(pages >= 0);
-      }
-      const int pg = __builtin_amdgcn_readlane(pages, 2 * (s & 31) + half);
-      return Moves{keys.rows(pg, key0 + 16 * half), lds0 + (s % kBuffers) * T::kBytes + dst0};
+      const int t = min(s, steps - 1);
+      const int key = (s_lo + t) * kKeys + 8 * wave;
+      const int pg = __builtin_amdgcn_readlane(pages, 2 * (t & 31) + (wave >> 1));
+      const uint32_t to = kFp8 ? 3 * T::kBytes + ((s & 1) * 4 + wave) * kCodes
+                               : s % kBuffers * T::kBytes + wave * (T::kBytes / 4);
+      return Moves{keys.rows(pg, key), lds0 + to};
     };
-    // Issues the i-th of them: bf16 into LDS, fp8 into raw.
+    constexpr int kLoads = kFp8 ? kCodeMoves : kMoves;
     auto issue = [&](const Moves& m, int i) {
-      if constexpr (kFp8)
-        raw[i] = ld8(m.from + src[i]);
-      else
+      if constexpr (!kFp8)
         lds_load16(m.from, src[i], m.to + 1024 * i);
+      else if (i < kWide)
+        lds_load16(m.from + 1024 * i, 16 * src[0], m.to + 1024 * i);
+      else
+        lds_load4(m.from + 1024 * kWide + 256 * (i - kWide), 4 * src[0],
+                  m.to + 1024 * kWide + 256 * (i - kWide));
     };
     auto load = [&](int s) {
       const Moves m = moves_of(s);
 #pragma unroll
-      for (int i = 0; i < kMoves; ++i) issue(m, i);
+      for (int i = 0; i < kLoads; ++i) issue(m, i);
     };
-    // fp8: what was loaded, as bf16, into step s's buffer.
-    auto put = [&](int s) {
-      uint8_t* const dst = lds + (s % kBuffers) * T::kBytes + dst0 + 16 * lane;
+    // Keys that the row does not see may hold anything, infinities and NaN among it, which a zero
+    // weight would not undo: their rows become zeros.  bf16: among this wave's rows of step s.
+    auto clear = [&](int s) {
+      const int n = seen(s, 8 * wave);
+      if (n >= 8) return;
+      uint8_t* const at = lds + s % kBuffers * T::kBytes + wave * (T::kBytes / 4) + 16 * lane;
 #pragma unroll
-      for (int i = 0; i < (kFp8 ? kMoves : 0); ++i) {
-        const uint2 a = fp8x4_to_bf16x4(raw[i].x), c = fp8x4_to_bf16x4(raw[i].y);
-        *reinterpret_cast<uint4*>(dst + 1024 * i) = make_uint4(a.x, a.y, c.x, c.y);
-      }
+      for (int i = 0; i < kMoves; ++i)
+        if (64 * i + lane >= max(n, 0) * T::kPieces)
+          *reinterpret_cast<uint4*>(at + 1024 * i) = make_uint4(0, 0, 0, 0);
     };
-    auto halves_of = [&](int s) -> uint32_t {
-      return (s / 32 == looked_up ? there : there_before) >> (2 * (s & 31)) & 3;
+    // fp8: this wave's codes of step s, which have come, become a tile's rows; the i-th 512 bytes.
+    // (Piece 64 i + lane of the eight rows: bytes 8 (64 i + lane) of the codes.)
+    uint32_t row_at[kFp8 ? kMoves : 1];
+#pragma unroll
+    for (int i = 0; i < (kFp8 ? kMoves : 0); ++i) {
+      const int piece = 64 * i + lane;
+      row_at[i] = T::at(8 * wave + piece / T::kPieces, piece % T::kPieces);
+    }
+    auto codes = [&](int s, int i) {
+      return *reinterpret_cast<const uint2*>(lds + 3 * T::kBytes + ((s & 1) * 4 + wave) * kCodes +
+                                             8 * lane + 512 * i);
     };
-    // Whether every column sees all keys of step s.
-    auto whole = [&](int s) { return (s_lo + s + 1) * kKeys <= all_hi && halves_of(s) == 3; };
-
+    auto convert = [&](int s, int n, int i, uint2 v) {
+      const bool ok = lane < n * T::kPieces - 64 * i;
+      v = make_uint2(ok ? v.x : 0, ok ? v.y : 0);
+      const uint2 a = fp8x4_to_bf16x4(v.x), c = fp8x4_to_bf16x4(v.y);
+      *reinterpret_cast<uint4*>(lds + s % kBuffers * T::kBytes + row_at[kFp8 ? i : 0]) =
+          make_uint4(a.x, a.y, c.x, c.y);
+    };
+    auto convert_all = [&](int s) {
+      const int n = min(max(seen(s, 8 * wave), 0), 8);
+#pragma unroll
+      for (int i = 0; i < kMoves; ++i) convert(s, n, i, codes(s, i));
+    };
     // The first steps' loads, and the queries behind them.
+    look_up(0);
     load(0);
-    if constexpr (kFp8) put(0);
     load(1);
     bf16x8_t qb[kCB][kKc];
 #pragma unroll
     for (int cb = 0; cb < kCB; ++cb) {
-      const int h = (su ? head0[kUnits - 1] : head0[0]) + (s_col + 16 * cb) % 32;
+      const int h = head0 + s_col + 16 * cb;
       const bool ok = h < A.num_heads;
       const uint16_t* const qp =
-          A.q + (sr.row0 + (su ? row_i[kUnits - 1] : row_i[0])) * A.q_row_stride +
-          (ok ? h : 0) * A.q_head_stride + 8 * g;
+          A.q + (sr.row0 + row) * A.q_row_stride + (ok ? h : 0) * A.q_head_stride + 8 * g;
 #pragma unroll
       for (int k = 0; k < kKc; ++k) {
         uint4 v = ok ? *reinterpret_cast<const uint4*>(qp + 32 * k) : make_uint4(0, 0, 0, 0);
@@ -392,13 +394,12 @@ __attribute__((amdgpu_waves_per_eu(1, 1))) void latent_decode_kernel(
     // (The weights are rounded to bf16 for P V, 2^-9 relative at most, of either sign; their sum
     // is of the unrounded ones.)
     auto logits = [&](int s, floatx4_t (&p)[kCB]) {
-      // (keys that this lane's column sees, from its first one on; without a branch, which would
-      // part the products around it)
-      const int seen = halves_of(s) >> ts & 1 ? my_hi - ((s_lo + s) * kKeys + 16 * ts + 4 * g) : 0;
+      // (without a branch, which would part the products around it)
+      const int n = seen(s, 16 * ts) - 4 * g;
 #pragma unroll
       for (int cb = 0; cb < kCB; ++cb)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) p[cb][i] = i < seen ? p[cb][i] * abs_s2 : kNegInf;
+        for (int i = 0; i < 4; ++i) p[cb][i] = i < n ? p[cb][i] * abs_s2 : kNegInf;
     };
     auto maxima = [&](int s, const floatx4_t (&p)[kCB]) {
 #pragma unroll
@@ -416,31 +417,12 @@ __attribute__((amdgpu_waves_per_eu(1, 1))) void latent_decode_kernel(
       *reinterpret_cast<uint2*>(p_at(s_col + 16 * cb, 16 * ts + 4 * g) + (s & 1) * kP) =
           make_uint2(pack2(e[0], e[1]), pack2(e[2], e[3]));
     };
-    // Whether a maximum is too far above its reference (uniform: every wave has the same ones);
-    // then the references move and the step's weights are made again.
+    // Whether a maximum is too far above its reference (uniform: every wave has the same ones).
     auto too_far = [&](const float (&t)[kUnits]) {
       bool far = false;
 #pragma unroll
-      for (int u = 0; u < kUnits; ++u) far |= t[u] > mo[u] + kLazyMax;
+      for (int u = 0; u < kUnits; ++u) far |= t[u] > mo[u] + kFar;
       return __ballot(far) != 0;
-    };
-    auto move = [&](int s, const floatx4_t (&p)[kCB], const float (&t)[kUnits]) {
-#pragma unroll
-      for (int u = 0; u < kUnits; ++u) {
-        const float m_new = fmaxf(mo[u], t[u]);
-        scale_acc(o[u], __builtin_amdgcn_exp2f(mo[u] - m_new));
-        mo[u] = m_new;
-      }
-      const float* const top = tops + (s & 1) * 2 * kCols;
-#pragma unroll
-      for (int cb = 0; cb < kCB; ++cb) {
-        const int c = s_col + 16 * cb;
-        const float m_new = fmaxf(ms[cb], fmaxf(top[c], top[kCols + c]));
-        l[cb] *= __builtin_amdgcn_exp2f(ms[cb] - m_new);
-        ms[cb] = m_new;
-        weights(s, p, cb);
-      }
-      __syncthreads();
     };
     auto count = [&] {
 #pragma unroll
@@ -482,26 +464,8 @@ __attribute__((amdgpu_waves_per_eu(1, 1))) void latent_decode_kernel(
         f.v[j] = v_operand(lds + (s % kBuffers) * T::kBytes, j);
     };
     // (among(x): what to do among the products of the x-th quarter)
-    auto values = [&](int s, const First& f, auto is_masked, auto among) {
-      constexpr bool kMasked = decltype(is_masked)::value;
+    auto values = [&](int s, const First& f, auto among) {
       const uint8_t* const tile = lds + (s % kBuffers) * T::kBytes;
-      // Keys that the row does not see may hold anything, infinities and NaN among it: zeros.
-      uint32_t mask[2][kUnits][4];
-      if constexpr (kMasked) {
-        const uint32_t halves = halves_of(s);
-#pragma unroll
-        for (int k = 0; k < 2; ++k)
-#pragma unroll
-          for (int u = 0; u < kUnits; ++u) {
-            uint32_t bits = 0;
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-              const int t = (s_lo + s) * kKeys + 16 * k + 8 * kh + i;
-              bits |= (halves >> k & 1) && t < hi[u] ? 1u << i : 0u;
-            }
-            word_masks(bits, mask[k][u]);
-          }
-      }
       bf16x8_t v[2][kVGroup];
 #pragma unroll
       for (int j = 0; j < kVGroup; ++j) v[0][j] = f.v[j];
@@ -518,8 +482,8 @@ __attribute__((amdgpu_waves_per_eu(1, 1))) void latent_decode_kernel(
           const int k = (x0 + j) / kOb, d = (x0 + j) % kOb;
 #pragma unroll
           for (int u = 0; u < kUnits; ++u)
-            o[u][d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(
-                kMasked ? masked(v[now][j], mask[k][u]) : v[now][j], f.w[k][u], o[u][d], 0, 0, 0);
+            o[u][d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(v[now][j], f.w[k][u], o[u][d], 0, 0,
+                                                              0);
         }
         among(x0 / kVGroup);
       }
@@ -527,12 +491,15 @@ __attribute__((amdgpu_waves_per_eu(1, 1))) void latent_decode_kernel(
 
     floatx4_t p[kCB], next[kCB];
     // A step's barrier: step s's weights and maxima and step s + 1's tile are in LDS, and step
-    // s - 1 is done with.  Its loads, of step s + 3, are issued among its products, so that the
-    // waves do not wait for their addresses to be taken.
+    // s - 1 is done with.  The loads (bf16: of step s + 3, fp8: of s + 4, with the conversion of
+    // s + 2) are issued among its products, so that the waves do not wait for their addresses to
+    // be taken.
     auto enter = [&](int s, float (&t)[kUnits]) {
-      if constexpr (!kFp8) wait_loads<kMoves>();
+      if constexpr (!kFp8) {
+        wait_loads<kLoads>();
+        clear(s + 1);
+      }
       __syncthreads();
-      if constexpr (kFp8) put(s + 2);
 #pragma unroll
       for (int u = 0; u < kUnits; ++u) {
         const float* const top = tops + (s & 1) * 2 * kCols + 32 * u + n;
@@ -542,15 +509,22 @@ __attribute__((amdgpu_waves_per_eu(1, 1))) void latent_decode_kernel(
     const auto nothing = [](int) {};
     float t[kUnits];
     First f;
-    if constexpr (!kFp8) wait_loads<0>();
+    __builtin_amdgcn_s_waitcnt(kNoLoads);
+    if constexpr (kFp8) {
+      convert_all(0);
+      convert_all(1);
+      load(2);
+      load(3);
+    } else {
+      clear(0);
+      load(2);
+    }
     __syncthreads();
-    if constexpr (kFp8) put(1);
-    load(2);
     scores(0, p, nothing);
     logits(0, p);
     maxima(0, p);
     __syncthreads();
-    // The first references.
+    // The references.
 #pragma unroll
     for (int u = 0; u < kUnits; ++u) {
       const int c = s_col + 16 * u;
@@ -559,49 +533,65 @@ __attribute__((amdgpu_waves_per_eu(1, 1))) void latent_decode_kernel(
       weights(0, p, u);
     }
     enter(0, t);
+    constexpr int kAhead = kFp8 ? 4 : 3;
     int s = 0;
 #pragma unroll 1
-    while (true) {  // (step s has been entered)
-      if (too_far(t)) move(s, p, t);
-      if (s + 1 < steps && whole(s)) {
-        // The steps that need nothing special, in a loop of their own: where such a step met
-        // another, the compiler would copy O around.
+    while (s + 1 < steps && !too_far(t)) {  // (step s has been entered)
+      look_up(s + kAhead);
+      // (The wait, which the compiler knows of, as it does not of the loads into LDS: with a load
+      // of its own unfinished here it would wait for it in the loop, and with it for those.)
+      __builtin_amdgcn_s_waitcnt(kNoLoads);
 #pragma unroll 1
-        do {
-          count();
-          const Moves m = moves_of(s + 3);
-          scores(s + 1, next, [&](int x) {
-            issue(m, x);
-            if (x == kKc / kGroup - 1) first_operands(s, f);
-          });
-          constexpr int kDone = kKc / kGroup;
-          static_assert(kDone <= kMoves && kDone + 8 >= kMoves, "every load is issued once");
-          values(s, f, std::false_type{}, [&](int x) {
-            if (x == 0) logits(s + 1, next);
-            if (x == 1) maxima(s + 1, next);
-            if (x >= 2 && x - 2 < kCB) weights(s + 1, next, x - 2);
-#pragma unroll
-            for (int i = 0; i < 2; ++i)
-              if (kDone + 2 * x + i < kMoves) issue(m, kDone + 2 * x + i);
-          });
-#pragma unroll
-          for (int cb = 0; cb < kCB; ++cb) p[cb] = next[cb];
-          ++s;
-          enter(s, t);
-        } while (s + 1 < steps && whole(s) && !too_far(t));
-      } else {
+      do {
         count();
-        load(s + 3);
-        first_operands(s, f);
-        values(s, f, std::true_type{}, nothing);
-        if (++s == steps) break;
-        scores(s, p, nothing);
-        logits(s, p);
-        maxima(s, p);
+        const Moves m = moves_of(s + kAhead);
+        constexpr int kGroups = kKc / kGroup;
+        int rows = 0;
+        uint2 raw[3];  // codes on their way from LDS
+        if constexpr (kFp8) {
+          wait_loads<kLoads>();
+          rows = min(max(seen(s + 2, 8 * wave), 0), 8);
 #pragma unroll
-        for (int cb = 0; cb < kCB; ++cb) weights(s, p, cb);
+          for (int i = 0; i < 3; ++i) raw[i] = codes(s + 2, i);
+        }
+        scores(s + 1, next, [&](int x) {
+          if constexpr (kFp8) {
+            convert(s + 2, rows, x, raw[x % 3]);
+            raw[x % 3] = codes(s + 2, x + 3);
+          } else {
+            issue(m, x);
+          }
+          if (x == kGroups - 1) first_operands(s, f);
+        });
+        values(s, f, [&](int x) {
+          if (x == 0) logits(s + 1, next);
+          if (x == 1) maxima(s + 1, next);
+          if (x >= 2 && x - 2 < kCB) weights(s + 1, next, x - 2);
+          if constexpr (kFp8) {
+            if (x < kMoves - kGroups) convert(s + 2, rows, kGroups + x, raw[x]);
+            if (x == 3) {
+              // (the codes have been read, whose place the loads take)
+              __builtin_amdgcn_sched_barrier(0);
+              asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+#pragma unroll
+              for (int i = 0; i < kLoads; ++i) issue(m, i);
+            }
+          } else if (x < kMoves - kGroups) {
+            issue(m, kGroups + x);
+          }
+        });
+        static_assert(kGroups % 3 == 0 && kMoves - kGroups == 3, "all of them once");
+        p[0] = next[0];
+        if constexpr (kCB == 2) p[1] = next[1];
+        ++s;
         enter(s, t);
-      }
+      } while (s + 1 < steps && !too_far(t) && known(s + kAhead));
+    }
+    if (!too_far(t)) {
+      count();
+      first_operands(s, f);
+      values(s, f, nothing);
+      ++s;
     }
     wait_loads<0>();
     __syncthreads();
@@ -610,42 +600,66 @@ __attribute__((amdgpu_waves_per_eu(1, 1))) void latent_decode_kernel(
     // theirs, and O, which leaves in whole rows.
     constexpr int kRow = R + 4;  // floats
     float* const xo = reinterpret_cast<float*>(lds);
-    static_assert(4 * kCols * kRow <= kBuffers * T::kBytes, "O fits");
+    static_assert(4 * kCols * kRow <= 4 * T::kBytes, "O fits");
 #pragma unroll
-    for (int cb = 0; cb < kCB; ++cb) {
-      l[cb] = pair_sum(l[cb]);
-      tops[kCols * ts + s_col + 16 * cb] = l[cb];
-    }
+    for (int cb = 0; cb < kCB; ++cb) tops[kCols * ts + s_col + 16 * cb] = pair_sum(l[cb]);
 #pragma unroll
     for (int u = 0; u < kUnits; ++u) {
       if (wave == 0) tops[2 * kCols + 32 * u + n] = mo[u];
-      float* const to = xo + (32 * u + n) * kRow + wave * (R / 4) + 4 * kh;
+      float* const at = xo + (32 * u + n) * kRow + wave * (R / 4) + 4 * kh;
 #pragma unroll
       for (int d = 0; d < kOb; ++d)
 #pragma unroll
         for (int i = 0; i < 4; ++i)
-          *reinterpret_cast<float4*>(to + 32 * d + 8 * i) = make_float4(
+          *reinterpret_cast<float4*>(at + 32 * d + 8 * i) = make_float4(
               o[u][d][4 * i], o[u][d][4 * i + 1], o[u][d][4 * i + 2], o[u][d][4 * i + 3]);
     }
     __syncthreads();
+    const bool last_go = s == steps;
+    const int64_t slot = last_go ? to : spare;
 #pragma unroll 4
     for (int i = threadIdx.x; i < kCols * (R / 4); i += kThreads) {
       const int c = i / (R / 4), dim = 4 * (i % (R / 4));
-      const int u = c / 32, head = (u ? head0[kUnits - 1] : head0[0]) + c % 32;
+      const int head = head0 + c;
       if (head >= A.num_heads) continue;
-      const float4 z = *reinterpret_cast<const float4*>(xo + c * kRow + dim);
-      const float L = tops[c] + tops[kCols + c], M = tops[2 * kCols + c];
+      Folded f;
+      f.o = *reinterpret_cast<const float4*>(xo + c * kRow + dim);
+      f.L = tops[c] + tops[kCols + c];
+      f.M = tops[2 * kCols + c];
+      if (more) {
+        const float2 y = *reinterpret_cast<const float2*>(A.ml + (spare * kCols + c) * 2);
+        f.add(y.x, y.y, *reinterpret_cast<const float4*>(A.o + (spare * kCols + c) * R + dim));
+      }
       if (slot < 0) {
-        write_out(A, sr.row0 + (u ? row_i[kUnits - 1] : row_i[0]), head, dim, z, M, L, vsc);
+        write_out(A, sr.row0 + row, head, dim, f.o, f.M, f.L, vsc);
       } else {
-        *reinterpret_cast<float4*>(A.o + (slot * kCols + c) * R + dim) = z;
-        if (dim == 0)
-          *reinterpret_cast<float2*>(A.ml + (slot * kCols + c) * 2) = make_float2(M, L);
+        *reinterpret_cast<float4*>(A.o + (slot * kCols + c) * R + dim) = f.o;
       }
     }
+    __syncthreads();  // (the state before has been read)
+    if (slot >= 0 && threadIdx.x < kCols) {
+      const int c = threadIdx.x;
+      Folded f;
+      f.reset();
+      f.L = tops[c] + tops[kCols + c];
+      f.M = tops[2 * kCols + c];
+      float2* const ml = reinterpret_cast<float2*>(A.ml + (slot * kCols + c) * 2);
+      if (more) f.add(ml->x, ml->y, f.o);
+      *ml = make_float2(f.M, f.L);
+    }
     __syncthreads();
+    return s_lo + s;
   };
-  walk_line<kThreads>(line, A.batch, A.wgs, blockIdx.x, 1, A.records,
+  auto body = [&](int b, const SeqRows& sr, const LineItems& x, int it, int s_lo, int s_hi,
+                  int64_t slot, int64_t free_slot) {
+    const int64_t spare = slot >= 0 ? slot : free_slot;
+    bool more = false;
+    while (s_lo < s_hi) {
+      s_lo = attempt(b, sr, x, it, s_lo, s_hi, slot, spare, more);
+      more = true;
+    }
+  };
+  walk_line(line, A.batch, A.wgs, blockIdx.x, 1, A.records,
                       [&](int b) { return seq_rows(cu, ctx_lens, b, A.rows, A.most); },
                       [&](const SeqRows& s) { return line_items(A, s, kUnits); }, body);
 }
@@ -666,17 +680,16 @@ __global__ __launch_bounds__(kMergeThreads) void latent_merge_kernel(
   const LineRecord rec = A.records[b];
   const float vsc = fp8 && A.cache_scale ? *A.cache_scale : 1.f;
   const int h0 = blockIdx.x * heads, h1 = min(h0 + heads, A.num_heads);
-  // Unit by unit of the row's heads.
+  // Item by item of the row.
   for (int h = h0; h < h1;) {
-    const int unit = i * A.head_blocks + h / 32;
-    const int in = 32 * (unit % A.units) + h % 32;
-    const int nc = min(h1, (h / 32 + 1) * 32) - h;
-    const LinePieces pieces(rec, unit / A.units);
+    const int per = 32 * A.units, block = h / per;
+    const int in = h - block * per, nc = min(h1, (block + 1) * per) - h;
+    const LinePieces pieces(rec, i * ((A.head_blocks + A.units - 1) / A.units) + block);
     if (pieces.n > 1) {
       merge_pieces<kDims>(
           0, nc, folded, [&](int) { return pieces.n; },
           [&](int k, int x, const float*& ml, const float*& o) {
-            const int64_t at = pieces.slot(k) * (32 * A.units) + in + x;
+            const int64_t at = pieces.slot(k) * per + in + x;
             ml = A.ml + 2 * at;
             o = A.o + at * R + dim0;
           },
@@ -695,7 +708,7 @@ struct LatentPlan {
 };
 LatentPlan plan_of(int64_t batch, int64_t max_seqlen_q, int num_heads, int latent_size) {
   LatentPlan p{};
-  p.units = max_seqlen_q * ((num_heads + 31) / 32) > 1 ? 2 : 1;
+  p.units = num_heads > 32 ? 2 : 1;
   p.wgs = num_cus();
   auto take = [&](int64_t bytes) {
     const int64_t at = p.bytes;
@@ -711,7 +724,7 @@ LatentPlan plan_of(int64_t batch, int64_t max_seqlen_q, int num_heads, int laten
 template <int R, int P, bool kFp8>
 void launch(const LatentParams& A, hipStream_t s, const int32_t* bt, const int32_t* ctx,
             const int32_t* cu) {
-  const unsigned lds = kBuffers * Tile<R, P>::kBytes + 2 * 32 * A.units * (kKeys * 2 + 2 * 4);
+  const unsigned lds = 4 * Tile<R, P>::kBytes + 2 * 32 * A.units * (kKeys * 2 + 2 * 4);
   if (A.units == 1)
     hipLaunchKernelGGL((latent_decode_kernel<R, P, 1, kFp8>), dim3(A.wgs + 1), dim3(kThreads),
                        lds, s, A, bt, ctx, cu);

@@ -105,21 +105,22 @@ __device__ __forceinline__ int64_t line_slot(int64_t wg, bool begins) {
   return 2 * wg + (begins ? 1 : 0);
 }
 
-// What walk_line holds in LDS.
-template <int kThreads>
+// What walk_line holds in LDS: kSeqs sequences at a time.
+template <int kThreads, int kSeqs = kThreads>
 struct LineLds {
-  SeqRows seq[kThreads];
+  SeqRows seq[kSeqs];
   int64_t sum[kThreads / 64];
-  uint64_t hits[kThreads / 64];
+  uint64_t hits[kSeqs / 64];
 };
 
 // Walks the share of work-group `wg` of `wgs` on the line of `batch` sequences, seq_at(b) their
-// rows and items_of(rows) their items: body(b, rows, items, item, first step, end step, slot) for
-// each item's part in it, uniform over the work-group; slot: -1 where the part is the whole item,
-// otherwise where its partial state goes.  Work-group wgs writes every sequence's record instead.
+// rows and items_of(rows) their items: body(b, rows, items, item, first step, end step, slot, free)
+// for each item's part in it, uniform over the work-group; slot: -1 where the part is the whole
+// item, otherwise where its partial state goes; free: a slot that is not in use yet where the part
+// is a whole item.  Work-group wgs writes every sequence's record instead.
 // Every thread of the work-group calls it; items have at least one step.
-template <int kThreads, class SeqAt, class ItemsOf, class Body>
-__device__ __forceinline__ void walk_line(LineLds<kThreads>& lds, int batch, int wgs, int wg,
+template <int kThreads, int kSeqs, class SeqAt, class ItemsOf, class Body>
+__device__ __forceinline__ void walk_line(LineLds<kThreads, kSeqs>& lds, int batch, int wgs, int wg,
                                           int quantum, LineRecord* __restrict__ records,
                                           SeqAt seq_at, ItemsOf items_of, Body body) {
   constexpr int kWaves = kThreads / 64;
@@ -140,7 +141,7 @@ __device__ __forceinline__ void walk_line(LineLds<kThreads>& lds, int batch, int
   };
   auto at = [&](int b) {
     SeqRows x{};
-    if (b < batch) x = seq_at(b);
+    if (tid < kSeqs && b < batch) x = seq_at(b);
     return x;
   };
   auto length = [&](const SeqRows& x) {
@@ -148,9 +149,8 @@ __device__ __forceinline__ void walk_line(LineLds<kThreads>& lds, int batch, int
     const LineItems it = items_of(x);
     return static_cast<int64_t>(it.steps) * it.items;
   };
-  const SeqRows first = at(tid);
-  int64_t sum = length(first), total;
-  for (int b = kThreads + tid; b < batch; b += kThreads) sum += length(at(b));
+  int64_t sum = 0, total;
+  for (int b = tid; b < batch; b += kSeqs) sum += length(at(b));
   scan_all(sum, total);
   if (total == 0) return;
   const int64_t S = range_of(total, wgs, quantum);
@@ -159,8 +159,8 @@ __device__ __forceinline__ void walk_line(LineLds<kThreads>& lds, int batch, int
   const int64_t t_lo = writes ? 0 : w * S;
   const int64_t t_hi = writes ? total : min(total, t_lo + S);
   int64_t line = 0;
-  for (int b0 = 0; t_lo < total && b0 < batch && line < t_hi; b0 += kThreads) {
-    SeqRows x = b0 == 0 ? first : at(b0 + tid);
+  for (int b0 = 0; t_lo < total && b0 < batch && line < t_hi; b0 += kSeqs) {
+    SeqRows x = at(b0 + tid);
     const int64_t mine = length(x);
     const int64_t end = line + scan_all(mine, sum);
     line += sum;
@@ -172,10 +172,10 @@ __device__ __forceinline__ void walk_line(LineLds<kThreads>& lds, int batch, int
     const bool in = mine > 0 && end > t_lo && x.start < t_hi;
     if (in) lds.seq[tid] = x;
     const uint64_t hits = __ballot(in);
-    if (lane == 0) lds.hits[wave] = hits;
+    if (lane == 0 && wave < kSeqs / 64) lds.hits[wave] = hits;
     __syncthreads();
 #pragma unroll 1
-    for (int k = 0; k < kWaves; ++k) {
+    for (int k = 0; k < kSeqs / 64; ++k) {
       uint64_t hit = lane64(lds.hits[k], 0);
       while (hit) {
         const int src = 64 * k + __builtin_ctzll(hit);
@@ -193,7 +193,8 @@ __device__ __forceinline__ void walk_line(LineLds<kThreads>& lds, int batch, int
           const int lo = static_cast<int>(max(t_lo, s0) - s0);
           const int hi = static_cast<int>(min(t_hi, s0 + z.steps) - s0);
           const bool whole = lo == 0 && hi == z.steps;
-          body(b0 + src, y, z, it, lo, hi, whole ? int64_t{-1} : line_slot(w, lo == 0));
+          body(b0 + src, y, z, it, lo, hi, whole ? int64_t{-1} : line_slot(w, lo == 0),
+               line_slot(w, true));
         }
       }
     }

@@ -191,7 +191,7 @@ __attribute__((amdgpu_waves_per_eu(2))) void mxfp4_decode_kernel(
     return x;
   };
   auto body = [&](int b, const SeqRows& sr, const LineItems& x, int it, int s_lo, int s_hi,
-                  int64_t slot) {
+                  int64_t slot, int64_t) {
     const int col_items = x.items / A.num_kv_heads;
     const int kvh = it / col_items;
     const int col0 = (it - kvh * col_items) * kCols;
@@ -335,7 +335,7 @@ __attribute__((amdgpu_waves_per_eu(2))) void mxfp4_decode_kernel(
                         });
     __syncthreads();
   };
-  walk_line<kThreads>(line, A.batch, P.wgs, blockIdx.x, kWaves, P.records,
+  walk_line(line, A.batch, P.wgs, blockIdx.x, kWaves, P.records,
                       [&](int b) { return seq_rows(cu, ctx_lens, b, P.rows, P.most); }, items_of,
                       body);
 }
