@@ -26,6 +26,7 @@ constexpr int kWaves = 4;
 constexpr int kThreads = kWaves * 64;
 constexpr int kSeqs = 128;   // sequences looked at together
 constexpr int kKeys = 32;    // of a tile
+constexpr int kPad = 14;     // what a part costs besides its steps, in steps
 // (Weights to 2^32: with values up to 2^90 their sums stay finite.  No logits of trained models come
 // near it.)
 constexpr float kFar = 32.f;
@@ -369,8 +370,13 @@ __attribute__((amdgpu_waves_per_eu(1, 1))) void latent_decode_kernel(
 #pragma unroll
       for (int j = 0; j < kGroup; ++j)
         kx[0][j] = *reinterpret_cast<const uint4*>(at[j & 1] + 128 * (j >> 1));
+      // (two chains of products at least: one alone would wait for each result)
+      constexpr int kChains = kCB == 1 ? 2 : 1;
+      floatx4_t x[kChains][kCB];
 #pragma unroll
-      for (int cb = 0; cb < kCB; ++cb) p[cb] = floatx4_t{0.f, 0.f, 0.f, 0.f};
+      for (int c = 0; c < kChains; ++c)
+#pragma unroll
+        for (int cb = 0; cb < kCB; ++cb) x[c][cb] = floatx4_t{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
       for (int k0 = 0; k0 < kKc; k0 += kGroup) {
         const int now = k0 / kGroup & 1;
@@ -386,9 +392,13 @@ __attribute__((amdgpu_waves_per_eu(1, 1))) void latent_decode_kernel(
         for (int j = 0; j < kGroup; ++j)
 #pragma unroll
           for (int cb = 0; cb < kCB; ++cb)
-            p[cb] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(
-                __builtin_bit_cast(bf16x8_t, kx[now][j]), qb[cb][k0 + j], p[cb], 0, 0, 0);
+            x[j % kChains][cb] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(
+                __builtin_bit_cast(bf16x8_t, kx[now][j]), qb[cb][k0 + j], x[j % kChains][cb], 0,
+                0, 0);
       }
+#pragma unroll
+      for (int cb = 0; cb < kCB; ++cb)
+        p[cb] = kChains == 1 ? x[0][cb] : x[0][cb] + x[kChains - 1][cb];
     };
     // The softmax of step s, in four parts: logits, their maxima, weights.
     // (The weights are rounded to bf16 for P V, 2^-9 relative at most, of either sign; their sum
@@ -538,13 +548,12 @@ __attribute__((amdgpu_waves_per_eu(1, 1))) void latent_decode_kernel(
 #pragma unroll 1
     while (s + 1 < steps && !too_far(t)) {  // (step s has been entered)
       look_up(s + kAhead);
+      Moves m = moves_of(s + kAhead);
       // (The wait, which the compiler knows of, as it does not of the loads into LDS: with a load
       // of its own unfinished here it would wait for it in the loop, and with it for those.)
       __builtin_amdgcn_s_waitcnt(kNoLoads);
 #pragma unroll 1
       do {
-        count();
-        const Moves m = moves_of(s + kAhead);
         constexpr int kGroups = kKc / kGroup;
         int rows = 0;
         uint2 raw[3];  // codes on their way from LDS
@@ -563,6 +572,8 @@ __attribute__((amdgpu_waves_per_eu(1, 1))) void latent_decode_kernel(
           }
           if (x == kGroups - 1) first_operands(s, f);
         });
+        if (too_far(t)) break;  // (looked at behind the products that do not depend on it)
+        count();
         values(s, f, [&](int x) {
           if (x == 0) logits(s + 1, next);
           if (x == 1) maxima(s + 1, next);
@@ -579,13 +590,14 @@ __attribute__((amdgpu_waves_per_eu(1, 1))) void latent_decode_kernel(
           } else if (x < kMoves - kGroups) {
             issue(m, kGroups + x);
           }
+          if (x == 3) m = moves_of(s + 1 + kAhead);
         });
         static_assert(kGroups % 3 == 0 && kMoves - kGroups == 3, "all of them once");
         p[0] = next[0];
         if constexpr (kCB == 2) p[1] = next[1];
         ++s;
         enter(s, t);
-      } while (s + 1 < steps && !too_far(t) && known(s + kAhead));
+      } while (s + 1 < steps && known(s + kAhead));
     }
     if (!too_far(t)) {
       count();
@@ -659,7 +671,7 @@ __attribute__((amdgpu_waves_per_eu(1, 1))) void latent_decode_kernel(
       more = true;
     }
   };
-  walk_line(line, A.batch, A.wgs, blockIdx.x, 1, A.records,
+  walk_line(line, A.batch, A.wgs, blockIdx.x, 1, kPad, A.records,
                       [&](int b) { return seq_rows(cu, ctx_lens, b, A.rows, A.most); },
                       [&](const SeqRows& s) { return line_items(A, s, kUnits); }, body);
 }
@@ -684,7 +696,7 @@ __global__ __launch_bounds__(kMergeThreads) void latent_merge_kernel(
   for (int h = h0; h < h1;) {
     const int per = 32 * A.units, block = h / per;
     const int in = h - block * per, nc = min(h1, (block + 1) * per) - h;
-    const LinePieces pieces(rec, i * ((A.head_blocks + A.units - 1) / A.units) + block);
+    const LinePieces pieces(rec, i * ((A.head_blocks + A.units - 1) / A.units) + block, kPad);
     if (pieces.n > 1) {
       merge_pieces<kDims>(
           0, nc, folded, [&](int) { return pieces.n; },

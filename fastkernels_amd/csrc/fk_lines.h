@@ -121,7 +121,8 @@ struct LineLds {
 // Every thread of the work-group calls it; items have at least one step.
 template <int kThreads, int kSeqs, class SeqAt, class ItemsOf, class Body>
 __device__ __forceinline__ void walk_line(LineLds<kThreads, kSeqs>& lds, int batch, int wgs, int wg,
-                                          int quantum, LineRecord* __restrict__ records,
+                                          int quantum, int pad,
+                                          LineRecord* __restrict__ records,
                                           SeqAt seq_at, ItemsOf items_of, Body body) {
   constexpr int kWaves = kThreads / 64;
   const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63;
@@ -147,7 +148,7 @@ __device__ __forceinline__ void walk_line(LineLds<kThreads, kSeqs>& lds, int bat
   auto length = [&](const SeqRows& x) {
     if (x.rows == 0) return int64_t{0};
     const LineItems it = items_of(x);
-    return static_cast<int64_t>(it.steps) * it.items;
+    return static_cast<int64_t>(it.steps + pad) * it.items;
   };
   int64_t sum = 0, total;
   for (int b = tid; b < batch; b += kSeqs) sum += length(at(b));
@@ -187,11 +188,13 @@ __device__ __forceinline__ void walk_line(LineLds<kThreads, kSeqs>& lds, int bat
         y.ctx = uniform(y.ctx);
         y.start = lane64(y.start, 0);
         const LineItems z = items_of(y);
-        for (int it = t_lo > y.start ? quotient(t_lo - y.start, z.steps) : 0;
-             it < z.items && y.start + static_cast<int64_t>(it) * z.steps < t_hi; ++it) {
-          const int64_t s0 = y.start + static_cast<int64_t>(it) * z.steps;
-          const int lo = static_cast<int>(max(t_lo, s0) - s0);
-          const int hi = static_cast<int>(min(t_hi, s0 + z.steps) - s0);
+        const int length = z.steps + pad;
+        for (int it = t_lo > y.start ? quotient(t_lo - y.start, length) : 0;
+             it < z.items && y.start + static_cast<int64_t>(it) * length < t_hi; ++it) {
+          const int64_t s0 = y.start + static_cast<int64_t>(it) * length + pad;
+          const int lo = static_cast<int>(max(t_lo - s0, int64_t{0}));
+          const int hi = static_cast<int>(min(t_hi - s0, static_cast<int64_t>(z.steps)));
+          if (hi <= 0) continue;
           const bool whole = lo == 0 && hi == z.steps;
           body(b0 + src, y, z, it, lo, hi, whole ? int64_t{-1} : line_slot(w, lo == 0),
                line_slot(w, true));
@@ -207,8 +210,8 @@ __device__ __forceinline__ void walk_line(LineLds<kThreads, kSeqs>& lds, int bat
 struct LinePieces {
   int64_t first;
   int n;
-  __device__ __forceinline__ LinePieces(const LineRecord& r, int it) {
-    const int64_t s0 = r.start + static_cast<int64_t>(it) * r.steps;
+  __device__ __forceinline__ LinePieces(const LineRecord& r, int it, int pad) {
+    const int64_t s0 = r.start + static_cast<int64_t>(it) * (r.steps + pad) + pad;
     first = quotient(s0, r.range);
     n = quotient(s0 + r.steps - 1, r.range) - static_cast<int>(first) + 1;
   }

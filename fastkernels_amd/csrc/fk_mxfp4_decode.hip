@@ -26,6 +26,7 @@ namespace {
 constexpr int kWaves = 4;
 constexpr int kThreads = kWaves * 64;
 constexpr int kStep = 32;  // keys
+constexpr int kPad = 8;    // what a part costs besides its steps, in steps
 
 struct Mxfp4Params {
   PageAttnParams A;
@@ -335,7 +336,7 @@ __attribute__((amdgpu_waves_per_eu(2))) void mxfp4_decode_kernel(
                         });
     __syncthreads();
   };
-  walk_line(line, A.batch, P.wgs, blockIdx.x, kWaves, P.records,
+  walk_line(line, A.batch, P.wgs, blockIdx.x, kWaves, kPad, P.records,
                       [&](int b) { return seq_rows(cu, ctx_lens, b, P.rows, P.most); }, items_of,
                       body);
 }
@@ -363,7 +364,7 @@ __global__ __launch_bounds__(kMergeThreads) void mxfp4_merge_kernel(
     const int c = i * A.gqa + j;
     const int it = kvh * col_items + c / kCols;
     const int in = c % kCols, nc = min(j1 - j, kCols - in);
-    const LinePieces pieces(rec, it);
+    const LinePieces pieces(rec, it, kPad);
     if (pieces.n > 1) {
       merge_pieces<D>(
           0, nc, folded, [&](int) { return pieces.n; },
