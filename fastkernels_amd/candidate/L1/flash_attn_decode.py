@@ -355,3 +355,23 @@ class FlashAttnDecode(nn.Module):
                               a["cache_seqlens"], picked, a["softmax_scale"], a["k_scale"],
                               a["v_scale"], a["sinks"], cu_seqlens_q)
         return a["out"]
+
+    def forward_mxfp4(self, q, cache, cache_seqlens, cu_seqlens_q=None,
+                      max_seqlen_q: int | None = None, **kwargs):
+        """``forward`` over a 4-bit cache (an ``ops.Mxfp4Cache``, written by
+        ``StoreKVCacheMxfp4``).  One row per sequence, or the rows of cu_seqlens_q (a step that
+        checks drafted tokens), at most max_seqlen_q (then required) per sequence.  kwargs as
+        forward's (without num_splits and the fp8 scales)."""
+        what = "FlashAttnDecode.forward_mxfp4"
+        for name in ("k_scale", "v_scale", "k_descale", "v_descale"):
+            if kwargs.pop(name, None) is not None:
+                raise TypeError(f"{what}: {name}: a 4-bit cache holds its own scales")
+        k_cache, v_cache, k_scales, v_scales = cache
+        a = self._page_args(what, q, k_cache, cache_seqlens, kwargs)
+        call = torch.ops.fastkernels_amd.mxfp4_paged_decode if torch.compiler.is_compiling() \
+            else ops.mxfp4_paged_decode
+        n = q.shape[0]
+        call(self._heads(a["out"], n), self._heads(q, n), k_cache, v_cache, k_scales, v_scales,
+             a["block_table"], a["cache_seqlens"], a["softmax_scale"], a["window_left"],
+             a["sinks"], cu_seqlens_q, max_seqlen_q)
+        return a["out"]

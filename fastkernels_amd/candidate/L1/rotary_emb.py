@@ -126,6 +126,29 @@ class RotaryEmbedding(nn.Module):
              self.is_neox_style, qw, kw, float(eps))
         return query, key
 
+    def forward_store_latent(self, positions: torch.Tensor, query_rope: torch.Tensor,
+                             latent: torch.Tensor, key_rope: torch.Tensor,
+                             cache: torch.Tensor, slot_mapping: torch.Tensor,
+                             latent_norm: nn.Module | None = None,
+                             query_out: torch.Tensor | None = None,
+                             cache_scale: torch.Tensor | None = None):
+        """The latent attention block's steps between its projections and attention, in one
+        launch: ``latent_norm`` (an RMSNorm module or None) of latent [T, R], this rotation of
+        key_rope [T, head_dim] and query_rope [T, H, head_dim], and the store of [latent |
+        key_rope] in the latent cache.  query_rope goes to query_out (e.g. the last head_dim
+        columns of the absorbed queries), without one it is rewritten in place; returned."""
+        if query_out is None:
+            query_out = query_rope
+        w, eps = None, 1e-6
+        if latent_norm is not None:
+            w, eps = self._norm_weight(latent_norm, latent), latent_norm.eps
+        positions = positions.to(torch.int64).contiguous()
+        call = torch.ops.fastkernels_amd.latent_norm_rope_store if torch.compiler.is_compiling() \
+            else ops.latent_norm_rope_store
+        call(cache, slot_mapping, positions, latent, key_rope, self._cache_for(query_rope),
+             self.is_neox_style, w, float(eps), cache_scale, query_rope, query_out)
+        return query_out
+
     def forward(self, positions: torch.Tensor, query: torch.Tensor, key: torch.Tensor | None):
         cache = self.cos_sin_cache
         if cache.device != query.device:

@@ -16,6 +16,8 @@ at +-448.
 [num_blocks, num_kv_heads, page_size, head_dim], head h of token i at
 ``[slot // page_size, h, slot % page_size]``, as ``_store_kvcache_hnd_kernel``
 (store_kvcache.py:36-68); key and cache dtypes must match there.
+
+``StoreKVCacheMxfp4`` writes the rows into a 4-bit cache (``ops.new_mxfp4_cache``).
 """
 from __future__ import annotations
 
@@ -55,3 +57,13 @@ class StoreKVCacheHND(nn.Module):
                                                         slot_mapping, self.page_size)
         else:
             ops.store_kvcache_hnd(key, value, k_cache, v_cache, slot_mapping, self.page_size)
+
+
+class StoreKVCacheMxfp4(nn.Module):
+    """Store into a 4-bit cache: an ``ops.Mxfp4Cache``, or its four tensors in that order."""
+
+    def forward(self, key, value, cache, slot_mapping):
+        if torch.compiler.is_compiling():
+            torch.ops.fastkernels_amd.store_kvcache_mxfp4(key, value, *cache, slot_mapping)
+        else:
+            ops.store_kvcache_mxfp4(key, value, *cache, slot_mapping)

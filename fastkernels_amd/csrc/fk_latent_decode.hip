@@ -688,7 +688,7 @@ __global__ __launch_bounds__(kMergeThreads) void latent_merge_kernel(
   if (!query_row(cu, ctx_lens, A.batch, t, b, vis)) return;
   const SeqRows s = seq_rows(cu, ctx_lens, b, A.rows, A.most);
   const int i = t - s.row0;
-  if (i >= s.rows) return;
+  if (i < 0 || i >= s.rows) return;
   const LineRecord rec = A.records[b];
   const float vsc = fp8 && A.cache_scale ? *A.cache_scale : 1.f;
   const int h0 = blockIdx.x * heads, h1 = min(h0 + heads, A.num_heads);

@@ -21,7 +21,7 @@ struct CacheParams {
   int units;  // of 8 dims, of a token's K row
 };
 
-// Writes or reads the eight codes of unit u (dims 8 u' of head h) at a token's place.
+// Where the codes of dims `dim` .. `dim` + 7 of a token lie.
 __device__ __forceinline__ uint8_t* k_codes(const CacheParams& P, int64_t head_page, int tok,
                                             int dim) {
   return P.k_cache + ((head_page << P.block_size_log2) + tok) * (P.head_size / 2) + dim / 2;
@@ -107,38 +107,48 @@ __global__ __launch_bounds__(kThreads) void store_mxfp4_kernel(
     (is_v ? P.v_scales : P.k_scales)[scale_at(P, hp, in, dim)] = static_cast<uint8_t>(e);
 }
 
-// A wave per row of the output.
+constexpr int kGatherRows = 32;  // of a work-group: their slots are looked up side by side
+
+// A thread takes the same 8 dims of several rows, whose loads are in flight together.  50 thousand
+// tokens of 8 heads of 128: 50.6 us, 5.1 TB/s (84 with stores through the caches, which push out
+// the lines of codes that four tokens share; 79 so with a wave per row).
 __global__ __launch_bounds__(kThreads) void gather_mxfp4_kernel(
     CacheParams P, uint16_t* __restrict__ key, int64_t key_stride, uint16_t* __restrict__ value,
     int64_t value_stride, const int32_t* __restrict__ bt, int64_t bt_row_stride, int bt_width,
     int64_t num_blocks, const int32_t* __restrict__ cu, int batch, int rows) {
-  const int t = __builtin_amdgcn_readfirstlane(blockIdx.x * (kThreads / 64) + (threadIdx.x >> 6));
-  if (t >= rows) return;
-  const int b = sequence_of(cu, batch, t);
-  if (b < 0) return;
-  const int pos = t - cu[b];
-  const int j = pos >> P.block_size_log2, in = pos & ((1 << P.block_size_log2) - 1);
-  const int page = j < bt_width ? bt[b * bt_row_stride + j] : -1;
-  const bool there = page >= 0 && page < num_blocks;
-  for (int u = threadIdx.x & 63; u < 2 * P.units; u += 64) {
+  __shared__ int64_t slots[kGatherRows];
+  const int64_t t0 = static_cast<int64_t>(blockIdx.x) * kGatherRows;
+  dense_slots(cu, batch, t0, rows, bt, bt_row_stride, bt_width, P.block_size_log2, num_blocks,
+              slots);
+  const int n = static_cast<int>(min(static_cast<int64_t>(kGatherRows), rows - t0));
+  // Short rows: several side by side.
+  const int cols = 2 * P.units;
+  const int per = cols < kThreads ? kThreads / cols : 1;
+  const int row0 = cols < kThreads ? threadIdx.x / cols : 0;
+  if (row0 >= per) return;
+  for (int u = cols < kThreads ? threadIdx.x % cols : threadIdx.x; u < cols; u += kThreads) {
     const bool is_v = u >= P.units;
     const int at = 8 * (is_v ? u - P.units : u);
-    uint4 x = make_uint4(0, 0, 0, 0);
-    if (there) {
-      const int head = at / P.head_size, dim = at - head * P.head_size;
-      const int64_t hp = static_cast<int64_t>(page) * P.num_kv_heads + head;
-      const uint32_t e = (is_v ? P.v_scales : P.k_scales)[scale_at(P, hp, in, dim)];
-      uint32_t codes;
-      if (!is_v)
-        codes = *reinterpret_cast<const uint32_t*>(k_codes(P, hp, in, dim));
-      else if (P.head_size == 64)
-        codes = *reinterpret_cast<const uint16_t*>(v_codes(P, hp, in, dim)) |
-                *reinterpret_cast<const uint16_t*>(v_codes(P, hp, in, dim + 4)) << 16;
-      else
-        codes = *reinterpret_cast<const uint32_t*>(v_codes(P, hp, in, dim));
-      x = fp4x8_to_bf16x8(codes, __uint_as_float(e << 23));
+    const int head = at / P.head_size, dim = at - head * P.head_size;
+    const uint8_t* const scales = is_v ? P.v_scales : P.k_scales;
+    uint16_t* const out = (is_v ? value + t0 * value_stride : key + t0 * key_stride) + at;
+    const int64_t stride = is_v ? value_stride : key_stride;
+#pragma unroll 8
+    for (int row = row0; row < n; row += per) {
+      const int64_t slot = slots[row], from = max(slot, int64_t{0});
+      const int in = static_cast<int>(from & ((1 << P.block_size_log2) - 1));
+      const int64_t hp = (from >> P.block_size_log2) * P.num_kv_heads + head;
+      const uint32_t e = scales[scale_at(P, hp, in, dim)];
+      const uint8_t* const p = is_v ? v_codes(P, hp, in, dim) : k_codes(P, hp, in, dim);
+      // (V at head size 64: two halves of two bytes)
+      const uint32_t codes = is_v && P.head_size == 64
+                                 ? *reinterpret_cast<const uint16_t*>(p) |
+                                       *reinterpret_cast<const uint16_t*>(p + 8) << 16
+                                 : *reinterpret_cast<const uint32_t*>(p);
+      uint4 x = fp4x8_to_bf16x8(codes, __uint_as_float(e << 23));
+      if (slot < 0) x = make_uint4(0, 0, 0, 0);
+      if (slot != -2) store_past(out + row * stride, x);
     }
-    *reinterpret_cast<uint4*>((is_v ? value + t * value_stride : key + t * key_stride) + at) = x;
   }
 }
 
@@ -258,7 +268,7 @@ extern "C" int fk_gather_kvcache_mxfp4(void* key, int64_t key_row_stride, void* 
                  cu_seqlens_k,
              "%s: null pointer", what);
   hipLaunchKernelGGL(gather_mxfp4_kernel,
-                     dim3(static_cast<unsigned>((rows + kThreads / 64 - 1) / (kThreads / 64))),
+                     dim3(static_cast<unsigned>((rows + kGatherRows - 1) / kGatherRows)),
                      dim3(kThreads), 0, as_stream(stream), P, static_cast<uint16_t*>(key),
                      key_row_stride, static_cast<uint16_t*>(value), value_row_stride,
                      block_tables, bt_row_stride, static_cast<int>(bt_width), num_blocks,

@@ -337,8 +337,7 @@ __attribute__((amdgpu_waves_per_eu(2))) void mxfp4_decode_kernel(
     __syncthreads();
   };
   walk_line(line, A.batch, P.wgs, blockIdx.x, kWaves, kPad, P.records,
-                      [&](int b) { return seq_rows(cu, ctx_lens, b, P.rows, P.most); }, items_of,
-                      body);
+            [&](int b) { return seq_rows(cu, ctx_lens, b, P.rows, P.most); }, items_of, body);
 }
 
 // One work-group per (query row, kv head, some of its columns): merges the pieces of an item that
@@ -354,7 +353,7 @@ __global__ __launch_bounds__(kMergeThreads) void mxfp4_merge_kernel(
   if (!query_row(cu, ctx_lens, A.batch, t, b, vis)) return;
   const SeqRows s = seq_rows(cu, ctx_lens, b, P.rows, P.most);
   const int i = t - s.row0;
-  if (i >= s.rows) return;
+  if (i < 0 || i >= s.rows) return;
   const LineRecord rec = P.records[b];
   const int col_items = (s.rows * A.gqa + kCols - 1) / kCols;
   const int j0 = blockIdx.z * P.merge_cols;

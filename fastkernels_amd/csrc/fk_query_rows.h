@@ -23,6 +23,36 @@ __device__ __forceinline__ int sequence_of(const int32_t* __restrict__ cu, int b
   return lo;
 }
 
+// Slots (page * block size + place) of the tokens that rows t0 .. t0 + kRows - 1 of a dense copy
+// of the sequences stand for, into LDS: -1 at a masked page, -2 for a row of no sequence.  cu may
+// not ascend; what is read stays inside the table.
+template <int kRows>
+__device__ __forceinline__ void dense_slots(const int32_t* __restrict__ cu, int batch, int64_t t0,
+                                            int64_t rows, const int32_t* __restrict__ bt,
+                                            int64_t bt_row_stride, int bt_width,
+                                            int block_size_log2, int64_t num_blocks,
+                                            int64_t (&slot)[kRows]) {
+  if (threadIdx.x < kRows) {
+    const int64_t t = t0 + threadIdx.x;
+    int64_t at = -2;
+    if (t < rows && t >= cu[0] && t < cu[batch]) {
+      int lo = 0, hi = batch;  // the last sequence that begins at t or before
+      while (hi - lo > 1) {
+        const int mid = lo + ((hi - lo) >> 1);
+        if (cu[mid] <= t) lo = mid; else hi = mid;
+      }
+      const int64_t pos = t - cu[lo], j = pos >> block_size_log2;
+      const int page = j < bt_width ? bt[lo * bt_row_stride + j] : -1;
+      at = page >= 0 && page < num_blocks
+               ? (static_cast<int64_t>(page) << block_size_log2) +
+                     (pos & ((int64_t{1} << block_size_log2) - 1))
+               : -1;
+    }
+    slot[threadIdx.x] = at;
+  }
+  __syncthreads();
+}
+
 // Sequence b of query row t and the keys the row sees, vis = ctx - n + i + 1 for the i-th
 // of the sequence's n rows (aligned to the end of its tokens; at most ctx).  cu == nullptr:
 // one row per sequence.  False for a row behind the last sequence.  Whole waves call it, with one
@@ -47,6 +77,13 @@ __device__ __forceinline__ bool query_row(const int32_t* __restrict__ cu,
 // Pages that hold the first `vis` keys (0 for none).
 __device__ __forceinline__ int pages_of(int vis, int block_size_log2) {
   return vis > 0 ? ((vis - 1) >> block_size_log2) + 1 : 0;
+}
+
+// A store past the caches, for dense copies larger than they are: the lines that a copy is read
+// from stay.
+__device__ __forceinline__ void store_past(uint16_t* p, const uint4& v) {
+  typedef uint32_t words __attribute__((ext_vector_type(4)));
+  __builtin_nontemporal_store(words{v.x, v.y, v.z, v.w}, reinterpret_cast<words*>(p));
 }
 
 }  // namespace fk
