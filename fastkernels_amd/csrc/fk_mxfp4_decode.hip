@@ -171,6 +171,10 @@ __attribute__((amdgpu_waves_per_eu(2))) void mxfp4_decode_kernel(
   constexpr int kCols = 16 * kCB;
   __shared__ LineLds<kThreads> line;
   extern __shared__ __align__(16) float lds[];
+  // The queries' operands, where they are 32 registers or more: of those that then have no
+  // register, a step's reload comes after the next step's loads, and waits for them.
+  constexpr bool kQLds = kCB * D >= 256;
+  uint4* const q_lds = reinterpret_cast<uint4*>(lds);  // (the merge's, until the part's last step)
   const PageAttnParams& A = P.A;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int lane = threadIdx.x & 63;
@@ -211,13 +215,29 @@ __attribute__((amdgpu_waves_per_eu(2))) void mxfp4_decode_kernel(
           A.q + (sr.row0 + i) * A.q_row_stride + static_cast<int64_t>(hq) * D + g * (D / 4);
 #pragma unroll
       for (int k = 0; k < D / 32; ++k) {
+        if (kQLds && (cb * (D / 32) + k) % kWaves != wave) continue;
         const uint32_t flip = s2 < 0.f ? 0x80008000u : 0u;
         uint4 v = ok ? *reinterpret_cast<const uint4*>(qp + 8 * k) : make_uint4(0, 0, 0, 0);
         v = make_uint4(v.x ^ flip, v.y ^ flip, v.z ^ flip, v.w ^ flip);
-        st.qb[cb][k] = __builtin_bit_cast(bf16x8_t, v);
+        if constexpr (kQLds)
+          q_lds[(cb * (D / 32) + k) * 64 + lane] = v;
+        else
+          st.qb[cb][k] = __builtin_bit_cast(bf16x8_t, v);
       }
       if (!ok) hi[cb] = lo[cb] = 0;
     }
+    if constexpr (kQLds) __syncthreads();
+    auto score = [&](int cb, const uint4 (&k)[D / 32]) {
+      if constexpr (!kQLds) {
+        return qk_scores_n(k, st.qb[cb]);
+      } else {
+        bf16x8_t q[D / 32];
+#pragma unroll
+        for (int x = 0; x < D / 32; ++x)
+          q[x] = __builtin_bit_cast(bf16x8_t, q_lds[(cb * (D / 32) + x) * 64 + lane]);
+        return qk_scores_n(k, q);
+      }
+    };
     const int row_a = col0 / A.gqa, row_z = (col0 + n_cols - 1) / A.gqa;
     int none;
     row_keys(sr, row_z, P.window_left, all_lo, none);
@@ -251,10 +271,10 @@ __attribute__((amdgpu_waves_per_eu(2))) void mxfp4_decode_kernel(
           uint4 k[D / 32];
           k_operands<D>(c, 0, r, k);
 #pragma unroll
-          for (int cb = 0; cb < kCB; ++cb) sa[cb] = qk_scores_n(k, st.qb[cb]);
+          for (int cb = 0; cb < kCB; ++cb) sa[cb] = score(cb, k);
           k_operands<D>(c, 1, r, k);
 #pragma unroll
-          for (int cb = 0; cb < kCB; ++cb) sb[cb] = qk_scores_n(k, st.qb[cb]);
+          for (int cb = 0; cb < kCB; ++cb) sb[cb] = score(cb, k);
         }
 #pragma unroll
         for (int cb = 0; cb < kCB; ++cb) {
