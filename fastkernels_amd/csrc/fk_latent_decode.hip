@@ -44,6 +44,7 @@ struct LatentParams {
   int num_heads;
   int head_blocks;  // units of 32 heads of a row
   int units;        // of an item
+  int team;         // work-groups that take the same keys side by side, an item each
   int batch, rows, most;
   int block_size_log2;
   int64_t num_blocks;
@@ -142,7 +143,7 @@ struct Halves {
   }
 };
 
-// A sequence's items: `units` units of 32 heads of a row each, in steps of a tile.
+// A sequence's items: teams of `units` units of 32 heads of a row each, in steps of a tile.
 __device__ __forceinline__ LineItems line_items(const LatentParams& P, const SeqRows& s,
                                                 int units) {
   LineItems x;
@@ -153,7 +154,7 @@ __device__ __forceinline__ LineItems line_items(const LatentParams& P, const Seq
   x.to = static_cast<int>(min(min(static_cast<int64_t>(x.to), int64_t{0x7fffff00}),
                               static_cast<int64_t>(P.bt_width) << P.block_size_log2));
   x.steps = x.to > 0 ? (x.to - 1) / kKeys + 1 : 1;
-  x.items = s.rows * ((P.head_blocks + units - 1) / units);
+  x.items = s.rows * ((P.head_blocks + units - 1) / units / P.team);
   return x;
 }
 
@@ -662,18 +663,31 @@ __attribute__((amdgpu_waves_per_eu(1, 1))) void latent_decode_kernel(
     __syncthreads();
     return s_lo + s;
   };
+  // The work-groups of a team are neighbours on an XCD, and read each tile at about the same time.
+  int team = blockIdx.x / A.team, member = blockIdx.x % A.team;
+  if (A.wgs % (8 * A.team) == 0) {
+    const int i = blockIdx.x >> 3;
+    team = i / A.team * 8 + (blockIdx.x & 7);
+    member = i % A.team;
+  }
+  const int teams = A.wgs / A.team;
+  if (blockIdx.x >= teams * A.team) {
+    if (blockIdx.x < A.wgs) return;
+    team = teams;  // (writes the records)
+  }
   auto body = [&](int b, const SeqRows& sr, const LineItems& x, int it, int s_lo, int s_hi,
                   int64_t slot, int64_t free_slot) {
-    const int64_t spare = slot >= 0 ? slot : free_slot;
+    const int64_t to = slot >= 0 ? slot * A.team + member : -1;
+    const int64_t spare = slot >= 0 ? to : free_slot * A.team + member;
     bool more = false;
     while (s_lo < s_hi) {
-      s_lo = attempt(b, sr, x, it, s_lo, s_hi, slot, spare, more);
+      s_lo = attempt(b, sr, x, it * A.team + member, s_lo, s_hi, to, spare, more);
       more = true;
     }
   };
-  walk_line(line, A.batch, A.wgs, blockIdx.x, 1, kPad, A.records,
-                      [&](int b) { return seq_rows(cu, ctx_lens, b, A.rows, A.most); },
-                      [&](const SeqRows& s) { return line_items(A, s, kUnits); }, body);
+  walk_line(line, A.batch, teams, team, 1, kPad, A.records,
+            [&](int b) { return seq_rows(cu, ctx_lens, b, A.rows, A.most); },
+            [&](const SeqRows& s) { return line_items(A, s, kUnits); }, body);
 }
 
 // One work-group per (query row, some of its heads, kDims of their dims): merges the pieces of an
@@ -696,12 +710,13 @@ __global__ __launch_bounds__(kMergeThreads) void latent_merge_kernel(
   for (int h = h0; h < h1;) {
     const int per = 32 * A.units, block = h / per;
     const int in = h - block * per, nc = min(h1, (block + 1) * per) - h;
-    const LinePieces pieces(rec, i * ((A.head_blocks + A.units - 1) / A.units) + block, kPad);
+    const int item = i * ((A.head_blocks + A.units - 1) / A.units) + block;
+    const LinePieces pieces(rec, item / A.team, kPad);
     if (pieces.n > 1) {
       merge_pieces<kDims>(
           0, nc, folded, [&](int) { return pieces.n; },
           [&](int k, int x, const float*& ml, const float*& o) {
-            const int64_t at = pieces.slot(k) * per + in + x;
+            const int64_t at = (pieces.slot(k) * A.team + item % A.team) * per + in + x;
             ml = A.ml + 2 * at;
             o = A.o + at * R + dim0;
           },
@@ -823,6 +838,7 @@ extern "C" int fk_latent_decode(void* out, int64_t out_row_stride, int64_t out_h
   A.wgs = plan.wgs;
   A.head_blocks = (num_heads + 31) / 32;
   A.units = plan.units;
+  A.team = (A.head_blocks + plan.units - 1) / plan.units % 2 == 0 ? 2 : 1;
   A.o = reinterpret_cast<float*>(ws + plan.o);
   A.ml = reinterpret_cast<float*>(ws + plan.ml);
   A.records = reinterpret_cast<LineRecord*>(ws + plan.records);
