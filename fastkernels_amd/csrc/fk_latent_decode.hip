@@ -692,7 +692,7 @@ __attribute__((amdgpu_waves_per_eu(1, 1))) void latent_decode_kernel(
 
 // One work-group per (query row, some of its heads, kDims of their dims): merges the pieces of an
 // item that ranges cut.
-template <int R, int kDims>
+template <int R, int kDims, int kAhead>
 __global__ __launch_bounds__(kMergeThreads) void latent_merge_kernel(
     LatentParams A, const int32_t* __restrict__ ctx_lens, const int32_t* __restrict__ cu,
     int heads, int fp8) {
@@ -713,7 +713,7 @@ __global__ __launch_bounds__(kMergeThreads) void latent_merge_kernel(
     const int item = i * ((A.head_blocks + A.units - 1) / A.units) + block;
     const LinePieces pieces(rec, item / A.team, kPad);
     if (pieces.n > 1) {
-      merge_pieces<kDims>(
+      merge_pieces<kDims, kAhead>(
           0, nc, folded, [&](int) { return pieces.n; },
           [&](int k, int x, const float*& ml, const float*& o) {
             const int64_t at = (pieces.slot(k) * A.team + item % A.team) * per + in + x;
@@ -759,15 +759,22 @@ void launch(const LatentParams& A, hipStream_t s, const int32_t* bt, const int32
     hipLaunchKernelGGL((latent_decode_kernel<R, P, 2, kFp8>), dim3(A.wgs + 1), dim3(kThreads),
                        lds, s, A, bt, ctx, cu);
   // Where rows and heads do not make two work-groups a CU, the dims are dealt out too, and with
-  // them threads to share a column's pieces.
+  // them threads to share a column's pieces; where they make so few that a thread would take more
+  // than two rounds of columns, so that its loads overlap others' (64 rows of 128 heads: 13 us, 17
+  // with whole rows; 128 rows of 16 heads 8 us with whole rows, 10 otherwise).  An item is rarely
+  // in more than four pieces then, and loads for eight of them cost 22 us in place of 17.
   const int heads = merge_cols(A.rows, 1, A.num_heads);
   const dim3 grid((A.num_heads + heads - 1) / heads, A.rows);
+  auto merge = [&](auto kernel, int dims) {
+    hipLaunchKernelGGL(kernel, dim3(grid.x, grid.y, R / dims), dim3(kMergeThreads), 0, s, A, ctx,
+                       cu, heads, kFp8 ? 1 : 0);
+  };
   if (static_cast<int64_t>(grid.x) * grid.y < num_cus())
-    hipLaunchKernelGGL((latent_merge_kernel<R, 64>), dim3(grid.x, grid.y, R / 64),
-                       dim3(kMergeThreads), 0, s, A, ctx, cu, heads, kFp8 ? 1 : 0);
+    merge(latent_merge_kernel<R, 64, 8>, 64);
+  else if (heads * (R / 4) > 2 * kMergeThreads)
+    merge(latent_merge_kernel<R, 128, 4>, 128);
   else
-    hipLaunchKernelGGL((latent_merge_kernel<R, R>), grid, dim3(kMergeThreads), 0, s, A, ctx, cu,
-                       heads, kFp8 ? 1 : 0);
+    merge(latent_merge_kernel<R, R, 4>, R);
 }
 
 }  // namespace

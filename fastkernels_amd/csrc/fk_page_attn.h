@@ -424,7 +424,7 @@ inline int merge_cols(int64_t rows, int vheads, int cols) {
   return static_cast<int>(per < 1 ? 1 : per < cols ? per : cols);
 }
 constexpr int kMergeAhead = 8;  // pieces whose loads are in flight
-template <int D, class Pieces, class At, class Emit>
+template <int D, int kAhead = kMergeAhead, class Pieces, class At, class Emit>
 __device__ __forceinline__ void merge_pieces(int j0, int nc, Folded* folded, Pieces pieces, At at,
                                              Emit emit) {
   const int tid = threadIdx.x;
@@ -439,18 +439,18 @@ __device__ __forceinline__ void merge_pieces(int j0, int nc, Folded* folded, Pie
     Folded f;
     f.reset();
     const int n = ok ? pieces(j) : 0;
-    for (int k0 = slice; k0 < n; k0 += kMergeAhead * slices) {
-      float2 s[kMergeAhead];
-      float4 o[kMergeAhead];
+    for (int k0 = slice; k0 < n; k0 += kAhead * slices) {
+      float2 s[kAhead];
+      float4 o[kAhead];
 #pragma unroll
-      for (int u = 0; u < kMergeAhead; ++u) {
+      for (int u = 0; u < kAhead; ++u) {
         const float *ml, *row;
         at(min(k0 + u * slices, n - 1), j, ml, row);
         s[u] = *reinterpret_cast<const float2*>(ml);
         o[u] = *reinterpret_cast<const float4*>(row + dim);
       }
 #pragma unroll
-      for (int u = 0; u < kMergeAhead; ++u)
+      for (int u = 0; u < kAhead; ++u)
         if (k0 + u * slices < n) f.add(s[u].x, s[u].y, o[u]);
     }
     if (slices > 1) {
