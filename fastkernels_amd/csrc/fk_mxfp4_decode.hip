@@ -52,28 +52,42 @@ struct Codes {
   uint2 vs;
 };
 
-// Loads a step whose halves of 16 keys are in rows h0 and h1 (of a kv head's tokens).
-template <int D>
-__device__ __forceinline__ void load_step(const Mxfp4Params& P, int64_t page0, int tok0,
-                                          int64_t page1, int tok1, int r, int g, Codes<D>& c) {
-  const int bs_log2 = P.A.block_size_log2;
-  const int64_t k_row = ((r >> 3 ? page1 : page0) << bs_log2) + (r >> 3 ? tok1 : tok0);
-  const int64_t v_row = ((g >> 1 ? page1 : page0) << bs_log2) + (g >> 1 ? tok1 : tok0);
-  const uint8_t* const k =
-      P.A.k_cache + (k_row + 8 * ((r >> 2) & 1) + (r & 3)) * (D / 2) + g * (D / 8);
+// Loads a step whose halves of 16 keys are in pages page0 and page1 (of a kv head), at places tok
+// and tok + 16 modulo a page.  kOne: pages hold whole steps.  Then what differs between lanes is
+// the same in every step, and a load is a scalar base and a lane's own 32 bits; in pages of 16 keys
+// the halves lie anywhere, and lanes select between them.
+template <int D, bool kOne>
+__device__ __forceinline__ void load_step(const Mxfp4Params& P, uint32_t page0, uint32_t page1,
+                                          uint32_t tok, int r, int g, Codes<D>& c) {
+  constexpr int kRow = D / 2, kBlocks = D / 32;
+  const int log2 = kOne ? P.A.block_size_log2 : 4;
+  const uint32_t k_row = 8 * ((r >> 2) & 1) + (r & 3), v_row = 8 * (g & 1);
+  const uint8_t *k, *v, *ks, *vs;
+  if constexpr (kOne) {
+    const uint64_t row = (static_cast<uint64_t>(page0) << log2) + tok;
+    const uint64_t s_row = (static_cast<uint64_t>(page0) * kBlocks << log2) + tok;
+    k = P.A.k_cache + row * kRow + ((16 * (r >> 3) + k_row) * kRow + g * (D / 8));
+    v = P.A.v_cache + row * kRow + ((16 * (g >> 1) + v_row) * kRow + r * (D / 8));
+    ks = P.k_scales + s_row +
+         ((static_cast<uint32_t>(g * D / 128) << log2) + 16 * (r >> 3) + (k_row & 8));
+    vs = P.v_scales + s_row + ((static_cast<uint32_t>(r * D / 512) << log2) + 16 * (g >> 1) + v_row);
+  } else {
+    const uint32_t rk = (r >> 3 ? page1 : page0) << log2, rv = (g >> 1 ? page1 : page0) << log2;
+    k = P.A.k_cache + static_cast<uint64_t>(rk) * kRow + (k_row * kRow + g * (D / 8));
+    v = P.A.v_cache + static_cast<uint64_t>(rv) * kRow + (v_row * kRow + r * (D / 8));
+    ks = P.k_scales + static_cast<uint64_t>(rk) * kBlocks +
+         ((static_cast<uint32_t>(g * D / 128) << log2) + (k_row & 8));
+    vs = P.v_scales + static_cast<uint64_t>(rv) * kBlocks +
+         ((static_cast<uint32_t>(r * D / 512) << log2) + v_row);
+  }
   ld_words(k, c.k[0]);
-  ld_words(k + 4 * (D / 2), c.k[1]);
-  const uint8_t* const ks = P.k_scales +
-                            (((r >> 3 ? page1 : page0) * (D / 32) + g * D / 128) << bs_log2) +
-                            (r >> 3 ? tok1 : tok0) + 8 * ((r >> 2) & 1);
+  ld_words(k + 4 * kRow, c.k[1]);
 #pragma unroll
   for (int i = 0; i < Codes<D>::kScales; ++i)
-    c.ks[i] = ld8(ks + (static_cast<int64_t>(i) << bs_log2));
-  const uint8_t* const v = P.A.v_cache + (v_row + 8 * (g & 1)) * (D / 2) + r * (D / 8);
+    c.ks[i] = ld8(ks + (static_cast<uint32_t>(i) << log2));
   ld_words(v, c.v[0]);
-  ld_words(v + 4 * (D / 2), c.v[1]);
-  c.vs = ld8(P.v_scales + (((g >> 1 ? page1 : page0) * (D / 32) + r * D / 512) << bs_log2) +
-             (g >> 1 ? tok1 : tok0) + 8 * (g & 1));
+  ld_words(v + 4 * kRow, c.v[1]);
+  c.vs = ld8(vs);
 }
 
 // K operands of tile t: chunk c is dims (D/4) g + 8 c .. + 7 of this lane's row.
@@ -163,7 +177,7 @@ __device__ __forceinline__ void values(ColumnState<kCB, D, false>& st, const Cod
   }
 }
 
-template <int kCB, int D>
+template <int kCB, int D, bool kOne>
 __global__ __launch_bounds__(kThreads)
 __attribute__((amdgpu_waves_per_eu(2))) void mxfp4_decode_kernel(
     Mxfp4Params P, const int32_t* __restrict__ bt, const int32_t* __restrict__ ctx_lens,
@@ -260,8 +274,8 @@ __attribute__((amdgpu_waves_per_eu(2))) void mxfp4_decode_kernel(
       const int n = min(32, (s_hi - s0 + kWaves - 1) / kWaves);
       auto load = [&](int m, Codes<D>& c) {
         const int t0 = x.from + (s0 + m * kWaves) * kStep;
-        load_step<D>(P, __builtin_amdgcn_readlane(page, 2 * m), t0 & page_mask,
-                     __builtin_amdgcn_readlane(page, 2 * m + 1), (t0 + 16) & page_mask, r, g, c);
+        load_step<D, kOne>(P, __builtin_amdgcn_readlane(page, 2 * m),
+                           __builtin_amdgcn_readlane(page, 2 * m + 1), t0 & page_mask, r, g, c);
       };
       auto attend = [&](int m, const Codes<D>& c) {
         const int t0 = x.from + (s0 + m * kWaves) * kStep;
@@ -426,8 +440,11 @@ template <int kCB, int D>
 void launch(const Mxfp4Params& P, hipStream_t s, const int32_t* bt, const int32_t* ctx,
             const int32_t* cu) {
   const unsigned lds = 4 * merge_lds_floats<kWaves, D>(16 * kCB);
-  hipLaunchKernelGGL((mxfp4_decode_kernel<kCB, D>), dim3(P.wgs + 1), dim3(kThreads), lds, s, P,
-                     bt, ctx, cu);
+  auto go = [&](auto kernel) {
+    hipLaunchKernelGGL(kernel, dim3(P.wgs + 1), dim3(kThreads), lds, s, P, bt, ctx, cu);
+  };
+  P.A.block_size_log2 >= 5 ? go(mxfp4_decode_kernel<kCB, D, true>)
+                           : go(mxfp4_decode_kernel<kCB, D, false>);
   hipLaunchKernelGGL((mxfp4_merge_kernel<kCB, D>),
                      dim3(P.A.num_kv_heads, P.rows,
                           (P.A.gqa + P.merge_cols - 1) / P.merge_cols),
@@ -459,8 +476,10 @@ extern "C" int fk_mxfp4_paged_decode(
   FK_REQUIRE(window_left >= -1, "%s: window_left %d must be -1 or >= 0", what, window_left);
   FK_REQUIRE(max_seqlen_q >= 1 && max_seqlen_q <= 65535, "%s: max_seqlen_q %lld", what,
              static_cast<long long>(max_seqlen_q));
-  FK_REQUIRE(num_blocks * num_kv_heads <= 0x7fffffff, "%s: %lld pages of %d heads", what,
-             static_cast<long long>(num_blocks), num_kv_heads);
+  // (more are more bytes than a GPU has)
+  FK_REQUIRE(num_blocks <= (int64_t{1} << 32) / block_size / num_kv_heads,
+             "%s: %lld pages of %d heads", what, static_cast<long long>(num_blocks),
+             num_kv_heads);
   if (batch == 0 || rows == 0) return FK_OK;
   FK_REQUIRE(out && q && k_cache && v_cache && k_scales && v_scales && block_tables &&
                  cache_seqlens,
