@@ -8,9 +8,6 @@
 // one line, cut into equal ranges, one per CU (fk_lines.h).  An item inside one range is finished
 // there; of the others each part leaves a partial state, which a second launch merges.
 //
-// LDS holds a tile (32 keys) as rows of bf16; the 16-byte pieces of row t are permuted within
-// each run of 8 by (t / 2) mod 8, which with the row's length of 128 bytes more than a multiple
-// of 256 spreads what 16 lanes read at a time over all banks.
 #include "fk_lines.h"
 #include "fk_page_attn.h"
 #include "fk_query_rows.h"
@@ -56,23 +53,28 @@ struct LatentParams {
   LineRecord* records;
 };
 
-// A tile in LDS.
-template <int R, int P>
+// A tile in LDS: rows of bf16 or of fp8 codes.  A wave loads eight of them.
+template <int R, int P, bool kFp8>
 struct Tile {
-  static constexpr int kRow = 2 * (R + P);        // bytes
+  static constexpr int kRow = (R + P) * (kFp8 ? 1 : 2);  // bytes
   static constexpr int kPieces = kRow / 16;
   static constexpr int kBytes = kKeys * kRow;
-  static constexpr int kMoves = kPieces / 8;  // of 64 pieces, of eight rows
-  static_assert(kPieces % 8 == 0, "whole runs of pieces, whole moves of eight rows");
+  static constexpr int kWide = kRow / 128;           // loads of 64 pieces, of eight rows
+  static constexpr int kLoads = kWide + kRow % 128 / 32;  // ... and of 64 words
+  static_assert(kRow % 32 == 0, "whole loads");
+  // Bytes of dims 32 k on: of the four pieces (bf16) or the two (fp8).  The pieces of row t are
+  // permuted: in runs of 8 by (t / 2) mod 8, or fp8, two by two, by (t / 4) mod 2; so 16 rows that
+  // are read together meet no bank twice.
   static __device__ __forceinline__ int at(int row, int piece) {
-    return row * kRow + 16 * ((piece & ~7) | ((piece ^ (row >> 1)) & 7));
+    return row * kRow + 16 * (kFp8 ? piece ^ (row >> 1 & 2)
+                                   : (piece & ~7) | ((piece ^ (row >> 1)) & 7));
   }
-  // Where in its eight rows of the cache a lane finds the piece that goes to LDS bytes
-  // 1024 m + 16 lane of them (rows from a multiple of 8 on, `odd`: not of 16).
+  // Where in its eight rows of the cache a lane finds what load m takes to LDS (rows from a
+  // multiple of 8 on, `odd`: not of 16).
   static __device__ __forceinline__ uint32_t source(int m, int lane, bool odd) {
-    const int x = 64 * m + lane;
-    const int row = x / kPieces, slot = x % kPieces;
-    return row * kRow + 16 * ((slot & ~7) | ((slot ^ ((row >> 1) + (odd ? 4 : 0))) & 7));
+    const int byte = m < kWide ? 1024 * m + 16 * lane : 1024 * kWide + 256 * (m - kWide) + 4 * lane;
+    const int row = byte / kRow, in = byte % kRow;
+    return at(row + (odd ? 8 : 0), in >> 4) - (odd ? 8 * kRow : 0) + (in & 15);
   }
 };
 
@@ -114,9 +116,23 @@ __device__ __forceinline__ short4_t transposed(const uint8_t* p) {
   typedef __attribute__((address_space(3))) short4_t* lds_short4;
   return __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_short4)p);
 }
-__device__ __forceinline__ bf16x8_t joined(short4_t a, short4_t b) {
+// (fp8: eight keys of a dim)
+__device__ __forceinline__ uint2 transposed8(const uint8_t* p) {
+  typedef int int2_t __attribute__((ext_vector_type(2)));
+  typedef __attribute__((address_space(3))) int2_t* lds_int2;
+  return __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr8_b64_v2i32((lds_int2)p));
+}
+__device__ __forceinline__ uint4 joined(short4_t a, short4_t b) {
   const uint2 x = __builtin_bit_cast(uint2, a), y = __builtin_bit_cast(uint2, b);
-  return __builtin_bit_cast(bf16x8_t, make_uint4(x.x, x.y, y.x, y.y));
+  return make_uint4(x.x, x.y, y.x, y.y);
+}
+// Eight values as a product's operand (of fp8 codes exactly).
+__device__ __forceinline__ bf16x8_t operand(const uint4& x) {
+  return __builtin_bit_cast(bf16x8_t, x);
+}
+__device__ __forceinline__ bf16x8_t operand(const uint2& x) {
+  const uint2 a = fp8x4_to_bf16x4(x.x), b = fp8x4_to_bf16x4(x.y);
+  return __builtin_bit_cast(bf16x8_t, make_uint4(a.x, a.y, b.x, b.y));
 }
 __device__ __forceinline__ uint32_t pack2(float a, float b) {
   const bf16x2_t x = {static_cast<__bf16>(a), static_cast<__bf16>(b)};
@@ -183,29 +199,34 @@ __device__ __forceinline__ void write_out(const LatentParams& P, int64_t row, in
 // hold great weights as exactly as small ones, and O is not rescaled.  Where a later maximum, which
 // all waves know behind the next barrier, is 2^kFar times that, the part is taken in two: the state
 // so far goes to memory, and what follows begins again with its own maximum and is merged with it.
-constexpr int tiles_of(bool fp8) { return fp8 ? 3 : 4; }
+constexpr int kBuffers = 4;  // tiles in LDS, of which two are on their way
+constexpr int kAhead = kBuffers - 1;
+// Bytes of the tiles, whose place the outputs take at the end.
+template <int R, int P, bool kFp8>
+constexpr int tiles_bytes(int units) {
+  const int tiles = kBuffers * Tile<R, P, kFp8>::kBytes, out = 32 * units * (R + 4) * 4;
+  return tiles > out ? tiles : out;
+}
+// Work-groups on a CU: a tile of codes is small enough for two.
+constexpr int wgs_per_cu(int units, bool fp8) { return units == 1 && fp8 ? 2 : 1; }
 template <int R, int P, int kUnits, bool kFp8>
 __global__ __launch_bounds__(kThreads)
-__attribute__((amdgpu_waves_per_eu(1, 1))) void latent_decode_kernel(
+__attribute__((amdgpu_waves_per_eu(wgs_per_cu(kUnits, kFp8), wgs_per_cu(kUnits, kFp8)))) void
+latent_decode_kernel(
     LatentParams A, const int32_t* __restrict__ bt, const int32_t* __restrict__ ctx_lens,
     const int32_t* __restrict__ cu) {
-  using T = Tile<R, P>;
+  using T = Tile<R, P, kFp8>;
+  using Raw = std::conditional_t<kFp8, uint2, uint4>;  // eight values in LDS
   constexpr int kCols = 32 * kUnits;
   constexpr int kCB = kUnits;            // blocks of 16 columns of a wave's S
   constexpr int kKc = (R + P) / 32;      // products of S
   constexpr int kOb = R / 4 / 32;        // blocks of 32 dims of a wave
   constexpr int kGroup = 3;              // K operands read from LDS at a time
-  constexpr int kMoves = T::kMoves;      // of a wave and tile: eight rows
+  constexpr int kLoads = T::kLoads;
   static_assert(kKc % kGroup == 0 && kOb % 2 == 0, "whole groups");
-  // Tiles in LDS: bf16 four, of which two are on their way; fp8 three, and the codes of two to
-  // come (a wave's own eight rows each).
-  constexpr int kBuffers = tiles_of(kFp8);
-  constexpr int kCodes = 8 * (R + P);    // bytes of a wave's codes of a tile
-  constexpr int kWide = kCodes / 1024, kCodeMoves = kWide + kCodes % 1024 / 256;
-  static_assert(kCodes % 512 == 0, "whole moves");
   __shared__ LineLds<kThreads, kSeqs> line;
   extern __shared__ __align__(16) uint8_t lds[];
-  uint8_t* const p_lds = lds + 4 * T::kBytes;  // of two steps, [columns][32 keys] bf16
+  uint8_t* const p_lds = lds + tiles_bytes<R, P, kFp8>(kUnits);  // of two steps, [columns][32 keys] bf16
   constexpr int kP = kCols * kKeys * 2;
   // [two steps][2 halves of the keys][columns]
   float* const tops = reinterpret_cast<float*>(p_lds + 2 * kP);
@@ -218,11 +239,9 @@ __attribute__((amdgpu_waves_per_eu(1, 1))) void latent_decode_kernel(
   const float s2 = A.scale_log2 * vsc;
   const float abs_s2 = __builtin_fabsf(s2);
   const uint32_t flip = s2 < 0.f ? 0x80008000u : 0u;
-  // A wave loads eight rows of a tile.
-  uint32_t src[kFp8 ? 1 : kMoves];
+  uint32_t src[kLoads];
 #pragma unroll
-  for (int m = 0; m < (kFp8 ? 1 : kMoves); ++m)
-    src[m] = kFp8 ? lane : T::source(m, lane, wave & 1);
+  for (int m = 0; m < kLoads; ++m) src[m] = T::source(m, lane, wave & 1);
   const uint32_t lds0 = lds_addr_of(lds);
   // 16 bytes (8 keys) of a column's weights, their pieces permuted against bank conflicts.
   auto p_at = [&](int col, int key) {
@@ -287,19 +306,14 @@ __attribute__((amdgpu_waves_per_eu(1, 1))) void latent_decode_kernel(
       const int t = min(s, steps - 1);
       const int key = (s_lo + t) * kKeys + 8 * wave;
       const int pg = __builtin_amdgcn_readlane(pages, 2 * (t & 31) + (wave >> 1));
-      const uint32_t to = kFp8 ? 3 * T::kBytes + ((s & 1) * 4 + wave) * kCodes
-                               : s % kBuffers * T::kBytes + wave * (T::kBytes / 4);
-      return Moves{keys.rows(pg, key), lds0 + to};
+      return Moves{keys.rows(pg, key),
+                   lds0 + s % kBuffers * T::kBytes + wave * (T::kBytes / 4)};
     };
-    constexpr int kLoads = kFp8 ? kCodeMoves : kMoves;
     auto issue = [&](const Moves& m, int i) {
-      if constexpr (!kFp8)
+      if (i < T::kWide)
         lds_load16(m.from, src[i], m.to + 1024 * i);
-      else if (i < kWide)
-        lds_load16(m.from + 1024 * i, 16 * src[0], m.to + 1024 * i);
       else
-        lds_load4(m.from + 1024 * kWide + 256 * (i - kWide), 4 * src[0],
-                  m.to + 1024 * kWide + 256 * (i - kWide));
+        lds_load4(m.from, src[i], m.to + 1024 * T::kWide + 256 * (i - T::kWide));
     };
     auto load = [&](int s) {
       const Moves m = moves_of(s);
@@ -307,39 +321,15 @@ __attribute__((amdgpu_waves_per_eu(1, 1))) void latent_decode_kernel(
       for (int i = 0; i < kLoads; ++i) issue(m, i);
     };
     // Keys that the row does not see may hold anything, infinities and NaN among it, which a zero
-    // weight would not undo: their rows become zeros.  bf16: among this wave's rows of step s.
+    // weight would not undo: their rows become zeros, among this wave's rows of step s.
     auto clear = [&](int s) {
       const int n = seen(s, 8 * wave);
       if (n >= 8) return;
       uint8_t* const at = lds + s % kBuffers * T::kBytes + wave * (T::kBytes / 4) + 16 * lane;
 #pragma unroll
-      for (int i = 0; i < kMoves; ++i)
-        if (64 * i + lane >= max(n, 0) * T::kPieces)
+      for (int i = 0; i < (8 * T::kPieces + 63) / 64; ++i)
+        if (64 * i + lane >= max(n, 0) * T::kPieces && 64 * i + lane < 8 * T::kPieces)
           *reinterpret_cast<uint4*>(at + 1024 * i) = make_uint4(0, 0, 0, 0);
-    };
-    // fp8: this wave's codes of step s, which have come, become a tile's rows; the i-th 512 bytes.
-    // (Piece 64 i + lane of the eight rows: bytes 8 (64 i + lane) of the codes.)
-    uint32_t row_at[kFp8 ? kMoves : 1];
-#pragma unroll
-    for (int i = 0; i < (kFp8 ? kMoves : 0); ++i) {
-      const int piece = 64 * i + lane;
-      row_at[i] = T::at(8 * wave + piece / T::kPieces, piece % T::kPieces);
-    }
-    auto codes = [&](int s, int i) {
-      return *reinterpret_cast<const uint2*>(lds + 3 * T::kBytes + ((s & 1) * 4 + wave) * kCodes +
-                                             8 * lane + 512 * i);
-    };
-    auto convert = [&](int s, int n, int i, uint2 v) {
-      const bool ok = lane < n * T::kPieces - 64 * i;
-      v = make_uint2(ok ? v.x : 0, ok ? v.y : 0);
-      const uint2 a = fp8x4_to_bf16x4(v.x), c = fp8x4_to_bf16x4(v.y);
-      *reinterpret_cast<uint4*>(lds + s % kBuffers * T::kBytes + row_at[kFp8 ? i : 0]) =
-          make_uint4(a.x, a.y, c.x, c.y);
-    };
-    auto convert_all = [&](int s) {
-      const int n = min(max(seen(s, 8 * wave), 0), 8);
-#pragma unroll
-      for (int i = 0; i < kMoves; ++i) convert(s, n, i, codes(s, i));
     };
     // The first steps' loads, and the queries behind them.
     look_up(0);
@@ -359,18 +349,21 @@ __attribute__((amdgpu_waves_per_eu(1, 1))) void latent_decode_kernel(
         qb[cb][k] = __builtin_bit_cast(bf16x8_t, v);
       }
     }
-    // S of step s, in logits.  Operands come in groups, one ahead of the products.  Piece 4 k + g
-    // of a row: of its place, k / 2 moves it by 128 bytes, k % 2 by a permutation.
-    const uint32_t k_at[2] = {static_cast<uint32_t>(T::at(16 * ts + r, g)),
-                              static_cast<uint32_t>(T::at(16 * ts + r, 4 + g))};
+    // S of step s, in logits.  Operands come in groups, one ahead of the products.  Dims 32 k + 8 g
+    // of a row: of their place, k / 2 moves it by two runs, k % 2 by a permutation.
+    constexpr int kRun = kFp8 ? 32 : 64;  // bytes of 32 dims
+    uint32_t k_at[2];
+#pragma unroll
+    for (int k = 0; k < 2; ++k)
+      k_at[k] = T::at(16 * ts + r, kFp8 ? 2 * k + (g >> 1) : 4 * k + g) + (kFp8 ? 8 * (g & 1) : 0);
     // (among(x): what to do among the products of the x-th group)
     auto scores = [&](int s, floatx4_t (&p)[kCB], auto among) {
       const uint8_t* const tile = lds + (s % kBuffers) * T::kBytes;
       const uint8_t* const at[2] = {tile + k_at[0], tile + k_at[1]};
-      uint4 kx[2][kGroup];
+      Raw kx[2][kGroup];
 #pragma unroll
       for (int j = 0; j < kGroup; ++j)
-        kx[0][j] = *reinterpret_cast<const uint4*>(at[j & 1] + 128 * (j >> 1));
+        kx[0][j] = *reinterpret_cast<const Raw*>(at[j & 1] + 2 * kRun * (j >> 1));
       // (two chains of products at least: one alone would wait for each result)
       constexpr int kChains = kCB == 1 ? 2 : 1;
       floatx4_t x[kChains][kCB];
@@ -384,8 +377,8 @@ __attribute__((amdgpu_waves_per_eu(1, 1))) void latent_decode_kernel(
         if (k0 + kGroup < kKc) {
 #pragma unroll
           for (int j = 0; j < kGroup; ++j)
-            kx[now ^ 1][j] = *reinterpret_cast<const uint4*>(at[(k0 + kGroup + j) & 1] +
-                                                             128 * ((k0 + kGroup + j) >> 1));
+            kx[now ^ 1][j] = *reinterpret_cast<const Raw*>(
+                at[(k0 + kGroup + j) & 1] + 2 * kRun * ((k0 + kGroup + j) >> 1));
         }
         among(k0 / kGroup);
         __builtin_amdgcn_sched_barrier(0);
@@ -394,8 +387,7 @@ __attribute__((amdgpu_waves_per_eu(1, 1))) void latent_decode_kernel(
 #pragma unroll
           for (int cb = 0; cb < kCB; ++cb)
             x[j % kChains][cb] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(
-                __builtin_bit_cast(bf16x8_t, kx[now][j]), qb[cb][k0 + j], x[j % kChains][cb], 0,
-                0, 0);
+                operand(kx[now][j]), qb[cb][k0 + j], x[j % kChains][cb], 0, 0, 0);
       }
 #pragma unroll
       for (int cb = 0; cb < kCB; ++cb)
@@ -440,27 +432,33 @@ __attribute__((amdgpu_waves_per_eu(1, 1))) void latent_decode_kernel(
       for (int cb = 0; cb < kCB; ++cb) l[cb] += last[cb];
     };
     // O += P V of step s.  Operands of 16 keys (k): lane (n, kh) has keys 16 k + 8 kh .. + 7.  In
-    // a transpose load, lane 4 a + q of each 16 addresses key a and dims 4 q .. 4 q + 3; block d's
-    // place in a row moves by 128 bytes with d / 2 and by a permutation with d % 2.
-    uint32_t v_at[2][2];
+    // a transpose load of bf16, lane 4 a + q of each 16 addresses key a (of four) and dims 4 q on;
+    // of fp8, lane 2 a + q key a (of eight) and dims 8 q on.  Block d's place in a row moves by
+    // two runs with d / 2 and by a permutation with d % 2.
+    uint32_t v_at[kFp8 ? 1 : 2][2];
 #pragma unroll
-    for (int h = 0; h < 2; ++h)
+    for (int h = 0; h < (kFp8 ? 1 : 2); ++h)
 #pragma unroll
       for (int d = 0; d < 2; ++d)
-        v_at[h][d] = 8 * (lane & 1) +
-                     T::at(8 * kh + 4 * h + (r >> 2),
-                           wave * (R / 32) + 4 * d + 2 * (g & 1) + ((lane & 3) >> 1));
+        v_at[h][d] =
+            kFp8 ? 8 * (lane & 1) + T::at(8 * kh + (r >> 1), wave * (R / 64) + 2 * d + (g & 1))
+                 : 8 * (lane & 1) + T::at(8 * kh + 4 * h + (r >> 2),
+                                          wave * (R / 32) + 4 * d + 2 * (g & 1) + ((lane & 3) >> 1));
     const uint8_t* const p_from = p_at(n, 8 * kh);  // keys 16 on: pieces 2 on, of four, permuted
     const int p_next = 32 - 64 * (((kh ^ (n >> 2)) & 3) >> 1);
-    auto v_operand = [&](const uint8_t* tile, int x) {  // keys 16 (x / kOb) on, block x % kOb
+    auto v_raw = [&](const uint8_t* tile, int x) -> Raw {  // keys 16 (x / kOb) on, block x % kOb
       const int k = x / kOb, d = x % kOb;
-      const int off = 16 * k * T::kRow + 128 * (d >> 1);
-      return joined(transposed(tile + v_at[0][d & 1] + off), transposed(tile + v_at[1][d & 1] + off));
+      const uint8_t* const at = tile + 16 * k * T::kRow + 2 * kRun * (d >> 1);
+      if constexpr (kFp8)
+        return transposed8(at + v_at[0][d & 1]);
+      else
+        return joined(transposed(at + v_at[0][d & 1]), transposed(at + v_at[1][d & 1]));
     };
     // The first operands of P V of step s: its weights, and V's of the first group.
     constexpr int kVGroup = kOb / 2;
     struct First {
-      bf16x8_t w[2][kUnits], v[kVGroup];
+      bf16x8_t w[2][kUnits];
+      Raw v[kVGroup];
     };
     auto first_operands = [&](int s, First& f) {
 #pragma unroll
@@ -472,12 +470,12 @@ __attribute__((amdgpu_waves_per_eu(1, 1))) void latent_decode_kernel(
                                                         k * p_next));
 #pragma unroll
       for (int j = 0; j < kVGroup; ++j)
-        f.v[j] = v_operand(lds + (s % kBuffers) * T::kBytes, j);
+        f.v[j] = v_raw(lds + (s % kBuffers) * T::kBytes, j);
     };
     // (among(x): what to do among the products of the x-th quarter)
     auto values = [&](int s, const First& f, auto among) {
       const uint8_t* const tile = lds + (s % kBuffers) * T::kBytes;
-      bf16x8_t v[2][kVGroup];
+      Raw v[2][kVGroup];
 #pragma unroll
       for (int j = 0; j < kVGroup; ++j) v[0][j] = f.v[j];
 #pragma unroll
@@ -485,7 +483,7 @@ __attribute__((amdgpu_waves_per_eu(1, 1))) void latent_decode_kernel(
         const int now = x0 / kVGroup & 1;
         if (x0 + kVGroup < 2 * kOb) {
 #pragma unroll
-          for (int j = 0; j < kVGroup; ++j) v[now ^ 1][j] = v_operand(tile, x0 + kVGroup + j);
+          for (int j = 0; j < kVGroup; ++j) v[now ^ 1][j] = v_raw(tile, x0 + kVGroup + j);
         }
         __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
@@ -493,8 +491,8 @@ __attribute__((amdgpu_waves_per_eu(1, 1))) void latent_decode_kernel(
           const int k = (x0 + j) / kOb, d = (x0 + j) % kOb;
 #pragma unroll
           for (int u = 0; u < kUnits; ++u)
-            o[u][d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(v[now][j], f.w[k][u], o[u][d], 0, 0,
-                                                              0);
+            o[u][d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(operand(v[now][j]), f.w[k][u],
+                                                              o[u][d], 0, 0, 0);
         }
         among(x0 / kVGroup);
       }
@@ -502,14 +500,11 @@ __attribute__((amdgpu_waves_per_eu(1, 1))) void latent_decode_kernel(
 
     floatx4_t p[kCB], next[kCB];
     // A step's barrier: step s's weights and maxima and step s + 1's tile are in LDS, and step
-    // s - 1 is done with.  The loads (bf16: of step s + 3, fp8: of s + 4, with the conversion of
-    // s + 2) are issued among its products, so that the waves do not wait for their addresses to
-    // be taken.
+    // s - 1 is done with.  The loads of step s + 3 are issued among its products, so that the
+    // waves do not wait for their addresses to be taken.
     auto enter = [&](int s, float (&t)[kUnits]) {
-      if constexpr (!kFp8) {
-        wait_loads<kLoads>();
-        clear(s + 1);
-      }
+      wait_loads<kLoads>();
+      clear(s + 1);
       __syncthreads();
 #pragma unroll
       for (int u = 0; u < kUnits; ++u) {
@@ -521,15 +516,8 @@ __attribute__((amdgpu_waves_per_eu(1, 1))) void latent_decode_kernel(
     float t[kUnits];
     First f;
     __builtin_amdgcn_s_waitcnt(kNoLoads);
-    if constexpr (kFp8) {
-      convert_all(0);
-      convert_all(1);
-      load(2);
-      load(3);
-    } else {
-      clear(0);
-      load(2);
-    }
+    clear(0);
+    load(2);
     __syncthreads();
     scores(0, p, nothing);
     logits(0, p);
@@ -544,7 +532,6 @@ __attribute__((amdgpu_waves_per_eu(1, 1))) void latent_decode_kernel(
       weights(0, p, u);
     }
     enter(0, t);
-    constexpr int kAhead = kFp8 ? 4 : 3;
     int s = 0;
 #pragma unroll 1
     while (s + 1 < steps && !too_far(t)) {  // (step s has been entered)
@@ -556,21 +543,8 @@ __attribute__((amdgpu_waves_per_eu(1, 1))) void latent_decode_kernel(
 #pragma unroll 1
       do {
         constexpr int kGroups = kKc / kGroup;
-        int rows = 0;
-        uint2 raw[3];  // codes on their way from LDS
-        if constexpr (kFp8) {
-          wait_loads<kLoads>();
-          rows = min(max(seen(s + 2, 8 * wave), 0), 8);
-#pragma unroll
-          for (int i = 0; i < 3; ++i) raw[i] = codes(s + 2, i);
-        }
         scores(s + 1, next, [&](int x) {
-          if constexpr (kFp8) {
-            convert(s + 2, rows, x, raw[x % 3]);
-            raw[x % 3] = codes(s + 2, x + 3);
-          } else {
-            issue(m, x);
-          }
+          if (x < kLoads) issue(m, x);
           if (x == kGroups - 1) first_operands(s, f);
         });
         if (too_far(t)) break;  // (looked at behind the products that do not depend on it)
@@ -579,21 +553,10 @@ __attribute__((amdgpu_waves_per_eu(1, 1))) void latent_decode_kernel(
           if (x == 0) logits(s + 1, next);
           if (x == 1) maxima(s + 1, next);
           if (x >= 2 && x - 2 < kCB) weights(s + 1, next, x - 2);
-          if constexpr (kFp8) {
-            if (x < kMoves - kGroups) convert(s + 2, rows, kGroups + x, raw[x]);
-            if (x == 3) {
-              // (the codes have been read, whose place the loads take)
-              __builtin_amdgcn_sched_barrier(0);
-              asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-#pragma unroll
-              for (int i = 0; i < kLoads; ++i) issue(m, i);
-            }
-          } else if (x < kMoves - kGroups) {
-            issue(m, kGroups + x);
-          }
+          if (x < kLoads - kGroups) issue(m, kGroups + x);
           if (x == 3) m = moves_of(s + 1 + kAhead);
         });
-        static_assert(kGroups % 3 == 0 && kMoves - kGroups == 3, "all of them once");
+        static_assert(kLoads - kGroups <= 3, "all of them once");
         p[0] = next[0];
         if constexpr (kCB == 2) p[1] = next[1];
         ++s;
@@ -613,7 +576,6 @@ __attribute__((amdgpu_waves_per_eu(1, 1))) void latent_decode_kernel(
     // theirs, and O, which leaves in whole rows.
     constexpr int kRow = R + 4;  // floats
     float* const xo = reinterpret_cast<float*>(lds);
-    static_assert(4 * kCols * kRow <= 4 * T::kBytes, "O fits");
 #pragma unroll
     for (int cb = 0; cb < kCB; ++cb) tops[kCols * ts + s_col + 16 * cb] = pair_sum(l[cb]);
 #pragma unroll
@@ -730,13 +692,13 @@ __global__ __launch_bounds__(kMergeThreads) void latent_merge_kernel(
 }
 
 struct LatentPlan {
-  int wgs, units;
+  int wgs, units;  // work-groups at most, units of an item
   int64_t o, ml, records, bytes;
 };
 LatentPlan plan_of(int64_t batch, int64_t max_seqlen_q, int num_heads, int latent_size) {
   LatentPlan p{};
   p.units = num_heads > 32 ? 2 : 1;
-  p.wgs = num_cus();
+  p.wgs = num_cus() * wgs_per_cu(p.units, true);
   auto take = [&](int64_t bytes) {
     const int64_t at = p.bytes;
     p.bytes += (bytes + 255) / 256 * 256;
@@ -751,7 +713,8 @@ LatentPlan plan_of(int64_t batch, int64_t max_seqlen_q, int num_heads, int laten
 template <int R, int P, bool kFp8>
 void launch(const LatentParams& A, hipStream_t s, const int32_t* bt, const int32_t* ctx,
             const int32_t* cu) {
-  const unsigned lds = 4 * Tile<R, P>::kBytes + 2 * 32 * A.units * (kKeys * 2 + 2 * 4);
+  const unsigned lds =
+      tiles_bytes<R, P, kFp8>(A.units) + 2 * 32 * A.units * (kKeys * 2 + 2 * 4);
   if (A.units == 1)
     hipLaunchKernelGGL((latent_decode_kernel<R, P, 1, kFp8>), dim3(A.wgs + 1), dim3(kThreads),
                        lds, s, A, bt, ctx, cu);
@@ -842,7 +805,7 @@ extern "C" int fk_latent_decode(void* out, int64_t out_row_stride, int64_t out_h
   A.num_blocks = num_blocks;
   A.bt_row_stride = bt_row_stride;
   A.bt_width = static_cast<int>(bt_width);
-  A.wgs = plan.wgs;
+  A.wgs = num_cus() * wgs_per_cu(plan.units, cache_dtype == FK_DTYPE_FP8_E4M3FN);
   A.head_blocks = (num_heads + 31) / 32;
   A.units = plan.units;
   A.team = (A.head_blocks + plan.units - 1) / plan.units % 2 == 0 ? 2 : 1;
