@@ -157,7 +157,7 @@ __global__ __launch_bounds__(kThreads) void latent_store_kernel(StoreParams P) {
   }
 }
 
-constexpr int kGatherRows = 32;  // of a work-group: their slots are looked up side by side
+constexpr int kGatherRows = 32;  // of a work-group at most: their slots are looked up side by side
 
 // 51 thousand rows from an fp8 cache: 15.8 us, 5.6 TB/s (17.9 with stores through the caches).
 
@@ -166,14 +166,14 @@ __global__ __launch_bounds__(kThreads) void latent_gather_kernel(
     uint16_t* __restrict__ out, int64_t out_stride, const uint8_t* __restrict__ cache,
     const float* __restrict__ scale, const int32_t* __restrict__ bt, int64_t bt_row_stride,
     int bt_width, const int32_t* __restrict__ cu, int batch, int rows, int block_size_log2,
-    int64_t num_blocks) {
+    int64_t num_blocks, int rows_of_wg) {
   constexpr int kPieces = (kLatent + kRope) / 8;
   __shared__ int64_t from[kGatherRows];
-  const int64_t t0 = static_cast<int64_t>(blockIdx.x) * kGatherRows;
-  dense_slots(cu, batch, t0, rows, bt, bt_row_stride, bt_width, block_size_log2, num_blocks, from);
+  const int64_t t0 = static_cast<int64_t>(blockIdx.x) * rows_of_wg;
+  dense_slots(cu, batch, t0, rows_of_wg, rows, bt, bt_row_stride, bt_width, block_size_log2, num_blocks, from);
   const float f = kFp8 && scale ? *scale : 1.f;
 #pragma unroll 3
-  for (int i = threadIdx.x; i < kGatherRows * kPieces; i += kThreads) {
+  for (int i = threadIdx.x; i < rows_of_wg * kPieces; i += kThreads) {
     const int row = i / kPieces, piece = i % kPieces;
     const int64_t at = from[row];
     if (at == -2) continue;
@@ -288,14 +288,15 @@ extern "C" int fk_gather_latent(void* out, int64_t out_row_stride, const void* c
              what);
   if (rows == 0 || batch == 0) return FK_OK;
   FK_REQUIRE(out && cache && block_tables && cu_seqlens_k, "%s: null pointer", what);
-  const dim3 grid(static_cast<unsigned>((rows + kGatherRows - 1) / kGatherRows));
+  const int per = dense_rows_of_wg(rows, kGatherRows);
+  const dim3 grid(static_cast<unsigned>((rows + per - 1) / per));
   const int log2 = 31 - __builtin_clz(static_cast<unsigned>(block_size));
   auto go = [&](auto kernel) {
     hipLaunchKernelGGL(kernel, grid, dim3(kThreads), 0, as_stream(stream),
                        static_cast<uint16_t*>(out), out_row_stride,
                        static_cast<const uint8_t*>(cache), cache_scale, block_tables,
                        bt_row_stride, static_cast<int>(bt_width), cu_seqlens_k,
-                       static_cast<int>(batch), static_cast<int>(rows), log2, num_blocks);
+                       static_cast<int>(batch), static_cast<int>(rows), log2, num_blocks, per);
   };
   if (cache_dtype == FK_DTYPE_FP8_E4M3FN)
     go(latent_gather_kernel<true>);

@@ -23,16 +23,23 @@ __device__ __forceinline__ int sequence_of(const int32_t* __restrict__ cu, int b
   return lo;
 }
 
-// Slots (page * block size + place) of the tokens that rows t0 .. t0 + kRows - 1 of a dense copy
-// of the sequences stand for, into LDS: -1 at a masked page, -2 for a row of no sequence.  cu may
+// Rows of a work-group of such a copy: two work-groups a CU at least, if there are the rows, and at
+// most `most` rows each.
+inline int dense_rows_of_wg(int64_t rows, int most) {
+  const int64_t per = rows / (2 * num_cus());
+  return static_cast<int>(per < 1 ? 1 : per < most ? per : most);
+}
+
+// Slots (page * block size + place) of the tokens that rows t0 .. t0 + per - 1 (at most kRows) of a
+// dense copy of the sequences stand for, into LDS: -1 at a masked page, -2 for a row of no sequence.  cu may
 // not ascend; what is read stays inside the table.
 template <int kRows>
 __device__ __forceinline__ void dense_slots(const int32_t* __restrict__ cu, int batch, int64_t t0,
-                                            int64_t rows, const int32_t* __restrict__ bt,
+                                            int per, int64_t rows, const int32_t* __restrict__ bt,
                                             int64_t bt_row_stride, int bt_width,
                                             int block_size_log2, int64_t num_blocks,
                                             int64_t (&slot)[kRows]) {
-  if (threadIdx.x < kRows) {
+  if (threadIdx.x < per) {
     const int64_t t = t0 + threadIdx.x;
     int64_t at = -2;
     if (t < rows && t >= cu[0] && t < cu[batch]) {
