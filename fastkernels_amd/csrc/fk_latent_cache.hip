@@ -160,7 +160,6 @@ __global__ __launch_bounds__(kThreads) void latent_store_kernel(StoreParams P) {
 constexpr int kGatherRows = 32;  // of a work-group at most: their slots are looked up side by side
 
 // 51 thousand rows from an fp8 cache: 15.8 us, 5.6 TB/s (17.9 with stores through the caches).
-
 template <bool kFp8>
 __global__ __launch_bounds__(kThreads) void latent_gather_kernel(
     uint16_t* __restrict__ out, int64_t out_stride, const uint8_t* __restrict__ cache,
@@ -196,10 +195,11 @@ __global__ __launch_bounds__(kThreads) void latent_gather_kernel(
   }
 }
 
-int check_cache(const char* what, int cache_dtype, const void* cache, int latent_size,
-                int rope_size) {
+int check_cache(const char* what, int cache_dtype, const void* cache, const float* scale,
+                int latent_size, int rope_size) {
   FK_REQUIRE(cache_dtype == FK_DTYPE_BF16 || cache_dtype == FK_DTYPE_FP8_E4M3FN,
              "%s: the cache must be bf16 or fp8 e4m3fn", what);
+  FK_REQUIRE(!scale || cache_dtype == FK_DTYPE_FP8_E4M3FN, "%s: a bf16 cache has no scale", what);
   if (latent_size != kLatent || rope_size != kRope)
     return set_error(FK_ERR_UNSUPPORTED, "%s: rows of %d + %d unsupported (512 + 64)", what,
                      latent_size, rope_size);
@@ -233,7 +233,8 @@ extern "C" int fk_latent_norm_rope_store(
     int64_t latent_out_row_stride, void* key_out, int64_t key_out_row_stride, int64_t tokens,
     int latent_size, int rope_size, void* stream) {
   const char* what = "fk_latent_norm_rope_store";
-  if (int rc = check_cache(what, cache_dtype, cache, latent_size, rope_size)) return rc;
+  if (int rc = check_cache(what, cache_dtype, cache, cache_scale, latent_size, rope_size))
+    return rc;
   FK_REQUIRE(tokens >= 0 && tokens <= 0x7fffffff && num_slots >= 0 && num_heads >= 0 &&
                  num_heads <= 65535 && max_position >= 0,
              "%s: %lld tokens, %lld slots, %d heads", what, static_cast<long long>(tokens),
@@ -274,7 +275,8 @@ extern "C" int fk_gather_latent(void* out, int64_t out_row_stride, const void* c
                                 int64_t rows, int latent_size, int rope_size, int block_size,
                                 int64_t num_blocks, void* stream) {
   const char* what = "fk_gather_latent";
-  if (int rc = check_cache(what, cache_dtype, cache, latent_size, rope_size)) return rc;
+  if (int rc = check_cache(what, cache_dtype, cache, cache_scale, latent_size, rope_size))
+    return rc;
   FK_REQUIRE(block_size >= 16 && block_size <= (1 << 30) && (block_size & (block_size - 1)) == 0,
              "%s: block_size %d must be a power of two >= 16", what, block_size);
   FK_REQUIRE(num_blocks > 0 && num_blocks <= 0x7fffffff, "%s: num_blocks %lld", what,

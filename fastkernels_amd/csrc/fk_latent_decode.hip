@@ -2,12 +2,21 @@
 // to the same keys, a token's row of R + P values, and the values are its first R,
 //   s[t, h, j] = scale q[t, h] . row_j,   out[t, h] = sum_j softmax_j(s) row_j[0 .. R).
 //
-// The query rows of a sequence times the heads are the columns of matrix products with the
-// keys: S^T = K Q^T, then O^T += V^T P^T.  Keys come through LDS once: S reads them as rows, P V
-// the same bytes with the transpose loads.  Items (sequence, 64 columns) of 32-key steps lie on
-// one line, cut into equal ranges, one per CU (fk_lines.h).  An item inside one range is finished
-// there; of the others each part leaves a partial state, which a second launch merges.
+// The heads of a query row are the columns of matrix products with the keys: S^T = K Q^T, then
+// O^T += V^T P^T.  Keys come through LDS once: S reads them as rows, P V the same bytes with the
+// transpose loads.  Items (query row, 32 or 64 heads) of 32-key steps lie on one line, cut into
+// equal ranges (fk_lines.h); where a row has an even number of items, pairs of work-groups take
+// the same range for one each, side by side on an XCD, so that the second finds the keys in the
+// L2 (64 rows of 128 heads: 154 us, 170 without).  An item inside one range is finished there; of
+// the others each part leaves a partial state, which a second launch merges.
 //
+// Measured (a call, captured): 64 rows of 128 heads over 512 .. 8192 tokens 126 us (650 TFLOP/s),
+// of 16 heads 74 us (4.6 TB/s), of 16 heads over fp8 51 us; 128 rows of 16 heads over fp8 up to
+// 16384 153 us (4.4 TB/s).  What bounds it: 1.3 us a step of 64 heads, where the products alone
+// take 0.5 and LDS 0.6.  With all tiles in the L2 a step is no shorter, without S's products or
+// those of P V neither: two tiles on their way (LDS holds no more) cover as much latency as the
+// chain scores, maximum, weights, barrier takes.  Slower: eight waves, four of which do S and four
+// P V (64 x 128: 170 us in place of 154); words of the lines loaded three steps ahead (175).
 #include "fk_lines.h"
 #include "fk_page_attn.h"
 #include "fk_query_rows.h"
@@ -23,9 +32,11 @@ constexpr int kWaves = 4;
 constexpr int kThreads = kWaves * 64;
 constexpr int kSeqs = 128;   // sequences looked at together
 constexpr int kKeys = 32;    // of a tile
-constexpr int kPad = 14;     // what a part costs besides its steps, in steps
-// (Weights to 2^32: with values up to 2^90 their sums stay finite.  No logits of trained models come
-// near it.)
+// What a part costs besides its steps, in steps: first tiles, queries, state.  (64 rows of 128
+// heads: 166 us with 6, 156 with 10, 151 with 14, 154 with 20; others change by less.)
+constexpr int kPad = 14;
+// (Weights to 2^32: with values up to 2^90 their sums stay finite.  Logits that rise so far above the
+// first 32 keys' are rare, and cost a part taken in two.)
 constexpr float kFar = 32.f;
 
 struct LatentParams {
@@ -394,7 +405,7 @@ latent_decode_kernel(
         p[cb] = kChains == 1 ? x[0][cb] : x[0][cb] + x[kChains - 1][cb];
     };
     // The softmax of step s, in four parts: logits, their maxima, weights.
-    // (The weights are rounded to bf16 for P V, 2^-9 relative at most, of either sign; their sum
+    // (The weights are rounded to bf16 for P V, 2^-8 relative at most, of either sign; their sum
     // is of the unrounded ones.)
     auto logits = [&](int s, floatx4_t (&p)[kCB]) {
       // (without a branch, which would part the products around it)
@@ -764,6 +775,8 @@ extern "C" int fk_latent_decode(void* out, int64_t out_row_stride, int64_t out_h
              "%s: max_seqlen_q %lld", what, static_cast<long long>(max_seqlen_q));
   FK_REQUIRE(cache_dtype == FK_DTYPE_BF16 || cache_dtype == FK_DTYPE_FP8_E4M3FN,
              "%s: the cache must be bf16 or fp8 e4m3fn", what);
+  FK_REQUIRE(!cache_scale || cache_dtype == FK_DTYPE_FP8_E4M3FN, "%s: a bf16 cache has no scale",
+             what);
   FK_REQUIRE(block_size >= 16 && block_size <= (1 << 30) && (block_size & (block_size - 1)) == 0,
              "%s: block_size %d must be a power of two >= 16", what, block_size);
   FK_REQUIRE(num_blocks > 0 && num_blocks <= 0x7fffffff, "%s: num_blocks %lld", what,

@@ -89,7 +89,8 @@ __device__ __forceinline__ void row_keys(const SeqRows& s, int i, int window_lef
 }
 
 // Its items on a line: `items` of `steps` steps each, laid end to end, over the keys [from, to)
-// that any of its rows sees.
+// that any of its rows sees.  Each has `pad` steps before its own that stand for what a part of it
+// costs besides them, so that a range of many short items has fewer steps.
 struct LineItems {
   int from, to;
   int steps, items;

@@ -1174,6 +1174,8 @@ def _check_latent(what, cache, scale) -> tuple[torch.Size, int, int | None]:
                          "rope]")
     if cache.dtype == torch.bfloat16:
         tag = _native.FK_DTYPE_BF16
+        if scale is not None:
+            raise ValueError(f"{what}: scale is a float8_e4m3fn cache's; a bf16 one has none")
     elif cache.dtype == _FP8:
         tag = _native.FK_DTYPE_FP8_E4M3FN
     else:
@@ -1200,9 +1202,9 @@ def latent_norm_rope_store(cache: torch.Tensor, slot_mapping: torch.Tensor,
                            key_rope_out: torch.Tensor | None = None) -> None:
     """One launch for the steps between the projections and attention over a latent cache
     ([num_blocks, block_size, latent + rope], bf16 or float8_e4m3fn): c = rmsnorm(latent) with
-    ``weight`` (without: latent as it is), k = key_rope rotated by ``positions``, the row [c | k]
-    (divided by ``scale``, float32 [1]) to slot_mapping[t] (-1 skips; otherwise distinct), and
-    query_out = query_rope rotated.
+    ``weight`` (without: latent as it is), k = key_rope rotated by ``positions`` (as it is where they
+    lie outside cos_sin_cache), the row [c | k] (fp8: divided by ``scale``, float32 [1]) to
+    slot_mapping[t] (-1 skips; otherwise distinct), and query_out = query_rope rotated.
 
     latent [N, R], key_rope [N, P], query_rope / query_out [N, H, P] are bf16, contiguous along the
     last dimension: views of the projections' outputs and of the absorbed queries.  latent_out and

@@ -617,8 +617,8 @@ int fk_mxfp4_paged_decode_plan(int64_t batch, int64_t max_seqlen_q, int num_head
 /* Attention with keys and values from one latent row a token (library version 2.4): the cache
  * side of MLA (fastkernels/tasks/baseline/L2/mla_attention_impl.py).  The cache is
  * [num_blocks, block_size, latent_size + rope_size] of BF16 or FP8_E4M3FN, 16-byte aligned;
- * latent_size 512, rope_size 64; block_size a power of two >= 16.  cache_scale: device fp32
- * scalar or NULL (1); a value is its code times the scale.  Block tables and cu_seqlens_q as in
+ * latent_size 512, rope_size 64; block_size a power of two >= 16.  cache_scale, of an FP8
+ * cache: device fp32 scalar or NULL (1); a value is its code times the scale.  Block tables and cu_seqlens_q as in
  * the section above.
  *
  * fk_latent_norm_rope_store: for each token t

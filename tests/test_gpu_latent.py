@@ -177,7 +177,8 @@ def test_store_in_place_and_special_values(cuda):
 
 @pytest.mark.parametrize("kv", ["bf16", "fp8"])
 @pytest.mark.parametrize("page,lens", [(16, [17, 0, 1, 300]), (64, [64, 65, 200]), (256, [1]),
-                                       (32, [0, 33, 0, 0, 90])])
+                                       (32, [0, 33, 0, 0, 90]), (16, [1500, 0, 1601]),
+                                       (64, [9000, 1, 8001])])
 def test_gather(cuda, kv, page, lens):
     from fastkernels_amd import ops
 

@@ -133,7 +133,9 @@ def test_store_every_rounding(cuda):
 
 @pytest.mark.parametrize("hk,d,page,lens", [(8, 128, 16, [17, 0, 1, 300]), (1, 64, 32, [1]),
                                             (3, 256, 64, [64, 65, 200]),
-                                            (20, 64, 256, [255, 257, 0]), (40, 128, 16, [33])])
+                                            (20, 64, 256, [255, 257, 0]), (40, 128, 16, [33]),
+                                            (2, 64, 16, [1500, 0, 1601]),
+                                            (1, 128, 64, [9000, 1, 8001])])
 def test_gather(cuda, hk, d, page, lens):
     """The rows in between, those of masked pages zero, those of no sequence left alone."""
     from fastkernels_amd import ops

@@ -126,8 +126,9 @@ BAD = [
         (dict(lat=torch.zeros(5, 9216, dtype=BF)), ValueError),
         (dict(lat=torch.zeros(5, 16, 640, dtype=BF)), ValueError),
         (dict(lat=torch.zeros(5, 32, 576, dtype=BF)[:, ::2]), ValueError),
-        (dict(scale=torch.ones(2)), ValueError),
-        (dict(scale=torch.ones(1, dtype=BF)), ValueError))],
+        (dict(scale=torch.ones(1)), ValueError),  # of a bf16 cache
+        (dict(lat=torch.zeros(5, 16, 576).to(FP8), scale=torch.ones(2)), ValueError),
+        (dict(lat=torch.zeros(5, 16, 576).to(FP8), scale=torch.ones(1, dtype=BF)), ValueError))],
     (lstore, dict(c=torch.zeros(3, 512)), ValueError),
     (lstore, dict(c=torch.zeros(2, 512, dtype=BF)), ValueError),
     (lstore, dict(c=torch.zeros(3, 1, 512, dtype=BF)), ValueError),
@@ -250,19 +251,20 @@ def test_c_abi_refusals():
             "fk_latent_norm_rope_store")
     refuses(ls, [dict(r=256), dict(pe=32)], "fk_latent_norm_rope_store", N.FK_ERR_UNSUPPORTED)
 
-    def lg(rows=1, batch=1, out=p, stride=576, page=16, nb=4, width=4, r=512, cu=p, tag=bf):
-        return lib.fk_gather_latent(out, stride, p, tag, None, p, 4, width, cu, batch, rows, r, 64,
+    def lg(rows=1, batch=1, out=p, stride=576, page=16, nb=4, width=4, r=512, cu=p, tag=bf,
+           scale=None):
+        return lib.fk_gather_latent(out, stride, p, tag, scale, p, 4, width, cu, batch, rows, r, 64,
                                     page, nb, None)
 
     assert lg(rows=0) == N.FK_OK and lg(batch=0) == N.FK_OK
     refuses(lg, [dict(rows=-1), dict(rows=1 << 31), dict(batch=-1), dict(out=odd),
                  dict(stride=577), dict(page=17), dict(nb=0), dict(width=-1), dict(cu=None),
-                 dict(tag=N.FK_DTYPE_F32)], "fk_gather_latent")
+                 dict(tag=N.FK_DTYPE_F32), dict(scale=p)], "fk_gather_latent")
     refuses(lg, [dict(r=448)], "fk_gather_latent", N.FK_ERR_UNSUPPORTED)
 
     def ld(rows=1, batch=1, most=1, heads=16, tag=bf, page=16, nb=4, r=512, ws=p, size=1 << 40,
-           q=p, head_stride=576, cu=None):
-        return lib.fk_latent_decode(p, 8192, 512, q, 9216, head_stride, p, tag, None, p, 4, 4, p,
+           q=p, head_stride=576, cu=None, scale=None):
+        return lib.fk_latent_decode(p, 8192, 512, q, 9216, head_stride, p, tag, scale, p, 4, 4, p,
                                     cu, batch, rows, most, heads, r, 64, page, nb, 0.1, None, 0,
                                     ws, size, None)
 
@@ -270,7 +272,7 @@ def test_c_abi_refusals():
     refuses(ld, [dict(rows=-1), dict(rows=65536), dict(batch=65536), dict(most=0),
                  dict(most=65536), dict(heads=0), dict(heads=65536), dict(page=48), dict(nb=0),
                  dict(tag=N.FK_DTYPE_F16), dict(q=odd), dict(q=None), dict(head_stride=577),
-                 dict(ws=odd)], "fk_latent_decode")
+                 dict(ws=odd), dict(scale=p)], "fk_latent_decode")
     refuses(ld, [dict(r=256)], "fk_latent_decode", N.FK_ERR_UNSUPPORTED)
     refuses(ld, [dict(ws=None), dict(size=1000)], "fk_latent_decode", N.FK_ERR_WORKSPACE)
 
