@@ -111,23 +111,43 @@ __global__ __launch_bounds__(kThreads) void store_mxfp4_kernel(
 // CUs idle (117 rows of 8 heads of 128: 3.5 us, 14.7 with 32 each).
 constexpr int kGatherRows = 32;
 
-// A thread takes the same 8 dims of several rows, whose loads are in flight together.  50 thousand
-// tokens of 8 heads of 128: 50.6 us, 5.1 TB/s (84 with stores through the caches, which push out
-// the lines of codes that four tokens share; 79 so with a wave per row).
+// The rows of four tokens that lie side by side in the cache go together: a thread takes 8 dims of
+// them, whose V codes and scales are then one load each.  50 thousand tokens of 8 heads of 128:
+// 51 us, 5.1 TB/s, and 70 where no cache holds any of it (86 with a row at a time; 84 and 88 with
+// stores through the caches).
 __global__ __launch_bounds__(kThreads) void gather_mxfp4_kernel(
     CacheParams P, uint16_t* __restrict__ key, int64_t key_stride, uint16_t* __restrict__ value,
     int64_t value_stride, const int32_t* __restrict__ bt, int64_t bt_row_stride, int bt_width,
     int64_t num_blocks, const int32_t* __restrict__ cu, int batch, int rows, int rows_of_wg) {
   __shared__ int64_t slots[kGatherRows];
+  __shared__ int first_row[kGatherRows + 1];  // of each group
+  __shared__ int groups_of_wg;
   const int64_t t0 = static_cast<int64_t>(blockIdx.x) * rows_of_wg;
-  dense_slots(cu, batch, t0, rows_of_wg, rows, bt, bt_row_stride, bt_width, P.block_size_log2, num_blocks,
-              slots);
+  dense_slots(cu, batch, t0, rows_of_wg, rows, bt, bt_row_stride, bt_width, P.block_size_log2,
+              num_blocks, slots);
   const int n = static_cast<int>(min(static_cast<int64_t>(rows_of_wg), rows - t0));
-  // Short rows: several side by side.
+  // A row begins a group unless it is the next token of the row before and in the same four.
+  bool begins = false;
+  if (threadIdx.x < n) {
+    const int64_t s = slots[threadIdx.x];
+    begins = threadIdx.x == 0 || s < 0 || s % 4 == 0 || slots[threadIdx.x - 1] != s - 1;
+  }
+  const uint64_t all = __ballot(begins);  // (the first wave has all of them)
+  if (threadIdx.x < 64) {
+    const int before = __builtin_popcountll(all & ((uint64_t{1} << threadIdx.x) - 1));
+    if (begins) first_row[before] = threadIdx.x;
+    if (threadIdx.x == 0) {
+      groups_of_wg = __builtin_popcountll(all);
+      first_row[groups_of_wg] = n;
+    }
+  }
+  __syncthreads();
+  const int groups = groups_of_wg;
+  // Short rows: several groups side by side.
   const int cols = 2 * P.units;
   const int per = cols < kThreads ? kThreads / cols : 1;
-  const int row0 = cols < kThreads ? threadIdx.x / cols : 0;
-  if (row0 >= per) return;
+  const int group0 = cols < kThreads ? threadIdx.x / cols : 0;
+  if (group0 >= per) return;
   for (int u = cols < kThreads ? threadIdx.x % cols : threadIdx.x; u < cols; u += kThreads) {
     const bool is_v = u >= P.units;
     const int at = 8 * (is_v ? u - P.units : u);
@@ -135,21 +155,36 @@ __global__ __launch_bounds__(kThreads) void gather_mxfp4_kernel(
     const uint8_t* const scales = is_v ? P.v_scales : P.k_scales;
     uint16_t* const out = (is_v ? value + t0 * value_stride : key + t0 * key_stride) + at;
     const int64_t stride = is_v ? value_stride : key_stride;
-#pragma unroll 8
-    for (int row = row0; row < n; row += per) {
-      const int64_t slot = slots[row], from = max(slot, int64_t{0});
+#pragma unroll 4
+    for (int k = group0; k < groups; k += per) {
+      const int row = first_row[k], end = first_row[k + 1];
+      const int64_t slot = slots[row], from = max(slot, int64_t{0}) & ~int64_t{3};
       const int in = static_cast<int>(from & ((1 << P.block_size_log2) - 1));
       const int64_t hp = (from >> P.block_size_log2) * P.num_kv_heads + head;
-      const uint32_t e = scales[scale_at(P, hp, in, dim)];
+      const uint32_t e = *reinterpret_cast<const uint32_t*>(scales + scale_at(P, hp, in, dim));
       const uint8_t* const p = is_v ? v_codes(P, hp, in, dim) : k_codes(P, hp, in, dim);
-      // (V at head size 64: two halves of two bytes)
-      const uint32_t codes = is_v && P.head_size == 64
-                                 ? *reinterpret_cast<const uint16_t*>(p) |
-                                       *reinterpret_cast<const uint16_t*>(p + 8) << 16
-                                 : *reinterpret_cast<const uint32_t*>(p);
-      uint4 x = fp4x8_to_bf16x8(codes, __uint_as_float(e << 23));
-      if (slot < 0) x = make_uint4(0, 0, 0, 0);
-      if (slot != -2) store_past(out + row * stride, x);
+      uint32_t w[4];  // codes of the four tokens
+      if (is_v && P.head_size != 256) {
+        const uint4 x = *reinterpret_cast<const uint4*>(p);
+        if (P.head_size == 128) {
+          w[0] = x.x, w[1] = x.y, w[2] = x.z, w[3] = x.w;
+        } else {  // the four tokens' first 4 dims, then the others
+          w[0] = lo_pair(x.x, x.z), w[1] = hi_pair(x.x, x.z);
+          w[2] = lo_pair(x.y, x.w), w[3] = hi_pair(x.y, x.w);
+        }
+      } else {
+        const int apart = is_v ? 8 : P.head_size / 2;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) w[i] = *reinterpret_cast<const uint32_t*>(p + i * apart);
+      }
+      const int first = slot < 0 ? 0 : static_cast<int>(slot & 3);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        if (i < first || row + i - first >= end || slot == -2) continue;
+        uint4 x = fp4x8_to_bf16x8(w[i], __uint_as_float((e >> (8 * i) & 0xff) << 23));
+        if (slot < 0) x = make_uint4(0, 0, 0, 0);
+        store_past(out + (row + i - first) * stride, x);
+      }
     }
   }
 }
