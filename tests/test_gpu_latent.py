@@ -208,6 +208,7 @@ BATCHES = {
     "drafts": ([300, 3, 40, 1, 900], [4, 3, 1, 1, 5]),
     "holes": ([300, 2, 0, 70], [0, 3, 2, 2]),  # more rows than tokens: the first see none
     "many": ([17 * i % 90 for i in range(70)], None),
+    "negative": ([40, -3, 20], None),  # a length below zero is none
 }
 
 
@@ -233,7 +234,8 @@ def run(cuda, cache, heads, bt, lens, rows, scale, s, g, spare=0, most=None, q=N
 @pytest.mark.parametrize("name", list(BATCHES))
 @pytest.mark.parametrize("kv,heads,page", [("bf16", 16, 16), ("bf16", 128, 64), ("bf16", 20, 256),
                                            ("fp8", 16, 64), ("fp8", 128, 16), ("bf16", 33, 32),
-                                           ("fp8", 1, 128), ("fp8", 70, 32), ("bf16", 64, 16)])
+                                           ("fp8", 1, 128), ("fp8", 70, 32), ("bf16", 64, 16),
+                                           ("bf16", 150, 16), ("fp8", 256, 64)])
 def test_decode(cuda, kv, heads, page, name):
     lens, rows = BATCHES[name]
     g = torch.Generator(device=cuda).manual_seed(heads + page + len(lens))

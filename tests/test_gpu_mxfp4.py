@@ -167,13 +167,14 @@ def test_gather(cuda, hk, d, page, lens):
 # decode attention
 # ---------------------------------------------------------------------------
 SHAPES = [(32, 8, 128, 16), (16, 2, 256, 16), (20, 20, 64, 32), (64, 8, 128, 64), (64, 8, 64, 256),
-          (8, 1, 128, 16), (40, 2, 256, 128), (34, 2, 128, 16)]
+          (8, 1, 128, 16), (40, 2, 256, 128), (34, 2, 128, 16), (128, 1, 64, 16)]
 BATCHES = {
     "one": ([1], None), "zeros": ([0, 0], None), "short": ([31, 33, 0, 1, 16], None),
     "mixed": ([700, 5, 0, 1300, 64, 63, 65], None),
     "drafts": ([300, 3, 40, 1, 900], [4, 3, 1, 1, 5]),
     "holes": ([300, 2, 0, 70], [0, 3, 2, 2]),  # more rows than tokens: the first see none
     "many": ([17 * i % 90 for i in range(70)], None),
+    "negative": ([40, -3, 20], None),  # a length below zero is none
 }
 
 
