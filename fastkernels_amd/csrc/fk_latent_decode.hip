@@ -509,7 +509,6 @@ latent_decode_kernel(
       }
     };
 
-    floatx4_t p[kCB], next[kCB];
     // A step's barrier: step s's weights and maxima and step s + 1's tile are in LDS, and step
     // s - 1 is done with.  The loads of step s + 3 are issued among its products, so that the
     // waves do not wait for their addresses to be taken.
@@ -530,6 +529,7 @@ latent_decode_kernel(
     clear(0);
     load(2);
     __syncthreads();
+    floatx4_t p[kCB];
     scores(0, p, nothing);
     logits(0, p);
     maxima(0, p);
@@ -554,22 +554,20 @@ latent_decode_kernel(
 #pragma unroll 1
       do {
         constexpr int kGroups = kKc / kGroup;
-        scores(s + 1, next, [&](int x) {
+        scores(s + 1, p, [&](int x) {
           if (x < kLoads) issue(m, x);
           if (x == kGroups - 1) first_operands(s, f);
         });
         if (too_far(t)) break;  // (looked at behind the products that do not depend on it)
         count();
         values(s, f, [&](int x) {
-          if (x == 0) logits(s + 1, next);
-          if (x == 1) maxima(s + 1, next);
-          if (x >= 2 && x - 2 < kCB) weights(s + 1, next, x - 2);
+          if (x == 0) logits(s + 1, p);
+          if (x == 1) maxima(s + 1, p);
+          if (x >= 2 && x - 2 < kCB) weights(s + 1, p, x - 2);
           if (x < kLoads - kGroups) issue(m, kGroups + x);
           if (x == 3) m = moves_of(s + 1 + kAhead);
         });
         static_assert(kLoads - kGroups <= 3, "all of them once");
-        p[0] = next[0];
-        if constexpr (kCB == 2) p[1] = next[1];
         ++s;
         enter(s, t);
       } while (s + 1 < steps && known(s + kAhead));
