@@ -539,3 +539,34 @@ def test_streams_and_compile(cuda):
     compiled = torch.compile(step, backend="aot_eager", fullgraph=True)
     for c, w in zip(ctxs, want):
         assert torch.equal(compiled(q, c), w)
+
+
+@pytest.mark.parametrize("kv", ["bf16", "fp8"])
+def test_compiled_step(cuda, kv):
+    """A store into a view of the queries and the attention behind it under torch.compile: the bits
+    of the eager step, in the cache, the queries and the result."""
+    g = torch.Generator(device=cuda).manual_seed(6)
+    cache, scale = make_cache(g, 20, 16, kv, cuda), scale_of(kv, cuda)
+    bt = torch.randperm(20, generator=g, device=cuda).to(torch.int32).view(2, 10)
+    q = torch.randn(2, 16, 576, generator=g, device=cuda).to(BF)
+    raw = torch.randn(2, 16, 64, generator=g, device=cuda).to(BF)
+    proj = torch.randn(2, 576, generator=g, device=cuda).to(BF)
+    pos, ctx = torch.tensor([8, 100], device=cuda), int32([9, 101], cuda)
+    slots = torch.stack([bt[0, 0] * 16 + 8, bt[1, 6] * 16 + 4]).long()
+    rope = load("rotary_emb", "RotaryEmbedding")(64, 512, 10000.0).to(cuda)
+    norm = load("rms_norm", "RMSNorm")(512).to(cuda, BF)
+    attn = load("latent_attn", "LatentAttnDecode")(16, 0.05)
+
+    def step(cache, q):
+        rope.forward_store_latent(pos, raw, proj[:, :512], proj[:, 512:], cache, slots, norm,
+                                  q[:, :, 512:], scale)
+        return attn(q, cache, ctx, bt, scale)
+
+    got = []
+    for f in (step, torch.compile(step, backend="aot_eager", fullgraph=True)):
+        c, x = cache.clone(), q.clone()
+        out = f(c, x)
+        got.append((out, x, c.view(torch.uint8) if kv == "fp8" else c.view(torch.int16)))
+    assert not torch.equal(got[0][1], q)
+    for a, b in zip(*got):
+        assert torch.equal(a, b)

@@ -510,3 +510,33 @@ def test_streams_and_compile(cuda):
     compiled = torch.compile(step, backend="aot_eager", fullgraph=True)
     for c, w in zip(ctxs, want):
         assert torch.equal(compiled(q, c), w)
+
+
+def test_compiled_step(cuda):
+    """A store, the read-back and the attention under torch.compile: the bits of the eager step."""
+    hq, hk, d, page = 16, 2, 128, 16
+    g = torch.Generator(device=cuda).manual_seed(6)
+    cache = random_cache(g, 20, page, hk, d, cuda)
+    bt = torch.randperm(20, generator=g, device=cuda).to(torch.int32).view(2, 10)
+    q = torch.randn(2, hq, d, generator=g, device=cuda).to(BF)
+    new = torch.randn(2, 2, hk, d, generator=g, device=cuda).to(BF)
+    ctx, cu = int32([9, 101], cuda), int32([0, 9, 110], cuda)
+    slots = torch.stack([bt[0, 0] * 16 + 8, bt[1, 6] * 16 + 4]).long()
+    attn = load("flash_attn_decode", "FlashAttnDecode")(hq, hk, d)
+    put = load("store_kvcache", "StoreKVCacheMxfp4")()
+
+    def step(k, v, ks, vs, q):
+        put(new[0], new[1], (k, v, ks, vs), slots)
+        key = torch.zeros(110, hk, d, dtype=BF, device=q.device)
+        value = torch.zeros_like(key)
+        torch.ops.fastkernels_amd.gather_kvcache_mxfp4(key, value, k, v, ks, vs, bt, cu)
+        return attn.forward_mxfp4(q, (k, v, ks, vs), ctx, block_table=bt), key, value
+
+    got = []
+    for f in (step, torch.compile(step, backend="aot_eager", fullgraph=True)):
+        c = [t.clone() for t in cache]
+        got.append((*f(*c, q), *c))
+    for a, b in zip(*got):
+        assert torch.equal(a, b)
+    want = ref.mxfp4_values(*ref.mxfp4_blocks(f64(new[0])))
+    assert np.array_equal(f64(got[1][1][[8, 109]]), want)
