@@ -489,6 +489,8 @@ extern "C" int fk_mxfp4_paged_decode(
   FK_REQUIRE(num_blocks <= (int64_t{1} << 32) / block_size / num_kv_heads,
              "%s: %lld pages of %d heads", what, static_cast<long long>(num_blocks),
              num_kv_heads);
+  // (a lane's offset to a block's scales is 32 bits)
+  FK_REQUIRE(block_size <= 1 << 28, "%s: block_size %d above 2^28", what, block_size);
   if (batch == 0 || rows == 0) return FK_OK;
   FK_REQUIRE(out && q && k_cache && v_cache && k_scales && v_scales && block_tables &&
                  cache_seqlens,

@@ -234,7 +234,8 @@ def test_c_abi_refusals():
     refuses(de, [dict(rows=-1), dict(rows=65536), dict(batch=65536), dict(most=0),
                  dict(most=65536), dict(hq=9), dict(hk=0), dict(page=24), dict(nb=0),
                  dict(nb=1 << 30), dict(window=-2), dict(scales=odd), dict(scales=None),
-                 dict(ws=odd), dict(stride=1025)], "fk_mxfp4_paged_decode")
+                 dict(ws=odd), dict(stride=1025), dict(page=1 << 29, nb=1)],
+            "fk_mxfp4_paged_decode")
     refuses(de, [dict(d=96)], "fk_mxfp4_paged_decode", N.FK_ERR_UNSUPPORTED)
     refuses(de, [dict(ws=None), dict(size=1000)], "fk_mxfp4_paged_decode", N.FK_ERR_WORKSPACE)
 
