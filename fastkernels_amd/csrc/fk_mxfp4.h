@@ -32,12 +32,14 @@ __device__ __forceinline__ uint4 fp4x8_to_bf16x8(uint32_t w, float scale) {
 // Scale byte of a block whose greatest magnitude is `top`: the exponent of top rounded to two
 // significant bits, less that of the format's greatest power (4).  Rounded so, top is at most 7
 // of the block's units, and every value at most half a step of the grid from its code.  (With
-// top's own exponent, 6 would stand for values up to 8.)
+// top's own exponent, 6 would stand for values up to 8.)  From 1.75 2^127 on that scale's code would
+// be 2^128, which reads back as an infinity: such values become 1.5 2^127, the greatest below it.
+constexpr uint32_t kTopScale = 252;
 __device__ __forceinline__ uint32_t block_scale(float top) {
   const uint32_t u = __float_as_uint(top);
   if (u >= 0x7f800000u) return 255;  // infinity, NaN
   const uint32_t e = (u + 0x200000u) >> 23;
-  return e > 2 ? e - 2 : 0;
+  return e > 2 ? min(e - 2, kTopScale) : 0;
 }
 
 }  // namespace fk

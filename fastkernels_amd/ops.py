@@ -1067,8 +1067,8 @@ def store_kvcache_mxfp4(key: torch.Tensor, value: torch.Tensor, k_cache: torch.T
     """:func:`store_kvcache` into a 4-bit cache (:class:`Mxfp4Cache`): key/value [N, Hk, D] of
     float32, float16 or bfloat16, slot_mapping (-1 skips; otherwise distinct).  Each 32 dims of a
     row share a power of two, the exponent of their greatest magnitude rounded to two significant
-    bits, less 2; values are rounded to the nearest of {0, 0.5, 1, 1.5, 2, 3, 4, 6} times it, ties
-    to the even code.  32 dims with an infinity or a NaN become NaN."""
+    bits, less 2 (at most 2^125); values are rounded to the nearest of {0, 0.5, 1, 1.5, 2, 3, 4, 6}
+    times it, ties to the even code.  32 dims with an infinity or a NaN become NaN."""
     what = "store_kvcache_mxfp4"
     if key.dim() != 3 or value.shape != key.shape:
         raise ValueError(f"{what}: key/value must be [N, num_kv_heads, head_dim]")

@@ -576,8 +576,9 @@ int fk_shared_prefix_decode_plan(int64_t batch, int64_t num_groups, int64_t max_
  * key_row_stride / value_row_stride elements apart) go to slot slot_mapping[t] = page *
  * block_size + place (int32 or int64; skipped outside [0, num_blocks * block_size); distinct).
  * A block's E is the exponent of its greatest magnitude, rounded to two significant bits, less
- * 2 (at least 0); values are rounded to the nearest code, ties to the even one, so that none is
- * off by more than half a step.  A block with an infinity or a NaN is NaN. */
+ * 2 (at least 0, at most 252); values are rounded to the nearest code, ties to the even one, so
+ * that none is off by more than half a step, but for magnitudes from 1.75 2^127 on, which become
+ * 1.5 2^127.  A block with an infinity or a NaN is NaN. */
 int fk_store_kvcache_mxfp4(const void* key, int64_t key_row_stride, const void* value,
                            int64_t value_row_stride, int dtype, void* k_cache, void* v_cache,
                            void* k_scales, void* v_scales, const void* slot_mapping,

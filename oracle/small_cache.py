@@ -20,7 +20,8 @@ def mxfp4_blocks(x):
     top = np.abs(b).max(-1)
     bad = ~np.isfinite(b).all(-1)
     m, e = np.frexp(np.where(bad, 1.0, top))  # top = m 2^e, 0.5 <= m < 1
-    scale = np.where(top > 0, np.maximum(e - 1 + (m >= 0.875) - 2 + 127, 0), 0).astype(np.int64)
+    # (at most 252: 253's code for the greatest values would be 2^128, which bf16 has not)
+    scale = np.where(top > 0, np.clip(e - 1 + (m >= 0.875) - 2 + 127, 0, 252), 0).astype(np.int64)
     v = np.abs(np.where(bad[..., None], 0.0, b)) / 2.0 ** (scale[..., None] - 127)
     code = np.zeros(b.shape, np.int64)
     for i in range(7):  # past the middle of codes i and i + 1; on it, to the even one

@@ -131,6 +131,30 @@ def test_store_every_rounding(cuda):
         assert np.array_equal(got.reshape(-1, 64)[:n], want)
 
 
+@pytest.mark.parametrize("dtype", [torch.float32, BF])
+@pytest.mark.parametrize("d", [64, 128, 256])
+def test_the_greatest_magnitudes_stay_finite(cuda, dtype, d):
+    """Blocks whose greatest value is next to the type's end, of both signs: what is read back is
+    finite, and what the definition says."""
+    from fastkernels_amd import ops
+
+    tops = [1.2 * 2.0 ** 127, 1.74 * 2.0 ** 127, 1.75 * 2.0 ** 127, 1.9 * 2.0 ** 127, 3.0e38,
+            float(torch.finfo(dtype).max), 1.74 * 2.0 ** 126, 1.75 * 2.0 ** 126]
+    n = len(tops)
+    x = torch.rand(n, 1, d // 32, 32, device=cuda) * 1.5
+    x[..., 5], x[..., 6] = 1.0, -1.0
+    x = (x.clamp(-1, 1) * torch.tensor(tops, device=cuda).view(n, 1, 1, 1)).flatten(2).to(dtype)
+    assert bool(x.isfinite().all())
+    cache = ops.new_mxfp4_cache(1, 16, 1, d, cuda)
+    ops.store_kvcache_mxfp4(x, -x, *cache, torch.arange(n, device=cuda))
+    key = torch.empty(n, 1, d, dtype=BF, device=cuda)
+    value = torch.empty_like(key)
+    ops.gather_kvcache_mxfp4(key, value, *cache, int32([[0]], cuda), int32([0, n], cuda))
+    want = ref.mxfp4_values(*ref.mxfp4_blocks(x.double().cpu().numpy()))
+    assert np.isfinite(f64(key)).all() and np.isfinite(f64(value)).all()
+    assert np.array_equal(f64(key), want) and np.array_equal(f64(value), -want)
+
+
 @pytest.mark.parametrize("hk,d,page,lens", [(8, 128, 16, [17, 0, 1, 300]), (1, 64, 32, [1]),
                                             (3, 256, 64, [64, 65, 200]),
                                             (20, 64, 256, [255, 257, 0]), (40, 128, 16, [33]),

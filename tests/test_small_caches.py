@@ -387,6 +387,17 @@ def test_blocks_are_nearest():
         assert np.isnan(y[32:]).all() and not np.isnan(y[:32]).any()
 
 
+def test_greatest_blocks_stay_finite():
+    """From 1.75 2^127 on values become 1.5 2^127: the next value of a greater scale is 2^128."""
+    for top, scale, want in ((1.25 * 2.0 ** 127, 252, 1.0), (1.74 * 2.0 ** 127, 252, 1.5),
+                             (1.75 * 2.0 ** 127, 252, 1.5), (3.0e38, 252, 1.5),
+                             (float(np.finfo(np.float32).max), 252, 1.5),
+                             (1.74 * 2.0 ** 126, 251, 0.75), (1.75 * 2.0 ** 126, 252, 1.0)):
+        s, c = ref.mxfp4_blocks(np.array([top, -top] + [0.0] * 30))
+        assert s[0] == scale and ref.mxfp4_values(s, c)[:2].tolist() == [want * 2.0 ** 127,
+                                                                         -want * 2.0 ** 127]
+
+
 def test_layouts():
     """The arrays of a cache, byte by byte."""
     rng = np.random.default_rng(1)
