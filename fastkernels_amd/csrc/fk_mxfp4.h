@@ -18,7 +18,8 @@ template <int kByte>
 __device__ __forceinline__ float scale_of(uint32_t w) {
   return __uint_as_float(kByte == 3 ? w >> 1 : w << (23 - 8 * kByte));
 }
-// The two codes of byte i of w as bf16 values times the scale: exact, whatever the scale.
+// The two codes of byte i of w as bf16 values times the scale: exact up to the scale 2^125, and
+// beyond it but for values of 2^128 and more (a store makes none), which become infinities.
 template <int kByte>
 __device__ __forceinline__ uint32_t fp4x2_to_bf16x2(uint32_t w, float scale) {
   return __builtin_bit_cast(uint32_t,
@@ -35,6 +36,8 @@ __device__ __forceinline__ uint4 fp4x8_to_bf16x8(uint32_t w, float scale) {
 // top's own exponent, 6 would stand for values up to 8.)  From 1.75 2^127 on that scale's code would
 // be 2^128, which reads back as an infinity: such values become 1.5 2^127, the greatest below it.
 constexpr uint32_t kTopScale = 252;
+// Scales above it may have infinities among their values, or NaN (255).
+__device__ __forceinline__ bool all_finite(uint32_t e) { return e <= kTopScale; }
 __device__ __forceinline__ uint32_t block_scale(float top) {
   const uint32_t u = __float_as_uint(top);
   if (u >= 0x7f800000u) return 255;  // infinity, NaN

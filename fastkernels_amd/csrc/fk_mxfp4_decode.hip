@@ -328,12 +328,14 @@ __attribute__((amdgpu_waves_per_eu(2))) void mxfp4_decode_kernel(
         // Any column's keys: the lanes of a group of 16 hold the same ones.
 #pragma unroll
         for (int off = 8; off; off >>= 1) keep |= __shfl_xor(keep, off, 64);
-        // A NaN among them that some of the columns do not see stays with the others: row by row.
-        bool nan = false;
+        // A NaN or an infinity among them that some of the columns do not see stays with the
+        // others: row by row.
+        bool odd = false;
 #pragma unroll
         for (int i = 0; i < 8; ++i)
-          nan |= (keep >> i & 1) && ((i < 4 ? c.vs.x : c.vs.y) >> (8 * (i & 3)) & 0xff) == 0xff;
-        if (row_a == row_z || __ballot(nan) == 0) {
+          odd |= (keep >> i & 1) &&
+                 !all_finite((i < 4 ? c.vs.x : c.vs.y) >> (8 * (i & 3)) & 0xff);
+        if (row_a == row_z || __ballot(odd) == 0) {
           values<kCB, D, false>(st, c, sa, sb, keep, 0);
           return;
         }

@@ -1096,8 +1096,9 @@ def gather_kvcache_mxfp4(key: torch.Tensor, value: torch.Tensor, k_cache: torch.
                          v_cache: torch.Tensor, k_scales: torch.Tensor, v_scales: torch.Tensor,
                          block_table: torch.Tensor, cu_seqlens_k: torch.Tensor) -> None:
     """key / value (bf16 [rows, Hk, D]): row cu_seqlens_k[b] + i becomes what a 4-bit cache holds
-    of position i of sequence b, exactly (zeros where block_table has no page); rows behind the
-    last sequence stay as they were.  The dense keys that :func:`varlen_prefill` takes for a chunk
+    of position i of sequence b, exactly (zeros where block_table has no page; infinities for values
+    of 2^128 and more, which a store does not make); rows behind the last sequence stay as they
+    were.  The dense keys that :func:`varlen_prefill` takes for a chunk
     of a prompt over such a cache."""
     what = "gather_kvcache_mxfp4"
     nb, hk, bs, d = _check_mxfp4(what, k_cache, v_cache, k_scales, v_scales)

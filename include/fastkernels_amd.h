@@ -586,7 +586,8 @@ int fk_store_kvcache_mxfp4(const void* key, int64_t key_row_stride, const void* 
                            int block_size, int64_t num_blocks, void* stream);
 
 /* Rows cu_seqlens_k[b] + i of key and value (bf16 [rows, Hk, D], row strides in elements,
- * 16-byte aligned) = what the cache holds of position i of sequence b, exactly; zeros at masked
+ * 16-byte aligned) = what the cache holds of position i of sequence b, exactly (values of 2^128
+ * and more, which scales of 253 and 254 allow and no store makes, are infinities); zeros at masked
  * pages.  cu_seqlens_k: int32 [batch + 1]; rows behind the last sequence are left as they
  * were.  Dense keys for fk_varlen_prefill over a context that is held in 4 bits. */
 int fk_gather_kvcache_mxfp4(void* key, int64_t key_row_stride, void* value,

@@ -187,6 +187,30 @@ def test_gather(cuda, hk, d, page, lens):
     assert bool((wide[:, 2 * hk * d + 8:] == 9.0).all())
 
 
+@pytest.mark.parametrize("d", [64, 128, 256])
+def test_gather_every_scale(cuda, d):
+    """All codes under all scale bytes: exact, from 2^-128 to the greatest bf16, and infinities for
+    what is beyond."""
+    from fastkernels_amd import ops
+
+    cache = ops.new_mxfp4_cache(1, 256, 1, d, cuda)
+    code = torch.arange(16, dtype=torch.uint8, device=cuda)
+    pairs = (code[0::2] | code[1::2] << 4).repeat(d // 16)
+    cache.k_cache[:] = pairs
+    cache.v_cache[:] = pairs.view(1, 1, 1, 16, 1, d // 32)
+    cache.k_scales[:] = torch.arange(256, dtype=torch.uint8, device=cuda)
+    cache.v_scales[:] = torch.arange(256, dtype=torch.uint8, device=cuda).flip(0)
+    key = torch.empty(256, 1, d, dtype=BF, device=cuda)
+    value = torch.empty_like(key)
+    ops.gather_kvcache_mxfp4(key, value, *cache, int32([[0]], cuda), int32([0, 256], cuda))
+    for got, want in zip((key, value), values(cache)):
+        want = want.reshape(256, 1, d)
+        big = np.abs(want) >= 2.0 ** 128
+        assert np.array_equal(big.any((1, 2)), np.isin(want[:, 0, 1], [2.0 ** 125, 2.0 ** 126]))
+        want[big] = np.copysign(np.inf, want[big])
+        assert np.array_equal(f64(got), want, equal_nan=True)
+
+
 # ---------------------------------------------------------------------------
 # decode attention
 # ---------------------------------------------------------------------------
@@ -308,6 +332,38 @@ def test_decode_nan_stays_with_the_rows_that_see_it(cuda, hq, hk, d):
     nan[2:4, :gqa, 32:64] = True
     nan[7, hq - gqa:] = True
     assert np.array_equal(~seen, nan)
+
+
+@pytest.mark.parametrize("byte,code", [(253, 6), (253, 15), (254, 4), (254, 14)])
+@pytest.mark.parametrize("hq,hk,d,page", [(8, 2, 128, 16), (16, 1, 64, 64), (8, 2, 256, 16),
+                                          (24, 1, 128, 32)])
+def test_decode_infinities_stay_with_the_rows_that_see_them(cuda, hq, hk, d, page, byte, code):
+    """A value of 2^128 or more in V, which bf16 does not have, at keys that the last rows of a
+    sequence see: infinite there, in its dim alone."""
+    from fastkernels_amd import ops
+
+    lens, rows = [70, 100, 45], [4, 4, 2]
+    g = torch.Generator(device=cuda).manual_seed(d)
+    bt, pool = tables(g, [-(-n // page) for n in lens], cuda)
+    cache = random_cache(g, pool, page, hk, d, cuda)
+    q = torch.randn(10, hq, d, generator=g, device=cuda).to(BF)
+    t = lens[0] - 2  # seen by rows 2 and 3 of the first sequence
+    p, s = int(bt[0, t // page]), t % page
+    cache.v_scales[p, 0, 1, s] = byte  # of dims 32 .. 63: their codes 0, but for dim 32's
+    first = 32 // (d // 16)
+    cache.v_cache[p, 0, s // 4, first:2 * first, s % 4] = 0
+    cache.v_cache[p, 0, s // 4, first, s % 4, 0] = code
+    assert abs(values(cache)[1][p, s, 0, 32]) >= 2.0 ** 128
+    out, cu = torch.empty_like(q), cu_of(rows, cuda)
+    ops.mxfp4_paged_decode(out, q, *cache, bt, int32(lens, cuda), d ** -0.5, cu_seqlens_q=cu,
+                           max_seqlen_q=4)
+    want, mean, mag = ref.paged_decode(f64(q), *values(cache), bt.cpu().numpy(), lens, d ** -0.5,
+                                       cu_seqlens_q=cu.tolist())
+    inf = np.zeros(out.shape, bool)
+    inf[2:4, :hq // hk, 32] = True
+    assert np.array_equal(f64(out)[inf], np.where(code & 8, -np.inf, np.inf).repeat(inf.sum()))
+    want[inf] = np.nan
+    assert np.array_equal(check(out, want, mean, mag, 100), ~inf)
 
 
 @pytest.mark.parametrize("d", [64, 128, 256])
