@@ -35,9 +35,14 @@ constexpr int kKeys = 32;    // of a tile
 // What a part costs besides its steps, in steps: first tiles, queries, state.  (64 rows of 128
 // heads: 166 us with 6, 156 with 10, 151 with 14, 154 with 20; others change by less.)
 constexpr int kPad = 14;
-// (Weights to 2^32: with values up to 2^90 their sums stay finite.  Logits that rise so far above the
-// first 32 keys' are rare, and cost a part taken in two.)
+// How far a part's logits may rise above those of its first 32 keys before it is taken in two, which
+// is rare and costs a state written and read.
 constexpr float kFar = 32.f;
+// All weights, and with them the sums, carry this factor, so that none exceeds 2^8, as in the
+// other decode kernels: n keys with values to 2^120 / n have finite sums.  (The first keys' are
+// about 2^-24: bf16 and the fp32 sums hold them as exactly, and products of values down to
+// 2^-102 with them are normal numbers.)
+constexpr float kUnit = 0x1p-24f;
 
 struct LatentParams {
   uint16_t* out;
@@ -188,12 +193,15 @@ __device__ __forceinline__ LineItems line_items(const LatentParams& P, const Seq
 // Output of four dims of a finished column, and with dim == 0 its log-sum-exp.
 __device__ __forceinline__ void write_out(const LatentParams& P, int64_t row, int head, int dim,
                                           const float4& o, float M, float L, float vsc) {
-  const float f = L > 0.f ? vsc / L : 0.f;
+  // (1 / L may be 1 / kUnit, and a great scale times that no float.)
+  const float unit = __builtin_fabsf(vsc) > 1.f ? kUnit : 1.f;
+  const float f = L > 0.f ? vsc * unit / L : 0.f, g = 1.f / unit;
   *reinterpret_cast<uint2*>(P.out + row * P.out_row_stride + head * P.out_head_stride + dim) =
-      make_uint2(pack2(o.x * f, o.y * f), pack2(o.z * f, o.w * f));
+      make_uint2(pack2(o.x * f * g, o.y * f * g), pack2(o.z * f * g, o.w * f * g));
   if (dim == 0 && P.lse)
     P.lse[head * P.lse_head_stride + row] =
-        L > 0.f ? (M + __builtin_amdgcn_logf(L)) * 0.6931471805599453f : L == 0.f ? kNegInf : L;
+        L > 0.f ? (M + __builtin_amdgcn_logf(L * (1.f / kUnit))) * 0.6931471805599453f
+                : L == 0.f ? kNegInf : L;
 }
 
 // One work-group: items of kUnits units of 32 heads of a query row, in steps of a tile.
@@ -206,8 +214,8 @@ __device__ __forceinline__ void write_out(const LatentParams& P, int64_t row, in
 // A step has one barrier.  Behind it come S of the next step and P V of this one, with the next
 // step's softmax among the products of the latter.
 //
-// A column's weights are 2^(logit - m), m the maximum of the first step: bf16 and the fp32 sums
-// hold great weights as exactly as small ones, and O is not rescaled.  Where a later maximum, which
+// A column's weights are kUnit 2^(logit - m), m the maximum of the first step: bf16 and the fp32
+// sums hold great weights as exactly as small ones, and O is not rescaled.  Where a later maximum, which
 // all waves know behind the next barrier, is 2^kFar times that, the part is taken in two: the state
 // so far goes to memory, and what follows begins again with its own maximum and is merged with it.
 constexpr int kBuffers = 4;  // tiles in LDS, of which two are on their way
@@ -426,7 +434,7 @@ latent_decode_kernel(
     auto weights = [&](int s, const floatx4_t (&p)[kCB], int cb) {
       float e[4];
 #pragma unroll
-      for (int i = 0; i < 4; ++i) e[i] = __builtin_amdgcn_exp2f(p[cb][i] - ms[cb]);
+      for (int i = 0; i < 4; ++i) e[i] = kUnit * __builtin_amdgcn_exp2f(p[cb][i] - ms[cb]);
       last[cb] = (e[0] + e[1]) + (e[2] + e[3]);
       *reinterpret_cast<uint2*>(p_at(s_col + 16 * cb, 16 * ts + 4 * g) + (s & 1) * kP) =
           make_uint2(pack2(e[0], e[1]), pack2(e[2], e[3]));

@@ -659,8 +659,9 @@ int fk_gather_latent(void* out, int64_t out_row_stride, const void* cache, int c
 /* The absorbed form: out[t, h] (bf16 [rows, num_heads, latent_size]) = sum_j w_j c_j, w the
  * softmax of scale q[t, h] . [c_j | k_j] over the first vis keys of the row's sequence; q bf16
  * [rows, num_heads, latent_size + rope_size].  Row and head strides in elements, 16-byte
- * aligned.  lse (or NULL): fp32 [num_heads, rows], heads lse_head_stride apart: the natural log of
- * the softmax's denominator.  A row that sees no key is zero, its lse -infinity.  Keys that a row
+ * aligned.  Weights reach 2^8 and their sums with the values are fp32: of n keys, values (fp8:
+ * codes) up to 2^120 / n.  lse (or NULL): fp32 [num_heads, rows], heads lse_head_stride apart: the
+ * natural log of the softmax's denominator.  A row that sees no key is zero, its lse -infinity.  Keys that a row
  * does not see may hold anything.  batch, rows and max_seqlen_q <= 65535. */
 int fk_latent_decode(void* out, int64_t out_row_stride, int64_t out_head_stride, const void* q,
                      int64_t q_row_stride, int64_t q_head_stride, const void* cache,

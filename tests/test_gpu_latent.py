@@ -330,6 +330,47 @@ def test_decode_of_great_magnitudes(cuda, kv, sign):
                           rtol=1e-6)
 
 
+@pytest.mark.parametrize("kv,power", [("bf16", 109), ("bf16", -100), ("bf16", -115), ("fp8", 110),
+                                      ("fp8", -110)])
+@pytest.mark.parametrize("heads", [16, 40])
+@pytest.mark.parametrize("raised", [True, False])
+def test_decode_of_great_and_small_values(cuda, kv, power, heads, raised):
+    """Values of one sign next to 2^119 / 700 keys, and small ones, under logits that rise by nearly
+    2^32 (base 2: by 32) behind the first 32 keys, or do not: what the sums come to is finite, and
+    as exact as elsewhere.  Many rows, so that parts hold whole sequences.
+
+    Small values: a weight is 2^-24 of the sum at least, a sum of n products is off by 2^-150 for
+    each where they are no normal numbers, so the result by n 2^-126; and by half of bf16's least
+    step, 2^-134."""
+    from fastkernels_amd import ops
+
+    n, page, batch = 700, 64, 600
+    g = torch.Generator(device=cuda).manual_seed(heads)
+    cache = torch.rand(11, page, 576, generator=g, device=cuda)
+    scale = torch.tensor([2.0 ** power], device=cuda) if kv == "fp8" else None
+    cache *= 440.0 if kv == "fp8" else 2.0 ** power
+    cache[:, :, 512:] = 0
+    if raised:
+        cache[:, :, 512] = 22.0 if kv == "fp8" else 21.75
+        cache[0, :32, 512] = 0
+    cache = cache.to(FP8 if kv == "fp8" else BF)
+    q = torch.zeros(batch, heads, 576, dtype=BF, device=cuda)
+    q[:, :, 512] = 1
+    s = 1.0 if kv == "bf16" else 2.0 ** -power
+    out = torch.empty(batch, heads, 512, dtype=BF, device=cuda)
+    lse = torch.empty(heads, batch, device=cuda)
+    ops.latent_decode(out, q, cache, int32([list(range(11))] * batch, cuda),
+                      int32([n] * batch, cuda), s, scale, lse=lse)
+    want, mean, _, want_lse = ref.latent_decode(f64(q[:1]), dense(cache, scale),
+                                                np.arange(11)[None], [n], s)
+    assert np.isfinite(f64(out)).all()
+    tol = attn_tolerance(want, mean, 22.0, 1) - 1e-30 + n * E24 * mean + \
+        (n * 2.0 ** -126 if kv == "bf16" else 0) + 2.0 ** -134
+    assert (np.abs(f64(out) - want) <= tol).all()
+    tol = 4 * E24 * 22 + n * E24 + 8 * E24 * (1 + np.abs(want_lse))
+    assert (np.abs(lse.double().cpu().numpy() - want_lse) <= tol).all()
+
+
 @pytest.mark.parametrize("kv,heads,page,n,rows", [("bf16", 16, 16, 33001, 1), ("fp8", 128, 64, 20000, 2),
                                                   ("bf16", 40, 256, 9000, 5)])
 def test_decode_of_one_long_sequence(cuda, kv, heads, page, n, rows):
