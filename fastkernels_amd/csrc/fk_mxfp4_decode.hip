@@ -81,12 +81,12 @@ __device__ __forceinline__ void load_step(const Mxfp4Params& P, uint32_t page0, 
          ((static_cast<uint32_t>(g * D / 128) << log2) + 16 * (r >> 3) + (k_row & 8));
     vs = P.v_scales + s_row + ((static_cast<uint32_t>(r * D / 512) << log2) + 16 * (g >> 1) + v_row);
   } else {
-    const uint32_t rk = (r >> 3 ? page1 : page0) << log2, rv = (g >> 1 ? page1 : page0) << log2;
-    k = P.A.k_cache + static_cast<uint64_t>(rk) * kRow + (k_row * kRow + g * (D / 8));
-    v = P.A.v_cache + static_cast<uint64_t>(rv) * kRow + (v_row * kRow + r * (D / 8));
-    ks = P.k_scales + static_cast<uint64_t>(rk) * kBlocks +
+    const uint64_t pk = r >> 3 ? page1 : page0, pv = g >> 1 ? page1 : page0;
+    k = P.A.k_cache + pk * (16 * kRow) + (k_row * kRow + g * (D / 8));
+    v = P.A.v_cache + pv * (16 * kRow) + (v_row * kRow + r * (D / 8));
+    ks = P.k_scales + pk * (16 * kBlocks) +
          ((static_cast<uint32_t>(g * D / 128) << log2) + (k_row & 8));
-    vs = P.v_scales + static_cast<uint64_t>(rv) * kBlocks +
+    vs = P.v_scales + pv * (16 * kBlocks) +
          ((static_cast<uint32_t>(r * D / 512) << log2) + v_row);
   }
   ld_words(k, c.k[0]);
@@ -487,10 +487,9 @@ extern "C" int fk_mxfp4_paged_decode(
   FK_REQUIRE(window_left >= -1, "%s: window_left %d must be -1 or >= 0", what, window_left);
   FK_REQUIRE(max_seqlen_q >= 1 && max_seqlen_q <= 65535, "%s: max_seqlen_q %lld", what,
              static_cast<long long>(max_seqlen_q));
-  // (more are more bytes than a GPU has)
-  FK_REQUIRE(num_blocks <= (int64_t{1} << 32) / block_size / num_kv_heads,
-             "%s: %lld pages of %d heads", what, static_cast<long long>(num_blocks),
-             num_kv_heads);
+  // (a head's page is counted in 32 bits; more are over 2 TB)
+  FK_REQUIRE(num_blocks * num_kv_heads <= 0x7fffffff, "%s: %lld pages of %d heads", what,
+             static_cast<long long>(num_blocks), num_kv_heads);
   // (a lane's offset to a block's scales is 32 bits)
   FK_REQUIRE(block_size <= 1 << 28, "%s: block_size %d above 2^28", what, block_size);
   if (batch == 0 || rows == 0) return FK_OK;

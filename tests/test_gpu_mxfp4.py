@@ -462,6 +462,28 @@ def test_caches_past_4_gib(cuda):
         assert torch.equal(a, b)
 
 
+@pytest.mark.parametrize("hk,d", [(8, 128), (1, 64)])
+def test_decode_of_small_pages_past_4_gib(cuda, hk, d):
+    """Pages of 16 tokens, two of them to a step, on both sides of the byte offset 2^32."""
+    from fastkernels_amd import ops
+
+    g = torch.Generator(device=cuda).manual_seed(4)
+    nb = (5 << 30) // (16 * hk * d // 2)
+    at = [nb - 1, 0, nb * 4 // 5 - 1, nb * 4 // 5 + 1, nb // 2, nb - 2]
+    small, big = random_cache(g, 6, 16, hk, d, cuda), ops.new_mxfp4_cache(nb, 16, hk, d, cuda)
+    for x, y in zip(big, small):
+        for i, p in enumerate(at):
+            x[p] = y[i]
+    q = torch.randn(3, 2 * hk, d, generator=g, device=cuda).to(BF)
+    got = []
+    for cache, pages in ((small, range(6)), (big, at)):
+        out = torch.empty_like(q)
+        ops.mxfp4_paged_decode(out, q, *cache, int32([list(pages)] * 3, cuda),
+                               int32([96, 33, 70], cuda), d ** -0.5)
+        got.append(out)
+    assert torch.equal(*got)
+
+
 # ---------------------------------------------------------------------------
 # together
 # ---------------------------------------------------------------------------

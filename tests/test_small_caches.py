@@ -287,6 +287,21 @@ def test_c_abi_refusals():
         assert f(*good, None) == N.FK_ERR_INVALID_ARG
 
 
+@pytest.mark.parametrize("page,hk,nb", [(16, 2, 1 << 28), (16, 1, (1 << 31) - 1), (64, 8, 1 << 27),
+                                        (1 << 20, 1, 4104)])
+def test_c_abi_takes_every_cache_that_fits_a_gpu(page, hk, nb):
+    """2^32 tokens and more of a head of 64 are 272 GiB; with pages counted in 32 bits there is
+    room for all."""
+    lib, p = N.lib(), ctypes.c_void_p(0x100000)
+
+    def de(nb):
+        return lib.fk_mxfp4_paged_decode(p, 64, p, 64, p, p, p, p, p, 4, 4, p, None, 0, 1, 1, hk, hk,
+                                         64, page, nb, 0.1, -1, None, p, 1 << 40, None)
+
+    assert de(nb) == N.FK_OK, lib.fk_last_error().decode()
+    assert de((1 << 31) // hk) == N.FK_ERR_INVALID_ARG
+
+
 def test_modules_refuse():
     from fastkernels_amd.candidate.L1.flash_attn_decode import FlashAttnDecode
     from fastkernels_amd.candidate.L1.latent_attn import LatentAttnDecode
