@@ -19,6 +19,8 @@ int set_error(int code, const char* fmt, ...);
 int check_launch(const char* what);
 // Compute units of the current device (queried once per device).
 int num_cus();
+// Work-groups of so many threads that a launch takes: a grid dimension has fewer than 2^32 threads.
+constexpr int64_t most_groups(int threads) { return 0xffffffffLL / threads; }
 
 #define FK_REQUIRE(cond, ...)                                  \
   do {                                                         \

@@ -235,7 +235,7 @@ extern "C" int fk_latent_norm_rope_store(
   const char* what = "fk_latent_norm_rope_store";
   if (int rc = check_cache(what, cache_dtype, cache, cache_scale, latent_size, rope_size))
     return rc;
-  FK_REQUIRE(tokens >= 0 && tokens <= 0x7fffffff && num_slots >= 0 && num_heads >= 0 &&
+  FK_REQUIRE(tokens >= 0 && tokens <= most_groups(kThreads) && num_slots >= 0 && num_heads >= 0 &&
                  num_heads <= 65535 && max_position >= 0,
              "%s: %lld tokens, %lld slots, %d heads", what, static_cast<long long>(tokens),
              static_cast<long long>(num_slots), num_heads);
@@ -281,7 +281,8 @@ extern "C" int fk_gather_latent(void* out, int64_t out_row_stride, const void* c
              "%s: block_size %d must be a power of two >= 16", what, block_size);
   FK_REQUIRE(num_blocks > 0 && num_blocks <= 0x7fffffff, "%s: num_blocks %lld", what,
              static_cast<long long>(num_blocks));
-  FK_REQUIRE(rows >= 0 && rows <= 0x7fffffff && batch >= 0 && batch <= 0x7fffffff,
+  FK_REQUIRE(rows >= 0 && rows <= most_groups(kThreads) * kGatherRows && batch >= 0 &&
+                 batch <= 0x7fffffff,
              "%s: %lld rows of %lld sequences", what, static_cast<long long>(rows),
              static_cast<long long>(batch));
   FK_REQUIRE(bt_width >= 0 && bt_width <= 0x7fffffff && bt_row_stride >= 0,

@@ -252,8 +252,8 @@ extern "C" int fk_store_kvcache_mxfp4(const void* key, int64_t key_row_stride, c
   if (int rc = fill(what, P, k_cache, v_cache, k_scales, v_scales, num_kv_heads, head_size,
                     block_size, num_blocks))
     return rc;
-  FK_REQUIRE(tokens >= 0 && tokens <= (int64_t{1} << 39) / (2 * P.units), "%s: %lld tokens", what,
-             static_cast<long long>(tokens));
+  FK_REQUIRE(tokens >= 0 && tokens <= most_groups(kThreads) * kThreads / (2 * P.units),
+             "%s: %lld tokens, more than a launch takes", what, static_cast<long long>(tokens));
   if (tokens == 0) return FK_OK;
   FK_REQUIRE(key && value && k_cache && v_cache && k_scales && v_scales && slot_mapping,
              "%s: null pointer", what);
@@ -292,7 +292,8 @@ extern "C" int fk_gather_kvcache_mxfp4(void* key, int64_t key_row_stride, void* 
                     const_cast<void*>(k_scales), const_cast<void*>(v_scales), num_kv_heads,
                     head_size, block_size, num_blocks))
     return rc;
-  FK_REQUIRE(rows >= 0 && rows <= 0x7fffffff && batch >= 0 && batch <= 0x7fffffff,
+  FK_REQUIRE(rows >= 0 && rows <= most_groups(kThreads) * kGatherRows && batch >= 0 &&
+                 batch <= 0x7fffffff,
              "%s: %lld rows of %lld sequences", what, static_cast<long long>(rows),
              static_cast<long long>(batch));
   FK_REQUIRE(bt_width >= 0 && bt_width <= 0x7fffffff && bt_row_stride >= 0,

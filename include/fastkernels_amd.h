@@ -578,7 +578,7 @@ int fk_shared_prefix_decode_plan(int64_t batch, int64_t num_groups, int64_t max_
  * A block's E is the exponent of its greatest magnitude, rounded to two significant bits, less
  * 2 (at least 0, at most 252); values are rounded to the nearest code, ties to the even one, so
  * that none is off by more than half a step, but for magnitudes from 1.75 2^127 on, which become
- * 1.5 2^127.  A block with an infinity or a NaN is NaN. */
+ * 1.5 2^127.  A block with an infinity or a NaN is NaN.  tokens * Hk * D / 4 < 2^32. */
 int fk_store_kvcache_mxfp4(const void* key, int64_t key_row_stride, const void* value,
                            int64_t value_row_stride, int dtype, void* k_cache, void* v_cache,
                            void* k_scales, void* v_scales, const void* slot_mapping,
@@ -589,7 +589,8 @@ int fk_store_kvcache_mxfp4(const void* key, int64_t key_row_stride, const void* 
  * 16-byte aligned) = what the cache holds of position i of sequence b, exactly (values of 2^128
  * and more, which scales of 253 and 254 allow and no store makes, are infinities); zeros at masked
  * pages.  cu_seqlens_k: int32 [batch + 1]; rows behind the last sequence are left as they
- * were.  Dense keys for fk_varlen_prefill over a context that is held in 4 bits. */
+ * were.  Dense keys for fk_varlen_prefill over a context that is held in 4 bits.
+ * rows <= 2^29 - 32. */
 int fk_gather_kvcache_mxfp4(void* key, int64_t key_row_stride, void* value,
                             int64_t value_row_stride, const void* k_cache, const void* v_cache,
                             const void* k_scales, const void* v_scales,
@@ -621,8 +622,8 @@ int fk_mxfp4_paged_decode_plan(int64_t batch, int64_t max_seqlen_q, int num_head
  * side of MLA (fastkernels/tasks/baseline/L2/mla_attention_impl.py).  The cache is
  * [num_blocks, block_size, latent_size + rope_size] of BF16 or FP8_E4M3FN, 16-byte aligned;
  * latent_size 512, rope_size 64; block_size a power of two >= 16.  cache_scale, of an FP8
- * cache: device fp32 scalar or NULL (1); a value is its code times the scale.  Block tables and cu_seqlens_q as in
- * the section above.
+ * cache: device fp32 scalar or NULL (1); a value is its code times the scale.  Block tables and
+ * cu_seqlens_q as in the section above.
  *
  * fk_latent_norm_rope_store: for each token t
  *   c = latent[t] / sqrt(mean(latent[t]^2) + eps) * weight   (as it is with weight NULL),
@@ -633,7 +634,7 @@ int fk_mxfp4_paged_decode_plan(int64_t batch, int64_t max_seqlen_q, int num_head
  * [0, num_slots); distinct), fp8 rounded to nearest even and saturated at 448.  latent_out and
  * key_out (or NULL) take c and k in bf16.  Everything is computed in fp32 and rounded once.
  * Tensors are bf16 with rows and heads 16-byte aligned; each output may be its input.
- * num_heads 0: no queries. */
+ * num_heads 0: no queries.  tokens < 2^24. */
 int fk_latent_norm_rope_store(void* cache, int cache_dtype, const float* cache_scale,
                               const void* slot_mapping, int slot_is_i64, int64_t num_slots,
                               const int64_t* positions, const void* latent,
@@ -650,7 +651,7 @@ int fk_latent_norm_rope_store(void* cache, int cache_dtype, const float* cache_s
 /* Row cu_seqlens_k[b] + i of out (bf16 [rows, latent_size + rope_size], 16-byte aligned) = the
  * cache's row of position i of sequence b (times cache_scale); zeros at masked pages; rows behind
  * the last sequence are left as they were.  What the expanded form projects up to keys and
- * values (fk_varlen_prefill at head sizes 192 / 128). */
+ * values (fk_varlen_prefill at head sizes 192 / 128).  rows <= 2^29 - 32. */
 int fk_gather_latent(void* out, int64_t out_row_stride, const void* cache, int cache_dtype,
                      const float* cache_scale, const int32_t* block_tables,
                      int64_t bt_row_stride, int64_t bt_width, const int32_t* cu_seqlens_k,
@@ -662,8 +663,9 @@ int fk_gather_latent(void* out, int64_t out_row_stride, const void* cache, int c
  * [rows, num_heads, latent_size + rope_size].  Row and head strides in elements, 16-byte
  * aligned.  Weights reach 2^8 and their sums with the values are fp32: of n keys, values (fp8:
  * codes) up to 2^120 / n.  lse (or NULL): fp32 [num_heads, rows], heads lse_head_stride apart: the
- * natural log of the softmax's denominator.  A row that sees no key is zero, its lse -infinity.  Keys that a row
- * does not see may hold anything.  batch, rows and max_seqlen_q <= 65535. */
+ * natural log of the softmax's denominator.  A row that sees no key is zero, its lse
+ * -infinity.  Keys that a row does not see may hold anything.  batch, rows and max_seqlen_q
+ * <= 65535. */
 int fk_latent_decode(void* out, int64_t out_row_stride, int64_t out_head_stride, const void* q,
                      int64_t q_row_stride, int64_t q_head_stride, const void* cache,
                      int cache_dtype, const float* cache_scale, const int32_t* block_tables,

@@ -287,6 +287,34 @@ def test_c_abi_refusals():
         assert f(*good, None) == N.FK_ERR_INVALID_ARG
 
 
+def test_c_abi_refuses_more_than_a_launch_takes():
+    """A grid has fewer than 2^32 threads: refused by the arguments' checks, before a launch."""
+    lib, p = N.lib(), ctypes.c_void_p(0x100000)
+
+    def st(tokens, hk, d):
+        return lib.fk_store_kvcache_mxfp4(p, hk * d, p, hk * d, N.FK_DTYPE_BF16, p, p, p, p, p, 0,
+                                          tokens, hk, d, 16, 4, None)
+
+    def ga(rows):
+        return lib.fk_gather_kvcache_mxfp4(p, 64, p, 64, p, p, p, p, p, 4, 4, p, 1, rows, 1, 64, 16,
+                                           4, None)
+
+    def ls(tokens):
+        return lib.fk_latent_norm_rope_store(p, N.FK_DTYPE_BF16, None, p, 0, 64, p, p, 512, p, 64,
+                                             None, 1e-6, p, N.FK_DTYPE_F32, 32, 0, None, 0, 0, 0,
+                                             None, 0, 0, None, 0, None, 0, tokens, 512, 64, None)
+
+    def lg(rows):
+        return lib.fk_gather_latent(p, 576, p, N.FK_DTYPE_BF16, None, p, 4, 4, p, 1, rows, 512, 64,
+                                    16, 4, None)
+
+    for f, bad in ((lambda n: st(n, 8, 128), 1 << 24), (lambda n: st(n, 1, 64), 1 << 28),
+                   (lambda n: st(n, 65535, 256), 1025), (ga, 1 << 29), (ls, 1 << 24),
+                   (lg, 1 << 29)):
+        assert f(bad) == N.FK_ERR_INVALID_ARG
+        assert str(bad) in lib.fk_last_error().decode()
+
+
 @pytest.mark.parametrize("page,hk,nb", [(16, 2, 1 << 28), (16, 1, (1 << 31) - 1), (64, 8, 1 << 27),
                                         (1 << 20, 1, 4104)])
 def test_c_abi_takes_every_cache_that_fits_a_gpu(page, hk, nb):
