@@ -10,13 +10,15 @@
 // L2 (64 rows of 128 heads: 154 us, 170 without).  An item inside one range is finished there; of
 // the others each part leaves a partial state, which a second launch merges.
 //
-// Measured (a call, captured): 64 rows of 128 heads over 512 .. 8192 tokens 126 us (650 TFLOP/s),
-// of 16 heads 74 us (4.6 TB/s), of 16 heads over fp8 51 us; 128 rows of 16 heads over fp8 up to
-// 16384 153 us (4.4 TB/s).  What bounds it: 1.3 us a step of 64 heads, where the products alone
+// Measured (a call, captured): 64 rows of 128 heads over 512 .. 8192 tokens 127 us (645 TFLOP/s),
+// of 16 heads 78 us (4.4 TB/s), of 16 heads over fp8 51 us; 128 rows of 16 heads over fp8 up to
+// 16384 158 us (4.3 TB/s).  What bounds it: 1.3 us a step of 64 heads, where the products alone
 // take 0.5 and LDS 0.6.  With all tiles in the L2 a step is no shorter, without S's products or
 // those of P V neither: two tiles on their way (LDS holds no more) cover as much latency as the
 // chain scores, maximum, weights, barrier takes.  Slower: eight waves, four of which do S and four
-// P V (64 x 128: 170 us in place of 154); words of the lines loaded three steps ahead (175).
+// P V (64 x 128: 170 us in place of 154); words of the lines loaded three steps ahead (175).  (The fp8
+// kernel of one unit spills 40 bytes a lane, touched where the line is walked, not among the loads
+// into LDS, whose waits it would make longer.)
 #include "fk_lines.h"
 #include "fk_page_attn.h"
 #include "fk_query_rows.h"

@@ -12,11 +12,13 @@
 // others each part leaves a partial state, which a second launch merges.
 //
 // Measured (a call, captured): 64 rows over 512 .. 8192 tokens, 32 / 8 heads of 128, pages of 16:
-// 68 us, 4.7 TB/s (bf16 pages 203, fp8 114); 8 rows over up to 65536, 64 / 8 heads 74 us; 32
-// sequences with up to 4 rows 94 us, 3.7 TB/s.  What bounds it: memory with one column block;
+// 69 us, 4.7 TB/s (bf16 pages 212, fp8 116); 8 rows over up to 65536, 64 / 8 heads 75 us; 32
+// sequences with up to 4 rows 99 us, 3.5 TB/s.  What bounds it: memory with one column block;
 // with two, the vector instructions between the loads (48% of the time; a step's 300, of which 64
-// are conversions), as with 20 / 20 heads of 64 (110 us), where one column of 16 is used.  A third
-// set of codes in registers costs 5% (spills, code), codes through LDS three steps ahead 3 to 20%.
+// are conversions), as with 20 / 20 heads of 64 (112 us), where one column of 16 is used.  (What the
+// kernels of two column blocks and of head size 256 spill, 132 and 176 bytes a lane, is touched once
+// a part.)  A third set of codes in registers costs 5% (more spills, code), codes through LDS three
+// steps ahead 3 to 20%.
 //
 // Lanes.  Lane (r, g), r = lane % 16, g = lane / 16.  A step's keys 8 j + i are row 4 j + i of
 // tile A and keys 8 j + 4 + i row 4 j + i of tile B, so that column r's scores of tile A and B

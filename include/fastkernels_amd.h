@@ -602,7 +602,8 @@ int fk_gather_kvcache_mxfp4(void* key, int64_t key_row_stride, void* value,
 /* out[t, hq] = softmax attention of q[t, hq] (bf16 [rows, num_heads, D], heads contiguous) over
  * the keys it sees: the last window_left + 1 (-1: all) of its sequence's first vis.  sinks as
  * fk_paged_decode; a row that sees no key is zero.  Keys that a row does not see may hold
- * anything.  rows and max_seqlen_q <= 65535, block_size <= 2^28, num_blocks * num_kv_heads
+ * anything.  Weights reach 2^8 and their sums with the values are fp32: of n keys, values up to
+ * 2^120 / n.  rows and max_seqlen_q <= 65535, block_size <= 2^28, num_blocks * num_kv_heads
  * < 2^31. */
 int fk_mxfp4_paged_decode(void* out, int64_t out_row_stride, const void* q, int64_t q_row_stride,
                           const void* k_cache, const void* v_cache, const void* k_scales,
